@@ -22,13 +22,17 @@ struct cpq_device {
   struct cpq_commands* eval_session = nullptr;
 };
 
+constexpr int kStatusWords = 7;  // of cpq_commands::status
+
 struct cpq_commands {
   cpq_device* dev = nullptr;
   hipStream_t stream = nullptr;
   bool owns_stream = false;
   // Device-side status words: kernels that can detect bad data count it
   // here ([0] gather rows with out-of-range indices, [1] embed ids out of
-  // range, [2] MoE combine positions out of range)
+  // range, [2] MoE combine positions out of range, [3] blocks that
+  // cpq_kv_release dropped, [4] tokens that cpq_kv_plan did not place, [5]
+  // slots past a key/value cache, [6] what cpq_kv_attention could not compute)
   // add to it; cpq_commands_wait reads and clears it.
   unsigned int* status = nullptr;
   // Scratch of the split-K reductions and the routing sort: arrival
@@ -292,6 +296,26 @@ bool gather_supported(int bits, int n_rows, int n, int k, int gs);
 hipError_t launch_gather_qmm(hipStream_t s, const QuantArgs& q, const void* x, int x_rows,
                              const uint32_t* lhs, const uint32_t* rhs, int n_rows, void* y,
                              int n_experts, int n, int k, bool sorted, unsigned int* status);
+
+// Key/value cache in 4 bits (kernels/kv_cache.hip; layouts in cpq.h).
+constexpr size_t kKvMaxSeqs = 8192;
+hipError_t launch_kv_release(hipStream_t s, const uint32_t* finished, const uint32_t* lens, const uint32_t* table,
+                             uint32_t n_seqs, uint32_t max_blocks, uint32_t block_size, uint32_t* free_list,
+                             uint32_t free_cap, const uint32_t* free_count, uint32_t* lens_out,
+                             uint32_t* free_count_out, unsigned int* bad);
+hipError_t launch_kv_plan(hipStream_t s, const uint32_t* lens, const uint32_t* new_lens, uint32_t* table,
+                          uint32_t n_seqs, uint32_t max_blocks, uint32_t block_size, const uint32_t* free_list,
+                          uint32_t free_cap, const uint32_t* free_count, uint32_t* starts, uint32_t* kv_lens,
+                          uint32_t* slots, uint32_t* positions, uint32_t cap, uint32_t* free_count_out,
+                          unsigned int* bad);
+hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k, size_t k_token, size_t k_head,
+                            const void* v, size_t v_token, size_t v_head, const uint32_t* slots, uint32_t n_tokens,
+                            unsigned int* bad);
+hipError_t launch_kv_gather(hipStream_t s, const cpq_kv_cache& c, const uint32_t* slots, uint32_t n_rows, void* k_out,
+                            void* v_out, unsigned int* bad);
+// Attention over it (kernels/kv_attention.hip).
+hipError_t launch_kv_attention(hipStream_t s, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                               unsigned int* bad);
 
 // Whether the small-M kernel's per-slab constants fit in LDS at this K and
 // group size (16 columns x (K/gs + 1) x 16 bytes next to its static LDS).

@@ -190,9 +190,9 @@ cpq_status cpq_write_buffer(cpq_device* dev, void* dev_ptr, const void* host, si
 static cpq_status make_commands(cpq_device* dev, hipStream_t stream, bool owns,
                                 cpq_commands** out) {
   unsigned int* status = nullptr;
-  hipError_t e = hipMalloc(&status, 3 * sizeof(unsigned int));
+  hipError_t e = hipMalloc(&status, kStatusWords * sizeof(unsigned int));
   if (e != hipSuccess) return hip_fail(e, "hipMalloc(status word)");
-  e = hipMemset(status, 0, 3 * sizeof(unsigned int));
+  e = hipMemset(status, 0, kStatusWords * sizeof(unsigned int));
   if (e != hipSuccess) {
     (void)hipFree(status);
     return hip_fail(e, "hipMemset(status word)");
@@ -259,10 +259,10 @@ cpq_status cpq_commands_wait(cpq_commands* cmds) {
   if (!cmds) return fail(CPQ_ERR_INVALID_ARGUMENT, "cpq_commands_wait: NULL session");
   hipError_t e = hipStreamSynchronize(cmds->stream);
   if (e != hipSuccess) return cpq_completion_result((int)e);
-  unsigned int bad[3] = {0u, 0u, 0u};
+  unsigned int bad[kStatusWords] = {};
   e = hipMemcpy(bad, cmds->status, sizeof(bad), hipMemcpyDeviceToHost);
   if (e != hipSuccess) return hip_fail(e, "hipMemcpy(status word)");
-  if (bad[0] || bad[1] || bad[2]) {
+  if (std::any_of(bad, bad + kStatusWords, [](unsigned int n) { return n != 0; })) {
     e = hipMemset(cmds->status, 0, sizeof(bad));
     if (e != hipSuccess) return hip_fail(e, "hipMemset(status word)");
     std::string msg;
@@ -276,6 +276,18 @@ cpq_status cpq_commands_wait(cpq_commands* cmds) {
     if (bad[2])
       msg += std::string(msg.empty() ? "" : "; ") + "moe_combine: " + std::to_string(bad[2]) +
              " (token, slot) position(s) outside the expert rows; they contributed 0";
+    const char* const kv[] = {
+        "kv_release: %u block(s) past the free list's capacity; they were dropped",
+        "kv_plan: %u token(s) without a place (past the slots, the block table's rows or the free blocks)",
+        "kv_append / kv_gather: %u slot(s) past the cache; they were skipped, or read as 0",
+        "kv_attention: %u time(s) a sequence's lengths passed max_q or the query rows (not computed), or a block "
+        "the cache or the block table (masked)"};
+    for (int i = 3; i < kStatusWords; ++i) {
+      if (!bad[i]) continue;
+      char text[200];
+      std::snprintf(text, sizeof(text), kv[i - 3], bad[i]);
+      msg += std::string(msg.empty() ? "" : "; ") + text;
+    }
     return fail(CPQ_ERR_INVALID_ARGUMENT, msg);
   }
   return CPQ_OK;

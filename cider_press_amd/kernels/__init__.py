@@ -8,6 +8,7 @@ crate, crates/cider-press-kernels/src/lib.rs:35-40), backed by libcpq.so.
     Commands.commit / wait         -> commands.rs:349-419
     KernelLibrary.quantized(dev)   -> library.rs:230 (kernels are compiled ahead of time)
     kernels.{qmv,qmm,dequantize,gather,embed}.*  -> kernels/{qmv,qmm,dequantize}.rs, nn.rs
+    kernels.{moe,kv}.*             -> no counterpart (routed experts; 4-bit key/value cache)
 
 Buffers are typed views over device memory; 16-bit float buffers hold raw
 uint16 bit patterns on the host side (numpy has no bfloat16).
@@ -136,6 +137,15 @@ class Buffer:
         """Same allocation viewed with another element type (buffer.rs reinterpret_as)."""
         n = self.byte_len // _SIZE[dtype]
         view = Buffer(self.device, self.ptr, n, dtype, self.alloc_len)
+        view._owner = self
+        return view
+
+    def slice(self, start: int, length: int) -> "Buffer":
+        """Elements [start, start + length) of the same allocation."""
+        if not (0 <= start and 0 <= length and start + length <= self._len):
+            raise ValueError(f"slice: [{start}, {start + length}) of a buffer of {self._len}")
+        at = start * _SIZE[self.dtype]
+        view = Buffer(self.device, self.ptr + at, length, self.dtype, self.alloc_len - at)
         view._owner = self
         return view
 
@@ -315,4 +325,4 @@ def _ptr(buf):
     return None if buf is None else buf.ptr
 
 
-from . import dequantize, embed, gather, moe, qmm, qmv  # noqa: E402,F401
+from . import dequantize, embed, gather, kv, moe, qmm, qmv  # noqa: E402,F401

@@ -411,6 +411,145 @@ cpq_status cpq_moe_combine(cpq_commands* cmds, cpq_dtype dtype, const void* y, s
                            size_t out_len);
 
 /* ------------------------------------------------------------------ */
+/* Key/value cache in 4 bits                                             */
+/* ------------------------------------------------------------------ */
+
+/* No reference counterpart: its KV cache (runtime/src/kv_cache.rs) holds
+ * dense T.  Keys and values are held in the affine format of the weights,
+ * x = scale * q + bias with q in 0..15 per group of group_size values along
+ * the head dimension, in blocks of block_size tokens.  A block table gives
+ * each sequence its blocks; slot = block * block_size + offset names one
+ * token's place in every head.  A slot of 0xffffffff (CPQ_KV_NO_SLOT) is
+ * none: a padding token.
+ *
+ * The descriptor is a plain struct of one layer's cache; the caller owns the
+ * four device buffers (16-byte aligned u32 words, W = head_dim / 8 words and
+ * G = head_dim / group_size constants per token and head, j the dimension
+ * 8 w + j of word w in bits [4 j, 4 j + 4)):
+ *   k_q  [n_blocks][n_kv_heads][block_size][W]
+ *   k_sb [n_blocks][n_kv_heads][block_size][G]        scale | bias << 16, of T
+ *   v_q  [n_blocks][n_kv_heads][block_size / 4][W][4] four tokens interleaved
+ *   v_sb [n_blocks][n_kv_heads][block_size / 4][G][4]
+ * (a value's matrix operand takes one dimension of four tokens, a key's four
+ * words of one token: either is one 16-byte load).  head_dim 64, 128 or 256;
+ * group_size 32, 64 or 128, dividing it; block_size a power of two, 16 ..
+ * 1024; n_blocks * block_size < 2^32 - 1. */
+#define CPQ_KV_NO_SLOT 0xffffffffu
+typedef struct cpq_kv_cache {
+  cpq_dtype dtype; /* T: BF16 or F16 */
+  uint32_t head_dim;
+  uint32_t n_kv_heads;
+  uint32_t group_size;
+  uint32_t block_size;
+  size_t n_blocks;
+  uint32_t* k_q;
+  size_t k_q_len; /* in words, as the layouts above */
+  uint32_t* k_sb;
+  size_t k_sb_len;
+  uint32_t* v_q;
+  size_t v_q_len;
+  uint32_t* v_sb;
+  size_t v_sb_len;
+} cpq_kv_cache;
+
+/* Words of k_q (= v_q) and of k_sb (= v_sb) for this geometry; the pointers
+ * and lengths of the descriptor are not read. */
+cpq_status cpq_kv_cache_words(const cpq_kv_cache* cache, size_t* q_words, size_t* sb_words);
+
+/* Blocks of finished sequences back to the free list.  free_list[0 ..
+ * *free_count) are the free blocks; for each sequence s with finished[s] != 0,
+ * in order, its blocks block_table[s][0 .. ceil(lens[s] / block_size)) are
+ * put on top of them, and lens_out[s] = 0; other sequences keep lens[s].
+ * *free_count_out is the new count.  Blocks past free_cap entries are dropped
+ * and reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.  block_table is
+ * [n_seqs][max_blocks]; n_seqs <= 8192.  Outputs must not overlap inputs. */
+cpq_status cpq_kv_release(cpq_commands* cmds, const uint32_t* finished, const uint32_t* lens,
+                          const uint32_t* block_table, size_t n_seqs, size_t max_blocks, uint32_t block_size,
+                          uint32_t* free_list, size_t free_cap, const uint32_t* free_count, uint32_t* lens_out,
+                          uint32_t* free_count_out);
+/* One step's places, from the sequences' lengths (lens[s] tokens cached,
+ * new_lens[s] to come), without the host knowing them:
+ *   query_starts[s]  first of sequence s's new tokens ([n_seqs + 1], ascending)
+ *   kv_lens[s]       lens[s] + new_lens[s]
+ *   slots[t], positions[t] (t < cap) of the new tokens, sequence by sequence;
+ *                    past the last one CPQ_KV_NO_SLOT and 0
+ *   block_table      the blocks that new tokens open are taken off the top of
+ *                    the free list, in token order, and entered
+ *   *free_count_out  free blocks left
+ * What does not fit is not placed: new tokens past cap are cut off (query_starts
+ * stays within cap), a token past max_blocks blocks or without a free block has
+ * no slot, and kv_lens counts the tokens that have their place.  Either is
+ * reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.  n_seqs <= 8192,
+ * cap < 2^31.  Outputs must not overlap inputs, but for block_table. */
+cpq_status cpq_kv_plan(cpq_commands* cmds, const uint32_t* lens, const uint32_t* new_lens, uint32_t* block_table,
+                       size_t n_seqs, size_t max_blocks, uint32_t block_size, const uint32_t* free_list,
+                       size_t free_cap, const uint32_t* free_count, uint32_t* query_starts, uint32_t* kv_lens,
+                       uint32_t* slots, uint32_t* positions, size_t cap, uint32_t* free_count_out);
+
+/* Quantizes n_tokens keys and values (T, [n_tokens, n_kv_heads, head_dim] at
+ * the given token and head strides in elements, both multiples of 8; 16-byte
+ * aligned) into their slots.  Per group: bias = its lowest value, scale =
+ * RNE_T((highest - lowest) / 15), q = clamp(rint((x - bias) / scale), 0, 15)
+ * in fp32, 0 where the scale is 0.  A group that holds an Inf or NaN, or whose
+ * range overflows, is stored as q = 0, scale = 0, bias = NaN.  Slots that are
+ * none are skipped; slots past the cache are skipped and reported by the next
+ * wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one slot: either wins, word
+ * by word. */
+cpq_status cpq_kv_append(cpq_commands* cmds, const cpq_kv_cache* cache, const void* k, size_t k_token_stride,
+                         size_t k_head_stride, const void* v, size_t v_token_stride, size_t v_head_stride,
+                         const uint32_t* slots, size_t n_tokens);
+/* Cached keys and values as dense T: RNE_T(fmaf(scale, q, bias)) into
+ * k_out, v_out [n_rows, n_kv_heads, head_dim].  Rows of a slot that is none
+ * are zero; so are rows of slots past the cache, which are reported as by
+ * cpq_kv_append.  Either output may be NULL. */
+cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const uint32_t* slots, size_t n_rows,
+                         void* k_out, void* v_out);
+
+/* Attention of a step's queries over the cache.  Query row i of sequence s
+ * (rows query_starts[s] .. query_starts[s+1], i counted within) stands at
+ * position p = kv_lens[s] - n_queries + i; query head h reads key/value head
+ * h / (n_heads / n_kv_heads).  Over the keys j < kv_lens[s] with, if causal,
+ * j <= p and, if window > 0, j > p - window:
+ *   out = sum_j softmax_j(scale * <q, k_j>) v_j,  k, v = fmaf(scale, q, bias)
+ * in fp32, rounded to T once; a row without keys is zero.  Masked keys and
+ * values are not seen at all, whatever they hold.
+ * q, out: T, [n_tokens, n_heads, head_dim] at token and head strides in
+ * elements (multiples of 8), 16-byte aligned.  block_table [n_seqs][max_blocks]
+ * as cpq_kv_plan keeps it.  max_q, max_kv: the largest number of queries and
+ * of keys of any sequence, as far as the host knows; max_kv only steers how
+ * the work is split, a sequence with more than max_q queries is not computed.
+ * Rows past query_starts[n_seqs] are not written.  Such sequences, sequences
+ * whose rows pass n_tokens, and blocks past n_blocks or max_blocks (their keys
+ * count as masked) are reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.
+ * Session scratch holds the partial results where keys are split. */
+typedef struct cpq_kv_attention_args {
+  const void* q;
+  size_t q_token_stride;
+  size_t q_head_stride;
+  void* out;
+  size_t out_token_stride;
+  size_t out_head_stride;
+  size_t n_tokens;
+  size_t n_heads;
+  const uint32_t* block_table;
+  size_t max_blocks;
+  const uint32_t* query_starts;
+  const uint32_t* kv_lens;
+  size_t n_seqs;
+  size_t max_q;
+  size_t max_kv;
+  float scale;
+  int causal;
+  size_t window; /* 0: none */
+} cpq_kv_attention_args;
+cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_attention_args* args);
+
+/* Host-only argument validators of the above (callable without a GPU; of the
+ * pointers only NULL and alignment are looked at). */
+cpq_status cpq_check_kv_cache(const cpq_kv_cache* cache);
+cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* args);
+
+/* ------------------------------------------------------------------ */
 /* Runtime node (runtime/src/{quantized,tensor,eval}.rs)                 */
 /* ------------------------------------------------------------------ */
 
