@@ -36,7 +36,7 @@ SOURCES = [
     "kernels/gather_decode.hip", "kernels/qmm_rows.hip",
     "kernels/moe.hip",
     "kernels/stream_read.hip",
-    "kv.cpp", "kernels/kv_cache.hip", "kernels/kv_attention.hip",
+    "kv.cpp", "kernels/kv_cache.hip", "kernels/kv_attention.hip", "kernels/kv_decode.hip",
 ]
 
 ARCH = "gfx950"

@@ -222,6 +222,14 @@ struct ExecCtx {
   size_t scratch_bytes;
 };
 ExecCtx session_ctx(const cpq_commands* cmds);
+// Attention over the key/value cache (kernels/kv_attention.hip) and its kernel
+// for few query rows per sequence (kernels/kv_decode.hip): at most kKvDecodeRows
+// of one key/value head.
+constexpr size_t kKvDecodeRows = 32;
+hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                               unsigned int* bad);
+hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                            unsigned int* bad);
 // Y = X . W^T with the kernel chosen by M (small-M kernels, else the prefill
 // plan), as affine_qmm_t and the runtime node run it.
 hipError_t launch_matmul(const ExecCtx& ex, const QuantArgs& q, const void* x, void* y, int m, int n, int k);
@@ -313,10 +321,6 @@ hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k,
                             unsigned int* bad);
 hipError_t launch_kv_gather(hipStream_t s, const cpq_kv_cache& c, const uint32_t* slots, uint32_t n_rows, void* k_out,
                             void* v_out, unsigned int* bad);
-// Attention over it (kernels/kv_attention.hip).
-hipError_t launch_kv_attention(hipStream_t s, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                               unsigned int* bad);
-
 // Whether the small-M kernel's per-slab constants fit in LDS at this K and
 // group size (16 columns x (K/gs + 1) x 16 bytes next to its static LDS).
 bool skinny_fits(int k, int gs);

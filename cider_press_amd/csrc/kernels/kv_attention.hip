@@ -93,11 +93,12 @@ __global__ __launch_bounds__(64) void kv_attention_rows_kernel(cpq_kv_cache c, c
 
 }  // namespace
 
-hipError_t launch_kv_attention(hipStream_t s, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                unsigned int* bad) {
+  if (a.max_q * (a.n_heads / c.n_kv_heads) <= kKvDecodeRows) return launch_kv_decode(ex, c, a, bad);
   const dim3 grid((uint32_t)a.n_tokens, (uint32_t)a.n_heads);
   auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64), 0, s, c, a, bad);
+    hipLaunchKernelGGL(kernel, grid, dim3(64), 0, ex.stream, c, a, bad);
     return hipGetLastError();
   };
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;

@@ -1,0 +1,157 @@
+// What the attention kernels over the 4-bit key/value cache share.
+//
+// Operands are f16 for both types of T.  A nibble left in bits 0..3 (4..7) of
+// a 16-bit half reads as the f16 subnormal q * 2^-24 (q * 2^-20), so one AND
+// extracts two of them and one v_pk_fma_f16 makes two values
+//   (s * 2^(24 - E)) * (q * 2^-24) + b * 2^-E = (s q + b) * 2^-E
+// with a single rounding.  E, uniform over the wave, keeps the largest
+// constant of the keys (of the values) met so far, max(|b|, 16 |s|), within
+// 2^(E - 5): then s * 2^(24 - E) <= 2^15 fits f16 and a value is off by at most
+// 2^-12 of itself or 2^-19 of that largest, whatever T's range.  E rises when a
+// tile brings a larger constant; a factor 2 is left free so that it seldom does.
+#pragma once
+
+#include <cfloat>
+
+#include "../cpq_internal.hpp"
+#include "common.hpp"
+
+namespace cpq {
+namespace dev {
+
+constexpr int kKvTop = 5;  // constants stay below 2^(E - kKvTop)
+constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ __forceinline__ f16x2 as_f16x2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
+__device__ __forceinline__ uint32_t pk_fma(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_f16x2(a), as_f16x2(b), as_f16x2(c)));
+}
+__device__ __forceinline__ uint32_t sixteenth(uint32_t a) {
+  return __builtin_bit_cast(uint32_t, as_f16x2(a) * f16x2{(_Float16)0.0625f, (_Float16)0.0625f});
+}
+// x * 2^e, also where 2^e is no float.
+__device__ __forceinline__ float scaled(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+// The exponent e with |x| < 2^e, from x's bits (x finite).
+__device__ __forceinline__ int exponent_above(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 126; }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
+
+// The largest |scale| and |bias| of constants as T patterns in one word (both
+// types order like integers; Inf and NaN come last).
+__device__ __forceinline__ uint32_t sizes(uint32_t m, uint32_t sb) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                __builtin_bit_cast(u16x2, sb & 0x7fff7fffu)));
+}
+// What `sizes` may reach at exponent E: scales 2^(E - 9), biases 2^(E - 5), finite.
+template <typename TT>
+__device__ __forceinline__ uint32_t size_limits(int e) {
+  const uint32_t top = Sig16<TT>::bf16 ? 0x7f7fu : 0x7bffu;
+  const uint32_t s = TT::from_f32(scaled(1.f, e - kKvTop - 4)), b = TT::from_f32(scaled(1.f, e - kKvTop));
+  return min(s, top) | min(b, top) << 16;
+}
+// max(|b|, 16 |s|) of a constant, 0 where it is not finite.
+template <typename TT>
+__device__ __forceinline__ float finite_size(uint32_t sb) {
+  const float s = fabsf(TT::lo(sb)), b = fabsf(TT::hi(sb));
+  return s <= FLT_MAX && b <= FLT_MAX ? fminf(fmaxf(b, 16.f * s), FLT_MAX) : 0.f;
+}
+// The exponent for constants up to m.
+__device__ __forceinline__ int size_exponent(float m) { return max(exponent_above(m), -110) + kKvTop + 1; }
+
+// Over the lanes that differ in bits 4 and 5 (16 columns are left).
+template <typename F>
+__device__ __forceinline__ float over_rows(float v, F f) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float w = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const uint32_t x = __float_as_uint(w);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// One sequence of a call as a workgroup sees it.
+struct KvSeq {
+  int rows0;  // first query row in q and out
+  int n_q;
+  int n;    // keys, bounded by what the table's row holds
+  int pos;  // position of its first query (n_q queries stand at the end; may be negative)
+  int lo;   // first key that any query sees
+};
+
+// Sequence s, or n_q = 0 where its rows are not within the call's.  `report`:
+// this thread counts what is wrong with it.
+__device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, int bs_shift, bool report,
+                                        unsigned int* bad) {
+  const uint32_t s0 = a.query_starts[s], s1 = a.query_starts[s + 1], len = a.kv_lens[s];
+  KvSeq q{};
+  if (s1 <= s0) {
+    if (s1 < s0 && report) atomicAdd(bad, 1u);
+    return q;
+  }
+  if (s1 > a.n_tokens || s1 - s0 > a.max_q) {
+    if (report) atomicAdd(bad, 1u);
+    return q;
+  }
+  const uint64_t room = (uint64_t)a.max_blocks << bs_shift, most = room < 0x7fff0000ull ? room : 0x7fff0000ull;
+  if (len > most && report) atomicAdd(bad, 1u);
+  q.rows0 = (int)s0;
+  q.n_q = (int)(s1 - s0);
+  q.n = (int)(len < most ? len : most);
+  q.pos = q.n - q.n_q;
+  q.lo = a.window && (uint64_t)(q.pos + 1 > 0 ? q.pos + 1 : 0) > a.window ? q.pos + 1 - (int)a.window : 0;
+  return q;
+}
+
+// Where 16 keys from t (a multiple of 16) of a sequence lie: the row of the
+// first in the cache's [block][head][offset] order.  Past the end the last
+// keys' place (their loads are in bounds, their results masked).
+struct KvPlace {
+  size_t row;
+  bool ok;  // the block is one of the cache's
+};
+__device__ __forceinline__ KvPlace kv_place(const cpq_kv_cache& c, const uint32_t* __restrict__ blocks, int t, int n,
+                                            int head, int bs_shift) {
+  const int at = min(t, (n - 1) & ~15);
+  const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane((int)blocks[at >> bs_shift]);
+  const bool ok = b < c.n_blocks;
+  return KvPlace{(((size_t)(ok ? b : 0) * c.n_kv_heads + head) << bs_shift) + (at & ((1 << bs_shift) - 1)), ok};
+}
+
+// Rows of q as f16 operands: 8 values of T times 2^-e, in the order of a key
+// word's nibbles once extracted: (0, 4) (1, 5) (2, 6) (3, 7).
+template <typename TT>
+__device__ __forceinline__ u32x4 query_slice(u32x4 raw, int e) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = scaled(TT::lo(raw[i]), -e);
+    x[2 * i + 1] = scaled(TT::hi(raw[i]), -e);
+  }
+  return u32x4{F16::pack2(x[0], x[4]), F16::pack2(x[1], x[5]), F16::pack2(x[2], x[6]), F16::pack2(x[3], x[7])};
+}
+template <typename TT>
+__device__ __forceinline__ float largest(u32x4 raw, float m) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(TT::lo(raw[i])), fabsf(TT::hi(raw[i]))));
+  return m;
+}
+// The exponent that brings a row's largest value into [2^14, 2^15): every
+// value of T down to 2^-28 of it stays exact in f16.
+__device__ __forceinline__ int query_exponent(float m) { return m > 0.f ? max(exponent_above(m), -100) - 15 : 0; }
+
+// A word of keys as an operand of 8 dimensions.
+__device__ __forceinline__ u32x4 key_slice(uint32_t w, uint32_t s, uint32_t s16, uint32_t b) {
+  const uint32_t w8 = w >> 8;
+  return u32x4{pk_fma(w & 0x000f000fu, s, b), pk_fma(w & 0x00f000f0u, s16, b), pk_fma(w8 & 0x000f000fu, s, b),
+               pk_fma(w8 & 0x00f000f0u, s16, b)};
+}
+
+}  // namespace dev
+}  // namespace cpq

@@ -228,6 +228,8 @@ cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_a
     return invalid(op, "n_tokens * n_heads must stay below 2^31");
   if (!mul(a->n_seqs, a->max_blocks, &entries) || entries >= (1ull << 31) || a->max_blocks >= (1ull << 31))
     return invalid(op, "n_seqs * max_blocks must stay below 2^31");
+  if (cache->n_blocks == 0 && a->n_tokens != 0) return invalid(op, "the cache has no blocks");
+  if (a->n_seqs * cache->n_kv_heads * 4096 >= (1ull << 31)) return invalid(op, "n_seqs * n_kv_heads past 2^19");
   if (!(a->scale > 0.f) || a->scale > 3.4e38f) return invalid(op, "scale must be positive and finite");
   if (a->n_tokens == 0 || a->n_seqs == 0) return CPQ_OK;
   st = check_strided(op, "q", a->q, a->n_tokens, a->n_heads, cache->head_dim, a->q_token_stride, a->q_head_stride);
@@ -251,7 +253,8 @@ cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const
   cpq_status st = cpq_check_kv_attention_args(cache, args);
   if (st != CPQ_OK) return st;
   if (args->n_tokens == 0 || args->n_seqs == 0) return CPQ_OK;
-  return launched(cpq::launch_kv_attention(cmds->stream, *cache, *args, cmds->status + 6), "kv_attention launch");
+  return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 6),
+                  "kv_attention launch");
 }
 
 }  // extern "C"
