@@ -223,13 +223,14 @@ struct ExecCtx {
 };
 ExecCtx session_ctx(const cpq_commands* cmds);
 // Attention over the key/value cache (kernels/kv_attention.hip) and its kernel
-// for few query rows per sequence (kernels/kv_decode.hip): at most kKvDecodeRows
-// of one key/value head.
+// for few query rows per sequence (kernels/kv_decode.hip): sequences of up to
+// rows_max <= kKvDecodeRows rows of one key/value head; `report` counts sequences
+// whose lengths are wrong.
 constexpr size_t kKvDecodeRows = 32;
 hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                unsigned int* bad);
-hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                            unsigned int* bad);
+hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a, int rows_max,
+                            bool report, unsigned int* bad);
 // Y = X . W^T with the kernel chosen by M (small-M kernels, else the prefill
 // plan), as affine_qmm_t and the runtime node run it.
 hipError_t launch_matmul(const ExecCtx& ex, const QuantArgs& q, const void* x, void* y, int m, int n, int k);

@@ -1,111 +1,621 @@
 // Attention of a step's queries over the 4-bit key/value cache (semantics:
-// cpq_kv_attention in cpq.h).
+// cpq_kv_attention in cpq.h): the kernel for many query rows per sequence, and
+// the choice between it and kv_decode.hip.
 //
-// One wave per (query row, head) walks its sequence's keys 64 at a time: lane
-// j scores key j in fp32, the running maximum and sum of the softmax are kept
-// in registers, then lane d adds the weighted values of its dimensions.
-#include "../cpq_internal.hpp"
-#include "common.hpp"
+// A workgroup of four waves takes 128 query rows of one key/value head (rows
+// run over the queries, then the heads of the group, so a group of any size
+// shares the keys) and walks tiles of 64 keys, 32 rows a wave:
+//   S^T = K Q^T     v_mfma_f32_32x32x16_f16, A = 32 keys, B = 32 query rows
+//   O^T += V^T P^T  A = 32 dimensions over 16 keys, B = the weights, which
+//                   S^T's result layout holds as B takes them: lane (row n, h)
+//                   has keys 8 x + 4 h + 0 .. 3, so a k step's 16 keys are
+//                   {4 h .. 4 h + 3, 8 + 4 h ..} of either operand.
+// Keys and values become f16 operands once per workgroup (kv_common.hpp): two
+// waves dequantize the next tile's keys and two its values into the other half
+// of LDS while all four compute on this one; one barrier a tile.  The packed
+// words of the tile after that are in flight meanwhile.
+//   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
+//   keys of a k step, XORed so that the 16 lanes of a b128 read that are served
+//   together (p, p + 4, ...) meet in 16 different units.
+// The running maximum moves only when a tile exceeds it by 2^8.
+//
+// Few tiles over long keys are split over workgroups and joined, in part order,
+// by the last to arrive.
+#include <algorithm>
+
+#include "kv_common.hpp"
 
 namespace cpq {
 namespace {
 
 using namespace dev;
 
-template <typename TT, int D>
-__global__ __launch_bounds__(64) void kv_attention_rows_kernel(cpq_kv_cache c, cpq_kv_attention_args a,
-                                                               unsigned int* bad) {
-  constexpr int W = D / 8, DL = D / 64;
-  __shared__ float qs[D];
-  __shared__ float ps[64];
-  __shared__ uint32_t blocks[64];
-  const int lane = threadIdx.x;
-  const uint32_t row = blockIdx.x, head = blockIdx.y, group = a.n_heads / c.n_kv_heads, kvh = head / group;
-  uint32_t lo = 0, hi = a.n_seqs;  // starts[lo] <= row < starts[hi], if any
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (a.query_starts[mid] <= row) lo = mid;
-    else hi = mid;
+constexpr int kKeys = 64;        // of a tile
+constexpr int kRows = 128;       // of a workgroup
+constexpr float kSlack = 8.f;    // log2 of how far a weight may pass 1
+constexpr int kPoison = 1 << 20;  // in a published exponent: a value constant is not finite
+
+struct TileArgs {
+  cpq_kv_cache c;
+  cpq_kv_attention_args a;
+  int few_rows;    // sequences of up to this many rows are another kernel's
+  int parts;       // most key parts of a tile
+  int part_tiles;  // least tiles of one part
+  unsigned int* counters;
+  float* partial;  // [workgroup tile][part][wave][D / 8 + 1][lane] f32x4: rows, then (maximum, sum)
+  unsigned int* bad;
+};
+
+__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Unit of a key's word: rows of W units; at 8 units a row, neighbouring rows
+// in storage are keys 4 apart.
+template <int W>
+__device__ __forceinline__ int key_unit(int key, int w) {
+  if constexpr (W == 8) {
+    const int r = (key & 32) | (key >> 2 & 7) | (key & 3) << 3;
+    return r * 8 + (w ^ (r & 6));
+  } else {
+    return key * W + (w ^ (key >> 2 & 7) << 1);
   }
-  const uint32_t s0 = a.query_starts[lo], s1 = a.query_starts[lo + 1];
-  if (row < s0 || row >= s1) return;
-  if (s1 - s0 > a.max_q || s1 > a.n_tokens) {
-    if (lane == 0 && head == 0 && row == s0) atomicAdd(bad, 1u);
-    return;
-  }
-  const long n = a.kv_lens[lo], pos = n - (long)(s1 - s0) + (row - s0);
-  const long first = a.window && pos + 1 > (long)a.window ? pos + 1 - (long)a.window : 0;
-  // Keys past the table's row are masked.
-  const uint32_t bs = c.block_size, shift = 31 - __builtin_clz(bs);
-  const long room = (long)a.max_blocks << shift, end = min(a.causal ? pos + 1 : n, room);
-  if (n > room && lane == 0 && head == 0 && row == s0) atomicAdd(bad, 1u);
-  const uint16_t* q = static_cast<const uint16_t*>(a.q) + row * a.q_token_stride + head * a.q_head_stride;
-  for (int d = lane; d < D; d += 64) qs[d] = TT::to_f32(q[d]);
-  __syncthreads();
-  const uint32_t gs = c.group_size, G = D / gs;
-  float m = -INFINITY, l = 0.f, acc[DL] = {};
-  for (long base = first; base < end; base += 64) {
-    const long j = base + lane;
-    float score = -INFINITY;
-    uint32_t block = 0xffffffffu;
-    if (j < end) {
-      const long at = j >> shift;
-      block = a.block_table[(size_t)lo * a.max_blocks + at];
-      if (block >= c.n_blocks) {
-        atomicAdd(bad, 1u);
-      } else {
-        const size_t krow = ((size_t)block * c.n_kv_heads + kvh) * bs + (j & (bs - 1));
-        float dot = 0.f;
-        for (int w = 0; w < W; ++w) {
-          const uint32_t word = c.k_q[krow * W + w], sb = c.k_sb[krow * G + w * 8 / gs];
-          const float s = TT::lo(sb), b = TT::hi(sb);
+}
+// Unit of a dimension's keys of half k step ts (2 * step + h).
+__device__ __forceinline__ int value_unit(int d, int ts) {
+  const int r = (d & ~31) | (d >> 2 & 7) | (d & 3) << 3;
+  return r * 8 + (ts ^ (r & 6));
+}
+
+// The packed words of one wave's 32 keys: as keys, lane (key, half of the
+// words); as values, lane (word, half k step) -- twice at head_dim 256.
+template <int D>
+struct Packed {
+  static constexpr int NK = D / 64;            // 16-byte loads of a key's half, and its constants
+  static constexpr int VS = D == 256 ? 2 : 1;  // value words per lane
+  static constexpr int N = NK > 2 * VS ? NK : 2 * VS;
+  u32x4 q[N];
+  u32x4 sb[2 * VS];  // values: constants of q's four keys each; keys: sb[0], one per 16-byte load
+};
+
+template <int D>
+__device__ __forceinline__ void load_keys(Packed<D>& t, const cpq_kv_cache& c, const KvPlace* p, int lane,
+                                          int gw_shift) {
+  constexpr int W = D / 8, NK = Packed<D>::NK;
+  const int G = W >> gw_shift, half = lane >> 5;
+  const size_t row = (lane & 16 ? p[1].row : p[0].row) + (lane & 15);
+  const u32x4* q = reinterpret_cast<const u32x4*>(c.k_q + row * W + half * (W / 2));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dot = fmaf(fmaf(s, (float)(word >> (4 * i) & 15u), b), qs[8 * w + i], dot);
-        }
-        score = dot * a.scale;
-      }
+  for (int i = 0; i < NK; ++i) {
+    t.q[i] = q[i];
+    t.sb[0][i] = c.k_sb[row * G + ((half * (W / 2) + 4 * i) >> gw_shift)];
+  }
+}
+template <int D>
+__device__ __forceinline__ void load_values(Packed<D>& t, const cpq_kv_cache& c, const KvPlace* p, int lane,
+                                            int gw_shift) {
+  constexpr int W = D / 8, L = W < 16 ? 8 : 16;  // lanes over words
+  const int G = W >> gw_shift, ts = lane / L & 3;
+  const size_t quad = ((ts & 2 ? p[1].row : p[0].row) >> 2) + (ts & 1);
+#pragma unroll
+  for (int v = 0; v < Packed<D>::VS; ++v) {
+    const int w = 16 * v + lane % L;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // keys 4 h .., 8 + 4 h ..
+      t.q[2 * v + e] = *reinterpret_cast<const u32x4*>(c.v_q + ((quad + 2 * e) * W + w) * 4);
+      t.sb[2 * v + e] = *reinterpret_cast<const u32x4*>(c.v_sb + ((quad + 2 * e) * G + (w >> gw_shift)) * 4);
     }
-    float top = score;
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new;
-    const float keep = expf(m - ref), p = block < c.n_blocks ? expf(score - ref) : 0.f;
-    l = l * keep + wave_sum(p);
-    m = m_new;
-    ps[lane] = p;
-    blocks[lane] = block;
+  }
+}
+
+// A wave's running exponent for the constants it has met, and the limits that
+// go with it.
+struct Range {
+  int e = 0;
+  uint32_t limits = 0;
+};
+template <typename TT>
+__device__ __forceinline__ void raise(Range& r, float largest_size) {
+  const int e = size_exponent(wave_max(largest_size));
+  if (r.limits == 0 || e > r.e) {
+    r.e = e;
+    r.limits = size_limits<TT>(e);
+  }
+}
+
+// 32 keys (key0 .. in the tile) as operands.
+template <typename TT, int D>
+__device__ __forceinline__ void store_keys(const Packed<D>& t, u32x4* lds, int key0, int lane, Range& range,
+                                           bool live) {
+  constexpr int W = D / 8, NK = Packed<D>::NK;
+  uint32_t sb[NK], m = range.limits;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    sb[i] = live ? t.sb[0][i] : 0u;
+    m = sizes(m, sb[i]);
+  }
+  if (__any(m != range.limits)) {
+    float f = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) f = fmaxf(f, finite_size<TT>(sb[i]));
+    raise<TT>(range, f);
+  }
+  const int key = key0 + (lane & 31), half = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const float s = scaled(TT::lo(sb[i]), 24 - range.e), b = scaled(TT::hi(sb[i]), -range.e);
+    const uint32_t s0 = F16::pack2(s, s), b0 = F16::pack2(b, b), s1 = sixteenth(s0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      lds[key_unit<W>(key, half * (W / 2) + 4 * i + e)] = key_slice(t.q[i][e], s0, s1, b0);
+  }
+}
+
+// 32 keys' values (half k steps ts0 ..) as operands; returns whether a
+// constant was not finite (those count as zeros).
+template <typename TT, int D>
+__device__ __forceinline__ bool store_values(Packed<D>& t, u32x4* lds, int ts0, int lane, Range& range,
+                                             uint32_t live) {
+  constexpr int W = D / 8, L = W < 16 ? 8 : 16, VS = Packed<D>::VS;
+  uint32_t m = range.limits;
+  if (live != 0xffu) {
+#pragma unroll
+    for (int i = 0; i < 2 * VS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t.sb[i][e] = live >> (4 * (i & 1) + e) & 1 ? t.sb[i][e] : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < 2 * VS; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = sizes(m, t.sb[i][e]);
+  bool poison = false;
+  if (__any(m != range.limits)) {
+    float f = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 * VS; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f = fmaxf(f, finite_size<TT>(t.sb[i][e]));
+        const bool ok = finite(TT::lo(t.sb[i][e])) && finite(TT::hi(t.sb[i][e]));
+        poison |= !ok;
+        t.sb[i][e] = ok ? t.sb[i][e] : 0u;
+      }
+    raise<TT>(range, f);
+    poison = __any(poison);
+  }
+  const int ts = ts0 + (lane / L & 3);
+#pragma unroll
+  for (int v = 0; v < VS; ++v) {
+    uint32_t s0[4], s1[4], b0[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const uint32_t c0 = t.sb[2 * v + (x >> 1)][2 * (x & 1)], c1 = t.sb[2 * v + (x >> 1)][2 * (x & 1) + 1];
+      s0[x] = F16::pack2(scaled(TT::lo(c0), 24 - range.e), scaled(TT::lo(c1), 24 - range.e));
+      b0[x] = F16::pack2(scaled(TT::hi(c0), -range.e), scaled(TT::hi(c1), -range.e));
+      s1[x] = sixteenth(s0[x]);
+    }
+    const int w = 16 * v + lane % L;
+    // At head_dim 64 the wave's halves take half of a word's dimensions each.
+    constexpr int NY = D == 64 ? 2 : 4;
+    const int y0 = D == 64 ? 2 * (lane >> 5) : 0;
+#pragma unroll
+    for (int y = 0; y < NY; ++y) {
+      const uint32_t sel = 0x0c040c00u + (uint32_t)(y + y0) * 0x00010001u;
+      u32x4 lo, hi;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const u32x4& q4 = t.q[2 * v + (x >> 1)];
+        const uint32_t b2 = __builtin_amdgcn_perm(q4[2 * (x & 1) + 1], q4[2 * (x & 1)], sel);
+        lo[x] = pk_fma(b2 & 0x000f000fu, s0[x], b0[x]);
+        hi[x] = pk_fma(b2 & 0x00f000f0u, s1[x], b0[x]);
+      }
+      lds[value_unit(8 * w + 2 * (y + y0), ts)] = lo;
+      lds[value_unit(8 * w + 2 * (y + y0) + 1, ts)] = hi;
+    }
+  }
+  return poison;
+}
+
+// Workgroup tile -> (sequence, tile of its rows), counted over the sequences
+// that this kernel takes.  False past the last.
+__device__ __forceinline__ bool find_tile(const TileArgs& p, int want, int group, int bs_shift, uint32_t* lds, int& s,
+                                          int& qt) {
+  const int tid = threadIdx.x, lane = tid & 63, n_seqs = (int)p.a.n_seqs;
+  int before = 0;
+  for (int base = 0; base < n_seqs; base += 256) {
+    int tiles = 0;
+    if (base + tid < n_seqs) {
+      const KvSeq q = kv_seq(p.a, base + tid, bs_shift, false, nullptr);
+      const int rows = q.n_q * group;
+      tiles = rows > p.few_rows ? (rows + kRows - 1) / kRows : 0;
+    }
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(sum, d, 64);
+      if (lane >= d) sum += o;
+    }
+    if (lane == 63) lds[tid >> 6] = (uint32_t)sum;
     __syncthreads();
-    for (int i = 0; i < DL; ++i) acc[i] *= keep;
-    for (int i = 0; i < 64; ++i) {
-      if (blocks[i] >= c.n_blocks) continue;
-      const uint32_t off = (uint32_t)(base + i) & (bs - 1);
-      const size_t quad = ((size_t)blocks[i] * c.n_kv_heads + kvh) * bs + (off & ~3u);
-      for (int e = 0; e < DL; ++e) {
-        const uint32_t d = lane + 64 * e;
-        const uint32_t word = c.v_q[quad * W + d / 8 * 4 + (off & 3)], sb = c.v_sb[quad * G + d / gs * 4 + (off & 3)];
-        acc[e] = fmaf(ps[i], fmaf(TT::lo(sb), (float)(word >> (4 * (d & 7)) & 15u), TT::hi(sb)), acc[e]);
+    int at = before;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < tid >> 6) at += (int)lds[w];
+      before += (int)lds[w];
+    }
+    if (want >= at + sum - tiles && want < at + sum) {
+      lds[4] = (uint32_t)(base + tid);
+      lds[5] = (uint32_t)(want - (at + sum - tiles));
+    }
+    __syncthreads();
+    if (want < before) {
+      s = (int)lds[4];
+      qt = (int)lds[5];
+      return true;
+    }
+  }
+  return false;
+}
+
+template <typename TT, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs p) {
+  constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
+  extern __shared__ u32x4 units[];  // [2][keys, values][kUnits]
+  __shared__ int meta[2][6];         // exponents of the halves' keys and values, which 16 keys have their block
+  __shared__ uint32_t words[8];
+  const cpq_kv_cache& c = p.c;
+  const cpq_kv_attention_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(c.group_size);
+  const int group = (int)a.n_heads / (int)c.n_kv_heads;
+  const int tile = blockIdx.x / (int)c.n_kv_heads, head = blockIdx.x % (int)c.n_kv_heads, part = blockIdx.y;
+  if (blockIdx.x == 0 && part == 0)
+    for (int s = tid; s < (int)a.n_seqs; s += 256) kv_seq(a, s, bs_shift, true, p.bad);
+  int s = 0, qt = 0;
+  if (!find_tile(p, tile, group, bs_shift, words, s, qt)) return;
+  s = __builtin_amdgcn_readfirstlane(s);
+  qt = __builtin_amdgcn_readfirstlane(qt);
+  const KvSeq q = kv_seq(a, s, bs_shift, false, nullptr);
+  const int rows = q.n_q * group;
+  qt = (rows + kRows - 1) / kRows - 1 - qt;  // the rows that see most first
+  const int row0 = qt * kRows, row1 = min(row0 + kRows, rows);
+
+  // Keys that any of the rows sees, in tiles; this part's.
+  const int pos0 = q.pos + row0 / group, pos1 = q.pos + (row1 - 1) / group;
+  const int end = max(a.causal ? min(pos1 + 1, q.n) : q.n, 0);
+  const int from = a.window ? (int)max((int64_t)pos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
+  const int first = from / kKeys, tiles = max((end + kKeys - 1) / kKeys - first, 0);
+  const int per = max(p.part_tiles, (tiles + p.parts - 1) / p.parts);
+  const int parts = max((tiles + per - 1) / per, 1);
+  if (part >= parts) return;
+  const int begin = first + part * per, stop = min(first + tiles, begin + per);
+
+  // This lane's query row.
+  const int r = min(row0 + wave * 32 + col, rows - 1), qi = r / group, hh = head * group + r - qi * group;
+  const int qpos = q.pos + qi;
+  u32x4 qs[NS];
+  int qe;
+  {
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (size_t)(q.rows0 + qi) * a.q_token_stride +
+                          (size_t)hh * a.q_head_stride + h * 8;
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      qs[i] = *reinterpret_cast<const u32x4*>(src + 16 * i);
+      m = largest<TT>(qs[i], m);
+    }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+    qe = query_exponent(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+#pragma unroll
+    for (int i = 0; i < NS; ++i) qs[i] = query_slice<TT>(qs[i], qe);
+  }
+  const int see_to = a.causal ? min(qpos + 1, q.n) : q.n;  // keys [see_from, see_to) of this row
+  const int see_from = a.window ? (int)max((int64_t)qpos + 1 - (int64_t)a.window, (int64_t)0) : 0;
+  // Of the wave's rows: any sees [any_from, any_to), all see [all_from, all_to).
+  const int wr0 = min(row0 + wave * 32, rows - 1), wr1 = min(row0 + wave * 32 + 31, rows - 1);
+  const int wpos0 = q.pos + wr0 / group, wpos1 = q.pos + wr1 / group;
+  const int any_to = a.causal ? min(wpos1 + 1, q.n) : q.n, all_to = a.causal ? min(wpos0 + 1, q.n) : q.n;
+  const int any_from = a.window ? (int)max((int64_t)wpos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
+  const int all_from = a.window ? (int)max((int64_t)wpos1 + 1 - (int64_t)a.window, (int64_t)0) : 0;
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
+  float top = -INFINITY, ref = -FLT_MAX, sum = 0.f;
+  int ev = -1000;                      // o, so far zeros, is in units of 2^ev
+  int ek0 = 1 << 30, ek1 = 1 << 30;    // key exponents that cl0, cl1 are for
+  float cl0 = 0.f, cl1 = 0.f;
+
+  // Staging: waves 0, 1 keys and 2, 3 values of the tile's halves.
+  const uint32_t* blocks = a.block_table + (size_t)s * a.max_blocks;
+  const bool is_values = wave >= 2;
+  const int half = wave & 1;
+  Range range;
+  Packed<D> packed;
+  int loaded_ok = 3;
+  auto load = [&](int t) {
+    const int key = t * kKeys + half * 32;
+    KvPlace pl[2];
+    pl[0] = kv_place(c, blocks, key, q.n, head, bs_shift);
+    pl[1] = bs_shift > 4 && key + 16 < q.n ? KvPlace{pl[0].row + 16, pl[0].ok}
+                                           : kv_place(c, blocks, key + 16, q.n, head, bs_shift);
+    loaded_ok = (pl[0].ok ? 1 : 0) | (pl[1].ok ? 2 : 0);
+    if (is_values) load_values<D>(packed, c, pl, lane, gw_shift);
+    else load_keys<D>(packed, c, pl, lane, gw_shift);
+  };
+  auto store = [&](int t, int buf) {
+    u32x4* keys = units + buf * 2 * kUnits;
+    const int key = t * kKeys + half * 32;
+    const bool all = key >= from && key + 32 <= q.n && loaded_ok == 3;
+    if (!all && !is_values && lane == 0 &&
+        ((!(loaded_ok & 1) && key < q.n) || (!(loaded_ok & 2) && key + 16 < q.n)))
+      atomicAdd(p.bad, 1u);
+    bool poison = false;
+    if (is_values) {
+      uint32_t live = 0xff;
+      if (!all) {
+        const int ts = lane / (W < 16 ? 8 : 16) & 3;
+        live = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = key + 16 * (ts >> 1) + 4 * (ts & 1) + (e & 3) + 8 * (e >> 2);
+          live |= (uint32_t)(k >= from && k < q.n && (loaded_ok >> (ts >> 1) & 1)) << e;
+        }
+      }
+      poison = store_values<TT, D>(packed, keys + kUnits, 4 * half, lane, range, live);
+    } else {
+      const int k = key + (lane & 31);
+      const bool live = all || (k >= from && k < q.n && (loaded_ok >> (lane >> 4 & 1) & 1));
+      store_keys<TT, D>(packed, keys, 32 * half, lane, range, live);
+    }
+    if (lane == 0) {
+      meta[buf][wave] = poison ? range.e + kPoison : range.e;
+      if (!is_values) meta[buf][4 + half] = loaded_ok;
+    }
+  };
+
+  if (begin < stop) {
+    load(begin);
+    store(begin, 0);
+    if (begin + 1 < stop) load(begin + 1);
+  }
+  __syncthreads();
+  for (int t = begin; t < stop; ++t) {
+    const int buf = (t - begin) & 1;
+    const int mk0 = __builtin_amdgcn_readfirstlane(meta[buf][0]), mk1 = __builtin_amdgcn_readfirstlane(meta[buf][1]);
+    int mv0 = __builtin_amdgcn_readfirstlane(meta[buf][2]), mv1 = __builtin_amdgcn_readfirstlane(meta[buf][3]);
+    const int ok = __builtin_amdgcn_readfirstlane(meta[buf][4] | meta[buf][5] << 2);
+    const bool poison = mv0 >= kPoison / 2 || mv1 >= kPoison / 2;
+    if (mv0 >= kPoison / 2) mv0 -= kPoison;
+    if (mv1 >= kPoison / 2) mv1 -= kPoison;
+    if (is_values && max(mv0, mv1) > range.e) {  // the halves' values share the larger exponent from here on
+      range.e = max(mv0, mv1);
+      range.limits = size_limits<TT>(range.e);
+    }
+    if (t + 1 < stop) {
+      store(t + 1, buf ^ 1);
+      if (t + 2 < stop) load(t + 2);
+    }
+    const int key0 = t * kKeys;
+    if (key0 < any_to && key0 + kKeys > any_from) {
+      const u32x4* keys = units + buf * 2 * kUnits;
+      const u32x4* values = keys + kUnits;
+      if (mk0 != ek0 || mk1 != ek1) {
+        ek0 = mk0;
+        ek1 = mk1;
+        cl0 = fmaxf(scaled(a.scale * kLog2e, ek0 + qe), FLT_MIN);
+        cl1 = fmaxf(scaled(a.scale * kLog2e, ek1 + qe), FLT_MIN);
+      }
+      f32x16 sc[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) sc[u] = mma(keys[key_unit<W>(32 * u + col, 2 * i + h)], qs[i], sc[u]);
+      }
+      const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = key0 + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+            sc[u][e] = key >= see_from && key < see_to && (ok >> (2 * u + (e >> 3)) & 1) ? sc[u][e] : -INFINITY;
+          }
+      }
+      float m0 = sc[0][0], m1 = sc[1][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) {
+        m0 = fmaxf(m0, sc[0][e]);
+        m1 = fmaxf(m1, sc[1][e]);
+      }
+      float m = fmaxf(m0 * cl0, m1 * cl1);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+      m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+      if (__any(m > top + kSlack)) {
+        const float was = ref;
+        top = fmaxf(top, m);
+        ref = fmaxf(top, -FLT_MAX);
+        const float keep = __builtin_amdgcn_exp2f(was - ref);
+        sum *= keep;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) o[j] *= keep;
+      }
+      float add = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          sc[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e], u ? cl1 : cl0, -ref));
+          add += sc[u][e];
+        }
+      sum += add;
+      if (mv0 != ev || mv1 != ev) {  // other exponents than o's: rare after the first tile
+        const int e = max(ev, max(mv0, mv1));
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], ev - e);
+        ev = e;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sc[u][x] = scaled(sc[u][x], (u ? mv1 : mv0) - e);
+      }
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k) {
+        const f32x16& w = sc[k >> 1];
+        const int x = 8 * (k & 1);
+        const u32x4 pw{F16::pack2(w[x], w[x + 1]), F16::pack2(w[x + 2], w[x + 3]), F16::pack2(w[x + 4], w[x + 5]),
+                       F16::pack2(w[x + 6], w[x + 7])};
+#pragma unroll
+        for (int j = 0; j < ND; ++j) o[j] = mma(values[value_unit(32 * j + col, 2 * k + h)], pw, o[j]);
+      }
+      if (poison) {  // rows that see a value that is not finite: not a number in its group's dimensions
+        for (int k = 0; k < kKeys / 16; ++k) {
+          const int at = key0 + 16 * k;
+          if (at >= q.n) break;
+          const KvPlace pl = kv_place(c, blocks, at, q.n, head, bs_shift);
+          u32x4 seen;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int key = at + 8 * (x >> 1) + 4 * h + 2 * (x & 1);
+            seen[x] = (key >= see_from && key < see_to && pl.ok ? 0x3c00u : 0u) |
+                      (key + 1 >= see_from && key + 1 < see_to && pl.ok ? 0x3c000000u : 0u);
+          }
+          for (int j = 0; j < ND; ++j) {
+            const int g = (32 * j + col) / 8 >> gw_shift, G = W >> gw_shift;
+            u32x4 flags;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t* sb = c.v_sb + (((pl.row >> 2) + 2 * (x >> 1) + h) * G + g) * 4 + 2 * (x & 1);
+              flags[x] = (finite(TT::lo(sb[0])) && finite(TT::hi(sb[0])) ? 0u : 0x3c00u) |
+                         (finite(TT::lo(sb[1])) && finite(TT::hi(sb[1])) ? 0u : 0x3c000000u);
+            }
+            f32x16 n;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) n[x] = 0.f;
+            n = mma(flags, seen, n);
+#pragma unroll
+            for (int jj = 0; jj < ND; ++jj)
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[jj][x] = jj == j && n[x] > 0.f ? NAN : o[jj][x];
+          }
+        }
       }
     }
     __syncthreads();
   }
-  uint16_t* out = static_cast<uint16_t*>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
-  for (int e = 0; e < DL; ++e) out[lane + 64 * e] = TT::from_f32(l == 0.f ? 0.f : acc[e] / l);
+
+  {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+    sum = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  const bool stored = row0 + wave * 32 + col < rows;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +
+                  (size_t)hh * a.out_head_stride + 4 * h;
+  if (parts > 1) {
+    const size_t slab = (size_t)4 * (D / 8 + 1) * 64;  // f32x4 per part
+    const f32x4* all = reinterpret_cast<const f32x4*>(p.partial) + (size_t)blockIdx.x * p.parts * slab +
+                       (size_t)wave * (D / 8 + 1) * 64;
+    const f32x4* mine = all + part * slab;
+    auto put = [&](int at, f32x4 v) { park_store(mine, (at * 64 + lane) * 16, v); };
+    auto get = [&](int k, int at) { return park_load(all + k * slab, (at * 64 + lane) * 16); };
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        put(4 * j + x, f32x4{scaled(o[j][4 * x], ev), scaled(o[j][4 * x + 1], ev),
+                             scaled(o[j][4 * x + 2], ev), scaled(o[j][4 * x + 3], ev)});
+    put(D / 8, f32x4{ref, sum, 0.f, 0.f});
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) words[6] = __hip_atomic_fetch_add(&p.counters[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (words[6] != (uint32_t)(parts - 1)) return;
+    float m = -FLT_MAX;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, get(k, D / 8)[0]);
+    sum = 0.f;
+    ev = 0;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[j][x] = 0.f;
+    for (int k = 0; k < parts; ++k) {
+      const f32x4 ml = get(k, D / 8);
+      const float w = __builtin_amdgcn_exp2f(ml[0] - m);
+      sum += ml[1] * w;
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const f32x4 v = get(k, 4 * j + x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[j][4 * x + e] += v[e] * w;
+        }
+    }
+    if (tid == 0) __hip_atomic_store(&p.counters[blockIdx.x], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (!stored) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+      *reinterpret_cast<u32x2*>(out + 32 * j + 8 * x) =
+          u32x2{TT::pack2(scaled(o[j][4 * x] * inv, ev), scaled(o[j][4 * x + 1] * inv, ev)),
+                TT::pack2(scaled(o[j][4 * x + 2] * inv, ev), scaled(o[j][4 * x + 3] * inv, ev))};
+}
+
+template <typename TT, int D>
+hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
+  const size_t lds = (size_t)2 * 2 * kKeys * (D / 8) * 16;
+  auto kernel = kv_tile_kernel<TT, D>;
+  static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (raised != hipSuccess) return raised;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                unsigned int* bad) {
-  if (a.max_q * (a.n_heads / c.n_kv_heads) <= kKvDecodeRows) return launch_kv_decode(ex, c, a, bad);
-  const dim3 grid((uint32_t)a.n_tokens, (uint32_t)a.n_heads);
-  auto run = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64), 0, ex.stream, c, a, bad);
-    return hipGetLastError();
-  };
+  const size_t group = a.n_heads / c.n_kv_heads;
+  if (a.max_q * group <= kKvDecodeRows) return launch_kv_decode(ex, c, a, (int)(a.max_q * group), true, bad);
+  TileArgs p{};
+  p.c = c;
+  p.a = a;
+  p.bad = bad;
+  // Beside long rows a batch may hold single tokens over long keys, whose rows
+  // would leave most of a tile empty and their keys to one workgroup.
+  p.few_rows = a.n_seqs > 1 && group <= 16 ? 16 : 0;
+  if (p.few_rows) {
+    const hipError_t e = launch_kv_decode(ex, c, a, p.few_rows, false, bad);
+    if (e != hipSuccess) return e;
+  }
+  // No more tiles than this, whatever the sequences' shares.
+  const size_t tiles = a.n_tokens * group / kRows + a.n_seqs, wgs = tiles * c.n_kv_heads;
+  const size_t keys = (std::min<size_t>(a.max_kv, a.max_blocks * c.block_size) + kKeys - 1) / kKeys;
+  const size_t slab = wgs * 4 * (c.head_dim / 8 + 1) * 64 * 16;
+  const size_t room = ex.scratch_bytes > kWideCounterBytes ? ex.scratch_bytes - kWideCounterBytes : 0;
+  p.part_tiles = 4;
+  size_t parts = std::max<size_t>(std::min(512 / wgs, keys / p.part_tiles), 1);
+  if (wgs * sizeof(unsigned int) > kWideCounterBytes) parts = 1;
+  p.parts = (int)std::max<size_t>(std::min(parts, room / slab), 1);
+  p.counters = static_cast<unsigned int*>(ex.scratch);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
+  const dim3 grid((uint32_t)wgs, (uint32_t)p.parts);
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   switch (c.head_dim) {
-    case 64: return bf16 ? run(kv_attention_rows_kernel<BF16, 64>) : run(kv_attention_rows_kernel<F16, 64>);
-    case 128: return bf16 ? run(kv_attention_rows_kernel<BF16, 128>) : run(kv_attention_rows_kernel<F16, 128>);
-    case 256: return bf16 ? run(kv_attention_rows_kernel<BF16, 256>) : run(kv_attention_rows_kernel<F16, 256>);
+    case 64: return bf16 ? launch_tiles<BF16, 64>(ex.stream, p, grid) : launch_tiles<F16, 64>(ex.stream, p, grid);
+    case 128: return bf16 ? launch_tiles<BF16, 128>(ex.stream, p, grid) : launch_tiles<F16, 128>(ex.stream, p, grid);
+    case 256: return bf16 ? launch_tiles<BF16, 256>(ex.stream, p, grid) : launch_tiles<F16, 256>(ex.stream, p, grid);
     default: return hipErrorInvalidValue;
   }
 }

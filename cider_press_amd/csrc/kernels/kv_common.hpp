@@ -76,6 +76,20 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// 16 bytes of a partial result that a workgroup on another XCD reads or wrote in
+// this launch: through to the memory side and from it.  `base` is the same for
+// the whole wave.
+constexpr int kSc1 = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t park_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ void park_store(const void* base, int off, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), park_rsrc(base), off, 0, kSc1);
+}
+__device__ __forceinline__ f32x4 park_load(const void* base, int off) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(park_rsrc(base), off, 0, kSc1));
+}
+
 // One sequence of a call as a workgroup sees it.
 struct KvSeq {
   int rows0;  // first query row in q and out

@@ -51,6 +51,7 @@ struct DecodeArgs {
   int parts;       // most parts per sequence and head
   int part_tiles;  // least tiles of one part
   int rows_max;    // query rows the scratch and LDS are laid out for
+  int report;      // this launch counts what is wrong with the sequences
   unsigned int* counters;
   float* partial;  // [seq * head][part][rows_max][D + 2]: rows, then maximum and sum
   unsigned int* bad;
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
   const int head = pair % (int)c.n_kv_heads, s = pair / (int)c.n_kv_heads;
   const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(c.group_size);
   const int group = (int)a.n_heads / (int)c.n_kv_heads;
-  const KvSeq q = kv_seq(a, s, bs_shift, tid == 0 && head == 0 && part == 0, p.bad);
+  const KvSeq q = kv_seq(a, s, bs_shift, p.report && tid == 0 && head == 0 && part == 0, p.bad);
   const int rows = q.n_q * group;
   if (rows == 0 || rows > p.rows_max) return;  // none, not computed, or many: another kernel's
 
@@ -481,14 +482,14 @@ hipError_t launch_d(hipStream_t s, const DecodeArgs& p) {
 
 }  // namespace
 
-hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                            unsigned int* bad) {
-  const int group = (int)(a.n_heads / c.n_kv_heads);
+hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a, int rows_max,
+                            bool report, unsigned int* bad) {
   DecodeArgs p{};
   p.c = c;
   p.a = a;
   p.bad = bad;
-  p.rows_max = (int)std::min<size_t>(a.max_q * group, kKvDecodeRows);
+  p.rows_max = rows_max;
+  p.report = report;
   const size_t pairs = a.n_seqs * c.n_kv_heads;
   // A part is at least one tile per wave; more parts than about 4096
   // workgroups in all bring nothing but their joining.
