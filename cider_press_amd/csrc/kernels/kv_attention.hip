@@ -330,21 +330,24 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   float cl0 = 0.f, cl1 = 0.f;
 
   // Staging: waves 0, 1 keys and 2, 3 values of the tile's halves.
-  const uint32_t* blocks = a.block_table + (size_t)s * a.max_blocks;
+  const KvBlocks blocks = kv_blocks(a, s);
   const bool is_values = wave >= 2;
   const int half = wave & 1;
   Range range;
   Packed<D> packed;
   int loaded_ok = 3;
+  KvIds ids{};  // blocks of the half tile that is loaded next
+  auto look = [&](int t) {
+    if (t < stop) ids = kv_ids(blocks, min(t * kKeys + half * 32, (q.n - 1) & ~31), q.n, bs_shift);
+  };
   auto load = [&](int t) {
     const int key = t * kKeys + half * 32;
     KvPlace pl[2];
-    pl[0] = kv_place(c, blocks, key, q.n, head, bs_shift);
-    pl[1] = bs_shift > 4 && key + 16 < q.n ? KvPlace{pl[0].row + 16, pl[0].ok}
-                                           : kv_place(c, blocks, key + 16, q.n, head, bs_shift);
+    kv_places(c, ids, min(key, (q.n - 1) & ~31), q.n, head, bs_shift, pl);
     loaded_ok = (pl[0].ok ? 1 : 0) | (pl[1].ok ? 2 : 0);
     if (is_values) load_values<D>(packed, c, pl, lane, gw_shift);
     else load_keys<D>(packed, c, pl, lane, gw_shift);
+    look(t + 1);
   };
   auto store = [&](int t, int buf) {
     u32x4* keys = units + buf * 2 * kUnits;
@@ -377,6 +380,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
     }
   };
 
+  look(begin);
   if (begin < stop) {
     load(begin);
     store(begin, 0);
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
         for (int k = 0; k < kKeys / 16; ++k) {
           const int at = key0 + 16 * k;
           if (at >= q.n) break;
-          const KvPlace pl = kv_place(c, blocks, at, q.n, head, bs_shift);
+          const KvPlace pl = kv_place(c, blocks[at >> bs_shift], at, head, bs_shift);
           u32x4 seen;
 #pragma unroll
           for (int x = 0; x < 4; ++x) {

@@ -58,6 +58,9 @@ __device__ __forceinline__ float finite_size(uint32_t sb) {
 // The exponent for constants up to m.
 __device__ __forceinline__ int size_exponent(float m) { return max(exponent_above(m), -110) + kKvTop + 1; }
 
+// Until the wave's LDS reads and writes are done.
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
+
 // Over the lanes that differ in bits 4 and 5 (16 columns are left).
 template <typename F>
 __device__ __forceinline__ float over_rows(float v, F f) {
@@ -123,19 +126,35 @@ __device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, i
   return q;
 }
 
-// Where 16 keys from t (a multiple of 16) of a sequence lie: the row of the
-// first in the cache's [block][head][offset] order.  Past the end the last
-// keys' place (their loads are in bounds, their results masked).
+// A block table's row, read through the scalar cache: nothing writes it while
+// the kernel runs.
+typedef const __attribute__((address_space(4))) uint32_t* KvBlocks;
+__device__ __forceinline__ KvBlocks kv_blocks(const cpq_kv_attention_args& a, int s) {
+  return (KvBlocks)(a.block_table + (size_t)s * a.max_blocks);
+}
+// The blocks of 32 keys from t (a multiple of 32, below n): of the first 16 and
+// of the others, which past the end are the last keys' (their loads are in
+// bounds, their results masked).
+struct KvIds {
+  uint32_t id[2];
+};
+__device__ __forceinline__ KvIds kv_ids(KvBlocks blocks, int t, int n, int bs_shift) {
+  return KvIds{{blocks[t >> bs_shift], blocks[min(t + 16, (n - 1) & ~15) >> bs_shift]}};
+}
+// Where they lie: the row of the first in the cache's [block][head][offset]
+// order, and whether the block is one of the cache's.
 struct KvPlace {
   size_t row;
-  bool ok;  // the block is one of the cache's
+  bool ok;
 };
-__device__ __forceinline__ KvPlace kv_place(const cpq_kv_cache& c, const uint32_t* __restrict__ blocks, int t, int n,
-                                            int head, int bs_shift) {
-  const int at = min(t, (n - 1) & ~15);
-  const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane((int)blocks[at >> bs_shift]);
-  const bool ok = b < c.n_blocks;
-  return KvPlace{(((size_t)(ok ? b : 0) * c.n_kv_heads + head) << bs_shift) + (at & ((1 << bs_shift) - 1)), ok};
+__device__ __forceinline__ KvPlace kv_place(const cpq_kv_cache& c, uint32_t id, int at, int head, int bs_shift) {
+  const bool ok = id < c.n_blocks;
+  return KvPlace{(((size_t)(ok ? id : 0) * c.n_kv_heads + head) << bs_shift) + (at & ((1 << bs_shift) - 1)), ok};
+}
+__device__ __forceinline__ void kv_places(const cpq_kv_cache& c, const KvIds& ids, int t, int n, int head,
+                                          int bs_shift, KvPlace* p) {
+  p[0] = kv_place(c, ids.id[0], t, head, bs_shift);
+  p[1] = kv_place(c, ids.id[1], min(t + 16, (n - 1) & ~15), head, bs_shift);
 }
 
 // Rows of q as f16 operands: 8 values of T times 2^-e, in the order of a key

@@ -5,21 +5,25 @@
 // group, at most 16 NC) share its keys and values, which are read once.  A
 // workgroup of four waves takes one (sequence, head, part of the keys); each
 // wave walks tiles of 32 keys with a softmax of its own:
-//   S^T = K Q^T   v_mfma_f32_16x16x32_f16, A = 16 keys, B = 16 query rows:
-//                 lane (key i, quarter h) holds a quarter of the key's words,
-//                 16 adjacent bytes at head_dim 128, as the cache lays them out
+//   S^T = K Q^T     v_mfma_f32_16x16x32_f16, A = 16 keys, B = 16 query rows:
+//                   lane (key i, quarter h) takes a quarter of the key's words
 //   O^T += V^T P^T  A = 16 words' j-th dimension over 32 keys, B = the weights.
-//                 The result layout of S^T (lane: query n, keys 4h .. 4h + 3)
-//                 is B's layout of P^T as it stands, with A's keys in the same
-//                 order: lane (word i, h) takes word i of keys 4h .. 4h + 3, one
-//                 16-byte load of the interleaved value layout.
-// So nothing goes through LDS until the waves' results are joined, and a
-// dimension pair of two keys costs one v_perm, two ANDs and two v_pk_fma_f16
-// (kv_common.hpp).  The running maximum moves only when a tile exceeds it by
-// 2^8 (weights stay below 2^8 in f16, sums are fp32).
+//                   The result layout of S^T (lane: query n, keys 4h .. 4h + 3)
+//                   is B's layout of P^T as it stands, with A's keys in the same
+//                   order: lane (word i, h) takes word i of keys 4h .. 4h + 3,
+//                   16 bytes of the interleaved value layout.
+// A dimension pair of two keys costs one v_perm, two ANDs and two v_pk_fma_f16
+// (kv_common.hpp).  A tile's words and constants come into the wave's own ring
+// in LDS by asynchronous copies, a tile ahead, each lane's 16 bytes as it will
+// read them; no barrier until the waves' results are joined.  The constants of
+// 32 keys' values are turned into f16 once per wave, not once per lane that uses
+// them.  The running maximum moves only when a tile exceeds it by 2^8 (weights
+// stay below 2^8 in f16, sums are fp32).
 //
-// Where keys are split, every part parks its maximum, sum and fp32 rows in the
-// session's scratch, and the last to arrive joins them in part order.
+// The workgroups divide the tiles of all sequences evenly, by the lengths on
+// the device.  Where a sequence's keys are split, every part parks its maximum,
+// sum and fp32 rows in the session's scratch, and the last to arrive joins them
+// in part order.
 #include <algorithm>
 
 #include "kv_common.hpp"
@@ -29,271 +33,226 @@ namespace {
 
 using namespace dev;
 
+#ifndef WPS
+#define WPS 2
+#endif
+#ifndef STAGES
+#define STAGES 2
+#endif
 constexpr int kWaves = 4;
 constexpr int kTile = 32;
+constexpr int kMaxParts = 256;
 constexpr float kSlack = 8.f;  // log2 of how far a weight may pass 1
 
-template <int D>
-struct Tile {
+template <int D, int GS>
+struct Geo {
+  static constexpr int W = D / 8;               // words of a row
+  static constexpr int G = D / GS;              // constants of a row
+  static constexpr int GW = GS / 8;             // words of a group
   static constexpr int WL = D / 32;             // key words per lane
-  static constexpr int NG = D == 256 ? 2 : 1;   // key constants per lane (32 dimensions each at least)
+  static constexpr int NG = WL > GW ? WL / GW : 1;  // key constants per lane
   static constexpr int VS = D == 256 ? 2 : 1;   // sets of 16 value words
-  static constexpr int NJ = D == 64 ? 4 : 8;    // dimensions of a word per result tile set
-  uint32_t kq[2][WL];
-  uint32_t ksb[2][NG];
-  u32x4 vq[2][VS];
-  u32x4 vsb[2][VS];
+  static constexpr int NJ = D == 64 ? 4 : 8;    // result tiles per set
+  static constexpr int NQ = D / 64;             // copies of 1 KiB per tile's keys (values)
+  static constexpr int NL = G > 2 ? G / 2 : 1;  // copies of 256 bytes per tile's constants
+  static constexpr int kLoads = 2 * NQ + 2 * NL;
+  // Byte offsets in a stage: keys, values, their constants.
+  static constexpr int kV = NQ * 1024, kKc = 2 * kV, kVc = kKc + NL * 256, kStage = kVc + NL * 256;
+  // Behind the ring: the values' constants in f16, scales, biases and flags [G][32].
+  static constexpr int kConst = STAGES * kStage, kWave = kConst + 3 * 64 * G;
 };
 
 struct DecodeArgs {
   cpq_kv_cache c;
   cpq_kv_attention_args a;
-  int parts;       // most parts per sequence and head
-  int part_tiles;  // least tiles of one part
-  int rows_max;    // query rows the scratch and LDS are laid out for
+  int rows_max;    // sequences of more rows are another kernel's
+  int target;      // workgroups to divide the tiles over
+  int part_tiles;  // least tiles of a part
   int report;      // this launch counts what is wrong with the sequences
-  unsigned int* counters;
-  float* partial;  // [seq * head][part][rows_max][D + 2]: rows, then maximum and sum
+  unsigned int* counters;  // per (sequence, head)
+  float* partial;          // [workgroup][rows_max][D + 4]: rows, then maximum and sum
   unsigned int* bad;
 };
 
-template <int D>
-__device__ __forceinline__ void load_tile(Tile<D>& t, const cpq_kv_cache& c, const KvPlace* p, int lane, int gw_shift) {
-  using T = Tile<D>;
-  constexpr int W = D / 8;
-  const int G = W >> gw_shift, i = lane & 15, h = lane >> 4;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+__device__ __forceinline__ void copy16(const void* src, unsigned char* lds) {
+  __builtin_amdgcn_global_load_lds((GlobalPtr)src, (LdsPtr)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void copy4(const void* src, unsigned char* lds) {
+  __builtin_amdgcn_global_load_lds((GlobalPtr)src, (LdsPtr)lds, 4, 0, 0);
+}
+
+// Starts the copies of one tile into a stage: kLoads instructions.
+template <int D, int GS>
+__device__ __forceinline__ void start_tile(const cpq_kv_cache& c, const KvPlace* p, int lane, unsigned char* stage) {
+  using X = Geo<D, GS>;
+  const int i = lane & 15, h = lane >> 4;
+  const size_t mine = lane & 32 ? p[1].row : p[0].row;  // lanes 32 .. take the second 16 keys
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const uint32_t* kq = c.k_q + p[u].row * W + i * W + h * T::WL;
-    if constexpr (T::WL == 2) {
-      const u32x2 v = *reinterpret_cast<const u32x2*>(kq);
-      t.kq[u][0] = v.x; t.kq[u][1] = v.y;
+  for (int q = 0; q < X::NQ; ++q) {
+    const uint32_t *k, *v;
+    if constexpr (D == 64) {  // lane: half a key; a word of four keys
+      k = c.k_q + mine * 8 + (lane & 31) * 4;
+      v = c.v_q + mine * 8 + (lane & 31) * 4;
     } else {
-#pragma unroll
-      for (int q = 0; q < T::WL / 4; ++q) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(kq + 4 * q);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t.kq[u][4 * q + e] = v[e];
-      }
+      const int u = q / (D / 128), part = q % (D / 128);
+      k = c.k_q + p[u].row * X::W + i * X::W + h * X::WL + 4 * part;
+      v = c.v_q + p[u].row * X::W + (h * X::W + 16 * part + i) * 4;
     }
+    copy16(k, stage + q * 1024);
+    copy16(v, stage + X::kV + q * 1024);
+  }
 #pragma unroll
-    for (int q = 0; q < T::NG; ++q)
-      t.ksb[u][q] = c.k_sb[p[u].row * G + i * G + ((h * T::WL + 4 * q) >> gw_shift)];
-#pragma unroll
-    for (int q = 0; q < T::VS; ++q) {
-      const int w = 16 * q + (i & (W - 1));
-      t.vq[u][q] = *reinterpret_cast<const u32x4*>(c.v_q + (p[u].row >> 2) * (4 * W) + (h * W + w) * 4);
-      t.vsb[u][q] =
-          *reinterpret_cast<const u32x4*>(c.v_sb + (p[u].row >> 2) * (4 * G) + (h * G + (w >> gw_shift)) * 4);
-    }
+  for (int q = 0; q < X::NL; ++q) {
+    const int e = min(64 * q + lane, 32 * X::G - 1);  // constant of the tile, 16 G of each place
+    const bool second = e >= 16 * X::G;
+    const size_t at = (second ? p[1].row : p[0].row) * X::G + (second ? e - 16 * X::G : e);
+    copy4(c.k_sb + at, stage + X::kKc + q * 256);
+    copy4(c.v_sb + at, stage + X::kVc + q * 256);
   }
 }
 
-template <typename TT, int D, int NC>
-__global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
-  using T = Tile<D>;
-  constexpr int W = D / 8, WL = T::WL, NJ = T::NJ, VS = T::VS;
-  extern __shared__ float lds[];  // [wave][rows][D + 4], then [wave][rows] maxima and sums
-  __shared__ unsigned int flag;
-  const cpq_kv_cache& c = p.c;
-  const cpq_kv_attention_args& a = p.a;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane & 15, h = lane >> 4;
-  const int pair = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
-  const int head = pair % (int)c.n_kv_heads, s = pair / (int)c.n_kv_heads;
-  const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(c.group_size);
-  const int group = (int)a.n_heads / (int)c.n_kv_heads;
-  const KvSeq q = kv_seq(a, s, bs_shift, p.report && tid == 0 && head == 0 && part == 0, p.bad);
-  const int rows = q.n_q * group;
-  if (rows == 0 || rows > p.rows_max) return;  // none, not computed, or many: another kernel's
-
-  // Tiles of this part.
-  const int base = q.lo & ~(kTile - 1);
-  const int tiles = (max(q.n - base, 0) + kTile - 1) / kTile;
-  const int per = max(p.part_tiles, (tiles + p.parts - 1) / p.parts);
-  const int parts = max((tiles + per - 1) / per, 1);
-  if (part >= parts) return;
-  const int last = min(tiles, (part + 1) * per);
-
-  // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
-  u32x4 qs[NC][WL];
-  float cl[NC];   // log2(e) * scale * 2^(query exponent)
-  int qpos[NC];   // position of the row's query
-  int qe[NC];
-#pragma unroll
-  for (int cc = 0; cc < NC; ++cc) {
-    const int r = min(16 * cc + i, rows - 1), qi = r / group, hh = head * group + r - qi * group;
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (size_t)(q.rows0 + qi) * a.q_token_stride +
-                          (size_t)hh * a.q_head_stride + h * (WL * 8);
-    u32x4 raw[WL];
-    float m = 0.f;
-#pragma unroll
-    for (int w = 0; w < WL; ++w) {
-      raw[w] = *reinterpret_cast<const u32x4*>(src + 8 * w);
-      m = largest<TT>(raw[w], m);
-    }
-    m = over_rows(m, max_of);
-    qe[cc] = query_exponent(m);
-#pragma unroll
-    for (int w = 0; w < WL; ++w) qs[cc][w] = query_slice<TT>(raw[w], qe[cc]);
-    qpos[cc] = q.pos + qi;
-  }
-
-  f32x4 o[VS][NJ][NC];
+// A wave's running result: o in units of 2^ev, relative to 2^ref per row.
+template <typename TT, int D, int GS, int NC>
+struct Rows {
+  using X = Geo<D, GS>;
+  u32x4 qs[NC][X::WL];
+  int qe[NC];    // exponents of the query rows
+  int qpos[NC];  // positions
+  float cl[NC];  // log2(e) * scale * 2^(qe + ek)
+  f32x4 o[X::VS][X::NJ][NC];
   float top[NC], ref[NC], sum[NC];
-#pragma unroll
-  for (int cc = 0; cc < NC; ++cc) {
-    top[cc] = -INFINITY;
-    ref[cc] = -FLT_MAX;
-    sum[cc] = 0.f;
-    cl[cc] = fmaxf(scaled(a.scale * kLog2e, qe[cc]), FLT_MIN);
-#pragma unroll
-    for (int v = 0; v < VS; ++v)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) o[v][j][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
   int ek = 0, ev = 0;  // exponents of keys and values; zeros alone fit them so far
   uint32_t klim = 0, vlim = 0;
-  const uint32_t* blocks = a.block_table + (size_t)s * a.max_blocks;
 
-  auto places = [&](int ti, KvPlace* pl) {
-    const int t = base + ti * kTile;
-    pl[0] = kv_place(c, blocks, t, q.n, head, bs_shift);
-    pl[1] = bs_shift > 4 && t + 16 < q.n ? KvPlace{pl[0].row + 16, pl[0].ok} : kv_place(c, blocks, t + 16, q.n, head, bs_shift);
-  };
-  // Every row sees all keys of [t, t + 32): nothing to mask.
-  const int seen_end = a.causal ? min(q.pos + 1, q.n) : q.n;
-  const int seen_from = a.window ? (int)max((int64_t)q.pos + q.n_q - (int64_t)a.window, (int64_t)0) : 0;
-
-  Tile<D> cur, nxt;
-  KvPlace now[2] = {}, then[2] = {};
-  int ti = part * per + wave;
-  if (ti < last) {
-    places(ti, now);
-    load_tile<D>(cur, c, now, lane, gw_shift);
-    if (ti + kWaves < last) places(ti + kWaves, then);
-  }
-  for (; ti < last; ti += kWaves) {
-    const bool ok0 = now[0].ok, ok1 = now[1].ok;
-    if (ti + kWaves < last) {
-      now[0] = then[0]; now[1] = then[1];
-      load_tile<D>(nxt, c, now, lane, gw_shift);
-      if (ti + 2 * kWaves < last) places(ti + 2 * kWaves, then);
+  // Raises the exponents to a tile's constants.
+  __device__ __forceinline__ void raise(float km, float vm, float scale) {
+    km = wave_max(km);
+    vm = wave_max(vm);
+    if (klim == 0 || size_exponent(km) > ek) {
+      ek = size_exponent(km);
+      klim = size_limits<TT>(ek);
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) cl[cc] = fmaxf(scaled(scale * kLog2e, ek + qe[cc]), FLT_MIN);
     }
-    const int t = base + ti * kTile;
-    const bool whole = t >= seen_from && t + kTile <= seen_end && ok0 && ok1;
-    if (!whole) {
-      if (lane == 0 && ((!ok0 && t < q.n) || (!ok1 && t + 16 < q.n))) atomicAdd(p.bad, 1u);
-      // Values that no row sees count as zeros, whatever they hold.
+    if (vlim == 0 || size_exponent(vm) > ev) {
+      const int e = size_exponent(vm);
+#pragma unroll
+      for (int v = 0; v < X::VS; ++v)
+#pragma unroll
+        for (int j = 0; j < X::NJ; ++j)
+#pragma unroll
+          for (int cc = 0; cc < NC; ++cc)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[v][j][cc][x] = scaled(o[v][j][cc][x], ev - e);
+      ev = e;
+      vlim = size_limits<TT>(ev);
+    }
+  }
+
+  // One tile in `stage`.  on(key of the tile, position) says what a row sees,
+  // any(key) whether a row may; whole: all rows see all of it.
+  template <typename On, typename Any>
+  __device__ __forceinline__ void add(unsigned char* wave_lds, const unsigned char* stage, int lane, bool whole,
+                                      float scale, On on, Any any) {
+    const int i = lane & 15, h = lane >> 4;
+    const uint32_t* kc = reinterpret_cast<const uint32_t*>(stage + X::kKc);
+    const uint32_t* vc = reinterpret_cast<const uint32_t*>(stage + X::kVc);
+    uint16_t* cs = reinterpret_cast<uint16_t*>(wave_lds + X::kConst);  // scales, [32 G] biases, flags
+
+    // Constants: whether they fit the exponents (and are finite).
+    uint32_t ksb[2][X::NG], vsb[X::NL];
+    uint32_t ks = klim, vs = vlim;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int g = 0; g < X::NG; ++g) {
+        ksb[u][g] = kc[(16 * u + i) * X::G + h * X::WL / X::GW + g];
+        ks = sizes(ks, ksb[u][g]);
+      }
+#pragma unroll
+    for (int q = 0; q < X::NL; ++q) {
+      vsb[q] = vc[64 * q + lane];
+      vs = sizes(vs, vsb[q]);
+    }
+    const bool careful = !whole || __any(ks != klim || vs != vlim);
+    bool poison = false;
+    if (careful) {  // what no row sees counts as zeros, as do values that are not finite (NaN below)
+      float km = 0.f, vm = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = t + 16 * u + 4 * h + e;
-          const bool any = key < q.n && key >= q.lo && (u ? ok1 : ok0);
+        for (int g = 0; g < X::NG; ++g)
+          km = fmaxf(km, any(16 * u + i) ? finite_size<TT>(ksb[u][g]) : 0.f);
 #pragma unroll
-          for (int v = 0; v < VS; ++v) cur.vsb[u][v][e] = any ? cur.vsb[u][v][e] : 0u;
-        }
+      for (int q = 0; q < X::NL; ++q) {
+        const int e = 64 * q + lane, key = e / (4 * X::G) * 4 + (e & 3);
+        const bool live = any(key & 31);
+        const bool ok = finite(TT::lo(vsb[q])) && finite(TT::hi(vsb[q]));
+        poison |= live && !ok && e < 32 * X::G;
+        if (e < 32 * X::G) cs[64 * X::G + e / 4 % X::G * 32 + key] = live && !ok ? 0x3c00 : 0;
+        vsb[q] = live && ok ? vsb[q] : 0u;
+        vm = fmaxf(vm, finite_size<TT>(vsb[q]));
+      }
+      raise(km, vm, scale);
+      poison = __any(poison);
+    }
+    // The values' constants in f16, each once: [group][key].
+    wave_lds_order();
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = t + 16 * u + i;
-        const bool any = key < q.n && key >= q.lo && (u ? ok1 : ok0);
-#pragma unroll
-        for (int g = 0; g < T::NG; ++g) cur.ksb[u][g] = any ? cur.ksb[u][g] : 0u;
+    for (int q = 0; q < X::NL; ++q) {
+      const int e = 64 * q + lane, at = e / 4 % X::G * 32 + e / (4 * X::G) * 4 + (e & 3);
+      if (X::G > 1 || lane < 32) {
+        cs[at] = F16::from_f32(scaled(TT::lo(vsb[q]), 24 - ev));
+        cs[32 * X::G + at] = F16::from_f32(scaled(TT::hi(vsb[q]), -ev));
       }
     }
+    wave_lds_order();
 
-    // Exponents: larger constants than before (or none finite) are rare.
-    uint32_t ks = klim, vs = vlim;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int g = 0; g < T::NG; ++g) ks = sizes(ks, cur.ksb[u][g]);
-#pragma unroll
-      for (int v = 0; v < VS; ++v)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vs = sizes(vs, cur.vsb[u][v][e]);
-    }
-    const bool careful = __any(ks != klim || vs != vlim);
-    if (careful) {
-      float km = 0.f, vm = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int g = 0; g < T::NG; ++g) km = fmaxf(km, finite_size<TT>(cur.ksb[u][g]));
-#pragma unroll
-        for (int v = 0; v < VS; ++v)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vm = fmaxf(vm, finite_size<TT>(cur.vsb[u][v][e]));
-      }
-      km = wave_max(km);
-      vm = wave_max(vm);
-      if (klim == 0 || size_exponent(km) > ek) {
-        ek = size_exponent(km);
-        klim = size_limits<TT>(ek);
-#pragma unroll
-        for (int cc = 0; cc < NC; ++cc) cl[cc] = fmaxf(scaled(a.scale * kLog2e, ek + qe[cc]), FLT_MIN);
-      }
-      if (vlim == 0 || size_exponent(vm) > ev) {
-        const int e = size_exponent(vm);
-#pragma unroll
-        for (int v = 0; v < VS; ++v)
-#pragma unroll
-          for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int cc = 0; cc < NC; ++cc)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) o[v][j][cc][x] = scaled(o[v][j][cc][x], ev - e);
-        ev = e;
-        vlim = size_limits<TT>(ev);
-      }
-    }
-
-    // S^T.
     f32x4 sc[2][NC];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      uint32_t s0[T::NG], s1[T::NG], bb[T::NG];
+      uint32_t s0[X::NG], s1[X::NG], bb[X::NG];
 #pragma unroll
-      for (int g = 0; g < T::NG; ++g) {
-        const float sv = scaled(TT::lo(cur.ksb[u][g]), 24 - ek), bv = scaled(TT::hi(cur.ksb[u][g]), -ek);
+      for (int g = 0; g < X::NG; ++g) {
+        const float sv = scaled(TT::lo(ksb[u][g]), 24 - ek), bv = scaled(TT::hi(ksb[u][g]), -ek);
         s0[g] = F16::pack2(sv, sv);
         bb[g] = F16::pack2(bv, bv);
         s1[g] = sixteenth(s0[g]);
       }
 #pragma unroll
       for (int cc = 0; cc < NC; ++cc) sc[u][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
+      uint32_t kw[X::WL];
+      if constexpr (D == 64) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(stage + (16 * u + i) * 32 + h * 8);
+        kw[0] = v.x;
+        kw[1] = v.y;
+      } else {
 #pragma unroll
-      for (int w = 0; w < WL; ++w) {
-        const int g = T::NG == 2 ? w / 4 : 0;
-        const u32x4 k = key_slice(cur.kq[u][w], s0[g], s1[g], bb[g]);
+        for (int q = 0; q < D / 128; ++q) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(stage + (u * (D / 128) + q) * 1024 + lane * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) kw[4 * q + e] = v[e];
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < X::WL; ++w) {
+        const int g = w / X::GW;
+        const u32x4 k = key_slice(kw[w], s0[g], s1[g], bb[g]);
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc) sc[u][cc] = Mfma16<F16>::run(k, qs[cc][w], sc[u][cc]);
       }
     }
 
-    // Weights.
-    u32x4 pw[NC], seen[NC];
+    u32x4 pw[NC];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       if (!whole) {
-        const int to = a.causal ? min(qpos[cc] + 1, q.n) : q.n;
-        const int from = a.window ? (int)max((int64_t)qpos[cc] + 1 - (int64_t)a.window, (int64_t)0) : 0;
-        uint32_t bits = 0;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = t + 16 * u + 4 * h + e;
-            const bool on = key >= from && key < to && (u ? ok1 : ok0);
-            sc[u][cc][e] = on ? sc[u][cc][e] : -INFINITY;
-            bits |= (uint32_t)on << (4 * u + e);
-          }
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          seen[cc][x] = ((bits >> (2 * x) & 1) ? 0x3c00u : 0u) | ((bits >> (2 * x + 1) & 1) ? 0x3c000000u : 0u);
-      } else {
-        seen[cc] = u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+          for (int e = 0; e < 4; ++e) sc[u][cc][e] = on(16 * u + 4 * h + e, qpos[cc]) ? sc[u][cc][e] : -INFINITY;
       }
       float m = fmaxf(fmaxf(fmaxf(sc[0][cc][0], sc[0][cc][1]), fmaxf(sc[0][cc][2], sc[0][cc][3])),
                       fmaxf(fmaxf(sc[1][cc][0], sc[1][cc][1]), fmaxf(sc[1][cc][2], sc[1][cc][3])));
@@ -305,9 +264,9 @@ __global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
         const float keep = __builtin_amdgcn_exp2f(was - ref[cc]);
         sum[cc] *= keep;
 #pragma unroll
-        for (int v = 0; v < VS; ++v)
+        for (int v = 0; v < X::VS; ++v)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) o[v][j][cc] *= keep;
+          for (int j = 0; j < X::NJ; ++j) o[v][j][cc] *= keep;
       }
       float w[8];
 #pragma unroll
@@ -319,32 +278,33 @@ __global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
       for (int x = 0; x < 4; ++x) pw[cc][x] = F16::pack2(w[2 * x], w[2 * x + 1]);
     }
 
-    // O^T.
 #pragma unroll
-    for (int v = 0; v < VS; ++v) {
+    for (int v = 0; v < X::VS; ++v) {
+      const int word = D == 64 ? i & 7 : 16 * v + i;
+      const uint16_t* mine = cs + word / X::GW * 32 + 4 * h;
       uint32_t s0[4], s1[4], bb[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        uint32_t c0 = cur.vsb[x >> 1][v][2 * (x & 1)], c1 = cur.vsb[x >> 1][v][2 * (x & 1) + 1];
-        if (careful) {  // constants that are not finite: zeros here, NaN below
-          const bool f0 = finite(TT::lo(c0)) && finite(TT::hi(c0)), f1 = finite(TT::lo(c1)) && finite(TT::hi(c1));
-          cur.vsb[x >> 1][v][2 * (x & 1)] = (f0 ? 0u : 0x3c00u) | (f1 ? 0u : 0x3c000000u);  // flags, as operands
-          c0 = f0 ? c0 : 0u;
-          c1 = f1 ? c1 : 0u;
-        }
-        s0[x] = F16::pack2(scaled(TT::lo(c0), 24 - ev), scaled(TT::lo(c1), 24 - ev));
-        bb[x] = F16::pack2(scaled(TT::hi(c0), -ev), scaled(TT::hi(c1), -ev));
-        s1[x] = sixteenth(s0[x]);
+      for (int u = 0; u < 2; ++u) {
+        const u32x2 s = *reinterpret_cast<const u32x2*>(mine + 16 * u);
+        const u32x2 b = *reinterpret_cast<const u32x2*>(mine + 32 * X::G + 16 * u);
+        s0[2 * u] = s.x; s0[2 * u + 1] = s.y;
+        bb[2 * u] = b.x; bb[2 * u + 1] = b.y;
       }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s1[x] = sixteenth(s0[x]);
+      u32x4 vq[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        vq[u] = *reinterpret_cast<const u32x4*>(
+            stage + X::kV + (D == 64 ? u * 512 + h * 128 + (i & 7) * 16 : (u * (D / 128) + v) * 1024 + lane * 16));
       const uint32_t lane_sel = D == 64 ? (uint32_t)(i >> 3) * 0x00020002u : 0u;
 #pragma unroll
-      for (int y = 0; y < NJ / 2; ++y) {
+      for (int y = 0; y < X::NJ / 2; ++y) {
         const uint32_t sel = (0x0c040c00u + (uint32_t)y * 0x00010001u) + lane_sel;
         u32x4 lo, hi;
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const u32x4& q4 = cur.vq[x >> 1][v];
-          const uint32_t b2 = __builtin_amdgcn_perm(q4[2 * (x & 1) + 1], q4[2 * (x & 1)], sel);
+          const uint32_t b2 = __builtin_amdgcn_perm(vq[x >> 1][2 * (x & 1) + 1], vq[x >> 1][2 * (x & 1)], sel);
           lo[x] = pk_fma(b2 & 0x000f000fu, s0[x], bb[x]);
           hi[x] = pk_fma(b2 & 0x00f000f0u, s1[x], bb[x]);
         }
@@ -354,50 +314,233 @@ __global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
           o[v][2 * y + 1][cc] = Mfma16<F16>::run(hi, pw[cc], o[v][2 * y + 1][cc]);
         }
       }
-      if (careful) {  // rows that see such a value: not a number in its group's dimensions
-        const u32x4 flags{cur.vsb[0][v][0], cur.vsb[0][v][2], cur.vsb[1][v][0], cur.vsb[1][v][2]};
+      if (poison) {  // rows that see such a value: not a number in its group's dimensions
+        const u32x2 f0 = *reinterpret_cast<const u32x2*>(mine + 64 * X::G);
+        const u32x2 f1 = *reinterpret_cast<const u32x2*>(mine + 64 * X::G + 16);
+        const u32x4 flags{f0.x, f0.y, f1.x, f1.y};
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc) {
-          const f32x4 n = Mfma16<F16>::run(flags, seen[cc], f32x4{0.f, 0.f, 0.f, 0.f});
+          u32x4 seen;
 #pragma unroll
-          for (int j = 0; j < NJ; ++j)
+          for (int x = 0; x < 4; ++x) {
+            const int key = 16 * (x >> 1) + 4 * h + 2 * (x & 1);
+            seen[x] = (on(key, qpos[cc]) ? 0x3c00u : 0u) | (on(key + 1, qpos[cc]) ? 0x3c000000u : 0u);
+          }
+          const f32x4 n = Mfma16<F16>::run(flags, seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+          for (int j = 0; j < X::NJ; ++j)
 #pragma unroll
             for (int x = 0; x < 4; ++x) o[v][j][cc][x] = n[x] > 0.f ? NAN : o[v][j][cc][x];
         }
       }
     }
-    cur = nxt;
+  }
+};
+
+// What a workgroup does: its sequence, head and part.
+struct Item {
+  int s, head, part, parts, first;  // first: workgroup of the same head's part 0
+};
+
+__device__ __forceinline__ int tiles_of(const KvSeq& q) {
+  return (max(q.n - (q.lo & ~(kTile - 1)), 0) + kTile - 1) / kTile;
+}
+// Exclusive sum over the workgroup's threads and *all, the sum (two barriers).
+__device__ __forceinline__ int block_scan(int v, int* words, int& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int sum = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(sum, d, 64);
+    if (lane >= d) sum += o;
+  }
+  __syncthreads();
+  if (lane == 63) words[wave] = sum;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += words[w];
+    all += words[w];
+  }
+  return before + sum - v;
+}
+// The tiles of all sequences divided evenly: workgroup b's item, if any.
+__device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group, int bs_shift, int* words, Item& it) {
+  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, tid = threadIdx.x;
+  constexpr int kThreads = kWaves * 64;
+  auto work = [&](int s, bool report) {
+    if (s >= n_seqs) return 0;
+    const KvSeq q = kv_seq(p.a, s, bs_shift, report, p.bad);
+    const int rows = q.n_q * group;
+    return rows == 0 || rows > p.rows_max ? 0 : max(tiles_of(q), 1);  // no keys: zeros to store
+  };
+  int total = 0, own = 0;
+  for (int base = 0; base < n_seqs; base += kThreads) {
+    own = work(base + tid, p.report && b == 0);
+    int all;
+    block_scan(own, words, all);
+    total += all;
+  }
+  const int per = max(p.part_tiles, p.target ? (int)(((long)total * heads + p.target - 1) / p.target) : 0x3fffffff);
+  int before = 0;
+  for (int base = 0; base < n_seqs; base += kThreads) {
+    if (n_seqs > kThreads) own = work(base + tid, false);
+    const int parts = min((own + per - 1) / per, kMaxParts);
+    int all;
+    const int at = before + block_scan(parts * heads, words, all);
+    before += all;
+    if (b >= at && b < at + parts * heads) {
+      words[4] = base + tid;
+      words[5] = b - at;
+      words[6] = parts;
+    }
+    if (b < before) {
+      __syncthreads();
+      const int k = __builtin_amdgcn_readfirstlane(words[5]);
+      it.s = __builtin_amdgcn_readfirstlane(words[4]);
+      it.parts = __builtin_amdgcn_readfirstlane(words[6]);
+      it.head = k % heads;
+      it.part = k / heads;
+      it.first = b - it.part * heads;
+      return true;
+    }
+  }
+  return false;
+}
+
+template <typename TT, int D, int GS, int NC>
+__global__ __launch_bounds__(kWaves * 64, WPS) void kv_decode_kernel(DecodeArgs p) {
+  using X = Geo<D, GS>;
+  extern __shared__ __align__(16) unsigned char lds_bytes[];  // the waves' rings; then the join
+  __shared__ int words[8];
+  const cpq_kv_cache& c = p.c;
+  const cpq_kv_attention_args& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, h = lane >> 4;
+  const int bs_shift = 31 - __builtin_clz(c.block_size);
+  const int group = (int)a.n_heads / (int)c.n_kv_heads;
+  Item it{};
+  if (!find_item(p, blockIdx.x, group, bs_shift, words, it)) return;
+  const KvSeq q = kv_seq(a, it.s, bs_shift, false, nullptr);
+  const int rows = q.n_q * group, head = it.head, parts = it.parts;
+  const int base = q.lo & ~(kTile - 1), tiles = tiles_of(q);
+  const int per = (tiles + parts - 1) / parts, last = min(tiles, (it.part + 1) * per);
+
+  // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
+  Rows<TT, D, GS, NC> R;
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc) {
+    const int r = min(16 * cc + i, rows - 1), qi = r / group, hh = head * group + r - qi * group;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (size_t)(q.rows0 + qi) * a.q_token_stride +
+                          (size_t)hh * a.q_head_stride + h * (X::WL * 8);
+    float m = 0.f;
+#pragma unroll
+    for (int w = 0; w < X::WL; ++w) {
+      R.qs[cc][w] = *reinterpret_cast<const u32x4*>(src + 8 * w);
+      m = largest<TT>(R.qs[cc][w], m);
+    }
+    m = over_rows(m, max_of);
+    R.qe[cc] = query_exponent(m);
+#pragma unroll
+    for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = query_slice<TT>(R.qs[cc][w], R.qe[cc]);
+    R.qpos[cc] = q.pos + qi;
+    R.cl[cc] = fmaxf(scaled(a.scale * kLog2e, R.qe[cc]), FLT_MIN);
+    R.top[cc] = -INFINITY;
+    R.ref[cc] = -FLT_MAX;
+    R.sum[cc] = 0.f;
+#pragma unroll
+    for (int v = 0; v < X::VS; ++v)
+#pragma unroll
+      for (int j = 0; j < X::NJ; ++j) R.o[v][j][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const KvBlocks blocks = kv_blocks(a, it.s);
+  unsigned char* ring = lds_bytes + wave * X::kWave;
+  const int t0 = it.part * per + wave;
+  int ok = 0;  // two bits a stage: whether the block of either 16 keys is the cache's
+  KvIds ids{};  // blocks of the tile that is copied next
+  auto look = [&](int ti) {
+    if (ti < last) ids = kv_ids(blocks, base + ti * kTile, q.n, bs_shift);
+  };
+  auto start = [&](int ti) {
+    const int stage = (ti - t0) / kWaves % STAGES;
+    KvPlace pl[2];
+    kv_places(c, ids, base + ti * kTile, q.n, head, bs_shift, pl);
+    ok = (ok & ~(3 << 2 * stage)) | (pl[0].ok ? 1 : 0) << 2 * stage | (pl[1].ok ? 2 : 0) << 2 * stage;
+    start_tile<D, GS>(c, pl, lane, ring + stage * X::kStage);
+    look(ti + kWaves);
+  };
+  // Every row sees the keys [seen_from, seen_end): nothing to mask among them.
+  const int seen_end = a.causal ? min(q.pos + 1, q.n) : q.n;
+  const int seen_from = a.window ? (int)max((int64_t)q.pos + q.n_q - (int64_t)a.window, (int64_t)0) : 0;
+  look(t0);
+#pragma unroll
+  for (int st = 0; st < STAGES - 1; ++st)
+    if (t0 + st * kWaves < last) start(t0 + st * kWaves);
+  for (int ti = t0; ti < last; ti += kWaves) {
+    // The stage that the wave read last is free once its reads are done.
+    wave_lds_order();
+    wait_lds();
+    if (ti + (STAGES - 1) * kWaves < last) {
+      start(ti + (STAGES - 1) * kWaves);
+      wait_vmcnt<(STAGES - 1) * X::kLoads>();
+    } else if (STAGES > 2 && ti + kWaves < last) {
+      wait_vmcnt<X::kLoads>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    wave_lds_order();
+    const int stage = (ti - t0) / kWaves % STAGES;
+    const int t = base + ti * kTile, oks = ok >> 2 * stage & 3;
+    const bool whole = t >= seen_from && t + kTile <= seen_end && oks == 3;
+    if (lane == 0 && ((!(oks & 1) && t < q.n) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
+    R.add(ring, ring + stage * X::kStage, lane, whole, a.scale,
+          [&](int k, int pos) {
+            const int key = t + k;
+            return key < q.n && !(a.causal && key > pos) &&
+                   !(a.window && (int64_t)key <= (int64_t)pos - (int64_t)a.window) && (oks >> (k >> 4) & 1);
+          },
+          [&](int k) { return t + k < q.n && t + k >= q.lo && (oks >> (k >> 4) & 1); });
   }
 
   // The waves' results: each one's rows relative to its own maximum.
+  __syncthreads();
+  float* lds = reinterpret_cast<float*>(lds_bytes);  // [wave][rows][LD], then maxima and sums
   constexpr int LD = D + 4;
   float* wmax = lds + kWaves * rows * LD;  // [wave][rows]
   float* wsum = wmax + kWaves * rows;
 #pragma unroll
   for (int cc = 0; cc < NC; ++cc) {
     const int r = 16 * cc + i;
-    const float total = over_rows(sum[cc], sum_of);
+    const float total = over_rows(R.sum[cc], sum_of);
     if (r < rows) {
       float* dst = lds + (wave * rows + r) * LD;
 #pragma unroll
-      for (int v = 0; v < VS; ++v)
+      for (int v = 0; v < X::VS; ++v)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < X::NJ; ++j)
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int w = 4 * h + x;  // of 16: word, or word and half of its dimensions
             const int d = D == 64 ? 8 * (w & 7) + 4 * (w >> 3) + j : 8 * (16 * v + w) + j;
-            dst[d] = scaled(o[v][j][cc][x], ev);
+            dst[d] = scaled(R.o[v][j][cc][x], R.ev);
           }
       if (h == 0) {
-        wmax[wave * rows + r] = ref[cc];
+        wmax[wave * rows + r] = R.ref[cc];
         wsum[wave * rows + r] = total;
       }
     }
   }
   __syncthreads();
-  const size_t slab = (size_t)p.rows_max * (D + 2);
-  float* park = p.partial + ((size_t)pair * p.parts + part) * slab;
+  const size_t slab = (size_t)p.rows_max * LD;
+  auto put = [&](int r, int d, f32x4 acc, float inv) {
+    const int qi = r / group, hh = head * group + r - qi * group;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +
+                    (size_t)hh * a.out_head_stride + d;
+    *reinterpret_cast<u32x2*>(out) = u32x2{TT::pack2(acc[0] * inv, acc[1] * inv), TT::pack2(acc[2] * inv, acc[3] * inv)};
+  };
   for (int e = tid; e < rows * (D / 4); e += kWaves * 64) {
     const int r = e / (D / 4), d = e % (D / 4) * 4;
     float m = wmax[r];
@@ -412,70 +555,105 @@ __global__ __launch_bounds__(kWaves * 64) void kv_decode_kernel(DecodeArgs p) {
       acc += *reinterpret_cast<const f32x4*>(lds + (w * rows + r) * LD + d) * k;
     }
     if (parts == 1) {
-      const float inv = total == 0.f ? 0.f : 1.f / total;
-      const int qi = r / group, hh = head * group + r - qi * group;
-      uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +
-                      (size_t)hh * a.out_head_stride + d;
-      *reinterpret_cast<u32x2*>(out) = u32x2{TT::pack2(acc[0] * inv, acc[1] * inv), TT::pack2(acc[2] * inv, acc[3] * inv)};
+      put(r, d, acc, total == 0.f ? 0.f : 1.f / total);
     } else {
-      float* dst = park + r * (D + 2);
-#pragma unroll
-      for (int x = 0; x < 4; ++x) __hip_atomic_store(dst + d + x, acc[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      if (d == 0) {
-        __hip_atomic_store(dst + D, m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(dst + D + 1, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
+      const float* park = p.partial + blockIdx.x * slab;
+      park_store(park, (r * LD + d) * 4, acc);
+      if (d == 0) park_store(park, (r * LD + D) * 4, f32x4{m, total, 0.f, 0.f});
     }
   }
   if (parts == 1) return;
 
-  // The last part to arrive joins them, in part order.
+  // The last part to arrive joins them: the parts' weights first (a lane a
+  // part), then their rows, every (threads / vectors)-th part to a thread, eight
+  // loads in flight.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  if (tid == 0) flag = __hip_atomic_fetch_add(&p.counters[pair], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  unsigned int* counter = p.counters + (it.s * (int)c.n_kv_heads + head);
+  if (tid == 0) words[7] = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (flag != (unsigned int)(parts - 1)) return;
-  const float* all = p.partial + (size_t)pair * p.parts * slab;
-  for (int e = tid; e < rows * D; e += kWaves * 64) {
-    const int r = e / D, d = e % D;
-    float m = -FLT_MAX;
-    for (int k = 0; k < parts; ++k)
-      m = fmaxf(m, __hip_atomic_load(all + k * slab + r * (D + 2) + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-    float acc = 0.f, total = 0.f;
-    for (int k = 0; k < parts; ++k) {
-      const float* src = all + k * slab + r * (D + 2);
-      const float w = __builtin_amdgcn_exp2f(
-          __hip_atomic_load(src + D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) - m);
-      total += __hip_atomic_load(src + D + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * w;
-      acc += __hip_atomic_load(src + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) * w;
+  if (words[7] != parts - 1) return;
+  const float* all = p.partial + it.first * slab;
+  const int stride = (int)(slab * c.n_kv_heads);  // from part to part
+  float* weight = lds;                   // [rows][parts]
+  float* share = weight + rows * parts;  // [rows]: 1 / sum
+  f32x4* acc_lds = reinterpret_cast<f32x4*>(lds + ((rows * parts + rows + 3) & ~3));
+  for (int r = wave; r < rows; r += kWaves) {
+    float m = -FLT_MAX, total = 0.f;
+    f32x4 ml[kMaxParts / 64];
+#pragma unroll
+    for (int u = 0; u < kMaxParts / 64; ++u) {
+      if (64 * u >= parts) break;
+      ml[u] = park_load(all, (min(64 * u + lane, parts - 1) * stride + r * LD + D) * 4);
+      m = fmaxf(m, ml[u][0]);
     }
-    const int qi = r / group, hh = head * group + r - qi * group;
-    static_cast<uint16_t*>(a.out)[(size_t)(q.rows0 + qi) * a.out_token_stride + (size_t)hh * a.out_head_stride + d] =
-        TT::from_f32(total == 0.f ? 0.f : acc / total);
+    m = wave_max(m);
+#pragma unroll
+    for (int u = 0; u < kMaxParts / 64; ++u) {
+      if (64 * u >= parts) break;
+      const float w = __builtin_amdgcn_exp2f(ml[u][0] - m);
+      if (64 * u + lane < parts) {
+        weight[r * parts + 64 * u + lane] = w;
+        total += ml[u][1] * w;
+      }
+    }
+    total = wave_sum(total);
+    if (lane == 0) share[r] = total == 0.f ? 0.f : 1.f / total;
   }
-  if (tid == 0) __hip_atomic_store(&p.counters[pair], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int vectors = rows * (D / 4), each = max(kWaves * 64 / vectors, 1);
+  for (int e = tid; e < vectors * each; e += kWaves * 64) {
+    const int k0 = e / vectors, v = e - k0 * vectors, r = v / (D / 4), d = v % (D / 4) * 4;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int k = k0; k < parts; k += 8 * each) {
+      f32x4 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = park_load(all, (min(k + u * each, parts - 1) * stride + r * LD + d) * 4);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (k + u * each < parts) acc += x[u] * weight[r * parts + k + u * each];
+    }
+    if (each == 1) put(r, d, acc, share[r]);
+    else acc_lds[e] = acc;
+  }
+  if (each > 1) {
+    __syncthreads();
+    for (int v = tid; v < vectors; v += kWaves * 64) {
+      f32x4 acc = acc_lds[v];
+      for (int k = 1; k < each; ++k) acc += acc_lds[k * vectors + v];
+      put(v / (D / 4), v % (D / 4) * 4, acc, share[v / (D / 4)]);
+    }
+  }
+  if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <typename TT, int D, int NC>
-hipError_t launch(hipStream_t s, const DecodeArgs& p) {
-  const size_t lds = (size_t)kWaves * p.rows_max * (D + 4 + 2) * sizeof(float);
-  auto kernel = kv_decode_kernel<TT, D, NC>;
+template <typename TT, int D, int GS, int NC>
+hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
+  const size_t ring = (size_t)kWaves * Geo<D, GS>::kWave;
+  const size_t waves = (size_t)kWaves * p.rows_max * (D + 4 + 2) * sizeof(float);
+  const size_t join = ((size_t)p.rows_max * (kMaxParts + 1) + 4 + (size_t)kWaves * 64 * 4) * sizeof(float);
+  const size_t lds = std::max(ring, std::max(waves, p.target ? join : 0));
+  auto kernel = kv_decode_kernel<TT, D, GS, NC>;
   if (lds > 60 * 1024) {
     static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024);
+                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024);
     if (raised != hipSuccess) return raised;
   }
-  const dim3 grid((uint32_t)(p.a.n_seqs * p.c.n_kv_heads * p.parts));
-  hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), lds, s, p);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kWaves * 64), lds, s, p);
   return hipGetLastError();
 }
 
 template <typename TT, int NC>
-hipError_t launch_d(hipStream_t s, const DecodeArgs& p) {
-  switch (p.c.head_dim) {
-    case 64: return launch<TT, 64, NC>(s, p);
-    case 128: return launch<TT, 128, NC>(s, p);
-    case 256: return launch<TT, 256, NC>(s, p);
+hipError_t launch_d(hipStream_t s, const DecodeArgs& p, size_t grid) {
+  switch (p.c.head_dim * 1000 + p.c.group_size) {
+    case 64032: return launch<TT, 64, 32, NC>(s, p, grid);
+    case 64064: return launch<TT, 64, 64, NC>(s, p, grid);
+    case 128032: return launch<TT, 128, 32, NC>(s, p, grid);
+    case 128064: return launch<TT, 128, 64, NC>(s, p, grid);
+    case 128128: return launch<TT, 128, 128, NC>(s, p, grid);
+    case 256032: return launch<TT, 256, 32, NC>(s, p, grid);
+    case 256064: return launch<TT, 256, 64, NC>(s, p, grid);
+    case 256128: return launch<TT, 256, 128, NC>(s, p, grid);
     default: return hipErrorInvalidValue;
   }
 }
@@ -491,21 +669,20 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.rows_max = rows_max;
   p.report = report;
   const size_t pairs = a.n_seqs * c.n_kv_heads;
-  // A part is at least one tile per wave; more parts than about 4096
-  // workgroups in all bring nothing but their joining.
-  const size_t tiles = (std::min<size_t>(a.max_kv, a.max_blocks * c.block_size) + kTile - 1) / kTile;
-  size_t parts = std::max<size_t>(std::min((tiles + kWaves - 1) / kWaves, std::max<size_t>(4096 / pairs, 1)), 1);
-  const size_t slab = pairs * (size_t)p.rows_max * (c.head_dim + 2) * sizeof(float);
-  const size_t room = ex.scratch_bytes > kWideCounterBytes ? ex.scratch_bytes - kWideCounterBytes : 0;
-  if (pairs * sizeof(unsigned int) > kWideCounterBytes) parts = 1;
-  parts = std::max<size_t>(std::min(parts, room / slab), 1);
-  p.parts = (int)parts;
-  p.part_tiles = kWaves;
+  const size_t slab = (size_t)p.rows_max * (c.head_dim + 4) * sizeof(float);
+  const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
+  size_t target = (size_t)env_int("CPQ_KV_ROUNDS", 4) * ex.cu_count;
+  // Each (sequence, head) rounds its parts up.
+  if (pairs * sizeof(unsigned int) > kWideCounterBytes || room <= pairs) target = 0;
+  else target = std::min(target, room - pairs);
+  p.target = (int)target;
+  p.part_tiles = env_int("CPQ_KV_MIN", 2) * kWaves;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
+  const size_t grid = pairs + target;
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
-  if (p.rows_max <= 16) return bf16 ? launch_d<BF16, 1>(ex.stream, p) : launch_d<F16, 1>(ex.stream, p);
-  return bf16 ? launch_d<BF16, 2>(ex.stream, p) : launch_d<F16, 2>(ex.stream, p);
+  if (p.rows_max <= 16) return bf16 ? launch_d<BF16, 1>(ex.stream, p, grid) : launch_d<F16, 1>(ex.stream, p, grid);
+  return bf16 ? launch_d<BF16, 2>(ex.stream, p, grid) : launch_d<F16, 2>(ex.stream, p, grid);
 }
 
 }  // namespace cpq
