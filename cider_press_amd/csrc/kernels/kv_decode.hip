@@ -33,13 +33,8 @@ namespace {
 
 using namespace dev;
 
-#ifndef WPS
-#define WPS 2
-#endif
-#ifndef STAGES
-#define STAGES 2
-#endif
 constexpr int kWaves = 4;
+constexpr int kStages = 2;  // of a wave's ring
 constexpr int kTile = 32;
 constexpr int kMaxParts = 256;
 constexpr float kSlack = 8.f;  // log2 of how far a weight may pass 1
@@ -58,8 +53,11 @@ struct Geo {
   static constexpr int kLoads = 2 * NQ + 2 * NL;
   // Byte offsets in a stage: keys, values, their constants.
   static constexpr int kV = NQ * 1024, kKc = 2 * kV, kVc = kKc + NL * 256, kStage = kVc + NL * 256;
+  // Waves per SIMD that the registers are to allow.
+  template <int NC>
+  static constexpr int kOccupancy = D == 256 ? 3 - NC : NC == 2 ? 2 : 3;
   // Behind the ring: the values' constants in f16, scales, biases and flags [G][32].
-  static constexpr int kConst = STAGES * kStage, kWave = kConst + 3 * 64 * G;
+  static constexpr int kConst = kStages * kStage, kWave = kConst + 3 * 64 * G;
 };
 
 struct DecodeArgs {
@@ -340,7 +338,10 @@ struct Rows {
 // What a workgroup does: its sequence, head and part.
 struct Item {
   int s, head, part, parts, first;  // first: workgroup of the same head's part 0
+  KvSeq q;
 };
+// LDS words of the search: the waves' sums, the item, its sequence, the join's flag.
+constexpr int kSearchWords = 16;
 
 __device__ __forceinline__ int tiles_of(const KvSeq& q) {
   return (max(q.n - (q.lo & ~(kTile - 1)), 0) + kTile - 1) / kTile;
@@ -370,9 +371,10 @@ __device__ __forceinline__ int block_scan(int v, int* words, int& all) {
 __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group, int bs_shift, int* words, Item& it) {
   const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, tid = threadIdx.x;
   constexpr int kThreads = kWaves * 64;
+  KvSeq q{};
   auto work = [&](int s, bool report) {
     if (s >= n_seqs) return 0;
-    const KvSeq q = kv_seq(p.a, s, bs_shift, report, p.bad);
+    q = kv_seq(p.a, s, bs_shift, report, p.bad);
     const int rows = q.n_q * group;
     return rows == 0 || rows > p.rows_max ? 0 : max(tiles_of(q), 1);  // no keys: zeros to store
   };
@@ -395,6 +397,10 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
       words[4] = base + tid;
       words[5] = b - at;
       words[6] = parts;
+      words[8] = q.rows0;
+      words[9] = q.n_q;
+      words[10] = q.n;
+      words[11] = q.lo;
     }
     if (b < before) {
       __syncthreads();
@@ -404,6 +410,11 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
       it.head = k % heads;
       it.part = k / heads;
       it.first = b - it.part * heads;
+      it.q.rows0 = __builtin_amdgcn_readfirstlane(words[8]);
+      it.q.n_q = __builtin_amdgcn_readfirstlane(words[9]);
+      it.q.n = __builtin_amdgcn_readfirstlane(words[10]);
+      it.q.lo = __builtin_amdgcn_readfirstlane(words[11]);
+      it.q.pos = it.q.n - it.q.n_q;
       return true;
     }
   }
@@ -411,10 +422,10 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
 }
 
 template <typename TT, int D, int GS, int NC>
-__global__ __launch_bounds__(kWaves * 64, WPS) void kv_decode_kernel(DecodeArgs p) {
+__global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>)) void kv_decode_kernel(DecodeArgs p) {
   using X = Geo<D, GS>;
   extern __shared__ __align__(16) unsigned char lds_bytes[];  // the waves' rings; then the join
-  __shared__ int words[8];
+  __shared__ int words[kSearchWords];
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -423,38 +434,10 @@ __global__ __launch_bounds__(kWaves * 64, WPS) void kv_decode_kernel(DecodeArgs 
   const int group = (int)a.n_heads / (int)c.n_kv_heads;
   Item it{};
   if (!find_item(p, blockIdx.x, group, bs_shift, words, it)) return;
-  const KvSeq q = kv_seq(a, it.s, bs_shift, false, nullptr);
+  const KvSeq& q = it.q;
   const int rows = q.n_q * group, head = it.head, parts = it.parts;
   const int base = q.lo & ~(kTile - 1), tiles = tiles_of(q);
   const int per = (tiles + parts - 1) / parts, last = min(tiles, (it.part + 1) * per);
-
-  // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
-  Rows<TT, D, GS, NC> R;
-#pragma unroll
-  for (int cc = 0; cc < NC; ++cc) {
-    const int r = min(16 * cc + i, rows - 1), qi = r / group, hh = head * group + r - qi * group;
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (size_t)(q.rows0 + qi) * a.q_token_stride +
-                          (size_t)hh * a.q_head_stride + h * (X::WL * 8);
-    float m = 0.f;
-#pragma unroll
-    for (int w = 0; w < X::WL; ++w) {
-      R.qs[cc][w] = *reinterpret_cast<const u32x4*>(src + 8 * w);
-      m = largest<TT>(R.qs[cc][w], m);
-    }
-    m = over_rows(m, max_of);
-    R.qe[cc] = query_exponent(m);
-#pragma unroll
-    for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = query_slice<TT>(R.qs[cc][w], R.qe[cc]);
-    R.qpos[cc] = q.pos + qi;
-    R.cl[cc] = fmaxf(scaled(a.scale * kLog2e, R.qe[cc]), FLT_MIN);
-    R.top[cc] = -INFINITY;
-    R.ref[cc] = -FLT_MAX;
-    R.sum[cc] = 0.f;
-#pragma unroll
-    for (int v = 0; v < X::VS; ++v)
-#pragma unroll
-      for (int j = 0; j < X::NJ; ++j) R.o[v][j][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
 
   const KvBlocks blocks = kv_blocks(a, it.s);
   unsigned char* ring = lds_bytes + wave * X::kWave;
@@ -465,34 +448,65 @@ __global__ __launch_bounds__(kWaves * 64, WPS) void kv_decode_kernel(DecodeArgs 
     if (ti < last) ids = kv_ids(blocks, base + ti * kTile, q.n, bs_shift);
   };
   auto start = [&](int ti) {
-    const int stage = (ti - t0) / kWaves % STAGES;
+    const int stage = (ti - t0) / kWaves % kStages;
     KvPlace pl[2];
     kv_places(c, ids, base + ti * kTile, q.n, head, bs_shift, pl);
     ok = (ok & ~(3 << 2 * stage)) | (pl[0].ok ? 1 : 0) << 2 * stage | (pl[1].ok ? 2 : 0) << 2 * stage;
     start_tile<D, GS>(c, pl, lane, ring + stage * X::kStage);
     look(ti + kWaves);
   };
+  look(t0);
+  // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
+  // Their loads, the first tile's blocks and its copies are under way together.
+  Rows<TT, D, GS, NC> R;
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc) {
+    const int r = min(16 * cc + i, rows - 1), qi = r / group, hh = head * group + r - qi * group;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (size_t)(q.rows0 + qi) * a.q_token_stride +
+                          (size_t)hh * a.q_head_stride + h * (X::WL * 8);
+#pragma unroll
+    for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = *reinterpret_cast<const u32x4*>(src + 8 * w);
+    R.qpos[cc] = q.pos + qi;
+  }
+#pragma unroll
+  for (int st = 0; st < kStages - 1; ++st)
+    if (t0 + st * kWaves < last) start(t0 + st * kWaves);
+#pragma unroll
+  for (int cc = 0; cc < NC; ++cc) {
+    float m = 0.f;
+#pragma unroll
+    for (int w = 0; w < X::WL; ++w) m = largest<TT>(R.qs[cc][w], m);
+    m = over_rows(m, max_of);
+    R.qe[cc] = query_exponent(m);
+#pragma unroll
+    for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = query_slice<TT>(R.qs[cc][w], R.qe[cc]);
+    R.cl[cc] = fmaxf(scaled(a.scale * kLog2e, R.qe[cc]), FLT_MIN);
+    R.top[cc] = -INFINITY;
+    R.ref[cc] = -FLT_MAX;
+    R.sum[cc] = 0.f;
+#pragma unroll
+    for (int v = 0; v < X::VS; ++v)
+#pragma unroll
+      for (int j = 0; j < X::NJ; ++j) R.o[v][j][cc] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
   // Every row sees the keys [seen_from, seen_end): nothing to mask among them.
   const int seen_end = a.causal ? min(q.pos + 1, q.n) : q.n;
   const int seen_from = a.window ? (int)max((int64_t)q.pos + q.n_q - (int64_t)a.window, (int64_t)0) : 0;
-  look(t0);
-#pragma unroll
-  for (int st = 0; st < STAGES - 1; ++st)
-    if (t0 + st * kWaves < last) start(t0 + st * kWaves);
   for (int ti = t0; ti < last; ti += kWaves) {
     // The stage that the wave read last is free once its reads are done.
     wave_lds_order();
     wait_lds();
-    if (ti + (STAGES - 1) * kWaves < last) {
-      start(ti + (STAGES - 1) * kWaves);
-      wait_vmcnt<(STAGES - 1) * X::kLoads>();
-    } else if (STAGES > 2 && ti + kWaves < last) {
+    if (ti + (kStages - 1) * kWaves < last) {
+      start(ti + (kStages - 1) * kWaves);
+      wait_vmcnt<(kStages - 1) * X::kLoads>();
+    } else if (kStages > 2 && ti + kWaves < last) {
       wait_vmcnt<X::kLoads>();
     } else {
       wait_vmcnt<0>();
     }
     wave_lds_order();
-    const int stage = (ti - t0) / kWaves % STAGES;
+    const int stage = (ti - t0) / kWaves % kStages;
     const int t = base + ti * kTile, oks = ok >> 2 * stage & 3;
     const bool whole = t >= seen_from && t + kTile <= seen_end && oks == 3;
     if (lane == 0 && ((!(oks & 1) && t < q.n) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
@@ -671,12 +685,12 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   const size_t pairs = a.n_seqs * c.n_kv_heads;
   const size_t slab = (size_t)p.rows_max * (c.head_dim + 4) * sizeof(float);
   const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
-  size_t target = (size_t)env_int("CPQ_KV_ROUNDS", 4) * ex.cu_count;
+  size_t target = (size_t)env_int("CPQ_KV_ROUNDS", 3) * ex.cu_count;
   // Each (sequence, head) rounds its parts up.
   if (pairs * sizeof(unsigned int) > kWideCounterBytes || room <= pairs) target = 0;
   else target = std::min(target, room - pairs);
   p.target = (int)target;
-  p.part_tiles = env_int("CPQ_KV_MIN", 2) * kWaves;
+  p.part_tiles = env_int("CPQ_KV_MIN", 4) * kWaves;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
   const size_t grid = pairs + target;

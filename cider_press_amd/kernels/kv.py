@@ -8,6 +8,7 @@ include/cpq.h (cpq_kv_cache and the functions after it).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from .. import _lib
 from . import Buffer, Commands, Device, _ptr
@@ -23,13 +24,18 @@ class _CacheArgs(ctypes.Structure):
                 ("v_sb", ctypes.c_void_p), ("v_sb_len", ctypes.c_size_t)]
 
 
-class _AttentionArgs(ctypes.Structure):
-    _fields_ = [("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_size_t), ("q_head_stride", ctypes.c_size_t),
-                ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_size_t), ("out_head_stride", ctypes.c_size_t),
-                ("n_tokens", ctypes.c_size_t), ("n_heads", ctypes.c_size_t), ("block_table", ctypes.c_void_p),
-                ("max_blocks", ctypes.c_size_t), ("query_starts", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
-                ("n_seqs", ctypes.c_size_t), ("max_q", ctypes.c_size_t), ("max_kv", ctypes.c_size_t),
-                ("scale", ctypes.c_float), ("causal", ctypes.c_int), ("window", ctypes.c_size_t)]
+# cpq_kv_attention_args, packed: a ctypes structure of its fields takes longer to fill than the launch.
+_ATTENTION_ARGS = struct.Struct("@PNNPNNNNPNPPNNNfiN")
+
+
+def _attention_args(*fields) -> bytes:
+    """q, its token and head strides, out, its strides, tokens, heads, block
+    table, max_blocks, query starts, key lengths, sequences, max_q, max_kv,
+    scale, causal, window."""
+    try:
+        return _ATTENTION_ARGS.pack(*fields)
+    except struct.error as e:  # a negative or too large count
+        raise _lib.InvalidArgument(f"kv_attention: {e}") from None
 
 
 class KvCache:
@@ -50,32 +56,28 @@ class KvCache:
             buffers = [device.alloc_buffer(n.value, "u32") for n in (q, sb, q, sb)]
         self.k_q, self.k_sb, self.v_q, self.v_sb = buffers
         for name, b in zip(("k_q", "k_sb", "v_q", "v_sb"), buffers):
-            _expect("KvCache", "u32", b)
+            _need("KvCache", "u32", (b, 0))
             setattr(self._args, name, b.ptr)
             setattr(self._args, name + "_len", len(b))
         _lib.check(_lib.lib().cpq_check_kv_cache(self._ref))
 
 
-def _expect(op: str, dtype: str, *buffers: Buffer) -> None:
-    for b in buffers:
+def _need(op: str, dtype: str, *pairs) -> None:
+    """Each (buffer, elements): TypeError when it is of another type,
+    InvalidArgument when it is shorter."""
+    for b, n in pairs:
         if b.dtype != dtype:
             raise TypeError(f"{op}: expected a {dtype} buffer, got {b.dtype}")
+        if b._len < n:
+            raise _lib.InvalidArgument(f"{op}: a buffer of {b._len} elements where {n} are needed")
 
 
-def _hold(op: str, *pairs) -> None:
-    """Each (buffer, elements): InvalidArgument when the buffer is shorter."""
-    for b, n in pairs:
-        if len(b) < n:
-            raise _lib.InvalidArgument(f"{op}: a buffer of {len(b)} elements where {n} are needed")
-
-
-def _strides(op: str, strides, b: Buffer, tokens: int, heads: int, dim: int):
+def _strides(op: str, dtype: str, strides, b: Buffer, tokens: int, heads: int, dim: int):
     """(token, head) strides in elements, dense by default, checked against the buffer."""
     token, head = strides if strides is not None else (heads * dim, dim)
     if token < 0 or head < 0:
         raise _lib.InvalidArgument(f"{op}: negative strides")
-    if tokens and heads:
-        _hold(op, (b, (tokens - 1) * token + (heads - 1) * head + dim))
+    _need(op, dtype, (b, (tokens - 1) * token + (heads - 1) * head + dim if tokens > 0 and heads > 0 else 0))
     return token, head
 
 
@@ -84,14 +86,12 @@ def kv_release(commands: Commands, finished: Buffer, lens: Buffer, block_table: 
                free_count_out: Buffer) -> None:
     """Blocks of sequences with finished != 0 go on top of the free list, their
     lens_out is 0.  Encodes only."""
-    bufs = (finished, lens, block_table, free_list, free_count, lens_out, free_count_out)
-    _expect("kv_release", "u32", *bufs)
-    n = len(lens)
-    _hold("kv_release", (finished, n), (block_table, n * max_blocks), (free_count, 1), (lens_out, n),
-          (free_count_out, 1))
+    n = lens._len
+    _need("kv_release", "u32", (finished, n), (lens, n), (block_table, n * max_blocks), (free_list, 0),
+          (free_count, 1), (lens_out, n), (free_count_out, 1))
     _lib.check(_lib.lib().cpq_kv_release(
-        commands.handle, _ptr(finished), _ptr(lens), _ptr(block_table), n, max_blocks, block_size, _ptr(free_list),
-        len(free_list), _ptr(free_count), _ptr(lens_out), _ptr(free_count_out)))
+        commands.handle, finished.ptr, lens.ptr, block_table.ptr, n, max_blocks, block_size, free_list.ptr,
+        len(free_list), free_count.ptr, lens_out.ptr, free_count_out.ptr))
 
 
 def kv_plan(commands: Commands, lens: Buffer, new_lens: Buffer, block_table: Buffer, max_blocks: int, block_size: int,
@@ -100,41 +100,34 @@ def kv_plan(commands: Commands, lens: Buffer, new_lens: Buffer, block_table: Buf
     """Query starts, key lengths, slots and positions of a step's new tokens,
     and the blocks they open entered in the block table; len(slots) is the
     step's capacity, unused entries are NO_SLOT.  Encodes only."""
-    bufs = (lens, new_lens, block_table, free_list, free_count, query_starts, kv_lens, slots, positions,
-            free_count_out)
-    _expect("kv_plan", "u32", *bufs)
-    n, cap = len(lens), len(slots)
-    _hold("kv_plan", (new_lens, n), (block_table, n * max_blocks), (free_count, 1), (query_starts, n + 1),
-          (kv_lens, n), (positions, cap), (free_count_out, 1))
+    n, cap = lens._len, slots._len
+    _need("kv_plan", "u32", (lens, n), (new_lens, n), (block_table, n * max_blocks), (free_list, 0), (free_count, 1),
+          (query_starts, n + 1), (kv_lens, n), (slots, cap), (positions, cap), (free_count_out, 1))
     _lib.check(_lib.lib().cpq_kv_plan(
-        commands.handle, _ptr(lens), _ptr(new_lens), _ptr(block_table), n, max_blocks, block_size, _ptr(free_list),
-        len(free_list), _ptr(free_count), _ptr(query_starts), _ptr(kv_lens), _ptr(slots), _ptr(positions), cap,
-        _ptr(free_count_out)))
+        commands.handle, lens.ptr, new_lens.ptr, block_table.ptr, n, max_blocks, block_size, free_list.ptr,
+        len(free_list), free_count.ptr, query_starts.ptr, kv_lens.ptr, slots.ptr, positions.ptr, cap,
+        free_count_out.ptr))
 
 
 def kv_append(commands: Commands, cache: KvCache, k: Buffer, v: Buffer, slots: Buffer, tokens: int, k_strides=None,
               v_strides=None) -> None:
     """Quantizes the keys and values of `tokens` tokens into their slots;
     strides are (token, head) in elements.  Encodes only."""
-    _expect("kv_append", cache.dtype, k, v)
-    _expect("kv_append", "u32", slots)
-    _hold("kv_append", (slots, tokens))
-    kt, kh = _strides("kv_append", k_strides, k, tokens, cache.n_kv_heads, cache.head_dim)
-    vt, vh = _strides("kv_append", v_strides, v, tokens, cache.n_kv_heads, cache.head_dim)
-    _lib.check(_lib.lib().cpq_kv_append(commands.handle, cache._ref, _ptr(k), kt, kh, _ptr(v), vt, vh, _ptr(slots),
+    _need("kv_append", "u32", (slots, tokens))
+    kt, kh = _strides("kv_append", cache.dtype, k_strides, k, tokens, cache.n_kv_heads, cache.head_dim)
+    vt, vh = _strides("kv_append", cache.dtype, v_strides, v, tokens, cache.n_kv_heads, cache.head_dim)
+    _lib.check(_lib.lib().cpq_kv_append(commands.handle, cache._ref, k.ptr, kt, kh, v.ptr, vt, vh, slots.ptr,
                                         tokens))
 
 
 def kv_gather(commands: Commands, cache: KvCache, slots: Buffer, rows: int, k_out=None, v_out=None) -> None:
     """Cached keys and values of `rows` slots as dense T [rows, n_kv_heads,
     head_dim]; either output may be None.  Encodes only."""
-    _expect("kv_gather", "u32", slots)
-    _hold("kv_gather", (slots, rows))
+    _need("kv_gather", "u32", (slots, rows))
     for b in (k_out, v_out):
         if b is not None:
-            _expect("kv_gather", cache.dtype, b)
-            _hold("kv_gather", (b, rows * cache.n_kv_heads * cache.head_dim))
-    _lib.check(_lib.lib().cpq_kv_gather(commands.handle, cache._ref, _ptr(slots), rows, _ptr(k_out), _ptr(v_out)))
+            _need("kv_gather", cache.dtype, (b, rows * cache.n_kv_heads * cache.head_dim))
+    _lib.check(_lib.lib().cpq_kv_gather(commands.handle, cache._ref, slots.ptr, rows, _ptr(k_out), _ptr(v_out)))
 
 
 def kv_attention(commands: Commands, cache: KvCache, q: Buffer, block_table: Buffer, max_blocks: int,
@@ -144,11 +137,9 @@ def kv_attention(commands: Commands, cache: KvCache, q: Buffer, block_table: Buf
     """Softmax attention of q [tokens, n_heads, head_dim] over each sequence's
     cached keys and values; strides are (token, head) in elements.  max_q and
     max_kv bound the sequences' queries and keys.  Encodes only."""
-    _expect("kv_attention", cache.dtype, q, out)
-    _expect("kv_attention", "u32", block_table, query_starts, kv_lens)
-    _hold("kv_attention", (block_table, n_seqs * max_blocks), (query_starts, n_seqs + 1), (kv_lens, n_seqs))
-    qt, qh = _strides("kv_attention", q_strides, q, tokens, n_heads, cache.head_dim)
-    ot, oh = _strides("kv_attention", out_strides, out, tokens, n_heads, cache.head_dim)
-    args = _AttentionArgs(_ptr(q), qt, qh, _ptr(out), ot, oh, tokens, n_heads, _ptr(block_table), max_blocks,
-                          _ptr(query_starts), _ptr(kv_lens), n_seqs, max_q, max_kv, scale, int(bool(causal)), window)
-    _lib.check(_lib.lib().cpq_kv_attention(commands.handle, cache._ref, ctypes.byref(args)))
+    _need("kv_attention", "u32", (block_table, n_seqs * max_blocks), (query_starts, n_seqs + 1), (kv_lens, n_seqs))
+    qt, qh = _strides("kv_attention", cache.dtype, q_strides, q, tokens, n_heads, cache.head_dim)
+    ot, oh = _strides("kv_attention", cache.dtype, out_strides, out, tokens, n_heads, cache.head_dim)
+    args = _attention_args(q.ptr, qt, qh, out.ptr, ot, oh, tokens, n_heads, block_table.ptr, max_blocks,
+                           query_starts.ptr, kv_lens.ptr, n_seqs, max_q, max_kv, scale, bool(causal), window)
+    _lib.check(_lib.lib().cpq_kv_attention(commands.handle, cache._ref, args))

@@ -61,12 +61,12 @@ def _attention(**over):
     a = dict(q=4096, qt=512, qh=128, out=8192, ot=512, oh=128, tokens=3, heads=4, table=4096, max_blocks=4,
              starts=4096, lens=4096, seqs=2, max_q=2, max_kv=10, scale=0.1, causal=1, window=0)
     a.update(over)
-    return kkv._AttentionArgs(*a.values())
+    return kkv._attention_args(*(v or 0 for v in a.values()))
 
 
 def test_attention_refusals():
     check, c = _lib.lib().cpq_check_kv_attention_args, _cache()
-    run = lambda **over: check(ctypes.byref(c), ctypes.byref(_attention(**over)))
+    run = lambda **over: check(ctypes.byref(c), _attention(**over))
     assert run() == _lib.OK
     assert run(tokens=0, q=None, out=None) == _lib.OK
     assert run(seqs=0, table=None) == _lib.OK
@@ -102,8 +102,10 @@ def test_buffer_checks():
         kkv.kv_release(None, u32(1), u32(2), u32(8), 4, 16, u32(8), u32(1), u32(2), u32(1))
     b = Buffer(None, None, 100, "bf16", 512)
     with pytest.raises(_lib.InvalidArgument):
-        kkv._strides("op", (50, 10), b, 3, 1, 8)  # 2 * 50 + 8 elements
-    assert kkv._strides("op", (46, 10), b, 3, 1, 8) == (46, 10)
+        kkv._attention_args(*[0] * 15, 1.0, 1, -1)
+    with pytest.raises(_lib.InvalidArgument):
+        kkv._strides("op", "bf16", (50, 10), b, 3, 1, 8)  # 2 * 50 + 8 elements
+    assert kkv._strides("op", "bf16", (46, 10), b, 3, 1, 8) == (46, 10)
     view = u32(10)
     view.ptr = 0
     with pytest.raises(ValueError):
