@@ -340,37 +340,26 @@ struct Item {
   int s, head, part, parts, first;  // first: workgroup of the same head's part 0
   KvSeq q;
 };
-// LDS words of the search: the waves' sums, the item, its sequence, the join's flag.
-constexpr int kSearchWords = 16;
+
 
 __device__ __forceinline__ int tiles_of(const KvSeq& q) {
   return (max(q.n - (q.lo & ~(kTile - 1)), 0) + kTile - 1) / kTile;
 }
-// Exclusive sum over the workgroup's threads and *all, the sum (two barriers).
-__device__ __forceinline__ int block_scan(int v, int* words, int& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int sum = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int o = __shfl_up(sum, d, 64);
-    if (lane >= d) sum += o;
-  }
-  __syncthreads();
-  if (lane == 63) words[wave] = sum;
-  __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += words[w];
-    all += words[w];
-  }
-  return before + sum - v;
+// Inclusive sum over the wave: within rows of 16 lanes, then from row to row.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2, 3
+  return v;
 }
-// The tiles of all sequences divided evenly: workgroup b's item, if any.
-__device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group, int bs_shift, int* words, Item& it) {
-  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, tid = threadIdx.x;
-  constexpr int kThreads = kWaves * 64;
+// The tiles of all sequences divided evenly: workgroup b's item, if any.  Every
+// wave goes over the sequences, 64 at a time: their tiles, the size of a part
+// from the sum of all, the sequence whose parts workgroup b falls among.
+__device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group, int bs_shift, Item& it) {
+  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, lane = threadIdx.x & 63;
   KvSeq q{};
   auto work = [&](int s, bool report) {
     if (s >= n_seqs) return 0;
@@ -379,41 +368,29 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
     return rows == 0 || rows > p.rows_max ? 0 : max(tiles_of(q), 1);  // no keys: zeros to store
   };
   int total = 0, own = 0;
-  for (int base = 0; base < n_seqs; base += kThreads) {
-    own = work(base + tid, p.report && b == 0);
-    int all;
-    block_scan(own, words, all);
-    total += all;
+  for (int base = 0; base < n_seqs; base += 64) {
+    own = work(base + lane, p.report && b == 0 && threadIdx.x < 64);
+    total += __builtin_amdgcn_readlane(wave_scan(own), 63);
   }
   const int per = max(p.part_tiles, p.target ? (int)(((long)total * heads + p.target - 1) / p.target) : 0x3fffffff);
   int before = 0;
-  for (int base = 0; base < n_seqs; base += kThreads) {
-    if (n_seqs > kThreads) own = work(base + tid, false);
+  for (int base = 0; base < n_seqs; base += 64) {
+    if (n_seqs > 64) own = work(base + lane, false);
     const int parts = min((own + per - 1) / per, kMaxParts);
-    int all;
-    const int at = before + block_scan(parts * heads, words, all);
-    before += all;
-    if (b >= at && b < at + parts * heads) {
-      words[4] = base + tid;
-      words[5] = b - at;
-      words[6] = parts;
-      words[8] = q.rows0;
-      words[9] = q.n_q;
-      words[10] = q.n;
-      words[11] = q.lo;
-    }
+    const int sum = wave_scan(parts * heads), at = before + sum - parts * heads;
+    before += __builtin_amdgcn_readlane(sum, 63);
     if (b < before) {
-      __syncthreads();
-      const int k = __builtin_amdgcn_readfirstlane(words[5]);
-      it.s = __builtin_amdgcn_readfirstlane(words[4]);
-      it.parts = __builtin_amdgcn_readfirstlane(words[6]);
+      const int l = __builtin_ctzll(__ballot(b >= at && b < at + parts * heads));
+      const int k = b - __builtin_amdgcn_readlane(at, l);
+      it.s = base + l;
+      it.parts = __builtin_amdgcn_readlane(parts, l);
       it.head = k % heads;
       it.part = k / heads;
       it.first = b - it.part * heads;
-      it.q.rows0 = __builtin_amdgcn_readfirstlane(words[8]);
-      it.q.n_q = __builtin_amdgcn_readfirstlane(words[9]);
-      it.q.n = __builtin_amdgcn_readfirstlane(words[10]);
-      it.q.lo = __builtin_amdgcn_readfirstlane(words[11]);
+      it.q.rows0 = __builtin_amdgcn_readlane(q.rows0, l);
+      it.q.n_q = __builtin_amdgcn_readlane(q.n_q, l);
+      it.q.n = __builtin_amdgcn_readlane(q.n, l);
+      it.q.lo = __builtin_amdgcn_readlane(q.lo, l);
       it.q.pos = it.q.n - it.q.n_q;
       return true;
     }
@@ -425,7 +402,7 @@ template <typename TT, int D, int GS, int NC>
 __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>)) void kv_decode_kernel(DecodeArgs p) {
   using X = Geo<D, GS>;
   extern __shared__ __align__(16) unsigned char lds_bytes[];  // the waves' rings; then the join
-  __shared__ int words[kSearchWords];
+  __shared__ int arrived;
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -433,7 +410,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   const int bs_shift = 31 - __builtin_clz(c.block_size);
   const int group = (int)a.n_heads / (int)c.n_kv_heads;
   Item it{};
-  if (!find_item(p, blockIdx.x, group, bs_shift, words, it)) return;
+  if (!find_item(p, blockIdx.x, group, bs_shift, it)) return;
   const KvSeq& q = it.q;
   const int rows = q.n_q * group, head = it.head, parts = it.parts;
   const int base = q.lo & ~(kTile - 1), tiles = tiles_of(q);
@@ -493,7 +470,16 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   // Every row sees the keys [seen_from, seen_end): nothing to mask among them.
   const int seen_end = a.causal ? min(q.pos + 1, q.n) : q.n;
   const int seen_from = a.window ? (int)max((int64_t)q.pos + q.n_q - (int64_t)a.window, (int64_t)0) : 0;
+  // The SIMD serves its oldest wave first, so of the workgroups on a CU one would
+  // end long before the last.  A wave gives way as it gets ahead.
+  const int quarter = (last - t0 + 3) / 4;
+  __builtin_amdgcn_s_setprio(3);
   for (int ti = t0; ti < last; ti += kWaves) {
+    if (ti - t0 >= quarter) {
+      if (ti - t0 >= 3 * quarter) __builtin_amdgcn_s_setprio(0);
+      else if (ti - t0 >= 2 * quarter) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(2);
+    }
     // The stage that the wave read last is free once its reads are done.
     wave_lds_order();
     wait_lds();
@@ -584,9 +570,9 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   unsigned int* counter = p.counters + (it.s * (int)c.n_kv_heads + head);
-  if (tid == 0) words[7] = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid == 0) arrived = (int)__hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (words[7] != parts - 1) return;
+  if (arrived != parts - 1) return;
   const float* all = p.partial + it.first * slab;
   const int stride = (int)(slab * c.n_kv_heads);  // from part to part
   float* weight = lds;                   // [rows][parts]
@@ -685,8 +671,10 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   const size_t pairs = a.n_seqs * c.n_kv_heads;
   const size_t slab = (size_t)p.rows_max * (c.head_dim + 4) * sizeof(float);
   const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
-  size_t target = (size_t)env_int("CPQ_KV_ROUNDS", 3) * ex.cu_count;
-  // Each (sequence, head) rounds its parts up.
+  // As many parts as workgroups are resident; each (sequence, head) rounds its
+  // own up, by half a part on average.
+  const size_t resident = (size_t)env_int("CPQ_KV_ROUNDS", c.head_dim == 256 || p.rows_max > 16 ? 2 : 3) * ex.cu_count;
+  size_t target = std::max(resident - std::min(resident, pairs / 2), resident / 4);
   if (pairs * sizeof(unsigned int) > kWideCounterBytes || room <= pairs) target = 0;
   else target = std::min(target, room - pairs);
   p.target = (int)target;
