@@ -15,8 +15,9 @@
 // of LDS while all four compute on this one; one barrier a tile.  The packed
 // words of the tile after that are in flight meanwhile.
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
-//   keys of a k step, XORed so that the 16 lanes of a b128 read that are served
-//   together (p, p + 4, ...) meet in 16 different units.
+//   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
+//   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
+//   a key that repeats among them doubles it).
 // The running maximum moves only when a tile exceeds it by 2^8.
 //
 // Few tiles over long keys are split over workgroups and joined, in part order,
@@ -50,22 +51,14 @@ __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Unit of a key's word: rows of W units; at 8 units a row, neighbouring rows
-// in storage are keys 4 apart.
+// Unit of a key's word.
 template <int W>
 __device__ __forceinline__ int key_unit(int key, int w) {
-  if constexpr (W == 8) {
-    const int r = (key & 32) | (key >> 2 & 7) | (key & 3) << 3;
-    return r * 8 + (w ^ (r & 6));
-  } else {
-    return key * W + (w ^ (key >> 2 & 7) << 1);
-  }
+  return key * W + (w ^ (key & (W < 16 ? 7 : 15)));
 }
-// Unit of a dimension's keys of half k step ts (2 * step + h).
-__device__ __forceinline__ int value_unit(int d, int ts) {
-  const int r = (d & ~31) | (d >> 2 & 7) | (d & 3) << 3;
-  return r * 8 + (ts ^ (r & 6));
-}
+// Unit of a dimension's keys of half k step ts (2 * step + h): read at
+// neighbouring dimensions, written at dimensions 8 apart.
+__device__ __forceinline__ int value_unit(int d, int ts) { return d * 8 + (ts ^ ((d ^ d >> 3) & 7)); }
 
 // The packed words of one wave's 32 keys: as keys, lane (key, half of the
 // words); as values, lane (word, half k step) -- twice at head_dim 256.
