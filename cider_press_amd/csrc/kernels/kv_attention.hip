@@ -47,6 +47,7 @@ struct TileArgs {
   unsigned int* bad;
 };
 
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 __device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
@@ -323,24 +324,29 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   float cl0 = 0.f, cl1 = 0.f;
 
   // Staging: waves 0, 1 keys and 2, 3 values of the tile's halves.
-  const KvBlocks blocks = kv_blocks(a, s);
+  const uint32_t* __restrict__ blocks = a.block_table + (size_t)s * a.max_blocks;
   const bool is_values = wave >= 2;
   const int half = wave & 1;
   Range range;
   Packed<D> packed;
   int loaded_ok = 3;
-  KvIds ids{};  // blocks of the half tile that is loaded next
+  // The blocks of this half of 32 tiles, a lane each 16 keys (scalar loads in
+  // flight would make every LDS wait a wait for all).
+  uint32_t ids = 0;
   auto look = [&](int t) {
-    if (t < stop) ids = kv_ids(blocks, min(t * kKeys + half * 32, (q.n - 1) & ~31), q.n, bs_shift);
+    const int key = min((t + (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1);
+    ids = blocks[key >> bs_shift];
   };
   auto load = [&](int t) {
     const int key = t * kKeys + half * 32;
     KvPlace pl[2];
-    kv_places(c, ids, min(key, (q.n - 1) & ~31), q.n, head, bs_shift, pl);
+    const int l = 2 * ((t - begin) & 31);
+    if (l == 0) look(t);
+    const KvIds id{{(uint32_t)__builtin_amdgcn_readlane((int)ids, l), (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1)}};
+    kv_places(c, id, min(key, (q.n - 1) & ~15), q.n, head, bs_shift, pl);
     loaded_ok = (pl[0].ok ? 1 : 0) | (pl[1].ok ? 2 : 0);
     if (is_values) load_values<D>(packed, c, pl, lane, gw_shift);
     else load_keys<D>(packed, c, pl, lane, gw_shift);
-    look(t + 1);
   };
   auto store = [&](int t, int buf) {
     u32x4* keys = units + buf * 2 * kUnits;
@@ -373,7 +379,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
     }
   };
 
-  look(begin);
   if (begin < stop) {
     load(begin);
     store(begin, 0);
@@ -406,14 +411,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
         cl0 = fmaxf(scaled(a.scale * kLog2e, ek0 + qe), FLT_MIN);
         cl1 = fmaxf(scaled(a.scale * kLog2e, ek1 + qe), FLT_MIN);
       }
+      // Operands are read a step ahead of the matrix instructions that take them.
       f32x16 sc[2];
+      u32x4 op[2][NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) op[0][i] = keys[key_unit<W>(col, 2 * i + h)];
+      fence();
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) sc[u] = mma(keys[key_unit<W>(32 * u + col, 2 * i + h)], qs[i], sc[u]);
+        for (int i = 0; i < NS; ++i) {
+          if (u == 0) op[1][i] = keys[key_unit<W>(32 + col, 2 * i + h)];
+          sc[u] = mma(op[u][i], qs[i], sc[u]);
+          fence();
+        }
       }
+      u32x4 vop[2][ND];
+#pragma unroll
+      for (int j = 0; j < ND; ++j) vop[0][j] = values[value_unit(32 * j + col, h)];
+      fence();
       const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
       if (!whole) {
 #pragma unroll
@@ -433,45 +451,46 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
       float m = fmaxf(m0 * cl0, m1 * cl1);
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
       m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-      if (__any(m > top + kSlack)) {
+      const int e = max(ev, max(mv0, mv1));  // o's unit: the largest exponent so far
+      if (e != ev || __any(m > top + kSlack)) {
         const float was = ref;
-        top = fmaxf(top, m);
-        ref = fmaxf(top, -FLT_MAX);
-        const float keep = __builtin_amdgcn_exp2f(was - ref);
+        if (__any(m > top + kSlack)) {
+          top = fmaxf(top, m);
+          ref = fmaxf(top, -FLT_MAX);
+        }
+        const float keep = __builtin_amdgcn_exp2f(was - ref), unit = scaled(keep, ev - e);
         sum *= keep;
 #pragma unroll
-        for (int j = 0; j < ND; ++j) o[j] *= keep;
-      }
-      float add = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          sc[u][e] = __builtin_amdgcn_exp2f(fmaf(sc[u][e], u ? cl1 : cl0, -ref));
-          add += sc[u][e];
-        }
-      sum += add;
-      if (mv0 != ev || mv1 != ev) {  // other exponents than o's: rare after the first tile
-        const int e = max(ev, max(mv0, mv1));
-#pragma unroll
-        for (int j = 0; j < ND; ++j)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], ev - e);
+        for (int j = 0; j < ND; ++j) o[j] *= unit;
         ev = e;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) sc[u][x] = scaled(sc[u][x], (u ? mv1 : mv0) - e);
       }
+      // A half whose values have a smaller exponent: smaller weights.
+      const int d0 = mv0 - e, d1 = mv1 - e;
+      const float r0 = ref - (float)d0, r1 = ref - (float)d1;
+      float add0 = 0.f, add1 = 0.f;
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k) {
-        const f32x16& w = sc[k >> 1];
-        const int x = 8 * (k & 1);
-        const u32x4 pw{F16::pack2(w[x], w[x + 1]), F16::pack2(w[x + 2], w[x + 3]), F16::pack2(w[x + 4], w[x + 5]),
-                       F16::pack2(w[x + 6], w[x + 7])};
-#pragma unroll
-        for (int j = 0; j < ND; ++j) o[j] = mma(values[value_unit(32 * j + col, 2 * k + h)], pw, o[j]);
+      for (int x = 0; x < 16; ++x) {
+        sc[0][x] = __builtin_amdgcn_exp2f(fmaf(sc[0][x], cl0, -r0));
+        sc[1][x] = __builtin_amdgcn_exp2f(fmaf(sc[1][x], cl1, -r1));
+        add0 += sc[0][x];
+        add1 += sc[1][x];
       }
+      sum += scaled(add0, -d0) + scaled(add1, -d1);
+      u32x4 pw[kKeys / 16];
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          pw[k][x] = F16::pack2(sc[k >> 1][8 * (k & 1) + 2 * x], sc[k >> 1][8 * (k & 1) + 2 * x + 1]);
+      fence();
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k)
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = values[value_unit(32 * j + col, 2 * (k + 1) + h)];
+          o[j] = mma(vop[k & 1][j], pw[k], o[j]);
+          fence();
+        }
       if (poison) {  // rows that see a value that is not finite: not a number in its group's dimensions
         for (int k = 0; k < kKeys / 16; ++k) {
           const int at = key0 + 16 * k;
