@@ -2,9 +2,10 @@
 // cpq_kv_attention in cpq.h): the kernel for many query rows per sequence, and
 // the choice between it and kv_decode.hip.
 //
-// A workgroup of four waves takes 128 query rows of one key/value head (rows
-// run over the queries, then the heads of the group, so a group of any size
-// shares the keys) and walks tiles of 64 keys, 32 rows a wave:
+// A workgroup of eight waves (four at head_dim 256, whose rows take twice the
+// registers) takes 32 query rows a wave of one key/value head (rows run over the
+// queries, then the heads of the group, so a group of any size shares the keys)
+// and walks tiles of 64 keys:
 //   S^T = K Q^T     v_mfma_f32_32x32x16_f16, A = 32 keys, B = 32 query rows
 //   O^T += V^T P^T  A = 32 dimensions over 16 keys, B = the weights, which
 //                   S^T's result layout holds as B takes them: lane (row n, h)
@@ -12,16 +13,17 @@
 //                   {4 h .. 4 h + 3, 8 + 4 h ..} of either operand.
 // Keys and values become f16 operands once per workgroup (kv_common.hpp): two
 // waves dequantize the next tile's keys and two its values into the other half
-// of LDS while all four compute on this one; one barrier a tile.  The packed
-// words of the tile after that are in flight meanwhile.
+// of LDS, of eight waves the two halves in turn, so that on each SIMD one wave's
+// dequantization meets the other's matrix instructions; one barrier a tile.  The
+// packed words of the next tile of the same four waves are in flight meanwhile.
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
 //   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
 //   a key that repeats among them doubles it).
 // The running maximum moves only when a tile exceeds it by 2^8.
 //
-// Few tiles over long keys are split over workgroups and joined, in part order,
-// by the last to arrive.
+// Where there are few row tiles their keys are split, evenly over the workgroups
+// by the lengths on the device, and joined, in part order, by the last to arrive.
 #include <algorithm>
 
 #include "kv_common.hpp"
@@ -32,7 +34,9 @@ namespace {
 using namespace dev;
 
 constexpr int kKeys = 64;        // of a tile
-constexpr int kRows = 128;       // of a workgroup
+constexpr int kMinTiles = 4;     // of a part
+template <int D>
+constexpr int kWaves = D == 256 ? 4 : 8;
 constexpr float kSlack = 8.f;    // log2 of how far a weight may pass 1
 constexpr int kPoison = 1 << 20;  // in a published exponent: a value constant is not finite
 
@@ -40,10 +44,10 @@ struct TileArgs {
   cpq_kv_cache c;
   cpq_kv_attention_args a;
   int few_rows;    // sequences of up to this many rows are another kernel's
-  int parts;       // most key parts of a tile
-  int part_tiles;  // least tiles of one part
-  unsigned int* counters;
-  float* partial;  // [workgroup tile][part][wave][D / 8 + 1][lane] f32x4: rows, then (maximum, sum)
+  int target;      // parts to divide the tiles into, 0: no splits
+  unsigned int* counters;  // per workgroup that is a first part
+  float* partial;          // [workgroup][wave][D / 8 + 1][lane] f32x4: rows, then (maximum, sum)
+  int report;  // this launch counts what is wrong with the sequences
   unsigned int* bad;
 };
 
@@ -210,41 +214,59 @@ __device__ __forceinline__ bool store_values(Packed<D>& t, u32x4* lds, int ts0, 
   return poison;
 }
 
-// Workgroup tile -> (sequence, tile of its rows), counted over the sequences
-// that this kernel takes.  False past the last.
-__device__ __forceinline__ bool find_tile(const TileArgs& p, int want, int group, int bs_shift, uint32_t* lds, int& s,
-                                          int& qt) {
-  const int tid = threadIdx.x, lane = tid & 63, n_seqs = (int)p.a.n_seqs;
+// What a workgroup does: rows tile `qt` of a sequence, a head, a part of the keys.
+struct Item {
+  int s, qt, head, part, parts;
+  KvSeq q;
+};
+// Workgroup b's item among the sequences that this kernel takes, if any: every
+// wave goes over them, 64 at a time, first for all their tiles (rows by keys)
+// and from that the size of a part.
+__device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, int bs_shift, int rows_per, Item& it) {
+  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, lane = threadIdx.x & 63;
+  KvSeq q{};
+  int row_tiles = 0, key_tiles = 0;
+  auto work = [&](int s, bool report) {
+    row_tiles = key_tiles = 0;
+    if (s >= n_seqs) return;
+    q = kv_seq(p.a, s, bs_shift, report, p.bad);
+    const int rows = q.n_q * group;
+    if (rows <= p.few_rows) return;
+    row_tiles = (rows + rows_per - 1) / rows_per;
+    // Of the last rows; a window leaves about its own length beside the rows'.
+    const int reach = p.a.window ? (int)min((uint64_t)q.n, (uint64_t)p.a.window + rows_per / group) : q.n;
+    key_tiles = (reach + kKeys - 1) / kKeys;
+  };
+  long total = 0;
+  if (p.target || p.report) {
+    for (int base = 0; base < n_seqs; base += 64) {
+      work(base + lane, p.report && b == 0 && threadIdx.x < 64);
+      long sum = (long)row_tiles * key_tiles;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+      total += sum;
+    }
+  }
+  const long per = p.target ? max((total * heads + p.target - 1) / p.target, (long)kMinTiles) : 1l << 40;
   int before = 0;
-  for (int base = 0; base < n_seqs; base += 256) {
-    int tiles = 0;
-    if (base + tid < n_seqs) {
-      const KvSeq q = kv_seq(p.a, base + tid, bs_shift, false, nullptr);
-      const int rows = q.n_q * group;
-      tiles = rows > p.few_rows ? (rows + kRows - 1) / kRows : 0;
-    }
-    int sum = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(sum, d, 64);
-      if (lane >= d) sum += o;
-    }
-    if (lane == 63) lds[tid >> 6] = (uint32_t)sum;
-    __syncthreads();
-    int at = before;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < tid >> 6) at += (int)lds[w];
-      before += (int)lds[w];
-    }
-    if (want >= at + sum - tiles && want < at + sum) {
-      lds[4] = (uint32_t)(base + tid);
-      lds[5] = (uint32_t)(want - (at + sum - tiles));
-    }
-    __syncthreads();
-    if (want < before) {
-      s = (int)lds[4];
-      qt = (int)lds[5];
+  for (int base = 0; base < n_seqs; base += 64) {
+    work(base + lane, false);
+    const int parts = max((int)min((key_tiles + per - 1) / per, (long)64), 1), items = row_tiles * parts * heads;
+    const int sum = wave_scan(items), at = before + sum - items;
+    before += __builtin_amdgcn_readlane(sum, 63);
+    if (b < before) {
+      const int l = __builtin_ctzll(__ballot(b >= at && b < at + items));
+      const int k = b - __builtin_amdgcn_readlane(at, l);
+      it.s = base + l;
+      it.parts = __builtin_amdgcn_readlane(parts, l);
+      it.head = k % heads;
+      it.part = k / heads % it.parts;
+      it.qt = k / heads / it.parts;
+      it.q.rows0 = __builtin_amdgcn_readlane(q.rows0, l);
+      it.q.n_q = __builtin_amdgcn_readlane(q.n_q, l);
+      it.q.n = __builtin_amdgcn_readlane(q.n, l);
+      it.q.lo = __builtin_amdgcn_readlane(q.lo, l);
+      it.q.pos = it.q.n - it.q.n_q;
       return true;
     }
   }
@@ -252,27 +274,24 @@ __device__ __forceinline__ bool find_tile(const TileArgs& p, int want, int group
 }
 
 template <typename TT, int D>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs p) {
+__global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
   extern __shared__ u32x4 units[];  // [2][keys, values][kUnits]
   __shared__ int meta[2][6];         // exponents of the halves' keys and values, which 16 keys have their block
-  __shared__ uint32_t words[8];
+  __shared__ unsigned int arrived;
+  constexpr int kRows = 32 * kWaves<D>;
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
   const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(c.group_size);
   const int group = (int)a.n_heads / (int)c.n_kv_heads;
-  const int tile = blockIdx.x / (int)c.n_kv_heads, head = blockIdx.x % (int)c.n_kv_heads, part = blockIdx.y;
-  if (blockIdx.x == 0 && part == 0)
-    for (int s = tid; s < (int)a.n_seqs; s += 256) kv_seq(a, s, bs_shift, true, p.bad);
-  int s = 0, qt = 0;
-  if (!find_tile(p, tile, group, bs_shift, words, s, qt)) return;
-  s = __builtin_amdgcn_readfirstlane(s);
-  qt = __builtin_amdgcn_readfirstlane(qt);
-  const KvSeq q = kv_seq(a, s, bs_shift, false, nullptr);
+  Item it{};
+  if (!find_item(p, blockIdx.x, group, bs_shift, kRows, it)) return;
+  const KvSeq& q = it.q;
+  const int head = it.head, part = it.part;
   const int rows = q.n_q * group;
-  qt = (rows + kRows - 1) / kRows - 1 - qt;  // the rows that see most first
+  const int qt = (rows + kRows - 1) / kRows - 1 - it.qt;  // the rows that see most first
   const int row0 = qt * kRows, row1 = min(row0 + kRows, rows);
 
   // Keys that any of the rows sees, in tiles; this part's.
@@ -280,8 +299,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   const int end = max(a.causal ? min(pos1 + 1, q.n) : q.n, 0);
   const int from = a.window ? (int)max((int64_t)pos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
   const int first = from / kKeys, tiles = max((end + kKeys - 1) / kKeys - first, 0);
-  const int per = max(p.part_tiles, (tiles + p.parts - 1) / p.parts);
-  const int parts = max((tiles + per - 1) / per, 1);
+  const int parts = max(min(it.parts, tiles / kMinTiles), 1), per = (tiles + parts - 1) / parts;
   if (part >= parts) return;
   const int begin = first + part * per, stop = min(first + tiles, begin + per);
 
@@ -309,7 +327,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   // Of the wave's rows: any sees [any_from, any_to), all see [all_from, all_to).
   const int wr0 = min(row0 + wave * 32, rows - 1), wr1 = min(row0 + wave * 32 + 31, rows - 1);
   const int wpos0 = q.pos + wr0 / group, wpos1 = q.pos + wr1 / group;
-  const int any_to = a.causal ? min(wpos1 + 1, q.n) : q.n, all_to = a.causal ? min(wpos0 + 1, q.n) : q.n;
+  const bool idle = row0 + wave * 32 >= rows;  // no rows of its own: it only stages
+  const int any_to = idle ? 0 : a.causal ? min(wpos1 + 1, q.n) : q.n, all_to = a.causal ? min(wpos0 + 1, q.n) : q.n;
   const int any_from = a.window ? (int)max((int64_t)wpos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
   const int all_from = a.window ? (int)max((int64_t)wpos1 + 1 - (int64_t)a.window, (int64_t)0) : 0;
 
@@ -323,9 +342,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   int ek0 = 1 << 30, ek1 = 1 << 30;    // key exponents that cl0, cl1 are for
   float cl0 = 0.f, cl1 = 0.f;
 
-  // Staging: waves 0, 1 keys and 2, 3 values of the tile's halves.
-  const uint32_t* __restrict__ blocks = a.block_table + (size_t)s * a.max_blocks;
-  const bool is_values = wave >= 2;
+  // Staging: of each four waves 0, 1 keys and 2, 3 values of the tile's halves.
+  const uint32_t* __restrict__ blocks = a.block_table + (size_t)it.s * a.max_blocks;
+  constexpr int kTeams = kWaves<D> / 4;
+  const int team = wave >> 2;
+  const bool is_values = wave & 2;
   const int half = wave & 1;
   Range range;
   Packed<D> packed;
@@ -334,13 +355,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   // flight would make every LDS wait a wait for all).
   uint32_t ids = 0;
   auto look = [&](int t) {
-    const int key = min((t + (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1);
+    const int key = min((t + kTeams * (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1);
     ids = blocks[key >> bs_shift];
   };
   auto load = [&](int t) {
     const int key = t * kKeys + half * 32;
     KvPlace pl[2];
-    const int l = 2 * ((t - begin) & 31);
+    const int l = 2 * ((t - begin) / kTeams & 31);
     if (l == 0) look(t);
     const KvIds id{{(uint32_t)__builtin_amdgcn_readlane((int)ids, l), (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1)}};
     kv_places(c, id, min(key, (q.n - 1) & ~15), q.n, head, bs_shift, pl);
@@ -374,15 +395,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
       store_keys<TT, D>(packed, keys, 32 * half, lane, range, live);
     }
     if (lane == 0) {
-      meta[buf][wave] = poison ? range.e + kPoison : range.e;
+      meta[buf][wave & 3] = poison ? range.e + kPoison : range.e;
       if (!is_values) meta[buf][4 + half] = loaded_ok;
     }
   };
 
-  if (begin < stop) {
-    load(begin);
+  if (begin + team < stop) load(begin + team);
+  if (team == 0 && begin < stop) {
     store(begin, 0);
-    if (begin + 1 < stop) load(begin + 1);
+    if (begin + kTeams < stop) load(begin + kTeams);
   }
   __syncthreads();
   for (int t = begin; t < stop; ++t) {
@@ -397,9 +418,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
       range.e = max(mv0, mv1);
       range.limits = size_limits<TT>(range.e);
     }
-    if (t + 1 < stop) {
+    if (t + 1 < stop && (t + 1 - begin) % kTeams == team) {
       store(t + 1, buf ^ 1);
-      if (t + 2 < stop) load(t + 2);
+      if (t + 1 + kTeams < stop) load(t + 1 + kTeams);
     }
     const int key0 = t * kKeys;
     if (key0 < any_to && key0 + kKeys > any_from) {
@@ -468,20 +489,20 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
       const int d0 = mv0 - e, d1 = mv1 - e;
       const float r0 = ref - (float)d0, r1 = ref - (float)d1;
       float add0 = 0.f, add1 = 0.f;
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        sc[0][x] = __builtin_amdgcn_exp2f(fmaf(sc[0][x], cl0, -r0));
-        sc[1][x] = __builtin_amdgcn_exp2f(fmaf(sc[1][x], cl1, -r1));
-        add0 += sc[0][x];
-        add1 += sc[1][x];
-      }
-      sum += scaled(add0, -d0) + scaled(add1, -d1);
       u32x4 pw[kKeys / 16];
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          pw[k][x] = F16::pack2(sc[k >> 1][8 * (k & 1) + 2 * x], sc[k >> 1][8 * (k & 1) + 2 * x + 1]);
+        for (int x = 0; x < 4; ++x) {
+          const int u = k >> 1, at = 8 * (k & 1) + 2 * x;
+          const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][at], u ? cl1 : cl0, u ? -r1 : -r0));
+          const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][at + 1], u ? cl1 : cl0, u ? -r1 : -r0));
+          pw[k][x] = F16::pack2(w0, w1);
+          // The sum is of the rounded weights, two at a time.
+          float& add = u ? add1 : add0;
+          add = F16::dot2(pw[k][x], 0x3c003c00u, add);
+        }
+      sum += scaled(add0, -d0) + scaled(add1, -d1);
       fence();
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
@@ -535,12 +556,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
   uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +
                   (size_t)hh * a.out_head_stride + 4 * h;
   if (parts > 1) {
-    const size_t slab = (size_t)4 * (D / 8 + 1) * 64;  // f32x4 per part
-    const f32x4* all = reinterpret_cast<const f32x4*>(p.partial) + (size_t)blockIdx.x * p.parts * slab +
-                       (size_t)wave * (D / 8 + 1) * 64;
-    const f32x4* mine = all + part * slab;
+    const size_t slab = (size_t)kWaves<D> * (D / 8 + 1) * 64;  // f32x4 of a workgroup
+    const size_t first = blockIdx.x - (size_t)part * c.n_kv_heads, stride = slab * c.n_kv_heads;
+    const f32x4* all = reinterpret_cast<const f32x4*>(p.partial) + first * slab + (size_t)wave * (D / 8 + 1) * 64;
+    const f32x4* mine = all + part * stride;
     auto put = [&](int at, f32x4 v) { park_store(mine, (at * 64 + lane) * 16, v); };
-    auto get = [&](int k, int at) { return park_load(all + k * slab, (at * 64 + lane) * 16); };
+    auto get = [&](int k, int at) { return park_load(all + k * stride, (at * 64 + lane) * 16); };
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
@@ -550,9 +571,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
     put(D / 8, f32x4{ref, sum, 0.f, 0.f});
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (tid == 0) words[6] = __hip_atomic_fetch_add(&p.counters[blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) arrived = __hip_atomic_fetch_add(&p.counters[first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (words[6] != (uint32_t)(parts - 1)) return;
+    if (arrived != (unsigned int)(parts - 1)) return;
     float m = -FLT_MAX;
     for (int k = 0; k < parts; ++k) m = fmaxf(m, get(k, D / 8)[0]);
     sum = 0.f;
@@ -574,7 +595,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs
           for (int e = 0; e < 4; ++e) o[j][4 * x + e] += v[e] * w;
         }
     }
-    if (tid == 0) __hip_atomic_store(&p.counters[blockIdx.x], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) __hip_atomic_store(&p.counters[first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!stored) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -594,7 +615,7 @@ hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
   static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return raised;
-  hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, p);
+  hipLaunchKernelGGL(kernel, grid, dim3(kWaves<D> * 64), lds, s, p);
   return hipGetLastError();
 }
 
@@ -615,18 +636,18 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
     const hipError_t e = launch_kv_decode(ex, c, a, p.few_rows, false, bad);
     if (e != hipSuccess) return e;
   }
-  // No more tiles than this, whatever the sequences' shares.
-  const size_t tiles = a.n_tokens * group / kRows + a.n_seqs, wgs = tiles * c.n_kv_heads;
-  const size_t keys = (std::min<size_t>(a.max_kv, a.max_blocks * c.block_size) + kKeys - 1) / kKeys;
-  const size_t slab = wgs * 4 * (c.head_dim / 8 + 1) * 64 * 16;
-  const size_t room = ex.scratch_bytes > kWideCounterBytes ? ex.scratch_bytes - kWideCounterBytes : 0;
-  p.part_tiles = 4;
-  size_t parts = std::max<size_t>(std::min(512 / wgs, keys / p.part_tiles), 1);
-  if (wgs * sizeof(unsigned int) > kWideCounterBytes) parts = 1;
-  p.parts = (int)std::max<size_t>(std::min(parts, room / slab), 1);
+  p.report = 1;
+  // No more row tiles than this, whatever the sequences' shares.
+  const size_t waves = c.head_dim == 256 ? 4 : 8;
+  const size_t wgs = (a.n_tokens * group / (32 * waves) + a.n_seqs) * c.n_kv_heads;
+  // Two parts per CU where there are fewer tiles than that, as far as the scratch goes.
+  const size_t slab = waves * (c.head_dim / 8 + 1) * 64 * 16;
+  const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
+  const size_t target = 2 * (size_t)ex.cu_count;
+  p.target = wgs < room && wgs < target ? (int)std::min(target, room - wgs) : 0;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
-  const dim3 grid((uint32_t)wgs, (uint32_t)p.parts);
+  const dim3 grid((uint32_t)(wgs + p.target));
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   switch (c.head_dim) {
     case 64: return bf16 ? launch_tiles<BF16, 64>(ex.stream, p, grid) : launch_tiles<F16, 64>(ex.stream, p, grid);

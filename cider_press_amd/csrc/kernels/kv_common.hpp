@@ -79,6 +79,16 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// Inclusive sum over the wave: within rows of 16 lanes, then from row to row.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2, 3
+  return v;
+}
 // 16 bytes of a partial result that a workgroup on another XCD reads or wrote in
 // this launch: through to the memory side and from it.  `base` is the same for
 // the whole wave.

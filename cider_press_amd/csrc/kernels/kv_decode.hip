@@ -345,16 +345,6 @@ struct Item {
 __device__ __forceinline__ int tiles_of(const KvSeq& q) {
   return (max(q.n - (q.lo & ~(kTile - 1)), 0) + kTile - 1) / kTile;
 }
-// Inclusive sum over the wave: within rows of 16 lanes, then from row to row.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1, 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2, 3
-  return v;
-}
 // The tiles of all sequences divided evenly: workgroup b's item, if any.  Every
 // wave goes over the sequences, 64 at a time: their tiles, the size of a part
 // from the sum of all, the sequence whose parts workgroup b falls among.
