@@ -20,7 +20,10 @@
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
 //   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
 //   a key that repeats among them doubles it).
-// The running maximum moves only when a tile exceeds it by 2^8.
+// No maximum is taken on the way: weights are 2^(score - reference), and only
+// where their sums show that one leaves f16's range (the first tile's do) is the
+// tile's maximum found, the reference raised to 2^-6 of it and the tile's scores
+// computed again.
 //
 // Where there are few row tiles their keys are split, evenly over the workgroups
 // by the lengths on the device, and joined, in part order, by the last to arrive.
@@ -37,7 +40,8 @@ constexpr int kKeys = 64;        // of a tile
 constexpr int kMinTiles = 4;     // of a part
 template <int D>
 constexpr int kWaves = D == 256 ? 4 : 8;
-constexpr float kSlack = 8.f;    // log2 of how far a weight may pass 1
+constexpr float kRaise = 6.f;     // log2 of the largest weight when the reference is set
+constexpr float kMost = 32768.f;  // of 16 weights' sum, so that each fits f16
 constexpr int kPoison = 1 << 20;  // in a published exponent: a value constant is not finite
 
 struct TileArgs {
@@ -62,8 +66,9 @@ __device__ __forceinline__ int key_unit(int key, int w) {
   return key * W + (w ^ (key & (W < 16 ? 7 : 15)));
 }
 // Unit of a dimension's keys of half k step ts (2 * step + h): read at
-// neighbouring dimensions, written at dimensions 8 apart.
-__device__ __forceinline__ int value_unit(int d, int ts) { return d * 8 + (ts ^ ((d ^ d >> 3) & 7)); }
+// neighbouring dimensions, written at dimensions 8 apart (two of eight lanes
+// meet there).  Dimensions 32 apart have the same place in their rows.
+__device__ __forceinline__ int value_unit(int d, int ts) { return d * 8 + (ts ^ ((d ^ (d >> 3 & 3)) & 7)); }
 
 // The packed words of one wave's 32 keys: as keys, lane (key, half of the
 // words); as values, lane (word, half k step) -- twice at head_dim 256.
@@ -337,7 +342,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   for (int j = 0; j < ND; ++j)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
-  float top = -INFINITY, ref = -FLT_MAX, sum = 0.f;
+  float ref = -FLT_MAX, sum = 0.f;
   int ev = -1000;                      // o, so far zeros, is in units of 2^ev
   int ek0 = 1 << 30, ek1 = 1 << 30;    // key exponents that cl0, cl1 are for
   float cl0 = 0.f, cl1 = 0.f;
@@ -400,6 +405,22 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     }
   };
 
+  // Byte offsets of the lane's operands in LDS; the half of LDS in turn is the
+  // other value of one bit.
+  constexpr uint32_t kHalf = 2 * kUnits * 16;
+  const unsigned char* lds = reinterpret_cast<const unsigned char*>(units);
+  uint32_t at_key[NS], at_value[kKeys / 16];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) at_key[i] = (uint32_t)key_unit<W>(col, 2 * i + h) * 16;
+#pragma unroll
+  for (int k = 0; k < kKeys / 16; ++k) at_value[k] = (uint32_t)(kUnits + value_unit(col, 2 * k + h)) * 16;
+  auto key_operand = [&](int u, int i) {
+    return *reinterpret_cast<const u32x4*>(lds + at_key[i] + u * (32 * W * 16));
+  };
+  auto value_operand = [&](int j, int k) {
+    return *reinterpret_cast<const u32x4*>(lds + at_value[k] + j * (32 * 8 * 16));
+  };
+
   if (begin + team < stop) load(begin + team);
   if (team == 0 && begin < stop) {
     store(begin, 0);
@@ -424,91 +445,94 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     }
     const int key0 = t * kKeys;
     if (key0 < any_to && key0 + kKeys > any_from) {
-      const u32x4* keys = units + buf * 2 * kUnits;
-      const u32x4* values = keys + kUnits;
       if (mk0 != ek0 || mk1 != ek1) {
         ek0 = mk0;
         ek1 = mk1;
         cl0 = fmaxf(scaled(a.scale * kLog2e, ek0 + qe), FLT_MIN);
         cl1 = fmaxf(scaled(a.scale * kLog2e, ek1 + qe), FLT_MIN);
       }
-      // Operands are read a step ahead of the matrix instructions that take them.
-      f32x16 sc[2];
-      u32x4 op[2][NS];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) op[0][i] = keys[key_unit<W>(col, 2 * i + h)];
-      fence();
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sc[u][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          if (u == 0) op[1][i] = keys[key_unit<W>(32 + col, 2 * i + h)];
-          sc[u] = mma(op[u][i], qs[i], sc[u]);
-          fence();
-        }
-      }
-      u32x4 vop[2][ND];
-#pragma unroll
-      for (int j = 0; j < ND; ++j) vop[0][j] = values[value_unit(32 * j + col, h)];
-      fence();
-      const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
-      if (!whole) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-            sc[u][e] = key >= see_from && key < see_to && (ok >> (2 * u + (e >> 3)) & 1) ? sc[u][e] : -INFINITY;
-          }
-      }
-      float m0 = sc[0][0], m1 = sc[1][0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) {
-        m0 = fmaxf(m0, sc[0][e]);
-        m1 = fmaxf(m1, sc[1][e]);
-      }
-      float m = fmaxf(m0 * cl0, m1 * cl1);
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
-      m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       const int e = max(ev, max(mv0, mv1));  // o's unit: the largest exponent so far
-      if (e != ev || __any(m > top + kSlack)) {
-        const float was = ref;
-        if (__any(m > top + kSlack)) {
-          top = fmaxf(top, m);
-          ref = fmaxf(top, -FLT_MAX);
-        }
-        const float keep = __builtin_amdgcn_exp2f(was - ref), unit = scaled(keep, ev - e);
-        sum *= keep;
+      if (e != ev) {
 #pragma unroll
-        for (int j = 0; j < ND; ++j) o[j] *= unit;
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], ev - e);
         ev = e;
       }
       // A half whose values have a smaller exponent: smaller weights.
       const int d0 = mv0 - e, d1 = mv1 - e;
-      const float r0 = ref - (float)d0, r1 = ref - (float)d1;
-      float add0 = 0.f, add1 = 0.f;
-      u32x4 pw[kKeys / 16];
+      const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
+      u32x4 pw[kKeys / 16], vop[2][ND];
+      float add0, add1;
+      for (bool again = false;; again = true) {
+        // Operands are read a step ahead of the matrix instructions that take them.
+        f32x16 sc[2];
+        u32x4 op[2][NS];
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k)
+        for (int i = 0; i < NS; ++i) op[0][i] = key_operand(0, i);
+        fence();
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int u = k >> 1, at = 8 * (k & 1) + 2 * x;
-          const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][at], u ? cl1 : cl0, u ? -r1 : -r0));
-          const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][at + 1], u ? cl1 : cl0, u ? -r1 : -r0));
-          pw[k][x] = F16::pack2(w0, w1);
-          // The sum is of the rounded weights, two at a time.
-          float& add = u ? add1 : add0;
-          add = F16::dot2(pw[k][x], 0x3c003c00u, add);
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            if (u == 0) op[1][i] = key_operand(1, i);
+            sc[u] = mma(op[u][i], qs[i], sc[u]);
+            fence();
+          }
         }
+#pragma unroll
+        for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
+        fence();
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+              const int key = key0 + 32 * u + 8 * (x >> 2) + 4 * h + (x & 3);
+              sc[u][x] = key >= see_from && key < see_to && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
+            }
+        }
+        if (again) {
+          float m0 = sc[0][0], m1 = sc[1][0];
+#pragma unroll
+          for (int x = 1; x < 16; ++x) {
+            m0 = fmaxf(m0, sc[0][x]);
+            m1 = fmaxf(m1, sc[1][x]);
+          }
+          const float mine = fmaxf(m0 * cl0, m1 * cl1);
+          const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
+          const float was = ref;
+          ref = fmaxf(ref, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kRaise);
+          const float keep = __builtin_amdgcn_exp2f(was - ref);
+          sum *= keep;
+#pragma unroll
+          for (int j = 0; j < ND; ++j) o[j] *= keep;
+        }
+        const float r0 = ref - (float)d0, r1 = ref - (float)d1;
+        add0 = add1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int u = k >> 1, at = 8 * (k & 1) + 2 * x;
+            const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][at], u ? cl1 : cl0, u ? -r1 : -r0));
+            const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][at + 1], u ? cl1 : cl0, u ? -r1 : -r0));
+            pw[k][x] = F16::pack2(w0, w1);
+            // The sum is of the rounded weights, two at a time.
+            float& add = u ? add1 : add0;
+            add = F16::dot2(pw[k][x], 0x3c003c00u, add);
+          }
+        if (again || !__any(!(fmaxf(add0, add1) < kMost))) break;
+      }
       sum += scaled(add0, -d0) + scaled(add1, -d1);
       fence();
 #pragma unroll
       for (int k = 0; k < kKeys / 16; ++k)
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
-          if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = values[value_unit(32 * j + col, 2 * (k + 1) + h)];
+          if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = value_operand(j, k + 1);
           o[j] = mma(vop[k & 1][j], pw[k], o[j]);
           fence();
         }
@@ -545,6 +569,10 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) at_key[i] ^= kHalf;
+#pragma unroll
+    for (int k = 0; k < kKeys / 16; ++k) at_value[k] ^= kHalf;
     __syncthreads();
   }
 
