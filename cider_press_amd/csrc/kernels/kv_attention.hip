@@ -82,11 +82,11 @@ struct Packed {
 };
 
 template <int D>
-__device__ __forceinline__ void load_keys(Packed<D>& t, const cpq_kv_cache& c, const KvPlace* p, int lane,
+__device__ __forceinline__ void load_keys(Packed<D>& t, const cpq_kv_cache& c, size_t row_a, size_t row_b, int lane,
                                           int gw_shift) {
   constexpr int W = D / 8, NK = Packed<D>::NK;
   const int G = W >> gw_shift, half = lane >> 5;
-  const size_t row = (lane & 16 ? p[1].row : p[0].row) + (lane & 15);
+  const size_t row = (lane & 16 ? row_b : row_a) + (lane & 15);
   const u32x4* q = reinterpret_cast<const u32x4*>(c.k_q + row * W + half * (W / 2));
 #pragma unroll
   for (int i = 0; i < NK; ++i) {
@@ -95,11 +95,11 @@ __device__ __forceinline__ void load_keys(Packed<D>& t, const cpq_kv_cache& c, c
   }
 }
 template <int D>
-__device__ __forceinline__ void load_values(Packed<D>& t, const cpq_kv_cache& c, const KvPlace* p, int lane,
+__device__ __forceinline__ void load_values(Packed<D>& t, const cpq_kv_cache& c, size_t row_a, size_t row_b, int lane,
                                             int gw_shift) {
   constexpr int W = D / 8, L = W < 16 ? 8 : 16;  // lanes over words
   const int G = W >> gw_shift, ts = lane / L & 3;
-  const size_t quad = ((ts & 2 ? p[1].row : p[0].row) >> 2) + (ts & 1);
+  const size_t quad = ((ts & 2 ? row_b : row_a) >> 2) + (ts & 1);
 #pragma unroll
   for (int v = 0; v < Packed<D>::VS; ++v) {
     const int w = 16 * v + lane % L;
@@ -343,6 +343,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
   float ref = -FLT_MAX, sum = 0.f;
+  uint32_t nan_groups = 0;             // groups of dimensions that are NaN in this row
   int ev = -1000;                      // o, so far zeros, is in units of 2^ev
   int ek0 = 1 << 30, ek1 = 1 << 30;    // key exponents that cl0, cl1 are for
   float cl0 = 0.f, cl1 = 0.f;
@@ -365,14 +366,14 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   };
   auto load = [&](int t) {
     const int key = t * kKeys + half * 32;
-    KvPlace pl[2];
     const int l = 2 * ((t - begin) / kTeams & 31);
     if (l == 0) look(t);
-    const KvIds id{{(uint32_t)__builtin_amdgcn_readlane((int)ids, l), (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1)}};
-    kv_places(c, id, min(key, (q.n - 1) & ~15), q.n, head, bs_shift, pl);
-    loaded_ok = (pl[0].ok ? 1 : 0) | (pl[1].ok ? 2 : 0);
-    if (is_values) load_values<D>(packed, c, pl, lane, gw_shift);
-    else load_keys<D>(packed, c, pl, lane, gw_shift);
+    const KvPlaces pl = kv_places(c, (uint32_t)__builtin_amdgcn_readlane((int)ids, l),
+                                  (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1), min(key, (q.n - 1) & ~15), q.n,
+                                  head, bs_shift);
+    loaded_ok = (pl.a.ok ? 1 : 0) | (pl.b.ok ? 2 : 0);
+    if (is_values) load_values<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
+    else load_keys<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
   };
   auto store = [&](int t, int buf) {
     u32x4* keys = units + buf * 2 * kUnits;
@@ -486,12 +487,13 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
         for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
         fence();
         if (!whole) {
+          const int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;  // of the lane's first key
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-              const int key = key0 + 32 * u + 8 * (x >> 2) + 4 * h + (x & 3);
-              sc[u][x] = key >= see_from && key < see_to && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
+              const int k = 32 * u + 8 * (x >> 2) + (x & 3);
+              sc[u][x] = k >= lo && k < hi && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
             }
         }
         if (again) {
@@ -536,37 +538,11 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
           o[j] = mma(vop[k & 1][j], pw[k], o[j]);
           fence();
         }
-      if (poison) {  // rows that see a value that is not finite: not a number in its group's dimensions
-        for (int k = 0; k < kKeys / 16; ++k) {
-          const int at = key0 + 16 * k;
-          if (at >= q.n) break;
-          const KvPlace pl = kv_place(c, blocks[at >> bs_shift], at, head, bs_shift);
-          u32x4 seen;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = at + 8 * (x >> 1) + 4 * h + 2 * (x & 1);
-            seen[x] = (key >= see_from && key < see_to && pl.ok ? 0x3c00u : 0u) |
-                      (key + 1 >= see_from && key + 1 < see_to && pl.ok ? 0x3c000000u : 0u);
-          }
-          for (int j = 0; j < ND; ++j) {
-            const int g = (32 * j + col) / 8 >> gw_shift, G = W >> gw_shift;
-            u32x4 flags;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const uint32_t* sb = c.v_sb + (((pl.row >> 2) + 2 * (x >> 1) + h) * G + g) * 4 + 2 * (x & 1);
-              flags[x] = (finite(TT::lo(sb[0])) && finite(TT::hi(sb[0])) ? 0u : 0x3c00u) |
-                         (finite(TT::lo(sb[1])) && finite(TT::hi(sb[1])) ? 0u : 0x3c000000u);
-            }
-            f32x16 n;
-#pragma unroll
-            for (int x = 0; x < 16; ++x) n[x] = 0.f;
-            n = mma(flags, seen, n);
-#pragma unroll
-            for (int jj = 0; jj < ND; ++jj)
-#pragma unroll
-              for (int x = 0; x < 16; ++x) o[jj][x] = jj == j && n[x] > 0.f ? NAN : o[jj][x];
-          }
-        }
+      if (poison) {
+#pragma clang loop unroll(disable)
+        for (int k = 0; k < kKeys && key0 + k < q.n; k += 16)
+          nan_groups |= poisoned_groups<TT>(c, kv_place(c, blocks[(key0 + k) >> bs_shift], key0 + k, head, bs_shift),
+                                            key0 + k, W >> gw_shift, see_from, see_to);
       }
     }
 #pragma unroll
@@ -579,6 +555,13 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   {
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
     sum = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  if (__any(nan_groups != 0)) {
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        if (nan_groups >> ((32 * j + 8 * (x >> 2)) / 8 >> gw_shift) & 1) o[j][x] = NAN;
   }
   const bool stored = row0 + wave * 32 + col < rows;
   uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +

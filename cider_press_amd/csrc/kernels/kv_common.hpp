@@ -142,16 +142,10 @@ typedef const __attribute__((address_space(4))) uint32_t* KvBlocks;
 __device__ __forceinline__ KvBlocks kv_blocks(const cpq_kv_attention_args& a, int s) {
   return (KvBlocks)(a.block_table + (size_t)s * a.max_blocks);
 }
-// The blocks of 32 keys from t (a multiple of 32, below n): of the first 16 and
-// of the others, which past the end are the last keys' (their loads are in
-// bounds, their results masked).
-struct KvIds {
-  uint32_t id[2];
-};
-__device__ __forceinline__ KvIds kv_ids(KvBlocks blocks, int t, int n, int bs_shift) {
-  return KvIds{{blocks[t >> bs_shift], blocks[min(t + 16, (n - 1) & ~15) >> bs_shift]}};
-}
-// Where they lie: the row of the first in the cache's [block][head][offset]
+// The table index of 16 keys from t (a multiple of 16); past the end of the last
+// keys' block (their loads are in bounds, their results masked).
+__device__ __forceinline__ int kv_index(int t, int n, int bs_shift) { return min(t, (n - 1) & ~15) >> bs_shift; }
+// Where 16 keys lie: the row of the first in the cache's [block][head][offset]
 // order, and whether the block is one of the cache's.
 struct KvPlace {
   size_t row;
@@ -161,10 +155,32 @@ __device__ __forceinline__ KvPlace kv_place(const cpq_kv_cache& c, uint32_t id, 
   const bool ok = id < c.n_blocks;
   return KvPlace{(((size_t)(ok ? id : 0) * c.n_kv_heads + head) << bs_shift) + (at & ((1 << bs_shift) - 1)), ok};
 }
-__device__ __forceinline__ void kv_places(const cpq_kv_cache& c, const KvIds& ids, int t, int n, int head,
-                                          int bs_shift, KvPlace* p) {
-  p[0] = kv_place(c, ids.id[0], t, head, bs_shift);
-  p[1] = kv_place(c, ids.id[1], min(t + 16, (n - 1) & ~15), head, bs_shift);
+// Of 32 keys.
+struct KvPlaces {
+  KvPlace a, b;
+};
+__device__ __forceinline__ KvPlaces kv_places(const cpq_kv_cache& c, uint32_t id0, uint32_t id1, int t, int n, int head,
+                                              int bs_shift) {
+  return KvPlaces{kv_place(c, id0, t, head, bs_shift), kv_place(c, id1, min(t + 16, (n - 1) & ~15), head, bs_shift)};
+}
+
+// A value constant that is not finite is taken as zero and makes its group's
+// dimensions NaN in the rows that see the key (a masked row would meet 0 * NaN
+// otherwise): the groups of such keys among 16 from `key` in [from, to).  Only
+// where a tile holds any, so a loop over memory does.
+template <typename TT>
+__device__ __forceinline__ uint32_t poisoned_groups(const cpq_kv_cache& c, const KvPlace& p, int key, int G, int from,
+                                                    int to) {
+  uint32_t groups = 0;
+  if (!p.ok) return groups;
+#pragma clang loop unroll(disable)
+  for (int e = 0; e < 16 * G; ++e) {
+    const uint32_t sb = c.v_sb[p.row * G + e];
+    if (finite(TT::lo(sb)) && finite(TT::hi(sb))) continue;
+    const int k = key + e / (4 * G) * 4 + (e & 3);
+    groups |= (uint32_t)(k >= from && k < to) << (e / 4 % G);
+  }
+  return groups;
 }
 
 // Rows of q as f16 operands: 8 values of T times 2^-e, in the order of a key

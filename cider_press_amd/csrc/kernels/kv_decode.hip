@@ -56,8 +56,8 @@ struct Geo {
   // Waves per SIMD that the registers are to allow.
   template <int NC>
   static constexpr int kOccupancy = D == 256 ? 3 - NC : NC == 2 ? 2 : 3;
-  // Behind the ring: the values' constants in f16, scales, biases and flags [G][32].
-  static constexpr int kConst = kStages * kStage, kWave = kConst + 3 * 64 * G;
+  // Behind the ring: the values' constants in f16, scales and biases [G][32].
+  static constexpr int kConst = kStages * kStage, kWave = kConst + 2 * 64 * G;
 };
 
 struct DecodeArgs {
@@ -83,10 +83,10 @@ __device__ __forceinline__ void copy4(const void* src, unsigned char* lds) {
 
 // Starts the copies of one tile into a stage: kLoads instructions.
 template <int D, int GS>
-__device__ __forceinline__ void start_tile(const cpq_kv_cache& c, const KvPlace* p, int lane, unsigned char* stage) {
+__device__ __forceinline__ void start_tile(const cpq_kv_cache& c, size_t row_a, size_t row_b, int lane, unsigned char* stage) {
   using X = Geo<D, GS>;
   const int i = lane & 15, h = lane >> 4;
-  const size_t mine = lane & 32 ? p[1].row : p[0].row;  // lanes 32 .. take the second 16 keys
+  const size_t mine = lane & 32 ? row_b : row_a;  // lanes 32 .. take the second 16 keys
 #pragma unroll
   for (int q = 0; q < X::NQ; ++q) {
     const uint32_t *k, *v;
@@ -95,8 +95,8 @@ __device__ __forceinline__ void start_tile(const cpq_kv_cache& c, const KvPlace*
       v = c.v_q + mine * 8 + (lane & 31) * 4;
     } else {
       const int u = q / (D / 128), part = q % (D / 128);
-      k = c.k_q + p[u].row * X::W + i * X::W + h * X::WL + 4 * part;
-      v = c.v_q + p[u].row * X::W + (h * X::W + 16 * part + i) * 4;
+      k = c.k_q + (u ? row_b : row_a) * X::W + i * X::W + h * X::WL + 4 * part;
+      v = c.v_q + (u ? row_b : row_a) * X::W + (h * X::W + 16 * part + i) * 4;
     }
     copy16(k, stage + q * 1024);
     copy16(v, stage + X::kV + q * 1024);
@@ -105,7 +105,7 @@ __device__ __forceinline__ void start_tile(const cpq_kv_cache& c, const KvPlace*
   for (int q = 0; q < X::NL; ++q) {
     const int e = min(64 * q + lane, 32 * X::G - 1);  // constant of the tile, 16 G of each place
     const bool second = e >= 16 * X::G;
-    const size_t at = (second ? p[1].row : p[0].row) * X::G + (second ? e - 16 * X::G : e);
+    const size_t at = (second ? row_b : row_a) * X::G + (second ? e - 16 * X::G : e);
     copy4(c.k_sb + at, stage + X::kKc + q * 256);
     copy4(c.v_sb + at, stage + X::kVc + q * 256);
   }
@@ -117,7 +117,6 @@ struct Rows {
   using X = Geo<D, GS>;
   u32x4 qs[NC][X::WL];
   int qe[NC];    // exponents of the query rows
-  int qpos[NC];  // positions
   float cl[NC];  // log2(e) * scale * 2^(qe + ek)
   f32x4 o[X::VS][X::NJ][NC];
   float top[NC], ref[NC], sum[NC];
@@ -149,15 +148,17 @@ struct Rows {
     }
   }
 
-  // One tile in `stage`.  on(key of the tile, position) says what a row sees,
-  // any(key) whether a row may; whole: all rows see all of it.
-  template <typename On, typename Any>
-  __device__ __forceinline__ void add(unsigned char* wave_lds, const unsigned char* stage, int lane, bool whole,
-                                      float scale, On on, Any any) {
+  // One tile in `stage`, keys t on.  whole: all rows see all of it; else rows see
+  // keys [from, to) of theirs in the 16-key halves whose bit in `oks` is set, and
+  // none any outside [any_from, any_to).  Returns whether a value's constants were
+  // not finite (they count as zeros).
+  __device__ __forceinline__ bool add(unsigned char* wave_lds, const unsigned char* stage, int lane, bool whole,
+                                      float scale, int t, int oks, const int (&from)[NC], const int (&to)[NC],
+                                      int any_from, int any_to) {
     const int i = lane & 15, h = lane >> 4;
     const uint32_t* kc = reinterpret_cast<const uint32_t*>(stage + X::kKc);
     const uint32_t* vc = reinterpret_cast<const uint32_t*>(stage + X::kVc);
-    uint16_t* cs = reinterpret_cast<uint16_t*>(wave_lds + X::kConst);  // scales, [32 G] biases, flags
+    uint16_t* cs = reinterpret_cast<uint16_t*>(wave_lds + X::kConst);  // scales, [32 G] biases
 
     // Constants: whether they fit the exponents (and are finite).
     uint32_t ksb[2][X::NG], vsb[X::NL];
@@ -174,9 +175,10 @@ struct Rows {
       vsb[q] = vc[64 * q + lane];
       vs = sizes(vs, vsb[q]);
     }
+    auto any = [&](int k) { return t + k >= any_from && t + k < any_to && (oks >> (k >> 4) & 1); };
     const bool careful = !whole || __any(ks != klim || vs != vlim);
     bool poison = false;
-    if (careful) {  // what no row sees counts as zeros, as do values that are not finite (NaN below)
+    if (careful) {  // what no row sees counts as zeros, as do values that are not finite
       float km = 0.f, vm = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -185,11 +187,10 @@ struct Rows {
           km = fmaxf(km, any(16 * u + i) ? finite_size<TT>(ksb[u][g]) : 0.f);
 #pragma unroll
       for (int q = 0; q < X::NL; ++q) {
-        const int e = 64 * q + lane, key = e / (4 * X::G) * 4 + (e & 3);
-        const bool live = any(key & 31);
+        const int e = 64 * q + lane, key = e / (4 * X::G) * 4 + (e & 3) & 31;
+        const bool live = any(key);
         const bool ok = finite(TT::lo(vsb[q])) && finite(TT::hi(vsb[q]));
-        poison |= live && !ok && e < 32 * X::G;
-        if (e < 32 * X::G) cs[64 * X::G + e / 4 % X::G * 32 + key] = live && !ok ? 0x3c00 : 0;
+        poison |= live && !ok;
         vsb[q] = live && ok ? vsb[q] : 0u;
         vm = fmaxf(vm, finite_size<TT>(vsb[q]));
       }
@@ -247,10 +248,14 @@ struct Rows {
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       if (!whole) {
+        const int lo = from[cc] - t - 4 * h, hi = to[cc] - t - 4 * h;  // of the lane's first key
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[u][cc][e] = on(16 * u + 4 * h + e, qpos[cc]) ? sc[u][cc][e] : -INFINITY;
+          for (int e = 0; e < 4; ++e) {
+            const int k = 16 * u + e;
+            sc[u][cc][e] = k >= lo && k < hi && (oks >> u & 1) ? sc[u][cc][e] : -INFINITY;
+          }
       }
       float m = fmaxf(fmaxf(fmaxf(sc[0][cc][0], sc[0][cc][1]), fmaxf(sc[0][cc][2], sc[0][cc][3])),
                       fmaxf(fmaxf(sc[1][cc][0], sc[1][cc][1]), fmaxf(sc[1][cc][2], sc[1][cc][3])));
@@ -312,26 +317,8 @@ struct Rows {
           o[v][2 * y + 1][cc] = Mfma16<F16>::run(hi, pw[cc], o[v][2 * y + 1][cc]);
         }
       }
-      if (poison) {  // rows that see such a value: not a number in its group's dimensions
-        const u32x2 f0 = *reinterpret_cast<const u32x2*>(mine + 64 * X::G);
-        const u32x2 f1 = *reinterpret_cast<const u32x2*>(mine + 64 * X::G + 16);
-        const u32x4 flags{f0.x, f0.y, f1.x, f1.y};
-#pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
-          u32x4 seen;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = 16 * (x >> 1) + 4 * h + 2 * (x & 1);
-            seen[x] = (on(key, qpos[cc]) ? 0x3c00u : 0u) | (on(key + 1, qpos[cc]) ? 0x3c000000u : 0u);
-          }
-          const f32x4 n = Mfma16<F16>::run(flags, seen, f32x4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-          for (int j = 0; j < X::NJ; ++j)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[v][j][cc][x] = n[x] > 0.f ? NAN : o[v][j][cc][x];
-        }
-      }
     }
+    return poison;
   }
 };
 
@@ -410,22 +397,24 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   unsigned char* ring = lds_bytes + wave * X::kWave;
   const int t0 = it.part * per + wave;
   int ok = 0;  // two bits a stage: whether the block of either 16 keys is the cache's
-  KvIds ids{};  // blocks of the tile that is copied next
+  uint32_t id0 = 0, id1 = 0;  // blocks of the tile that is copied next
   auto look = [&](int ti) {
-    if (ti < last) ids = kv_ids(blocks, base + ti * kTile, q.n, bs_shift);
+    if (ti >= last) return;
+    id0 = blocks[kv_index(base + ti * kTile, q.n, bs_shift)];
+    id1 = blocks[kv_index(base + ti * kTile + 16, q.n, bs_shift)];
   };
   auto start = [&](int ti) {
     const int stage = (ti - t0) / kWaves % kStages;
-    KvPlace pl[2];
-    kv_places(c, ids, base + ti * kTile, q.n, head, bs_shift, pl);
-    ok = (ok & ~(3 << 2 * stage)) | (pl[0].ok ? 1 : 0) << 2 * stage | (pl[1].ok ? 2 : 0) << 2 * stage;
-    start_tile<D, GS>(c, pl, lane, ring + stage * X::kStage);
+    const KvPlaces pl = kv_places(c, id0, id1, base + ti * kTile, q.n, head, bs_shift);
+    ok = (ok & ~(3 << 2 * stage)) | (pl.a.ok ? 1 : 0) << 2 * stage | (pl.b.ok ? 2 : 0) << 2 * stage;
+    start_tile<D, GS>(c, pl.a.row, pl.b.row, lane, ring + stage * X::kStage);
     look(ti + kWaves);
   };
   look(t0);
   // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
   // Their loads, the first tile's blocks and its copies are under way together.
   Rows<TT, D, GS, NC> R;
+  int from[NC], to[NC];  // keys that a row sees
 #pragma unroll
   for (int cc = 0; cc < NC; ++cc) {
     const int r = min(16 * cc + i, rows - 1), qi = r / group, hh = head * group + r - qi * group;
@@ -433,7 +422,9 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
                           (size_t)hh * a.q_head_stride + h * (X::WL * 8);
 #pragma unroll
     for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = *reinterpret_cast<const u32x4*>(src + 8 * w);
-    R.qpos[cc] = q.pos + qi;
+    const int pos = q.pos + qi;
+    from[cc] = a.window ? (int)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
+    to[cc] = a.causal ? min(pos + 1, q.n) : q.n;
   }
 #pragma unroll
   for (int st = 0; st < kStages - 1; ++st)
@@ -460,6 +451,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   // Every row sees the keys [seen_from, seen_end): nothing to mask among them.
   const int seen_end = a.causal ? min(q.pos + 1, q.n) : q.n;
   const int seen_from = a.window ? (int)max((int64_t)q.pos + q.n_q - (int64_t)a.window, (int64_t)0) : 0;
+  uint32_t nan_groups[NC] = {};  // groups of dimensions that are NaN in a row
   // The SIMD serves its oldest wave first, so of the workgroups on a CU one would
   // end long before the last.  A wave gives way as it gets ahead.
   const int quarter = (last - t0 + 3) / 4;
@@ -486,13 +478,16 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     const int t = base + ti * kTile, oks = ok >> 2 * stage & 3;
     const bool whole = t >= seen_from && t + kTile <= seen_end && oks == 3;
     if (lane == 0 && ((!(oks & 1) && t < q.n) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
-    R.add(ring, ring + stage * X::kStage, lane, whole, a.scale,
-          [&](int k, int pos) {
-            const int key = t + k;
-            return key < q.n && !(a.causal && key > pos) &&
-                   !(a.window && (int64_t)key <= (int64_t)pos - (int64_t)a.window) && (oks >> (k >> 4) & 1);
-          },
-          [&](int k) { return t + k < q.n && t + k >= q.lo && (oks >> (k >> 4) & 1); });
+    const bool poison = R.add(ring, ring + stage * X::kStage, lane, whole, a.scale, t, oks, from, to, q.lo, q.n);
+    if (poison) {
+      const KvPlaces pl = kv_places(c, blocks[kv_index(t, q.n, bs_shift)], blocks[kv_index(t + 16, q.n, bs_shift)], t,
+                                    q.n, head, bs_shift);
+#pragma unroll
+      for (int cc = 0; cc < NC; ++cc) {
+        nan_groups[cc] |= poisoned_groups<TT>(c, pl.a, t, X::G, from[cc], to[cc]);
+        if (t + 16 < q.n) nan_groups[cc] |= poisoned_groups<TT>(c, pl.b, t + 16, X::G, from[cc], to[cc]);
+      }
+    }
   }
 
   // The waves' results: each one's rows relative to its own maximum.
@@ -515,7 +510,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
           for (int x = 0; x < 4; ++x) {
             const int w = 4 * h + x;  // of 16: word, or word and half of its dimensions
             const int d = D == 64 ? 8 * (w & 7) + 4 * (w >> 3) + j : 8 * (16 * v + w) + j;
-            dst[d] = scaled(R.o[v][j][cc][x], R.ev);
+            dst[d] = nan_groups[cc] >> (d / GS) & 1 ? NAN : scaled(R.o[v][j][cc][x], R.ev);
           }
       if (h == 0) {
         wmax[wave * rows + r] = R.ref[cc];
