@@ -365,6 +365,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     ids = blocks[key >> bs_shift];
   };
   auto load = [&](int t) {
+    const int lane = (int)opaque((uint32_t)(tid & 63));
     const int key = t * kKeys + half * 32;
     const int l = 2 * ((t - begin) / kTeams & 31);
     if (l == 0) look(t);
@@ -376,6 +377,9 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     else load_keys<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
   };
   auto store = [&](int t, int buf) {
+    // (The lane hidden from the optimiser: addresses made anew each time take a few
+    // instructions, kept through the loop they spill registers.)
+    const int lane = (int)opaque((uint32_t)(tid & 63));
     u32x4* keys = units + buf * 2 * kUnits;
     const int key = t * kKeys + half * 32;
     const bool all = key >= from && key + 32 <= q.n && loaded_ok == 3;
