@@ -577,27 +577,30 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     const f32x4* mine = all + part * stride;
     auto put = [&](int at, f32x4 v) { park_store(mine, (at * 64 + lane) * 16, v); };
     auto get = [&](int k, int at) { return park_load(all + k * stride, (at * 64 + lane) * 16); };
+    if (!idle) {
 #pragma unroll
-    for (int j = 0; j < ND; ++j)
+      for (int j = 0; j < ND; ++j)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        put(4 * j + x, f32x4{scaled(o[j][4 * x], ev), scaled(o[j][4 * x + 1], ev),
-                             scaled(o[j][4 * x + 2], ev), scaled(o[j][4 * x + 3], ev)});
-    put(D / 8, f32x4{ref, sum, 0.f, 0.f});
+        for (int x = 0; x < 4; ++x)
+          put(4 * j + x, f32x4{scaled(o[j][4 * x], ev), scaled(o[j][4 * x + 1], ev),
+                               scaled(o[j][4 * x + 2], ev), scaled(o[j][4 * x + 3], ev)});
+      put(D / 8, f32x4{ref, sum, 0.f, 0.f});
+    }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid == 0) arrived = __hip_atomic_fetch_add(&p.counters[first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (arrived != (unsigned int)(parts - 1)) return;
     float m = -FLT_MAX;
-    for (int k = 0; k < parts; ++k) m = fmaxf(m, get(k, D / 8)[0]);
+    const int joined = idle ? 0 : parts;
+    for (int k = 0; k < joined; ++k) m = fmaxf(m, get(k, D / 8)[0]);
     sum = 0.f;
     ev = 0;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[j][x] = 0.f;
-    for (int k = 0; k < parts; ++k) {
+    for (int k = 0; k < joined; ++k) {
       const f32x4 ml = get(k, D / 8);
       const float w = __builtin_amdgcn_exp2f(ml[0] - m);
       sum += ml[1] * w;
