@@ -42,7 +42,13 @@ template <int D>
 constexpr int kWaves = D == 256 ? 4 : 8;
 constexpr float kRaise = 6.f;     // log2 of the largest weight when the reference is set
 constexpr float kMost = 32768.f;  // of 16 weights' sum, so that each fits f16
-constexpr int kPoison = 1 << 20;  // in a published exponent: a value constant is not finite
+// What a wave publishes of its half of a tile: the exponent (0: all constants so
+// far are zeros), which 16 keys have their block, whether a value constant is not
+// finite.
+constexpr int kExpBias = 1 << 12, kOkShift = 16, kPoison = 1 << 20;
+// Halves of values whose exponents differ by no more than this are joined by
+// smaller weights, others are dequantized again to the same exponent.
+constexpr int kMostApart = 10;
 
 struct TileArgs {
   cpq_kv_cache c;
@@ -282,7 +288,7 @@ template <typename TT, int D>
 __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
   extern __shared__ u32x4 units[];  // [2][keys, values][kUnits]
-  __shared__ int meta[2][6];         // exponents of the halves' keys and values, which 16 keys have their block
+  __shared__ int meta[2][4];         // of the halves' keys, then their values
   __shared__ unsigned int arrived;
   constexpr int kRows = 32 * kWaves<D>;
   const cpq_kv_cache& c = p.c;
@@ -345,8 +351,8 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   float ref = -FLT_MAX, sum = 0.f;
   uint32_t nan_groups = 0;             // groups of dimensions that are NaN in this row
   int ev = -1000;                      // o, so far zeros, is in units of 2^ev
-  int ek0 = 1 << 30, ek1 = 1 << 30;    // key exponents that cl0, cl1 are for
-  float cl0 = 0.f, cl1 = 0.f;
+  float cl0 = 0.f, cl1 = 0.f;          // of the halves: log2(e) * scale * 2^(exponents of q and the keys)
+  int d0 = 0, d1 = 0;                  // and the values' exponents less ev
 
   // Staging: of each four waves 0, 1 keys and 2, 3 values of the tile's halves.
   const uint32_t* __restrict__ blocks = a.block_table + (size_t)it.s * a.max_blocks;
@@ -360,15 +366,12 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   // The blocks of this half of 32 tiles, a lane each 16 keys (scalar loads in
   // flight would make every LDS wait a wait for all).
   uint32_t ids = 0;
-  auto look = [&](int t) {
-    const int key = min((t + kTeams * (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1);
-    ids = blocks[key >> bs_shift];
-  };
-  auto load = [&](int t) {
+  auto load = [&](int t, bool again) {
     const int lane = (int)opaque((uint32_t)(tid & 63));
     const int key = t * kKeys + half * 32;
     const int l = 2 * ((t - begin) / kTeams & 31);
-    if (l == 0) look(t);
+    if (l == 0 || again)
+      ids = blocks[min((t + kTeams * ((lane - l) >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1) >> bs_shift];
     const KvPlaces pl = kv_places(c, (uint32_t)__builtin_amdgcn_readlane((int)ids, l),
                                   (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1), min(key, (q.n - 1) & ~15), q.n,
                                   head, bs_shift);
@@ -404,10 +407,8 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
       const bool live = all || (k >= from && k < q.n && (loaded_ok >> (lane >> 4 & 1) & 1));
       store_keys<TT, D>(packed, keys, 32 * half, lane, range, live);
     }
-    if (lane == 0) {
-      meta[buf][wave & 3] = poison ? range.e + kPoison : range.e;
-      if (!is_values) meta[buf][4 + half] = loaded_ok;
-    }
+    if (lane == 0)
+      meta[buf][wave & 3] = (range.limits ? range.e + kExpBias : 0) + (loaded_ok << kOkShift) + (poison ? kPoison : 0);
   };
 
   // Byte offsets of the lane's operands in LDS; the half of LDS in turn is the
@@ -426,37 +427,42 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     return *reinterpret_cast<const u32x4*>(lds + at_value[k] + j * (32 * 8 * 16));
   };
 
-  if (begin + team < stop) load(begin + team);
+  if (begin + team < stop) load(begin + team, false);
   if (team == 0 && begin < stop) {
     store(begin, 0);
-    if (begin + kTeams < stop) load(begin + kTeams);
+    if (begin + kTeams < stop) load(begin + kTeams, false);
   }
   __syncthreads();
+  int known = -1, ok = 0;  // the published words that cl, d and ok are of
+  bool poison = false;
   for (int t = begin; t < stop; ++t) {
     const int buf = (t - begin) & 1;
-    const int mk0 = __builtin_amdgcn_readfirstlane(meta[buf][0]), mk1 = __builtin_amdgcn_readfirstlane(meta[buf][1]);
-    int mv0 = __builtin_amdgcn_readfirstlane(meta[buf][2]), mv1 = __builtin_amdgcn_readfirstlane(meta[buf][3]);
-    const int ok = __builtin_amdgcn_readfirstlane(meta[buf][4] | meta[buf][5] << 2);
-    const bool poison = mv0 >= kPoison / 2 || mv1 >= kPoison / 2;
-    if (mv0 >= kPoison / 2) mv0 -= kPoison;
-    if (mv1 >= kPoison / 2) mv1 -= kPoison;
-    if (is_values && max(mv0, mv1) > range.e) {  // the halves' values share the larger exponent from here on
-      range.e = max(mv0, mv1);
-      range.limits = size_limits<TT>(range.e);
-    }
-    if (t + 1 < stop && (t + 1 - begin) % kTeams == team) {
-      store(t + 1, buf ^ 1);
-      if (t + 1 + kTeams < stop) load(t + 1 + kTeams);
-    }
-    const int key0 = t * kKeys;
-    if (key0 < any_to && key0 + kKeys > any_from) {
-      if (mk0 != ek0 || mk1 != ek1) {
-        ek0 = mk0;
-        ek1 = mk1;
-        cl0 = fmaxf(scaled(a.scale * kLog2e, ek0 + qe), FLT_MIN);
-        cl1 = fmaxf(scaled(a.scale * kLog2e, ek1 + qe), FLT_MIN);
+    int news = meta[buf][lane & 3];
+    if (__any(news != known)) {
+      auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
+      auto exponent = [&](int i, int none) { return word(i) & 0xffff ? (word(i) & 0xffff) - kExpBias : none; };
+      const int e = max(ev, max(exponent(2, ev), exponent(3, ev)));  // o's unit: the largest exponent so far
+      if (is_values && e > range.e) {  // the values share it from here on
+        range.e = e;
+        range.limits = size_limits<TT>(e);
       }
-      const int e = max(ev, max(mv0, mv1));  // o's unit: the largest exponent so far
+      if (e - min(exponent(2, e), exponent(3, e)) > kMostApart) {  // (all waves alike: they read the same words)
+        __syncthreads();
+        if (is_values && (t - begin) % kTeams == team) {
+          load(t, true);
+          store(t, buf);
+          if (t + kTeams < stop) load(t + kTeams, true);
+        }
+        __syncthreads();
+        news = meta[buf][lane & 3];
+      }
+      known = news;
+      poison = (word(2) | word(3)) >= kPoison;
+      ok = (word(0) >> kOkShift & 3) | (word(1) >> kOkShift & 3) << 2;
+      cl0 = fmaxf(scaled(a.scale * kLog2e, exponent(0, 0) + qe), FLT_MIN);
+      cl1 = fmaxf(scaled(a.scale * kLog2e, exponent(1, 0) + qe), FLT_MIN);
+      d0 = exponent(2, e) - e;
+      d1 = exponent(3, e) - e;
       if (e != ev) {
 #pragma unroll
         for (int j = 0; j < ND; ++j)
@@ -464,11 +470,17 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
           for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], ev - e);
         ev = e;
       }
-      // A half whose values have a smaller exponent: smaller weights.
-      const int d0 = mv0 - e, d1 = mv1 - e;
+    }
+    if (t + 1 < stop && (t + 1 - begin) % kTeams == team) {
+      store(t + 1, buf ^ 1);
+      if (t + 1 + kTeams < stop) load(t + 1 + kTeams, false);
+    }
+    const int key0 = t * kKeys;
+    if (key0 < any_to && key0 + kKeys > any_from) {
       const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
       u32x4 pw[kKeys / 16], vop[2][ND];
       float add0, add1;
+      uint64_t redo = 0;  // lanes whose weights left f16's range
       for (bool again = false;; again = true) {
         // Operands are read a step ahead of the matrix instructions that take them.
         f32x16 sc[2];
@@ -491,7 +503,10 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
         for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
         fence();
         if (!whole) {
-          const int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;  // of the lane's first key
+          // Of the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
+          // the scalar registers and every tile selects.)
+          int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;
+          asm volatile("" : "+v"(lo), "+v"(hi));
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -510,7 +525,9 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
           const float mine = fmaxf(m0 * cl0, m1 * cl1);
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
           const float was = ref;
-          ref = fmaxf(ref, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kRaise);
+          // (Rows that need none keep theirs: a row's result is its own.)
+          if ((redo | redo >> 32) >> col & 1)
+            ref = fmaxf(ref, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kRaise);
           const float keep = __builtin_amdgcn_exp2f(was - ref);
           sum *= keep;
 #pragma unroll
@@ -530,7 +547,8 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
             float& add = u ? add1 : add0;
             add = F16::dot2(pw[k][x], 0x3c003c00u, add);
           }
-        if (again || !__any(!(fmaxf(add0, add1) < kMost))) break;
+        redo = __ballot(!(add0 < kMost && add1 < kMost));
+        if (again || !redo) break;
       }
       sum += scaled(add0, -d0) + scaled(add1, -d1);
       fence();

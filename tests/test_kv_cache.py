@@ -686,6 +686,42 @@ def test_value_ranges(device, dtype, k_size, v_size):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("q", [1, 40])
+@pytest.mark.parametrize("n,sizes", [
+    (20, (1e-8, 1e-8, 1e-8, 1e-8)),     # less than a tile
+    (64, (1e-6, 1e4, 1e4, 1e4)), (64, (1e4, 1e-6, 1e-6, 1e-6)), (130, (1e-3, 1.0, 1e3, 1e-3)),
+    (100, (0.0, 1.0, 1.0, 0.0)), (40, (0.0, 0.0, 0.0, 0.0)), (140, (1.0, 1e-30, 1e30, 0.0))])
+def test_value_sizes_apart(device, q, n, sizes):
+    """Runs of 16 keys whose values' sizes differ, zeros among them: weights of
+    tiny or zero values still count in the sum."""
+    rng = np.random.default_rng(n)
+    b = Batch(rng, device, "bf16", 128, 64, 16, 1, 4, [q], [n])
+    j = np.arange(n)
+    x = rng.standard_normal((n, 1, 128)) * np.array(sizes)[j // 16 % 4][:, None, None]
+    parts = quantize(from_bits(to_bits(x.astype(np.float32), "bf16"), "bf16").astype(np.float32), 64, "bf16")
+    kx = _rows(rng, n, 1, 128, "bf16", 0.8)[1]
+    keys = quantize(kx, 64, "bf16")
+    b.host.put(b.table[0][j // 16] * 16 + j % 16, keys, parts)
+    b.k[0], b.v[0] = dequantize(*keys, 64, "bf16"), dequantize(*parts, 64, "bf16")
+    want, bound = b.expect(causal=False)
+    got = from_bits(b.run(causal=False), "bf16").astype(np.float64)
+    largest = np.abs(b.v[0]).max()
+    assert (np.abs(got - want) <= 2.0 ** -9 * 1.02 * np.abs(want) + bound + 2.0 ** -18 * largest).all()
+
+
+@pytest.mark.gpu
+def test_many_sequences(device):
+    """More sequences than a wave has lanes, lengths of zero among them, one and
+    several queries each."""
+    rng = np.random.default_rng(11)
+    kv = rng.integers(0, 90, 150)
+    kv[::17] = 0
+    for q in (np.minimum(kv, 1), np.minimum(kv, rng.integers(0, 30, 150))):
+        b = Batch(rng, device, "bf16", 64, 32, 16, 2, 3, q.tolist(), kv.tolist())
+        b.check(b.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q", [1, 40])
 def test_masked_poison(device, q):
     """Inf and NaN keys and values that no row may see: future tokens, tokens
     outside the window, what a block holds past the sequence's end."""
