@@ -37,6 +37,13 @@ constexpr int kWaves = 4;
 constexpr int kStages = 2;  // of a wave's ring
 constexpr int kTile = 32;
 constexpr int kMaxParts = 256;
+// Least tiles of a part (two a wave), and most that are one part all the same where
+// parts are that small: a join costs 3 us, a wave's tile 1.1 us while its SIMD has
+// no other.  (One request
+// of 4001 tokens, 8 heads: 12.6 us at two tiles a wave, 14.4 at four; one of 391
+// tokens, 2 heads: 11.4 us as one part, 13.1 as two.)
+constexpr int kPartTiles = 2 * kWaves, kWholeTiles = 3 * kPartTiles;
+constexpr size_t kScanSeqs = 128;
 constexpr float kSlack = 8.f;  // log2 of how far a weight may pass 1
 
 template <int D, int GS>
@@ -65,10 +72,11 @@ struct DecodeArgs {
   cpq_kv_attention_args a;
   int rows_max;    // sequences of more rows are another kernel's
   int target;      // workgroups to divide the tiles over
-  int part_tiles;  // least tiles of a part
   int report;      // this launch counts what is wrong with the sequences
+  int joined;      // the parts are joined by kv_join_kernel, not by the last to arrive
   unsigned int* counters;  // per (sequence, head)
   float* partial;          // [workgroup][rows_max][D + 4]: rows, then maximum and sum
+  int* starts;             // of many sequences: [n_seqs + 1] first workgroups, else null
   unsigned int* bad;
 };
 
@@ -328,32 +336,66 @@ struct Item {
   KvSeq q;
 };
 
-
 __device__ __forceinline__ int tiles_of(const KvSeq& q) {
   return (max(q.n - (q.lo & ~(kTile - 1)), 0) + kTile - 1) / kTile;
+}
+// Sequence s and its tiles that this kernel takes.
+__device__ __forceinline__ int seq_tiles(const DecodeArgs& p, int s, int group, int bs_shift, bool report, KvSeq& q) {
+  if (s >= (int)p.a.n_seqs) return 0;
+  q = kv_seq(p.a, s, bs_shift, report, p.bad);
+  const int rows = q.n_q * group;
+  return rows == 0 || rows > p.rows_max ? 0 : max(tiles_of(q), 1);  // no keys: zeros to store
+}
+// Tiles of a part, by those of all sequences; parts of a sequence.
+__device__ __forceinline__ int part_of(const DecodeArgs& p, int total) {
+  return max(kPartTiles, p.target ? (int)(((long)total * (int)p.c.n_kv_heads + p.target - 1) / p.target) : 0x3fffffff);
+}
+__device__ __forceinline__ int parts_of(int own, int per) {
+  return per == kPartTiles && own <= kWholeTiles ? min(own, 1) : min((own + per - 1) / per, kMaxParts);
+}
+// The item of workgroup b where kv_starts_kernel has run: two steps of a search
+// 64 wide (more past 4096 sequences).
+__device__ __forceinline__ bool look_up(const DecodeArgs& p, int b, int group, int bs_shift, Item& it) {
+  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, lane = threadIdx.x & 63;
+  if (b >= p.starts[n_seqs]) return false;
+  int lo = 0, hi = n_seqs;  // starts[lo] <= b < starts[hi]
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = min(lo + lane * step, hi);
+    const int k = (int)__builtin_popcountll(__ballot(p.starts[at] <= b)) - 1;  // lane 0's is
+    lo = min(lo + k * step, hi - 1);
+    hi = min(lo + step, hi);
+  }
+  const int first = __builtin_amdgcn_readfirstlane(p.starts[lo]), k = b - first;
+  const KvSeq q = kv_seq(p.a, lo, bs_shift, false, p.bad);
+  it.s = lo;
+  it.parts = (__builtin_amdgcn_readfirstlane(p.starts[lo + 1]) - first) / heads;
+  it.head = k % heads;
+  it.part = k / heads;
+  it.first = first + it.head;
+  it.q.rows0 = __builtin_amdgcn_readfirstlane(q.rows0);
+  it.q.n_q = __builtin_amdgcn_readfirstlane(q.n_q);
+  it.q.n = __builtin_amdgcn_readfirstlane(q.n);
+  it.q.lo = __builtin_amdgcn_readfirstlane(q.lo);
+  it.q.pos = it.q.n - it.q.n_q;
+  return true;
 }
 // The tiles of all sequences divided evenly: workgroup b's item, if any.  Every
 // wave goes over the sequences, 64 at a time: their tiles, the size of a part
 // from the sum of all, the sequence whose parts workgroup b falls among.
 __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group, int bs_shift, Item& it) {
   const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, lane = threadIdx.x & 63;
+  if (p.starts) return look_up(p, b, group, bs_shift, it);
   KvSeq q{};
-  auto work = [&](int s, bool report) {
-    if (s >= n_seqs) return 0;
-    q = kv_seq(p.a, s, bs_shift, report, p.bad);
-    const int rows = q.n_q * group;
-    return rows == 0 || rows > p.rows_max ? 0 : max(tiles_of(q), 1);  // no keys: zeros to store
-  };
   int total = 0, own = 0;
   for (int base = 0; base < n_seqs; base += 64) {
-    own = work(base + lane, p.report && b == 0 && threadIdx.x < 64);
+    own = seq_tiles(p, base + lane, group, bs_shift, p.report && b == 0 && threadIdx.x < 64, q);
     total += __builtin_amdgcn_readlane(wave_scan(own), 63);
   }
-  const int per = max(p.part_tiles, p.target ? (int)(((long)total * heads + p.target - 1) / p.target) : 0x3fffffff);
+  const int per = part_of(p, total);
   int before = 0;
   for (int base = 0; base < n_seqs; base += 64) {
-    if (n_seqs > 64) own = work(base + lane, false);
-    const int parts = min((own + per - 1) / per, kMaxParts);
+    if (n_seqs > 64) own = seq_tiles(p, base + lane, group, bs_shift, false, q);
+    const int parts = parts_of(own, per);
     const int sum = wave_scan(parts * heads), at = before + sum - parts * heads;
     before += __builtin_amdgcn_readlane(sum, 63);
     if (b < before) {
@@ -373,6 +415,42 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
     }
   }
   return false;
+}
+
+// Each sequence's first workgroup.
+constexpr int kStartsThreads = 1024;
+__global__ __launch_bounds__(kStartsThreads) void kv_starts_kernel(DecodeArgs p) {
+  __shared__ int waves[kStartsThreads / 64];
+  const int n_seqs = (int)p.a.n_seqs, heads = (int)p.c.n_kv_heads, group = (int)p.a.n_heads / heads;
+  const int tid = threadIdx.x, lane = tid & 63, bs_shift = 31 - __builtin_clz(p.c.block_size);
+  KvSeq q{};
+  auto sum_all = [&](int v, int& before) {  // over the workgroup; before: over earlier threads
+    const int sum = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) waves[tid >> 6] = sum;
+    __syncthreads();
+    int all = 0;
+    before = sum - v;
+#pragma unroll
+    for (int w = 0; w < kStartsThreads / 64; ++w) {
+      if (w < tid >> 6) before += waves[w];
+      all += waves[w];
+    }
+    return all;
+  };
+  int total = 0, own = 0, before = 0, at = 0;
+  for (int base = 0; base < n_seqs; base += kStartsThreads) {
+    own = seq_tiles(p, base + tid, group, bs_shift, p.report, q);
+    total += sum_all(own, before);
+  }
+  const int per = part_of(p, total);
+  for (int base = 0; base < n_seqs; base += kStartsThreads) {
+    if (n_seqs > kStartsThreads) own = seq_tiles(p, base + tid, group, bs_shift, false, q);
+    const int all = sum_all(parts_of(own, per) * heads, before);
+    if (base + tid < n_seqs) p.starts[base + tid] = at + before;
+    at += all;
+  }
+  if (tid == 0) p.starts[n_seqs] = at;
 }
 
 template <typename TT, int D, int GS, int NC>
@@ -547,11 +625,11 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
       if (d == 0) park_store(park, (r * LD + D) * 4, f32x4{m, total, 0.f, 0.f});
     }
   }
-  if (parts == 1) return;
+  if (parts == 1 || p.joined) return;
 
-  // The last part to arrive joins them: the parts' weights first (a lane a
-  // part), then their rows, every (threads / vectors)-th part to a thread, eight
-  // loads in flight.
+  // The last part to arrive joins them: the parts' weights (a lane a part) and
+  // their rows, every (threads / vectors)-th part to a thread, eight loads in
+  // flight, the first of them while the weights are made.
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
   unsigned int* counter = p.counters + (it.s * (int)c.n_kv_heads + head);
@@ -563,6 +641,15 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   float* weight = lds;                   // [rows][parts]
   float* share = weight + rows * parts;  // [rows]: 1 / sum
   f32x4* acc_lds = reinterpret_cast<f32x4*>(lds + ((rows * parts + rows + 3) & ~3));
+  const int vectors = rows * (D / 4), each = max(kWaves * 64 / vectors, 1), items = vectors * each;
+  constexpr int U = 8;
+  f32x4 x[U];
+  auto fetch = [&](int e, int k) {
+    const int v = e % vectors, r = v / (D / 4), d = v % (D / 4) * 4;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = park_load(all, (min(k + u * each, parts - 1) * stride + r * LD + d) * 4);
+  };
+  fetch(min(tid, items - 1), min(tid, items - 1) / vectors);
   for (int r = wave; r < rows; r += kWaves) {
     float m = -FLT_MAX, total = 0.f;
     f32x4 ml[kMaxParts / 64];
@@ -586,17 +673,17 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     if (lane == 0) share[r] = total == 0.f ? 0.f : 1.f / total;
   }
   __syncthreads();
-  const int vectors = rows * (D / 4), each = max(kWaves * 64 / vectors, 1);
-  for (int e = tid; e < vectors * each; e += kWaves * 64) {
+  for (int e = tid; e < items; e += kWaves * 64) {
     const int k0 = e / vectors, v = e - k0 * vectors, r = v / (D / 4), d = v % (D / 4) * 4;
+    if (e != tid) fetch(e, k0);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int k = k0; k < parts; k += 8 * each) {
-      f32x4 x[8];
+    for (int k = k0;;) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = park_load(all, (min(k + u * each, parts - 1) * stride + r * LD + d) * 4);
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < U; ++u)
         if (k + u * each < parts) acc += x[u] * weight[r * parts + k + u * each];
+      k += U * each;
+      if (k >= parts) break;
+      fetch(e, k);
     }
     if (each == 1) put(r, d, acc, share[r]);
     else acc_lds[e] = acc;
@@ -612,6 +699,79 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// Joins the parts of few heads' long keys.  The last workgroup to arrive takes 8 us
+// to read 94 parts alone (one request of 60001 tokens, 8 heads, 4 rows of 128: 192 KB a
+// head; 33 us in all), 32 workgroups together 4.5 us with their launch (24 us in all).
+// At 15 parts the two come out even, at 31 it is 15 us to 13.  A workgroup joins 32
+// vectors of four dimensions, a thread every eighth part.
+constexpr size_t kJoinParts = 16;
+constexpr int kJoinVectors = 32, kJoinSlices = kWaves * 64 / kJoinVectors;
+template <typename TT, int D>
+__global__ __launch_bounds__(kWaves * 64) void kv_join_kernel(DecodeArgs p) {
+  constexpr int LD = D + 4, kRows = D < 128 ? 128 / D : 1, U = 16;  // rows of a workgroup
+  static_assert(kMaxParts <= 2 * U * kJoinSlices);
+  __shared__ float weight[kRows][kMaxParts];
+  __shared__ float share[kRows];
+  __shared__ f32x4 slices[kJoinSlices][kJoinVectors];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int heads = (int)p.c.n_kv_heads, group = (int)p.a.n_heads / heads, s = blockIdx.x / heads, head = blockIdx.x % heads;
+  KvSeq q{};
+  const int own = seq_tiles(p, lane, group, 31 - __builtin_clz(p.c.block_size), false, q);
+  const int per = part_of(p, __builtin_amdgcn_readlane(wave_scan(own), 63));
+  const int mine = parts_of(own, per), sum = wave_scan(mine * heads);
+  const int parts = __builtin_amdgcn_readlane(mine, s), first = __builtin_amdgcn_readlane(sum - mine * heads, s) + head;
+  const int rows = __builtin_amdgcn_readlane(q.n_q, s) * group, rows0 = __builtin_amdgcn_readlane(q.rows0, s);
+  const int v0 = blockIdx.y * kJoinVectors, r0 = v0 / (D / 4);
+  if (parts <= 1 || r0 >= rows) return;
+  const size_t slab = (size_t)p.rows_max * LD;
+  const float* all = p.partial + first * slab;
+  const int stride = (int)(slab * heads);
+  const int v = min(v0 + tid % kJoinVectors, rows * (D / 4) - 1), r = v / (D / 4), d = v % (D / 4) * 4;
+  f32x4 x[U];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      x[u] = *reinterpret_cast<const f32x4*>(all + (size_t)min(k + u * kJoinSlices, parts - 1) * stride + r * LD + d);
+  };
+  fetch(tid / kJoinVectors);
+  if (wave < kRows && r0 + wave < rows) {
+    float m = -FLT_MAX, total = 0.f;
+    f32x4 ml[kMaxParts / 64];
+#pragma unroll
+    for (int u = 0; u < kMaxParts / 64; ++u) {
+      ml[u] = *reinterpret_cast<const f32x4*>(all + (size_t)min(64 * u + lane, parts - 1) * stride + (r0 + wave) * LD + D);
+      m = fmaxf(m, ml[u][0]);
+    }
+    m = wave_max(m);
+#pragma unroll
+    for (int u = 0; u < kMaxParts / 64; ++u) {
+      const float w = 64 * u + lane < parts ? __builtin_amdgcn_exp2f(ml[u][0] - m) : 0.f;
+      weight[wave][64 * u + lane] = w;
+      total += ml[u][1] * w;
+    }
+    total = wave_sum(total);
+    if (lane == 0) share[wave] = total == 0.f ? 0.f : 1.f / total;
+  }
+  __syncthreads();
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k = tid / kJoinVectors; k < parts; k += U * kJoinSlices) {
+    if (k >= U * kJoinSlices) fetch(k);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u * kJoinSlices < parts) acc += x[u] * weight[r - r0][k + u * kJoinSlices];
+  }
+  slices[tid / kJoinVectors][tid % kJoinVectors] = acc;
+  __syncthreads();
+  if (tid >= kJoinVectors || v0 + tid >= rows * (D / 4)) return;
+#pragma unroll
+  for (int k = 1; k < kJoinSlices; ++k) acc += slices[k][tid];
+  const int qi = r / group, hh = head * group + r - qi * group;
+  uint16_t* out = static_cast<uint16_t*>(p.a.out) + (size_t)(rows0 + qi) * p.a.out_token_stride +
+                  (size_t)hh * p.a.out_head_stride + d;
+  acc *= share[r - r0];
+  *reinterpret_cast<u32x2*>(out) = u32x2{TT::pack2(acc[0], acc[1]), TT::pack2(acc[2], acc[3])};
+}
+
 template <typename TT, int D, int GS, int NC>
 hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
   const size_t ring = (size_t)kWaves * Geo<D, GS>::kWave;
@@ -625,6 +785,11 @@ hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
     if (raised != hipSuccess) return raised;
   }
   hipLaunchKernelGGL(kernel, dim3((uint32_t)grid), dim3(kWaves * 64), lds, s, p);
+  const hipError_t launched = hipGetLastError();
+  if (launched != hipSuccess || !p.joined) return launched;
+  const dim3 joins((uint32_t)(p.a.n_seqs * p.c.n_kv_heads),
+                   (uint32_t)((p.rows_max * (D / 4) + kJoinVectors - 1) / kJoinVectors));
+  hipLaunchKernelGGL((kv_join_kernel<TT, D>), joins, dim3(kWaves * 64), 0, s, p);
   return hipGetLastError();
 }
 
@@ -655,17 +820,31 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.report = report;
   const size_t pairs = a.n_seqs * c.n_kv_heads;
   const size_t slab = (size_t)p.rows_max * (c.head_dim + 4) * sizeof(float);
-  const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
+  const size_t left = ex.scratch_bytes > kWideCounterBytes ? ex.scratch_bytes - kWideCounterBytes : 0;
+  // Every wave goes over the sequences, 64 at a time; over many a kernel before does
+  // (up to 600 keys each: 700 sequences 67 us, 117 without; 100 sequences 18 and 16).
+  const size_t starts = a.n_seqs > kScanSeqs ? (a.n_seqs + 4) / 4 * 16 : 0;
+  const size_t room = left > starts ? (left - starts) / slab : 0;
   // As many parts as workgroups are resident; each (sequence, head) rounds its
   // own up, by half a part on average.
-  const size_t resident = (size_t)env_int("CPQ_KV_ROUNDS", c.head_dim == 256 || p.rows_max > 16 ? 2 : 3) * ex.cu_count;
+  const size_t resident = (size_t)(c.head_dim == 256 || p.rows_max > 16 ? 2 : 3) * ex.cu_count;
   size_t target = std::max(resident - std::min(resident, pairs / 2), resident / 4);
   if (pairs * sizeof(unsigned int) > kWideCounterBytes || room <= pairs) target = 0;
   else target = std::min(target, room - pairs);
   p.target = (int)target;
-  p.part_tiles = env_int("CPQ_KV_MIN", 4) * kWaves;
+  // Parts of a head, at most; many are joined by a kernel of its own.
+  const size_t most = std::min(target / pairs + 1, (a.max_kv + kTile - 1) / kTile / kPartTiles);
+  p.joined = a.n_seqs <= 64 && most >= kJoinParts;
   p.counters = static_cast<unsigned int*>(ex.scratch);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
+  char* rest = static_cast<char*>(ex.scratch) + kWideCounterBytes;
+  if (starts && left >= starts) {
+    p.starts = reinterpret_cast<int*>(rest);
+    rest += starts;
+    hipLaunchKernelGGL(kv_starts_kernel, dim3(1), dim3(kStartsThreads), 0, ex.stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  p.partial = reinterpret_cast<float*>(rest);
   const size_t grid = pairs + target;
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   if (p.rows_max <= 16) return bf16 ? launch_d<BF16, 1>(ex.stream, p, grid) : launch_d<F16, 1>(ex.stream, p, grid);

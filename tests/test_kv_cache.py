@@ -721,6 +721,34 @@ def test_many_sequences(device):
 
 
 @pytest.mark.gpu
+def test_many_sequences_some_long(device):
+    """Of 140 sequences two are split over workgroups."""
+    rng = np.random.default_rng(12)
+    kv = rng.integers(1, 40, 140)
+    kv[70], kv[139] = 3001, 1700
+    for q in (np.ones(140, int), np.minimum(kv, rng.integers(0, 4, 140))):
+        b = Batch(rng, device, "f16", 64, 64, 16, 1, 4, q.tolist(), kv.tolist())
+        first = b.run()
+        b.check(first)
+        assert np.array_equal(b.run(), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,gs,group,q,n", [("bf16", 64, 32, 7, 1, 9000), ("f16", 64, 64, 1, 3, 4200),
+                                                    ("bf16", 128, 64, 4, 1, 12345), ("f16", 128, 32, 2, 9, 6000),
+                                                    ("bf16", 256, 128, 1, 1, 5001), ("f16", 256, 64, 8, 4, 7000)])
+def test_one_long_sequence(device, dtype, dim, gs, group, q, n):
+    """More parts than one workgroup joins, beside a sequence of one part and one
+    without keys that any row sees."""
+    rng = np.random.default_rng(n)
+    b = Batch(rng, device, dtype, dim, gs, 32, 1, group, [q, q, 0], [n, q, 0])
+    first = b.run()
+    b.check(first)
+    assert np.array_equal(b.run(), first)
+    b.check(b.run(window=4500), window=4500)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("q", [1, 40])
 def test_masked_poison(device, q):
     """Inf and NaN keys and values that no row may see: future tokens, tokens
