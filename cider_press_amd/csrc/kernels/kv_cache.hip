@@ -5,8 +5,7 @@
 #include <cfloat>
 #include <type_traits>
 
-#include "../cpq_internal.hpp"
-#include "common.hpp"
+#include "kv_common.hpp"
 
 namespace cpq {
 namespace {
@@ -14,6 +13,8 @@ namespace {
 using namespace dev;
 
 constexpr int kPlanThreads = 1024;
+// Heads to a thread of the gather where that leaves enough workgroups.
+constexpr uint32_t kHeads = 4, kEnough = 1024;
 
 // ceil(n / block) bounded by a table row's blocks.
 __device__ __forceinline__ uint32_t blocks_of(uint64_t n, int bs_shift, uint32_t max_blocks) {
@@ -190,10 +191,36 @@ __device__ __forceinline__ float group_extreme(float v, int lanes) {
   return v;
 }
 
+// d / s correctly rounded, as IEEE division gives it, for d >= 0 and an s of at
+// most 11 significant bits, r within a unit of 1 / s: one step of the remainder,
+// which is exact in an fma.  It leaves 2^-45 of the quotient, and no quotient of 24
+// bits by 11 is nearer than 2^-36 to a value halfway between two floats (nor on
+// one).  In `plain` range, where no remainder falls below the normal numbers.  A
+// quarter of a division's instructions, which bound the append.
+__device__ __forceinline__ float quotient(float d, float s, float r) {
+  const float q = d * r;
+  return fmaf(fmaf(-q, s, d), r, q);
+}
+__device__ __forceinline__ bool plain(float v) { return v >= 0x1p-100f && v <= 0x1p100f; }
+
+// Of three, where none is a NaN that counts (the builtins quiet each first).
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float o;
+  asm("v_min3_f32 %0, %1, %2, %3" : "=v"(o) : "v"(a), "v"(b), "v"(c));
+  return o;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float o;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(o) : "v"(a), "v"(b), "v"(c));
+  return o;
+}
+
 // A workgroup takes consecutive tokens of one head, keys or values: thread =
 // one word (8 values) of one token, so a group is 4, 8 or 16 adjacent lanes
 // and the words of four tokens in adjacent slots, which the value layout
-// interleaves, come from one wave (head_dim 128).
+// interleaves, come from one wave (head_dim 128).  Bound by its instructions, 183 a
+// wave of 512 values: 8191 tokens of 8 heads of 128 in 14.5 us (3.0 TB/s; with
+// IEEE divisions 17.4).  Four heads to a thread, as in the gather: no faster.
 template <typename TT>
 __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const uint16_t* __restrict__ k,
                                                         size_t k_token, size_t k_head,
@@ -214,31 +241,41 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
   const uint16_t* src = values ? v + t * v_token + head * v_head : k + t * k_token + head * k_head;
   const u32x4 raw = *reinterpret_cast<const u32x4*>(src + wi * 8);
   float x[8];
-  bool finite = true;
+  uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = TT::lo(raw[i]);
     x[2 * i + 1] = TT::hi(raw[i]);
-    finite &= (raw[i] & kExpBits<TT>) != kExpBits<TT> && (raw[i] >> 16 & kExpBits<TT>) != kExpBits<TT>;
+    most = sizes(most, raw[i]);
   }
-  float lo = x[0], hi = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-  lo = group_extreme<false>(lo, lanes);
+  const bool finite = (most & 0xffff) < kExpBits<TT> && most >> 16 < kExpBits<TT>;
+  float lo = min3(min3(min3(x[0], x[1], x[2]), x[3], x[4]), min3(x[5], x[6], x[7]), x[0]);
+  float hi = max3(max3(max3(x[0], x[1], x[2]), x[3], x[4]), max3(x[5], x[6], x[7]), x[0]);
+  lo = group_extreme<false>(finite ? lo : 0.f, lanes);
   hi = group_extreme<true>(finite ? hi : INFINITY, lanes);  // not finite anywhere: no finite range
   const float span = hi - lo;
   const bool ok = span <= FLT_MAX;
-  const uint16_t s = ok ? TT::from_f32(span / 15.f) : 0;
+  // (Opaque: an fma and a conversion become one instruction of one rounding, where
+  // the definition rounds to float first.)
+  const float step = !Sig16<TT>::bf16 || plain(span) ? quotient(span, 15.f, 1.f / 15.f) : span / 15.f;
+  const uint16_t s = ok ? TT::from_f32(__uint_as_float(opaque(__float_as_uint(step)))) : 0;
   const uint16_t b = ok ? TT::from_f32(lo) : (uint16_t)(kExpBits<TT> | kExpBits<TT> >> 1);  // NaN
   const float sf = TT::to_f32(s);
   uint32_t word = 0;
-  if (ok && sf != 0.f) {
+  if (ok && sf != 0.f) {  // the quotient correctly rounded: ties as in the definition
+    float q[8];
+    if (!Sig16<TT>::bf16 || plain(sf)) {
+      const float r = __builtin_amdgcn_rcpf(sf);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)  // the quotient correctly rounded: ties as in the definition
-      word |= (uint32_t)fminf(fmaxf(rintf((x[i] - lo) / sf), 0.f), 15.f) << (4 * i);
+      for (int i = 0; i < 8; ++i) q[i] = quotient(x[i] - lo, sf, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[i] = (x[i] - lo) / sf;
+    }
+    float half[2] = {0.f, 0.f};  // four values each, exact
+#pragma unroll
+    for (int i = 7; i >= 0; --i) half[i >> 2] = fmaf(half[i >> 2], 16.f, rintf(fminf(q[i], 15.f)));
+    word = (uint32_t)half[0] | (uint32_t)half[1] << 16;
   }
   const uint32_t w = 1u << w_shift, g = w / lanes, gi = wi / lanes;
   const size_t row = ((size_t)block * c.n_kv_heads + head) * bs;
@@ -253,34 +290,54 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
   }
 }
 
-// The same split; thread = one word in, 16 bytes out.
-template <typename TT>
+// The same split, U heads to a thread (their loads in flight together, and what
+// neighbouring workgroups write lies together); a word in, 16 bytes out.  Bound by
+// HBM: 65536 rows of 8 heads of 128 in 67 us, 5.1 TB/s read and written (99 us with
+// one head to a thread, 91 with two, 69 with eight).  Few rows: one head to a
+// thread, or the launch fills a part of the chip.
+template <typename TT, int U>
 __global__ __launch_bounds__(256) void kv_gather_kernel(cpq_kv_cache c, const uint32_t* __restrict__ slots,
                                                         uint32_t n_rows, uint16_t* __restrict__ k_out,
                                                         uint16_t* __restrict__ v_out, int w_shift, int lanes,
                                                         unsigned int* bad) {
   const uint32_t wi = threadIdx.x & ((1u << w_shift) - 1), t = blockIdx.x * (256u >> w_shift) + (threadIdx.x >> w_shift);
-  const uint32_t head = blockIdx.y;
+  const uint32_t head0 = blockIdx.y * U, heads = c.n_kv_heads;
   const bool values = k_out ? blockIdx.z : true;
   if (t >= n_rows) return;
   const uint32_t slot = slots[t];
   const uint32_t bs = c.block_size, bs_shift = 31 - __builtin_clz(bs);
   const uint32_t block = slot >> bs_shift, off = slot & (bs - 1);
   const uint32_t w = 1u << w_shift, g = w / lanes, gi = wi / lanes;
-  u32x4 o = {0u, 0u, 0u, 0u};
-  if (block < c.n_blocks) {
-    const size_t row = ((size_t)block * c.n_kv_heads + head) * bs, quad = row + (off & ~3u);
-    const uint32_t word = values ? c.v_q[quad * w + wi * 4 + (off & 3)] : c.k_q[(row + off) * w + wi];
-    const uint32_t sb = values ? c.v_sb[quad * g + gi * 4 + (off & 3)] : c.k_sb[(row + off) * g + gi];
-    const float s = TT::lo(sb), b = TT::hi(sb);
+  uint16_t* out = (values ? v_out : k_out) + (((size_t)t * heads + head0) << (w_shift + 3)) + wi * 8;
+  if (block >= c.n_blocks) {
+    if (slot != CPQ_KV_NO_SLOT && wi == 0 && head0 == 0 && blockIdx.z == 0) atomicAdd(bad, 1u);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (head0 + u < heads) *reinterpret_cast<u32x4*>(out + ((size_t)u << (w_shift + 3))) = u32x4{0u, 0u, 0u, 0u};
+    return;
+  }
+  uint32_t word[U], sb[U];
+  const uint32_t* q = values ? c.v_q + wi * 4 + (off & 3) : c.k_q + wi;
+  const uint32_t* p = values ? c.v_sb + gi * 4 + (off & 3) : c.k_sb + gi;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t row = ((size_t)block * heads + min(head0 + u, heads - 1)) * bs + (values ? off & ~3u : off);
+    word[u] = q[row * w];
+    sb[u] = p[row * g];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const float s = TT::lo(sb[u]), b = TT::hi(sb[u]);
+    u32x4 o;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      o[i] = TT::pack2(fmaf(s, (float)(word >> (8 * i) & 15u), b), fmaf(s, (float)(word >> (8 * i + 4) & 15u), b));
-  } else if (slot != CPQ_KV_NO_SLOT && wi == 0 && head == 0 && blockIdx.z == 0) {
-    atomicAdd(bad, 1u);
+      o[i] = TT::pack2(fmaf(s, (float)(word[u] >> (8 * i) & 15u), b), fmaf(s, (float)(word[u] >> (8 * i + 4) & 15u), b));
+    u32x4* dst = reinterpret_cast<u32x4*>(out + ((size_t)u << (w_shift + 3)));
+    if (head0 + u < heads) {
+      if (U > 1) __builtin_nontemporal_store(o, dst);  // more than the caches keep
+      else *dst = o;
+    }
   }
-  uint16_t* out = values ? v_out : k_out;
-  *reinterpret_cast<u32x4*>(out + (((size_t)t * c.n_kv_heads + head) << (w_shift + 3)) + wi * 8) = o;
 }
 
 int log2_of(uint32_t v) { return 31 - __builtin_clz(v); }
@@ -332,13 +389,16 @@ hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k,
 hipError_t launch_kv_gather(hipStream_t s, const cpq_kv_cache& c, const uint32_t* slots, uint32_t n_rows, void* k_out,
                             void* v_out, unsigned int* bad) {
   const int w_shift = log2_of(c.head_dim / 8), lanes = (int)c.group_size / 8;
-  const dim3 grid((n_rows + (256u >> w_shift) - 1) / (256u >> w_shift), c.n_kv_heads, k_out && v_out ? 2 : 1);
+  const uint32_t blocks = (n_rows + (256u >> w_shift) - 1) / (256u >> w_shift), sides = k_out && v_out ? 2 : 1;
+  const bool wide = (size_t)blocks * ((c.n_kv_heads + kHeads - 1) / kHeads) * sides >= kEnough;
+  const dim3 grid(blocks, wide ? (c.n_kv_heads + kHeads - 1) / kHeads : c.n_kv_heads, sides);
   auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, c, slots, n_rows, static_cast<uint16_t*>(k_out),
                        static_cast<uint16_t*>(v_out), w_shift, lanes, bad);
     return hipGetLastError();
   };
-  return c.dtype == CPQ_DTYPE_BF16 ? run(kv_gather_kernel<BF16>) : run(kv_gather_kernel<F16>);
+  if (wide) return c.dtype == CPQ_DTYPE_BF16 ? run(kv_gather_kernel<BF16, kHeads>) : run(kv_gather_kernel<F16, kHeads>);
+  return c.dtype == CPQ_DTYPE_BF16 ? run(kv_gather_kernel<BF16, 1>) : run(kv_gather_kernel<F16, 1>);
 }
 
 }  // namespace cpq

@@ -488,9 +488,9 @@ cpq_status cpq_kv_plan(cpq_commands* cmds, const uint32_t* lens, const uint32_t*
 
 /* Quantizes n_tokens keys and values (T, [n_tokens, n_kv_heads, head_dim] at
  * the given token and head strides in elements, both multiples of 8; 16-byte
- * aligned) into their slots.  Per group: bias = its lowest value, scale =
- * RNE_T((highest - lowest) / 15), q = clamp(rint((x - bias) / scale), 0, 15)
- * in fp32, 0 where the scale is 0.  A group that holds an Inf or NaN, or whose
+ * aligned) into their slots.  Per group, with the arithmetic in fp32: bias = its
+ * lowest value (-0 lies below 0), scale = RNE_T((highest - lowest) / 15), q =
+ * clamp(rint((x - bias) / scale), 0, 15), 0 where the scale is 0.  A group that holds an Inf or NaN, or whose
  * range overflows, is stored as q = 0, scale = 0, bias = NaN.  Slots that are
  * none are skipped; slots past the cache are skipped and reported by the next
  * wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one slot: either wins, word

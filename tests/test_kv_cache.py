@@ -303,6 +303,7 @@ def quantize(x, gs, dtype):
     g = x.astype(np.float32).reshape(*x.shape[:2], x.shape[2] // gs, gs)
     with np.errstate(all="ignore"):
         lo, hi = g.min(-1), g.max(-1)
+        lo = np.where((lo == 0) & np.signbit(g).any(-1), np.float32(-0.0), lo)  # -0 lies below 0
         span = (hi - lo).astype(np.float32)
         ok = np.isfinite(span) & np.isfinite(g).all(-1)
         s = np.where(ok, to_bits((np.where(ok, span, 0) / np.float32(15)).astype(np.float32), dtype), 0)
@@ -460,6 +461,33 @@ def test_append_special_values(device, dtype):
         assert np.array_equal(np.isnan(got), np.isnan(ref))
         assert np.array_equal(got[~np.isnan(got)], ref[~np.isnan(ref)])
     assert np.isnan(want[1, 0, 32:64]).all() and np.isfinite(want[1, 0, 64:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,low,high", [("bf16", -132, 122), ("f16", -22, 10)])
+def test_append_near_halves(device, dtype, low, high):
+    """Values next to half steps, over the type's whole range: bit for bit."""
+    dim, gs, bs, n = 128, 32, 64, 2048
+    rng = np.random.default_rng(17)
+    span = np.exp2(rng.uniform(low, high, (n, dim // gs, 1)))
+    base = rng.choice([0.0, 1.0, -1.0, -0.3], (n, dim // gs, 1)) * span * rng.choice([1, 0.01], (n, dim // gs, 1))
+    step = rng.integers(0, 31, (n, dim // gs, gs)) / 30.0
+    step[..., 0], step[..., 5] = 0.0, 1.0
+    bits = to_bits((base + span * step).astype(np.float32).reshape(n, 1, dim), dtype)
+    near = bits.astype(np.int64) + rng.integers(-1, 2, bits.shape)  # a unit of T off
+    bits = np.where((bits & 0x7FFF) > 0, near, bits).astype(np.uint16)
+    x = from_bits(bits, dtype).astype(np.float32)
+    assert np.isfinite(x).all()
+    host = Host(rng, dtype, n // bs, bs, 1, dim, gs)
+    cache = host.upload(device)
+    X, S = device.upload(bits.reshape(-1), dtype), device.upload(np.arange(n, dtype=np.uint32), "u32")
+    cmds = device.commands()
+    kkv.kv_append(cmds, cache, X, X, S, n)
+    cmds.commit_and_wait()
+    want = quantize(x, gs, dtype)
+    host.put(np.arange(n), want, want)
+    for name, w in zip(("k_q", "k_sb", "v_q", "v_sb"), host.arrays()):
+        assert np.array_equal(getattr(cache, name).to_numpy().reshape(w.shape), w), name
 
 
 @pytest.mark.gpu
