@@ -2,8 +2,7 @@
 // cpq_kv_attention in cpq.h): the kernel for many query rows per sequence, and
 // the choice between it and kv_decode.hip.
 //
-// A workgroup of eight waves (four at head_dim 256, whose rows take twice the
-// registers) takes 32 query rows a wave of one key/value head (rows run over the
+// A workgroup takes 32 query rows a wave of one key/value head (rows run over the
 // queries, then the heads of the group, so a group of any size shares the keys)
 // and walks tiles of 64 keys:
 //   S^T = K Q^T     v_mfma_f32_32x32x16_f16, A = 32 keys, B = 32 query rows
@@ -11,22 +10,35 @@
 //                   S^T's result layout holds as B takes them: lane (row n, h)
 //                   has keys 8 x + 4 h + 0 .. 3, so a k step's 16 keys are
 //                   {4 h .. 4 h + 3, 8 + 4 h ..} of either operand.
-// Keys and values become f16 operands once per workgroup (kv_common.hpp): two
-// waves dequantize the next tile's keys and two its values into the other half
-// of LDS, of eight waves the two halves in turn, so that on each SIMD one wave's
-// dequantization meets the other's matrix instructions; one barrier a tile.  The
-// packed words of the next tile of the same four waves are in flight meanwhile.
+// Keys and values become f16 operands in LDS once per workgroup (kv_common.hpp).  Of
+// four waves two dequantize a tile's keys and two its values.  At head_dim 128 a
+// workgroup has two such teams: each stages every second tile, one team before and
+// one between the products of two tiles, into the other half of four tiles of LDS,
+// so that on each SIMD one wave's dequantization meets the other's matrix
+// instructions; one barrier every two tiles.  At head_dim 256 (the rows take twice
+// the registers) and 64 (three workgroups share a CU) it has one team, two tiles of
+// LDS and a barrier every tile.  The packed words of a team's next tile are in
+// flight meanwhile.  (4096 queries of 32 heads over 8192 keys of 8: head_dim 128 429
+// us, 462 with a barrier every tile, 607 with four waves a workgroup; head_dim 64
+// 337 us, 429 with eight.)
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
 //   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
 //   a key that repeats among them doubles it).
 // No maximum is taken on the way: weights are 2^(score - reference), and only
 // where their sums show that one leaves f16's range (the first tile's do) is the
-// tile's maximum found, the reference raised to 2^-6 of it and the tile's scores
-// computed again.
+// maximum of the half tile found, the reference raised to 2^-6 of it and its weights
+// made again.  The weights of a tile's first 32 keys are made between the matrix
+// instructions of the other 32 keys' scores, theirs between those of the first
+// keys' values (head_dim 64 350 -> 337 us, 256 411 -> 354).
 //
-// Where there are few row tiles their keys are split, evenly over the workgroups
-// by the lengths on the device, and joined, in part order, by the last to arrive.
+// Bound by its instructions: 4096 queries over 8192 keys at head_dim 128 run at 960
+// TFLOP/s (a large f16 product of the library: 1322), with the matrix pipes busy for
+// 41% and the vector pipes for 46% of the cycles.
+//
+// Where there are few row tiles their keys are split, evenly over the resident
+// workgroups by the lengths on the device, and joined, in part order, by the last
+// to arrive.
 #include <algorithm>
 
 #include "kv_common.hpp"
@@ -39,7 +51,7 @@ using namespace dev;
 constexpr int kKeys = 64;        // of a tile
 constexpr int kMinTiles = 4;     // of a part
 template <int D>
-constexpr int kWaves = D == 256 ? 4 : 8;
+constexpr int kWaves = D == 128 ? 8 : 4;
 constexpr float kRaise = 6.f;     // log2 of the largest weight when the reference is set
 constexpr float kMost = 32768.f;  // of 16 weights' sum, so that each fits f16
 // What a wave publishes of its half of a tile: the exponent (0: all constants so
@@ -249,16 +261,20 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
     key_tiles = (reach + kKeys - 1) / kKeys;
   };
   long total = 0;
+  int items = 0;
   if (p.target || p.report) {
     for (int base = 0; base < n_seqs; base += 64) {
       work(base + lane, p.report && b == 0 && threadIdx.x < 64);
       long sum = (long)row_tiles * key_tiles;
+      items += __builtin_amdgcn_readlane(wave_scan(row_tiles * heads), 63);
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
       total += sum;
     }
   }
-  const long per = p.target ? max((total * heads + p.target - 1) / p.target, (long)kMinTiles) : 1l << 40;
+  // (Each row tile rounds its parts up, by half a part on average.)
+  const int target = max(p.target - items / 2, p.target / 4);
+  const long per = p.target ? max((total * heads + target - 1) / target, (long)kMinTiles) : 1l << 40;
   int before = 0;
   for (int base = 0; base < n_seqs; base += 64) {
     work(base + lane, false);
@@ -285,10 +301,11 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
 }
 
 template <typename TT, int D>
-__global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kernel(TileArgs p) {
+__global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
-  extern __shared__ u32x4 units[];  // [2][keys, values][kUnits]
-  __shared__ int meta[2][4];         // of the halves' keys, then their values
+  constexpr int kTeams = kWaves<D> / 4, kBufs = 2 * kTeams;
+  extern __shared__ u32x4 units[];  // [kBufs][keys, values][kUnits]
+  __shared__ int meta[kBufs][4];         // of the halves' keys, then their values
   __shared__ unsigned int arrived;
   constexpr int kRows = 32 * kWaves<D>;
   const cpq_kv_cache& c = p.c;
@@ -354,11 +371,10 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   float cl0 = 0.f, cl1 = 0.f;          // of the halves: log2(e) * scale * 2^(exponents of q and the keys)
   int d0 = 0, d1 = 0;                  // and the values' exponents less ev
 
-  // Staging: of each four waves 0, 1 keys and 2, 3 values of the tile's halves.
+  // Staging: of each four waves two keys and two values of the tile's halves.
   const uint32_t* __restrict__ blocks = a.block_table + (size_t)it.s * a.max_blocks;
-  constexpr int kTeams = kWaves<D> / 4;
   const int team = wave >> 2;
-  const bool is_values = wave & 2;
+  const bool is_values = ((wave >> 1) ^ team) & 1;  // on each SIMD one wave of either kind
   const int half = wave & 1;
   Range range;
   Packed<D> packed;
@@ -408,7 +424,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
       store_keys<TT, D>(packed, keys, 32 * half, lane, range, live);
     }
     if (lane == 0)
-      meta[buf][wave & 3] = (range.limits ? range.e + kExpBias : 0) + (loaded_ok << kOkShift) + (poison ? kPoison : 0);
+      meta[buf][2 * is_values + half] = (range.limits ? range.e + kExpBias : 0) + (loaded_ok << kOkShift) + (poison ? kPoison : 0);
   };
 
   // Byte offsets of the lane's operands in LDS; the half of LDS in turn is the
@@ -428,15 +444,15 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
   };
 
   if (begin + team < stop) load(begin + team, false);
-  if (team == 0 && begin < stop) {
-    store(begin, 0);
-    if (begin + kTeams < stop) load(begin + kTeams, false);
+  if (begin + team < stop) {
+    store(begin + team, team);
+    if (begin + team + kTeams < stop) load(begin + team + kTeams, false);
   }
   __syncthreads();
   int known = -1, ok = 0;  // the published words that cl, d and ok are of
   bool poison = false;
   for (int t = begin; t < stop; ++t) {
-    const int buf = (t - begin) & 1;
+    const int buf = (t - begin) & (kBufs - 1);
     int news = meta[buf][lane & 3];
     if (__any(news != known)) {
       auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
@@ -471,58 +487,48 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
         ev = e;
       }
     }
-    if (t + 1 < stop && (t + 1 - begin) % kTeams == team) {
-      store(t + 1, buf ^ 1);
-      if (t + 1 + kTeams < stop) load(t + 1 + kTeams, false);
+    if (t + kTeams < stop && (t - begin) % kTeams == team) {
+      store(t + kTeams, (t + kTeams - begin) & (kBufs - 1));
+      if (t + 2 * kTeams < stop) load(t + 2 * kTeams, false);
     }
     const int key0 = t * kKeys;
     if (key0 < any_to && key0 + kKeys > any_from) {
       const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
-      u32x4 pw[kKeys / 16], vop[2][ND];
-      float add0, add1;
-      uint64_t redo = 0;  // lanes whose weights left f16's range
-      for (bool again = false;; again = true) {
-        // Operands are read a step ahead of the matrix instructions that take them.
-        f32x16 sc[2];
-        u32x4 op[2][NS];
+      // Operands are read a step ahead of the matrix instructions that take them, and
+      // the weights of one half of the keys are made between those of the other.
+      f32x16 sc[2];
+      constexpr int kAhead = 4;
+      u32x4 op[kAhead], pw[kKeys / 16], vop[2][ND];
+      float add[2] = {0.f, 0.f};
+      auto mask = [&](int u) {
+        if (whole) return;
+        // Of the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
+        // the scalar registers and every tile selects.)
+        int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;
+        asm volatile("" : "+v"(lo), "+v"(hi));
 #pragma unroll
-        for (int i = 0; i < NS; ++i) op[0][i] = key_operand(0, i);
-        fence();
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int x = 0; x < 16; ++x) sc[u][x] = 0.f;
-#pragma unroll
-          for (int i = 0; i < NS; ++i) {
-            if (u == 0) op[1][i] = key_operand(1, i);
-            sc[u] = mma(op[u][i], qs[i], sc[u]);
-            fence();
-          }
+        for (int x = 0; x < 16; ++x) {
+          const int k = 32 * u + 8 * (x >> 2) + (x & 3);
+          sc[u][x] = k >= lo && k < hi && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
         }
+      };
+      auto weights = [&](int u, float rel, int i) {  // two of a half's
+        const float cl = u ? cl1 : cl0;
+        const uint32_t w = F16::pack2(__builtin_amdgcn_exp2f(fmaf(sc[u][2 * i], cl, rel)),
+                                      __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i + 1], cl, rel)));
+        pw[2 * u + (i >> 2)][i & 3] = w;
+        // The sum is of the rounded weights, two at a time.
+        add[u] = F16::dot2(w, 0x3c003c00u, add[u]);
+      };
+      // Where a weight of half u left f16's range: a new reference, the weights again.
+      auto settle = [&](int u) {
+        const uint64_t redo = __ballot(!(add[u] < kMost));
+        if (redo) {
+          const float cl = u ? cl1 : cl0;
+          float mine = sc[u][0];
 #pragma unroll
-        for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
-        fence();
-        if (!whole) {
-          // Of the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
-          // the scalar registers and every tile selects.)
-          int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;
-          asm volatile("" : "+v"(lo), "+v"(hi));
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) {
-              const int k = 32 * u + 8 * (x >> 2) + (x & 3);
-              sc[u][x] = k >= lo && k < hi && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
-            }
-        }
-        if (again) {
-          float m0 = sc[0][0], m1 = sc[1][0];
-#pragma unroll
-          for (int x = 1; x < 16; ++x) {
-            m0 = fmaxf(m0, sc[0][x]);
-            m1 = fmaxf(m1, sc[1][x]);
-          }
-          const float mine = fmaxf(m0 * cl0, m1 * cl1);
+          for (int x = 1; x < 16; ++x) mine = fmaxf(mine, sc[u][x]);
+          mine *= cl;
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
           const float was = ref;
           // (Rows that need none keep theirs: a row's result is its own.)
@@ -532,34 +538,56 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
           sum *= keep;
 #pragma unroll
           for (int j = 0; j < ND; ++j) o[j] *= keep;
+          add[u] = 0.f;
+          const float rel = (float)(u ? d1 : d0) - ref;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) weights(u, rel, i);
         }
-        const float r0 = ref - (float)d0, r1 = ref - (float)d1;
-        add0 = add1 = 0.f;
+        sum += scaled(add[u], u ? -d1 : -d0);
+      };
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int u = k >> 1, at = 8 * (k & 1) + 2 * x;
-            const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][at], u ? cl1 : cl0, u ? -r1 : -r0));
-            const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][at + 1], u ? cl1 : cl0, u ? -r1 : -r0));
-            pw[k][x] = F16::pack2(w0, w1);
-            // The sum is of the rounded weights, two at a time.
-            float& add = u ? add1 : add0;
-            add = F16::dot2(pw[k][x], 0x3c003c00u, add);
-          }
-        redo = __ballot(!(add0 < kMost && add1 < kMost));
-        if (again || !redo) break;
-      }
-      sum += scaled(add0, -d0) + scaled(add1, -d1);
+      for (int i = 0; i < kAhead; ++i) op[i] = key_operand(i / NS, i % NS);
       fence();
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k)
+      for (int x = 0; x < 16; ++x) sc[0][x] = sc[1][x] = 0.f;
+      auto score = [&](int i) {
+        sc[i / NS] = mma(op[i % kAhead], qs[i % NS], sc[i / NS]);
+        if (i + kAhead < 2 * NS) op[i % kAhead] = key_operand((i + kAhead) / NS, (i + kAhead) % NS);
+      };
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        score(i);
+        fence();
+      }
+#pragma unroll
+      for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
+      fence();
+      mask(0);
+      const float rel0 = (float)d0 - ref;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        score(NS + i);
+#pragma unroll
+        for (int x = i * 8 / NS; x < (i + 1) * 8 / NS; ++x) weights(0, rel0, x);
+        fence();
+      }
+      settle(0);
+      mask(1);
+      const float rel1 = (float)d1 - ref;
+#pragma unroll
+      for (int k = 0; k < kKeys / 16; ++k) {
+        if (k == 2) settle(1);
 #pragma unroll
         for (int j = 0; j < ND; ++j) {
           if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = value_operand(j, k + 1);
           o[j] = mma(vop[k & 1][j], pw[k], o[j]);
+          if (k < 2) {
+#pragma unroll
+            for (int x = (k * ND + j) * 4 / ND; x < (k * ND + j + 1) * 4 / ND; ++x) weights(1, rel1, x);
+          }
           fence();
         }
+      }
       if (poison) {
 #pragma clang loop unroll(disable)
         for (int k = 0; k < kKeys && key0 + k < q.n; k += 16)
@@ -567,11 +595,12 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
                                             key0 + k, W >> gw_shift, see_from, see_to);
       }
     }
+    const uint32_t next = kTeams > 1 && (t - begin) % kTeams ? 3 * kHalf : kHalf;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) at_key[i] ^= kHalf;
+    for (int i = 0; i < NS; ++i) at_key[i] ^= next;
 #pragma unroll
-    for (int k = 0; k < kKeys / 16; ++k) at_value[k] ^= kHalf;
-    __syncthreads();
+    for (int k = 0; k < kKeys / 16; ++k) at_value[k] ^= next;
+    if ((t + 1 - begin) % kTeams == 0) __syncthreads();
   }
 
   {
@@ -618,18 +647,25 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
     for (int j = 0; j < ND; ++j)
 #pragma unroll
       for (int x = 0; x < 16; ++x) o[j][x] = 0.f;
-    for (int k = 0; k < joined; ++k) {
-      const f32x4 ml = get(k, D / 8);
-      const float w = __builtin_amdgcn_exp2f(ml[0] - m);
-      sum += ml[1] * w;
+    constexpr int U = D == 256 ? 1 : 2;  // parts whose rows are under way together
+    for (int k = 0; k < joined; k += U) {
+      f32x4 v[U][D / 8], ml[U];
 #pragma unroll
-      for (int j = 0; j < ND; ++j)
+      for (int u = 0; u < U; ++u) {
+        ml[u] = get(min(k + u, joined - 1), D / 8);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const f32x4 v = get(k, 4 * j + x);
+        for (int x = 0; x < D / 8; ++x) v[u][x] = get(min(k + u, joined - 1), x);
+      }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][4 * x + e] += v[e] * w;
-        }
+      for (int u = 0; u < U; ++u) {
+        if (k + u >= joined) break;
+        const float w = __builtin_amdgcn_exp2f(ml[u][0] - m);
+        sum += ml[u][1] * w;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[x >> 2][4 * (x & 3) + e] += v[u][x][e] * w;
+      }
     }
     if (tid == 0) __hip_atomic_store(&p.counters[first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
@@ -646,7 +682,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : 2) void kv_tile_kern
 
 template <typename TT, int D>
 hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
-  const size_t lds = (size_t)2 * 2 * kKeys * (D / 8) * 16;
+  const size_t lds = (size_t)(kWaves<D> / 2) * 2 * kKeys * (D / 8) * 16;
   auto kernel = kv_tile_kernel<TT, D>;
   static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -674,12 +710,13 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
   }
   p.report = 1;
   // No more row tiles than this, whatever the sequences' shares.
-  const size_t waves = c.head_dim == 256 ? 4 : 8;
+  const size_t waves = c.head_dim == 128 ? 8 : 4;
   const size_t wgs = (a.n_tokens * group / (32 * waves) + a.n_seqs) * c.n_kv_heads;
-  // Two parts per CU where there are fewer tiles than that, as far as the scratch goes.
+  // As many parts as workgroups are resident where there are fewer tiles than that,
+  // as far as the scratch goes.
   const size_t slab = waves * (c.head_dim / 8 + 1) * 64 * 16;
   const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
-  const size_t target = 2 * (size_t)ex.cu_count;
+  const size_t target = (size_t)(c.head_dim == 64 ? 3 : 1) * ex.cu_count;
   p.target = wgs < room && wgs < target ? (int)std::min(target, room - wgs) : 0;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
