@@ -33,16 +33,20 @@ namespace {
 
 using namespace dev;
 
-constexpr int kWaves = 4;
 constexpr int kStages = 2;  // of a wave's ring
 constexpr int kTile = 32;
 constexpr int kMaxParts = 256;
-// Least tiles of a part (two a wave), and most that are one part all the same where
-// parts are that small: a join costs 3 us, a wave's tile 1.1 us while its SIMD has
-// no other.  (One request
-// of 4001 tokens, 8 heads: 12.6 us at two tiles a wave, 14.4 at four; one of 391
-// tokens, 2 heads: 11.4 us as one part, 13.1 as two.)
-constexpr int kPartTiles = 2 * kWaves, kWholeTiles = 3 * kPartTiles;
+// Least tiles of a part, and most that are one part all the same where parts are
+// that small: a join costs 3 us, a wave's tile 1.1 us while its SIMD has no other.
+// (One request of 4001 tokens, 8 heads: 12.6 us at 8 tiles a part, 14.4 at 16; one
+// of 391 tokens, 2 heads: 11.4 us as one part, 13.1 as two.)
+constexpr int kPartTiles = 8, kWholeTiles = 24;
+// Eight waves a workgroup instead of four halve what a wave goes over, but are
+// slower to start and leave one workgroup to a CU.  They are taken where that is
+// enough and a sequence is more than a tile a wave and at most this many tiles (16
+// requests of 701 tokens, 8 heads: 12.1 us, with four waves 13.9; 32 requests of 251:
+// 11.7 and 10.0; one of 8001: 15.8 and 13.0).
+constexpr size_t kEightWaves = 64;
 constexpr size_t kScanSeqs = 128;
 constexpr float kSlack = 8.f;  // log2 of how far a weight may pass 1
 
@@ -73,6 +77,7 @@ struct DecodeArgs {
   int rows_max;    // sequences of more rows are another kernel's
   int target;      // workgroups to divide the tiles over
   int report;      // this launch counts what is wrong with the sequences
+  int waves;       // of a workgroup: 4 or 8
   int joined;      // the parts are joined by kv_join_kernel, not by the last to arrive
   unsigned int* counters;  // per (sequence, head)
   float* partial;          // [workgroup][rows_max][D + 4]: rows, then maximum and sum
@@ -350,7 +355,7 @@ __device__ __forceinline__ int seq_tiles(const DecodeArgs& p, int s, int group, 
 __device__ __forceinline__ int part_of(const DecodeArgs& p, int total) {
   return max(kPartTiles, p.target ? (int)(((long)total * (int)p.c.n_kv_heads + p.target - 1) / p.target) : 0x3fffffff);
 }
-__device__ __forceinline__ int parts_of(int own, int per) {
+__device__ __forceinline__ int parts_of(const DecodeArgs& p, int own, int per) {
   return per == kPartTiles && own <= kWholeTiles ? min(own, 1) : min((own + per - 1) / per, kMaxParts);
 }
 // The item of workgroup b where kv_starts_kernel has run: two steps of a search
@@ -395,7 +400,7 @@ __device__ __forceinline__ bool find_item(const DecodeArgs& p, int b, int group,
   int before = 0;
   for (int base = 0; base < n_seqs; base += 64) {
     if (n_seqs > 64) own = seq_tiles(p, base + lane, group, bs_shift, false, q);
-    const int parts = parts_of(own, per);
+    const int parts = parts_of(p, own, per);
     const int sum = wave_scan(parts * heads), at = before + sum - parts * heads;
     before += __builtin_amdgcn_readlane(sum, 63);
     if (b < before) {
@@ -446,14 +451,14 @@ __global__ __launch_bounds__(kStartsThreads) void kv_starts_kernel(DecodeArgs p)
   const int per = part_of(p, total);
   for (int base = 0; base < n_seqs; base += kStartsThreads) {
     if (n_seqs > kStartsThreads) own = seq_tiles(p, base + tid, group, bs_shift, false, q);
-    const int all = sum_all(parts_of(own, per) * heads, before);
+    const int all = sum_all(parts_of(p, own, per) * heads, before);
     if (base + tid < n_seqs) p.starts[base + tid] = at + before;
     at += all;
   }
   if (tid == 0) p.starts[n_seqs] = at;
 }
 
-template <typename TT, int D, int GS, int NC>
+template <typename TT, int D, int GS, int NC, int kWaves>
 __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>)) void kv_decode_kernel(DecodeArgs p) {
   using X = Geo<D, GS>;
   extern __shared__ __align__(16) unsigned char lds_bytes[];  // the waves' rings; then the join
@@ -705,9 +710,9 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
 // At 15 parts the two come out even, at 31 it is 15 us to 13.  A workgroup joins 32
 // vectors of four dimensions, a thread every eighth part.
 constexpr size_t kJoinParts = 16;
-constexpr int kJoinVectors = 32, kJoinSlices = kWaves * 64 / kJoinVectors;
+constexpr int kJoinVectors = 32, kJoinSlices = 8, kJoinThreads = kJoinSlices * kJoinVectors;
 template <typename TT, int D>
-__global__ __launch_bounds__(kWaves * 64) void kv_join_kernel(DecodeArgs p) {
+__global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(DecodeArgs p) {
   constexpr int LD = D + 4, kRows = D < 128 ? 128 / D : 1, U = 16;  // rows of a workgroup
   static_assert(kMaxParts <= 2 * U * kJoinSlices);
   __shared__ float weight[kRows][kMaxParts];
@@ -718,7 +723,7 @@ __global__ __launch_bounds__(kWaves * 64) void kv_join_kernel(DecodeArgs p) {
   KvSeq q{};
   const int own = seq_tiles(p, lane, group, 31 - __builtin_clz(p.c.block_size), false, q);
   const int per = part_of(p, __builtin_amdgcn_readlane(wave_scan(own), 63));
-  const int mine = parts_of(own, per), sum = wave_scan(mine * heads);
+  const int mine = parts_of(p, own, per), sum = wave_scan(mine * heads);
   const int parts = __builtin_amdgcn_readlane(mine, s), first = __builtin_amdgcn_readlane(sum - mine * heads, s) + head;
   const int rows = __builtin_amdgcn_readlane(q.n_q, s) * group, rows0 = __builtin_amdgcn_readlane(q.rows0, s);
   const int v0 = blockIdx.y * kJoinVectors, r0 = v0 / (D / 4);
@@ -772,13 +777,13 @@ __global__ __launch_bounds__(kWaves * 64) void kv_join_kernel(DecodeArgs p) {
   *reinterpret_cast<u32x2*>(out) = u32x2{TT::pack2(acc[0], acc[1]), TT::pack2(acc[2], acc[3])};
 }
 
-template <typename TT, int D, int GS, int NC>
+template <typename TT, int D, int GS, int NC, int kWaves>
 hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
   const size_t ring = (size_t)kWaves * Geo<D, GS>::kWave;
   const size_t waves = (size_t)kWaves * p.rows_max * (D + 4 + 2) * sizeof(float);
   const size_t join = ((size_t)p.rows_max * (kMaxParts + 1) + 4 + (size_t)kWaves * 64 * 4) * sizeof(float);
   const size_t lds = std::max(ring, std::max(waves, p.target ? join : 0));
-  auto kernel = kv_decode_kernel<TT, D, GS, NC>;
+  auto kernel = kv_decode_kernel<TT, D, GS, NC, kWaves>;
   if (lds > 60 * 1024) {
     static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024);
@@ -789,21 +794,21 @@ hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
   if (launched != hipSuccess || !p.joined) return launched;
   const dim3 joins((uint32_t)(p.a.n_seqs * p.c.n_kv_heads),
                    (uint32_t)((p.rows_max * (D / 4) + kJoinVectors - 1) / kJoinVectors));
-  hipLaunchKernelGGL((kv_join_kernel<TT, D>), joins, dim3(kWaves * 64), 0, s, p);
+  hipLaunchKernelGGL((kv_join_kernel<TT, D>), joins, dim3(kJoinThreads), 0, s, p);
   return hipGetLastError();
 }
 
-template <typename TT, int NC>
+template <typename TT, int NC, int kWaves>
 hipError_t launch_d(hipStream_t s, const DecodeArgs& p, size_t grid) {
   switch (p.c.head_dim * 1000 + p.c.group_size) {
-    case 64032: return launch<TT, 64, 32, NC>(s, p, grid);
-    case 64064: return launch<TT, 64, 64, NC>(s, p, grid);
-    case 128032: return launch<TT, 128, 32, NC>(s, p, grid);
-    case 128064: return launch<TT, 128, 64, NC>(s, p, grid);
-    case 128128: return launch<TT, 128, 128, NC>(s, p, grid);
-    case 256032: return launch<TT, 256, 32, NC>(s, p, grid);
-    case 256064: return launch<TT, 256, 64, NC>(s, p, grid);
-    case 256128: return launch<TT, 256, 128, NC>(s, p, grid);
+    case 64032: return launch<TT, 64, 32, NC, kWaves>(s, p, grid);
+    case 64064: return launch<TT, 64, 64, NC, kWaves>(s, p, grid);
+    case 128032: return launch<TT, 128, 32, NC, kWaves>(s, p, grid);
+    case 128064: return launch<TT, 128, 64, NC, kWaves>(s, p, grid);
+    case 128128: return launch<TT, 128, 128, NC, kWaves>(s, p, grid);
+    case 256032: return launch<TT, 256, 32, NC, kWaves>(s, p, grid);
+    case 256064: return launch<TT, 256, 64, NC, kWaves>(s, p, grid);
+    case 256128: return launch<TT, 256, 128, NC, kWaves>(s, p, grid);
     default: return hipErrorInvalidValue;
   }
 }
@@ -818,6 +823,12 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.bad = bad;
   p.rows_max = rows_max;
   p.report = report;
+  const size_t reach = a.window ? std::min<size_t>(a.max_kv, (size_t)a.window + a.max_q) : a.max_kv;
+  const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : most_tiles / kPartTiles;
+  p.waves = p.rows_max <= 16 && most_tiles > 9 && most_tiles <= kEightWaves &&
+                    a.n_seqs * c.n_kv_heads * most_parts <= (size_t)ex.cu_count
+                ? 8
+                : 4;
   const size_t pairs = a.n_seqs * c.n_kv_heads;
   const size_t slab = (size_t)p.rows_max * (c.head_dim + 4) * sizeof(float);
   const size_t left = ex.scratch_bytes > kWideCounterBytes ? ex.scratch_bytes - kWideCounterBytes : 0;
@@ -847,8 +858,9 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.partial = reinterpret_cast<float*>(rest);
   const size_t grid = pairs + target;
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
-  if (p.rows_max <= 16) return bf16 ? launch_d<BF16, 1>(ex.stream, p, grid) : launch_d<F16, 1>(ex.stream, p, grid);
-  return bf16 ? launch_d<BF16, 2>(ex.stream, p, grid) : launch_d<F16, 2>(ex.stream, p, grid);
+  if (p.rows_max > 16) return bf16 ? launch_d<BF16, 2, 4>(ex.stream, p, grid) : launch_d<F16, 2, 4>(ex.stream, p, grid);
+  if (p.waves == 8) return bf16 ? launch_d<BF16, 1, 8>(ex.stream, p, grid) : launch_d<F16, 1, 8>(ex.stream, p, grid);
+  return bf16 ? launch_d<BF16, 1, 4>(ex.stream, p, grid) : launch_d<F16, 1, 4>(ex.stream, p, grid);
 }
 
 }  // namespace cpq
