@@ -806,7 +806,7 @@ hipError_t launch_d(hipStream_t s, const DecodeArgs& p, size_t grid) {
     case 128032: return launch<TT, 128, 32, NC, kWaves>(s, p, grid);
     case 128064: return launch<TT, 128, 64, NC, kWaves>(s, p, grid);
     case 128128: return launch<TT, 128, 128, NC, kWaves>(s, p, grid);
-    case 256032: return launch<TT, 256, 32, NC, kWaves>(s, p, grid);
+    case 256032: return launch<TT, 256, 32, NC, 4>(s, p, grid);
     case 256064: return launch<TT, 256, 64, NC, kWaves>(s, p, grid);
     case 256128: return launch<TT, 256, 128, NC, kWaves>(s, p, grid);
     default: return hipErrorInvalidValue;
@@ -825,7 +825,8 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.report = report;
   const size_t reach = a.window ? std::min<size_t>(a.max_kv, (size_t)a.window + a.max_q) : a.max_kv;
   const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : most_tiles / kPartTiles;
-  p.waves = p.rows_max <= 16 && most_tiles > 9 && most_tiles <= kEightWaves &&
+  const bool fits = c.head_dim < 256 || c.group_size > 32;  // the rings of eight waves in LDS
+  p.waves = fits && p.rows_max <= 16 && most_tiles > 9 && most_tiles <= kEightWaves &&
                     a.n_seqs * c.n_kv_heads * most_parts <= (size_t)ex.cu_count
                 ? 8
                 : 4;
