@@ -490,11 +490,11 @@ cpq_status cpq_kv_plan(cpq_commands* cmds, const uint32_t* lens, const uint32_t*
  * the given token and head strides in elements, both multiples of 8; 16-byte
  * aligned) into their slots.  Per group, with the arithmetic in fp32: bias = its
  * lowest value (-0 lies below 0), scale = RNE_T((highest - lowest) / 15), q =
- * clamp(rint((x - bias) / scale), 0, 15), 0 where the scale is 0.  A group that holds an Inf or NaN, or whose
- * range overflows, is stored as q = 0, scale = 0, bias = NaN.  Slots that are
- * none are skipped; slots past the cache are skipped and reported by the next
- * wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one slot: either wins, word
- * by word. */
+ * clamp(rint((x - bias) / scale), 0, 15), 0 where the scale is 0.  A group that
+ * holds an Inf or NaN, or whose range overflows, is stored as q = 0, scale = 0,
+ * bias = NaN.  Slots that are none are skipped; slots past the cache are skipped
+ * and reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one
+ * slot: either wins, word by word. */
 cpq_status cpq_kv_append(cpq_commands* cmds, const cpq_kv_cache* cache, const void* k, size_t k_token_stride,
                          size_t k_head_stride, const void* v, size_t v_token_stride, size_t v_head_stride,
                          const uint32_t* slots, size_t n_tokens);
