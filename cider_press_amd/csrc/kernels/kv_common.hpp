@@ -9,6 +9,12 @@
 // 2^(E - 5): then s * 2^(24 - E) <= 2^15 fits f16 and a value is off by at most
 // 2^-12 of itself or 2^-19 of that largest, whatever T's range.  E rises when a
 // tile brings a larger constant; a factor 2 is left free so that it seldom does.
+//
+// fp32 operands would run the matrix instructions at a sixteenth of the rate.  What
+// one rounding each of keys, values and weights costs: nothing at T = bf16, where
+// the output's own is eight times coarser (2-norm 0.0017 against 64 bits either
+// way); at T = f16 outputs are off by 0.0004 to 0.0011 where the output's rounding
+// alone is 0.0002.
 #pragma once
 
 #include <cfloat>

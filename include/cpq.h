@@ -510,9 +510,12 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
  * position p = kv_lens[s] - n_queries + i; query head h reads key/value head
  * h / (n_heads / n_kv_heads).  Over the keys j < kv_lens[s] with, if causal,
  * j <= p and, if window > 0, j > p - window:
- *   out = sum_j softmax_j(scale * <q, k_j>) v_j,  k, v = fmaf(scale, q, bias)
- * in fp32, rounded to T once; a row without keys is zero.  Masked keys and
- * values are not seen at all, whatever they hold.
+ *   out = sum_j softmax_j(scale * <q, k_j>) v_j,  k, v = scale * q + bias
+ * with scores, softmax and sums in fp32; keys, values and weights enter the
+ * matrix products as f16 for either T, each rounded once (2^-12 of itself, and
+ * 2^-19 of the largest constant near it), whatever the range of T; out is
+ * rounded to T once.  A row without keys is zero.  Masked keys and values are
+ * not seen at all, whatever they hold.
  * q, out: T, [n_tokens, n_heads, head_dim] at token and head strides in
  * elements (multiples of 8), 16-byte aligned.  block_table [n_seqs][max_blocks]
  * as cpq_kv_plan keeps it.  max_q, max_kv: the largest number of queries and
