@@ -737,6 +737,40 @@ def test_value_sizes_apart(device, q, n, sizes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,gs", [("bf16", 64, 32), ("f16", 64, 64), ("bf16", 256, 128), ("f16", 256, 32),
+                                          ("f16", 128, 128)])
+def test_prompt_values_apart(device, dtype, dim, gs):
+    """Prompts whose values' sizes rise and fall by 10^3 from run to run, in every
+    width, whole and split."""
+    rng = np.random.default_rng(dim + gs)
+    for q, n in ((90, 90), (40, 700), (300, 333)):
+        b = Batch(rng, device, dtype, dim, gs, 16, 1, 3, [q], [n])
+        j = np.arange(n)
+        size = np.array((1.0, 1e-3, 30.0, 0.0, 1e-2, 1.0, 0.0))[j // 16 % 7]
+        x = rng.standard_normal((n, 1, dim)) * size[:, None, None]
+        vq = quantize(from_bits(to_bits(x.astype(np.float32), dtype), dtype).astype(np.float32), gs, dtype)
+        kq = quantize(_rows(rng, n, 1, dim, dtype, 0.8)[1], gs, dtype)
+        b.host.put(b.table[0][j // 16] * 16 + j % 16, kq, vq)
+        b.k[0], b.v[0] = dequantize(*kq, gs, dtype), dequantize(*vq, gs, dtype)
+        unit = 2.0 ** -9 if dtype == "bf16" else 2.0 ** -12
+        for causal in (True, False):
+            want, bound = b.expect(causal=causal)
+            got = from_bits(b.run(causal=causal), dtype).astype(np.float64)
+            assert (np.abs(got - want) <= unit * 1.02 * np.abs(want) + bound + 2.0 ** -18 * np.abs(b.v[0]).max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,gs,group", [(64, 64, 4), (128, 64, 4), (256, 64, 2)])
+def test_long_token_beside_a_prompt(device, dim, gs, group):
+    """A single token over keys in many parts, beside a prompt and a draft."""
+    rng = np.random.default_rng(dim)
+    b = Batch(rng, device, "bf16", dim, gs, 32, 1, group, [1, 150, 3], [9001, 170, 4500])
+    first = b.run()
+    b.check(first)
+    assert np.array_equal(b.run(), first)
+
+
+@pytest.mark.gpu
 def test_many_sequences(device):
     """More sequences than a wave has lanes, lengths of zero among them, one and
     several queries each."""
