@@ -16,10 +16,11 @@
 // one between the products of two tiles, into the other half of four tiles of LDS,
 // so that on each SIMD one wave's dequantization meets the other's matrix
 // instructions; one barrier every two tiles.  At head_dim 256 (the rows take twice
-// the registers) and 64 (three workgroups share a CU) it has one team, two tiles of
-// LDS and a barrier every tile.  The packed words of a team's next tile are in
+// the registers), at 64 (three workgroups share a CU) and where eight waves a
+// workgroup would leave CUs without one, it has one team, two tiles of LDS and a
+// barrier every tile.  The packed words of a team's next tile are in
 // flight meanwhile.  (4096 queries of 32 heads over 8192 keys of 8: head_dim 128 429
-// us, 462 with a barrier every tile, 607 with four waves a workgroup; head_dim 64
+// us, 470 with a barrier every tile, 607 with four waves a workgroup; head_dim 64
 // 337 us, 429 with eight.)
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
@@ -50,8 +51,6 @@ using namespace dev;
 
 constexpr int kKeys = 64;        // of a tile
 constexpr int kMinTiles = 4;     // of a part
-template <int D>
-constexpr int kWaves = D == 128 ? 8 : 4;
 constexpr float kRaise = 6.f;     // log2 of the largest weight when the reference is set
 constexpr float kMost = 32768.f;  // of 16 weights' sum, so that each fits f16
 // What a wave publishes of its half of a tile: the exponent (0: all constants so
@@ -300,14 +299,14 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
   return false;
 }
 
-template <typename TT, int D>
-__global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(TileArgs p) {
+template <typename TT, int D, int kWaves>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
-  constexpr int kTeams = kWaves<D> / 4, kBufs = 2 * kTeams;
+  constexpr int kTeams = kWaves / 4, kBufs = 2 * kTeams;
   extern __shared__ u32x4 units[];  // [kBufs][keys, values][kUnits]
   __shared__ int meta[kBufs][4];         // of the halves' keys, then their values
   __shared__ unsigned int arrived;
-  constexpr int kRows = 32 * kWaves<D>;
+  constexpr int kRows = 32 * kWaves;
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -618,7 +617,7 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : D == 64 ? 3 : 2) voi
   uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t)(q.rows0 + qi) * a.out_token_stride +
                   (size_t)hh * a.out_head_stride + 4 * h;
   if (parts > 1) {
-    const size_t slab = (size_t)kWaves<D> * (D / 8 + 1) * 64;  // f32x4 of a workgroup
+    const size_t slab = (size_t)kWaves * (D / 8 + 1) * 64;  // f32x4 of a workgroup
     const size_t first = blockIdx.x - (size_t)part * c.n_kv_heads, stride = slab * c.n_kv_heads;
     const f32x4* all = reinterpret_cast<const f32x4*>(p.partial) + first * slab + (size_t)wave * (D / 8 + 1) * 64;
     const f32x4* mine = all + part * stride;
@@ -680,14 +679,14 @@ __global__ __launch_bounds__(kWaves<D> * 64, D == 256 ? 1 : D == 64 ? 3 : 2) voi
                 TT::pack2(scaled(o[j][4 * x + 2] * inv, ev), scaled(o[j][4 * x + 3] * inv, ev))};
 }
 
-template <typename TT, int D>
+template <typename TT, int D, int kWaves>
 hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
-  const size_t lds = (size_t)(kWaves<D> / 2) * 2 * kKeys * (D / 8) * 16;
-  auto kernel = kv_tile_kernel<TT, D>;
+  const size_t lds = (size_t)(kWaves / 2) * 2 * kKeys * (D / 8) * 16;
+  auto kernel = kv_tile_kernel<TT, D, kWaves>;
   static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return raised;
-  hipLaunchKernelGGL(kernel, grid, dim3(kWaves<D> * 64), lds, s, p);
+  hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), lds, s, p);
   return hipGetLastError();
 }
 
@@ -710,22 +709,29 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
   }
   p.report = 1;
   // No more row tiles than this, whatever the sequences' shares.
-  const size_t waves = c.head_dim == 128 ? 8 : 4;
-  const size_t wgs = (a.n_tokens * group / (32 * waves) + a.n_seqs) * c.n_kv_heads;
+  auto row_tiles = [&](size_t waves) { return (a.n_tokens * group / (32 * waves) + a.n_seqs) * c.n_kv_heads; };
+  // At head_dim 128 eight waves share a workgroup's dequantization; where that
+  // leaves compute units without one, workgroups of four, two to a CU (a step of 13
+  // requests, 590 and 115 tokens of prompts: 46.6 us, 52.6 with eight; 1024 queries
+  // of 48 heads on one key/value head: 75 and 87; 4096 of 32 on 8: 502 and 432).
+  const size_t waves = c.head_dim == 128 && row_tiles(8) >= (size_t)ex.cu_count ? 8 : 4;
+  const size_t wgs = row_tiles(waves);
   // As many parts as workgroups are resident where there are fewer tiles than that,
   // as far as the scratch goes.
   const size_t slab = waves * (c.head_dim / 8 + 1) * 64 * 16;
   const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
-  const size_t target = (size_t)(c.head_dim == 64 ? 3 : 1) * ex.cu_count;
+  const size_t target = (size_t)(c.head_dim == 64 ? 3 : c.head_dim == 128 && waves == 4 ? 2 : 1) * ex.cu_count;
   p.target = wgs < room && wgs < target ? (int)std::min(target, room - wgs) : 0;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
   const dim3 grid((uint32_t)(wgs + p.target));
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   switch (c.head_dim) {
-    case 64: return bf16 ? launch_tiles<BF16, 64>(ex.stream, p, grid) : launch_tiles<F16, 64>(ex.stream, p, grid);
-    case 128: return bf16 ? launch_tiles<BF16, 128>(ex.stream, p, grid) : launch_tiles<F16, 128>(ex.stream, p, grid);
-    case 256: return bf16 ? launch_tiles<BF16, 256>(ex.stream, p, grid) : launch_tiles<F16, 256>(ex.stream, p, grid);
+    case 64: return bf16 ? launch_tiles<BF16, 64, 4>(ex.stream, p, grid) : launch_tiles<F16, 64, 4>(ex.stream, p, grid);
+    case 128:
+      if (waves == 4) return bf16 ? launch_tiles<BF16, 128, 4>(ex.stream, p, grid) : launch_tiles<F16, 128, 4>(ex.stream, p, grid);
+      return bf16 ? launch_tiles<BF16, 128, 8>(ex.stream, p, grid) : launch_tiles<F16, 128, 8>(ex.stream, p, grid);
+    case 256: return bf16 ? launch_tiles<BF16, 256, 4>(ex.stream, p, grid) : launch_tiles<F16, 256, 4>(ex.stream, p, grid);
     default: return hipErrorInvalidValue;
   }
 }
