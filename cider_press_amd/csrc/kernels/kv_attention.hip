@@ -457,9 +457,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
       auto exponent = [&](int i, int none) { return word(i) & 0xffff ? (word(i) & 0xffff) - kExpBias : none; };
       const int e = max(ev, max(exponent(2, ev), exponent(3, ev)));  // o's unit: the largest exponent so far
-      if (is_values && e > range.e) {  // the values share it from here on
-        range.e = e;
-        range.limits = size_limits<TT>(e);
+      const int own = is_values ? e : max(exponent(0, range.e), exponent(1, range.e));
+      if (own > range.e) {  // the keys, and the values, share the largest from here on
+        range.e = own;
+        range.limits = size_limits<TT>(own);
       }
       if (e - min(exponent(2, e), exponent(3, e)) > kMostApart) {  // (all waves alike: they read the same words)
         __syncthreads();

@@ -4,11 +4,12 @@
 // a 16-bit half reads as the f16 subnormal q * 2^-24 (q * 2^-20), so one AND
 // extracts two of them and one v_pk_fma_f16 makes two values
 //   (s * 2^(24 - E)) * (q * 2^-24) + b * 2^-E = (s q + b) * 2^-E
-// with a single rounding.  E, uniform over the wave, keeps the largest
-// constant of the keys (of the values) met so far, max(|b|, 16 |s|), within
-// 2^(E - 5): then s * 2^(24 - E) <= 2^15 fits f16 and a value is off by at most
-// 2^-12 of itself or 2^-19 of that largest, whatever T's range.  E rises when a
-// tile brings a larger constant; a factor 2 is left free so that it seldom does.
+// with a single rounding.  E, uniform over the wave, keeps the largest constant of
+// the keys (of the values) met so far, max(|b|, 16 |s|), within 2^(E - 5): then
+// s * 2^(24 - E) <= 2^15 fits f16, whatever T's range.  A value is off by at most
+// 2^-12 of itself or, where it lies among f16's subnormals, by its bias's rounding
+// and its own, 2^-19 each of that largest.  E rises when a tile brings a larger
+// constant.
 //
 // fp32 operands would run the matrix instructions at a sixteenth of the rate.  What
 // one rounding each of keys, values and weights costs: nothing at T = bf16, where
@@ -62,7 +63,7 @@ __device__ __forceinline__ float finite_size(uint32_t sb) {
   return s <= FLT_MAX && b <= FLT_MAX ? fminf(fmaxf(b, 16.f * s), FLT_MAX) : 0.f;
 }
 // The exponent for constants up to m.
-__device__ __forceinline__ int size_exponent(float m) { return max(exponent_above(m), -110) + kKvTop + 1; }
+__device__ __forceinline__ int size_exponent(float m) { return max(exponent_above(m), -110) + kKvTop; }
 
 // Until the wave's LDS reads and writes are done.
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }

@@ -513,7 +513,7 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
  *   out = sum_j softmax_j(scale * <q, k_j>) v_j,  k, v = scale * q + bias
  * with scores, softmax and sums in fp32; keys, values and weights enter the
  * matrix products as f16 for either T, each rounded once (2^-12 of itself, and
- * 2^-19 of the largest constant near it), whatever the range of T; out is
+ * 2^-18 of the largest constant near it), whatever the range of T; out is
  * rounded to T once.  A row without keys is zero.  Masked keys and values are
  * not seen at all, whatever they hold.
  * q, out: T, [n_tokens, n_heads, head_dim] at token and head strides in

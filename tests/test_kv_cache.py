@@ -759,6 +759,46 @@ def test_prompt_values_apart(device, dtype, dim, gs):
             assert (np.abs(got - want) <= unit * 1.02 * np.abs(want) + bound + 2.0 ** -18 * np.abs(b.v[0]).max()).all()
 
 
+def _prompts(rng, device, dtype, gs):
+    """Enough row tiles for workgroups of eight waves: 34 prompts over 8 heads."""
+    q = rng.integers(6, 60, 34)
+    kv = q + rng.integers(0, 500, 34)
+    q[3], kv[3], kv[4], q[5], kv[5] = 130, 130, q[4], 200, 1200
+    return Batch(rng, device, dtype, 128, gs, 16, 8, 3, q.tolist(), kv.tolist())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gs,causal,window", [("bf16", 64, True, 0), ("f16", 32, False, 0), ("f16", 128, True, 70),
+                                                    ("bf16", 32, True, 333)])
+def test_many_prompts(device, dtype, gs, causal, window):
+    b = _prompts(np.random.default_rng(gs), device, dtype, gs)
+    first = b.run(causal, window)
+    b.check(first, causal, window)
+    assert np.array_equal(b.run(causal, window), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gs", [("bf16", 64), ("f16", 32)])
+def test_many_prompts_values_apart(device, dtype, gs):
+    """Values of very different sizes in neighbouring runs of 16, and what no row
+    may see after every sequence's end not finite."""
+    rng = np.random.default_rng(gs + 1)
+    b = _prompts(rng, device, dtype, gs)
+    for i, n in enumerate(b.kv_lens):
+        j = np.arange(n)
+        size = np.array((1.0, 1e-3, 30.0, 0.0, 1e-2, 1.0, 0.0))[(j // 16 + i) % 7]
+        x = rng.standard_normal((n, 8, 128)) * size[:, None, None]
+        vq = quantize(from_bits(to_bits(x.astype(np.float32), dtype), dtype).astype(np.float32), gs, dtype)
+        kq = quantize(_rows(rng, n, 8, 128, dtype, 0.8)[1], gs, dtype)
+        b.host.put(b.table[i][j // 16] * 16 + j % 16, kq, vq)
+        b.k[i], b.v[i] = dequantize(*kq, gs, dtype), dequantize(*vq, gs, dtype)
+    want, bound = b.expect()
+    got = from_bits(b.run(), dtype).astype(np.float64)
+    unit = 2.0 ** -9 if dtype == "bf16" else 2.0 ** -12
+    largest = max(np.abs(v).max() for v in b.v)
+    assert (np.abs(got - want) <= unit * 1.02 * np.abs(want) + bound + 2.0 ** -18 * largest).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim,gs,group", [(64, 64, 4), (128, 64, 4), (256, 64, 2)])
 def test_long_token_beside_a_prompt(device, dim, gs, group):
