@@ -14,8 +14,10 @@
 // fp32 operands would run the matrix instructions at a sixteenth of the rate.  What
 // one rounding each of keys, values and weights costs: nothing at T = bf16, where
 // the output's own is eight times coarser (2-norm 0.0017 against 64 bits either
-// way); at T = f16 outputs are off by 0.0004 to 0.0011 where the output's rounding
-// alone is 0.0002.
+// way).  At T = f16 outputs would be off by 0.0004 to 0.0013, most of it the keys',
+// where the output's rounding alone is 0.0002: for few rows keys and weights are
+// kept whole there (kv_decode.hip), for many, which the matrix instructions bound,
+// they are not (0.0005).
 #pragma once
 
 #include <cfloat>

@@ -25,8 +25,9 @@
 // sum and fp32 rows in the session's scratch, and the last to arrive joins them
 // in part order, or a kernel after this one where there are many.
 //
-// Bound by HBM where the keys are long (three requests of 120002 tokens, 8 heads of
-// 128 in groups of 32: 92 us, 5.0 TB/s, the vector pipes busy for 65%), by fixed
+// Bound by HBM where the keys are long (64 requests of 4097 tokens, 8 heads of 128 in
+// groups of 64: 65 us, 4.7 TB/s), at T = f16 by its instructions too (three requests
+// of 120002 tokens, groups of 32: 105 us, 4.4 TB/s), by fixed
 // phases of 9 us where they are not: launch, search, first tile, join (48 requests of
 // up to 8193 tokens: 25 us, 2.9 TB/s; one of 391 tokens, 2 heads of 64: 10.3 us).
 #include <algorithm>
@@ -133,7 +134,14 @@ __device__ __forceinline__ void start_tile(const cpq_kv_cache& c, size_t row_a, 
 template <typename TT, int D, int GS, int NC>
 struct Rows {
   using X = Geo<D, GS>;
+  // At T = f16 a key's and a weight's one rounding to f16 would show in the output: a
+  // scale enters in two parts whose products with a nibble are exact, the biases by
+  // a product of their own with the queries' sums, a weight with what it lost.
+  // (Three requests of 120002 tokens: off by 0.0002 to 0.0003 from 64 bits instead of
+  // 0.0006 to 0.0013, in 105 us instead of 92.)
+  static constexpr bool kExact = !Sig16<TT>::bf16;
   u32x4 qs[NC][X::WL];
+  u32x4 qsum[NC];  // sums over a lane's words of each group, in units of 2^6: high and low part
   int qe[NC];    // exponents of the query rows
   float cl[NC];  // log2(e) * scale * 2^(qe + ek)
   f32x4 o[X::VS][X::NJ][NC];
@@ -230,12 +238,18 @@ struct Rows {
     f32x4 sc[2][NC];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      uint32_t s0[X::NG], s1[X::NG], bb[X::NG];
+      uint32_t s0[X::NG], s1[X::NG], bb[X::NG], r0[X::NG], r1[X::NG];
 #pragma unroll
       for (int g = 0; g < X::NG; ++g) {
-        const float sv = scaled(TT::lo(ksb[u][g]), 24 - ek), bv = scaled(TT::hi(ksb[u][g]), -ek);
+        const float sv = scaled(TT::lo(ksb[u][g]), 24 - ek), bv = scaled(TT::hi(ksb[u][g]), (kExact ? 6 : 0) - ek);
         s0[g] = F16::pack2(sv, sv);
         bb[g] = F16::pack2(bv, bv);
+        if constexpr (kExact) {  // 7 bits and the other 4
+          const uint32_t all = s0[g];
+          s0[g] = all & 0xfff0fff0u;
+          r0[g] = __builtin_bit_cast(uint32_t, as_f16x2(all) - as_f16x2(s0[g]));
+          r1[g] = sixteenth(r0[g]);
+        }
         s1[g] = sixteenth(s0[g]);
       }
 #pragma unroll
@@ -256,13 +270,27 @@ struct Rows {
 #pragma unroll
       for (int w = 0; w < X::WL; ++w) {
         const int g = w / X::GW;
-        const u32x4 k = key_slice(kw[w], s0[g], s1[g], bb[g]);
+        if constexpr (kExact) {
+          const u32x4 high = key_slice(kw[w], s0[g], s1[g], 0u), low = key_slice(kw[w], r0[g], r1[g], 0u);
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) sc[u][cc] = Mfma16<F16>::run(k, qs[cc][w], sc[u][cc]);
+          for (int cc = 0; cc < NC; ++cc) {
+            sc[u][cc] = Mfma16<F16>::run(high, qs[cc][w], sc[u][cc]);
+            sc[u][cc] = Mfma16<F16>::run(low, qs[cc][w], sc[u][cc]);
+          }
+        } else {
+          const u32x4 k = key_slice(kw[w], s0[g], s1[g], bb[g]);
+#pragma unroll
+          for (int cc = 0; cc < NC; ++cc) sc[u][cc] = Mfma16<F16>::run(k, qs[cc][w], sc[u][cc]);
+        }
+      }
+      if constexpr (kExact) {
+        const u32x4 b{bb[0], X::NG > 1 ? bb[X::NG - 1] : 0u, 0u, 0u};
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc) sc[u][cc] = Mfma16<F16>::run(b, qsum[cc], sc[u][cc]);
       }
     }
 
-    u32x4 pw[NC];
+    u32x4 pw[NC], lost[NC];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       if (!whole) {
@@ -296,7 +324,11 @@ struct Rows {
         for (int e = 0; e < 4; ++e) w[4 * u + e] = __builtin_amdgcn_exp2f(fmaf(sc[u][cc][e], cl[cc], -ref[cc]));
       sum[cc] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
-      for (int x = 0; x < 4; ++x) pw[cc][x] = F16::pack2(w[2 * x], w[2 * x + 1]);
+      for (int x = 0; x < 4; ++x) {
+        pw[cc][x] = F16::pack2(w[2 * x], w[2 * x + 1]);
+        if constexpr (kExact)
+          lost[cc][x] = F16::pack2(w[2 * x] - F16::lo(pw[cc][x]), w[2 * x + 1] - F16::hi(pw[cc][x]));
+      }
     }
 
 #pragma unroll
@@ -333,6 +365,10 @@ struct Rows {
         for (int cc = 0; cc < NC; ++cc) {
           o[v][2 * y][cc] = Mfma16<F16>::run(lo, pw[cc], o[v][2 * y][cc]);
           o[v][2 * y + 1][cc] = Mfma16<F16>::run(hi, pw[cc], o[v][2 * y + 1][cc]);
+          if constexpr (kExact) {
+            o[v][2 * y][cc] = Mfma16<F16>::run(lo, lost[cc], o[v][2 * y][cc]);
+            o[v][2 * y + 1][cc] = Mfma16<F16>::run(hi, lost[cc], o[v][2 * y + 1][cc]);
+          }
         }
       }
     }
@@ -526,6 +562,20 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     R.qe[cc] = query_exponent(m);
 #pragma unroll
     for (int w = 0; w < X::WL; ++w) R.qs[cc][w] = query_slice<TT>(R.qs[cc][w], R.qe[cc]);
+    if constexpr (R.kExact) {
+      R.qsum[cc] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int g = 0; g < X::NG; ++g) {
+        float all = 0.f;
+#pragma unroll
+        for (int w = g * X::WL / X::NG; w < (g + 1) * X::WL / X::NG; ++w)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) all = F16::dot2(R.qs[cc][w][e], 0x3c003c00u, all);
+        all *= 0x1p-6f;
+        const float high = F16::lo(F16::pack2(all, 0.f));
+        R.qsum[cc][g] = F16::pack2(high, all - high);
+      }
+    }
     R.cl[cc] = fmaxf(scaled(a.scale * kLog2e, R.qe[cc]), FLT_MIN);
     R.top[cc] = -INFINITY;
     R.ref[cc] = -FLT_MAX;
