@@ -21,7 +21,7 @@
 // barrier every tile.  The packed words of a team's next tile are in
 // flight meanwhile.  (4096 queries of 32 heads over 8192 keys of 8: head_dim 128 429
 // us, 470 with a barrier every tile, 607 with four waves a workgroup; head_dim 64
-// 337 us, 429 with eight.)
+// 344 us, 429 with eight.)
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
 //   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
@@ -31,11 +31,11 @@
 // maximum of the half tile found, the reference raised to 2^-6 of it and its weights
 // made again.  The weights of a tile's first 32 keys are made between the matrix
 // instructions of the other 32 keys' scores, theirs between those of the first
-// keys' values (head_dim 64 350 -> 337 us, 256 411 -> 354).
+// keys' values (when that came in: head_dim 64 350 -> 337 us, 256 411 -> 354).
 //
 // Bound by its instructions: 4096 queries over 8192 keys at head_dim 128 run at 960
-// TFLOP/s (a large f16 product of the library: 1322), with the matrix pipes busy for
-// 41% and the vector pipes for 46% of the cycles.
+// TFLOP/s (a large f16 product of the library: 1322), with the vector pipes busy for
+// 55% of the cycles, the matrix pipes for 43%, both at once for 18%.
 //
 // Where there are few row tiles their keys are split, evenly over the resident
 // workgroups by the lengths on the device, and joined, in part order, by the last
