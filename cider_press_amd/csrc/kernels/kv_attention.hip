@@ -693,10 +693,17 @@ hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
 
 }  // namespace
 
-hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& given,
                                unsigned int* bad) {
+  // Bounds past what a sequence can have mean no more than that, and would wrap.
+  constexpr size_t kLongest = 1ull << 31;
+  cpq_kv_attention_args a = given;
+  a.max_q = std::min(a.max_q, a.n_tokens);
+  a.max_kv = std::min(a.max_kv, kLongest);
+  a.window = std::min(a.window, kLongest - 1);
   const size_t group = a.n_heads / c.n_kv_heads;
-  if (a.max_q * group <= kKvDecodeRows) return launch_kv_decode(ex, c, a, (int)(a.max_q * group), true, bad);
+  if (a.max_q * group <= kKvDecodeRows)
+    return launch_kv_decode(ex, c, a, (int)std::max<size_t>(a.max_q * group, 1), true, bad);
   TileArgs p{};
   p.c = c;
   p.a = a;

@@ -920,6 +920,24 @@ def test_layouts_streams_and_graph(device):
 
 
 @pytest.mark.gpu
+def test_bounds_at_their_ends(device):
+    """max_q, max_kv and window of zero, and as large as their type."""
+    rng = np.random.default_rng(4)
+    top = 2 ** 64 - 1
+    for q in ([1, 1], [3, 40]):
+        b = Batch(rng, device, "bf16", 128, 64, 16, 2, 4, q, [70, 300])
+        want = b.run()
+        for over in (dict(max_q=top), dict(max_q=2 ** 62), dict(max_kv=top), dict(max_kv=0), dict(window=top),
+                     dict(window=2 ** 63), dict(window=2 ** 31 + 5), dict(max_q=top, max_kv=top, window=top)):
+            b.check(b.run(**over))
+        b.check(b.run(window=301))
+        with pytest.raises(_lib.InvalidArgument, match="kv_attention"):
+            b.run(max_q=0)
+        assert np.all(b.keep[-1].to_numpy() == 0x5A5A)  # not computed
+        assert np.array_equal(b.run(), want)
+
+
+@pytest.mark.gpu
 def test_bad_lengths_and_blocks(device):
     """What the device finds wrong is masked or left out, and reported."""
     rng = np.random.default_rng(2)
