@@ -214,7 +214,8 @@ struct Rows {
 #pragma unroll
       for (int q = 0; q < X::NL; ++q) {
         const int e = 64 * q + lane, key = e / (4 * X::G) * 4 + (e & 3) & 31;
-        const bool live = any(key);
+        // (One group a head: 32 constants, the lanes after them hold copies of the last.)
+        const bool live = (X::G > 1 || lane < 32) && any(key);
         const bool ok = finite(TT::lo(vsb[q])) && finite(TT::hi(vsb[q]));
         poison |= live && !ok;
         vsb[q] = live && ok ? vsb[q] : 0u;
