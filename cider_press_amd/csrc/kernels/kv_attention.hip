@@ -271,8 +271,9 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
       total += sum;
     }
   }
-  // (Each row tile rounds its parts up, by half a part on average.)
-  const int target = max(p.target - items / 2, p.target / 4);
+  // (Each row tile rounds its parts up, by half a part on average.  At least 1: where
+  // the scratch leaves room for a few parts only, these come to nothing.)
+  const int target = max(max(p.target - items / 2, p.target / 4), 1);
   const long per = p.target ? max((total * heads + target - 1) / target, (long)kMinTiles) : 1l << 40;
   int before = 0;
   for (int base = 0; base < n_seqs; base += 64) {
