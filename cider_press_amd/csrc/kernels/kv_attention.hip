@@ -259,13 +259,12 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
     const int reach = p.a.window ? (int)min((uint64_t)q.n, (uint64_t)p.a.window + rows_per / group) : q.n;
     key_tiles = (reach + kKeys - 1) / kKeys;
   };
-  long total = 0;
-  int items = 0;
+  long total = 0, items = 0;
   if (p.target || p.report) {
     for (int base = 0; base < n_seqs; base += 64) {
       work(base + lane, p.report && b == 0 && threadIdx.x < 64);
       long sum = (long)row_tiles * key_tiles;
-      items += __builtin_amdgcn_readlane(wave_scan(row_tiles * heads), 63);
+      items += __builtin_amdgcn_readlane(wave_scan(min(row_tiles * heads, 1 << 24)), 63);
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
       total += sum;
@@ -273,8 +272,12 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
   }
   // (Each row tile rounds its parts up, by half a part on average.  At least 1: where
   // the scratch leaves room for a few parts only, these come to nothing.)
-  const int target = max(max(p.target - items / 2, p.target / 4), 1);
-  const long per = p.target ? max((total * heads + target - 1) / target, (long)kMinTiles) : 1l << 40;
+  const long target = max(max(p.target - items / 2, (long)p.target / 4), 1l);
+  // Query starts that are not ascending (reported) can name more row tiles than the
+  // grid was made for: no splits then, or parts without a workgroup would leave their
+  // arrival counters behind.
+  const bool split = p.target && items <= (long)gridDim.x - p.target;
+  const long per = split ? max((total * heads + target - 1) / target, (long)kMinTiles) : 1l << 40;
   int before = 0;
   for (int base = 0; base < n_seqs; base += 64) {
     work(base + lane, false);

@@ -1,8 +1,10 @@
 """Attention over the key/value cache where the session's scratch is small or
-missing: keys are split as far as it goes (test_kv_cache.py: Batch)."""
+missing: keys are split as far as it goes; and what a call leaves there
+(test_kv_cache.py: Batch)."""
 import numpy as np
 import pytest
 
+from cider_press_amd import _lib
 from test_kv_cache import Batch
 
 # Parts of a workgroup of four waves that 1 MiB holds behind the arrival counters.
@@ -50,3 +52,22 @@ def test_small_scratch(device, monkeypatch, mib, q, kv):
     first = b.run(cmds=cmds)
     b.check(first)
     assert np.array_equal(b.run(cmds=cmds), first)
+
+
+@pytest.mark.gpu
+def test_query_starts_that_overlap(device):
+    """Starts that are not ascending are reported, and leave nothing behind that a
+    later call on the session meets."""
+    rng = np.random.default_rng(3)
+    cmds = device.commands()
+    b = Batch(rng, device, "bf16", 64, 64, 16, 1, 4, [640], [2000])
+    n = 65
+    b.starts = np.array([0, 640] * n, np.uint32)
+    b.kv_lens, b.table = b.kv_lens * (2 * n - 1), np.repeat(b.table, 2 * n - 1, 0)
+    with pytest.raises(_lib.InvalidArgument, match="kv_attention"):
+        b.run(cmds=cmds)
+    for q in (1, 20, 70):
+        after = Batch(rng, device, "bf16", 64, 64, 16, 1, 4, [q], [3000])
+        want = after.run(cmds=cmds)
+        after.check(want)
+        assert np.array_equal(after.run(cmds=cmds), want)
