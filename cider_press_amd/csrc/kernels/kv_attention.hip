@@ -405,8 +405,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     u32x4* keys = units + buf * 2 * kUnits;
     const int key = t * kKeys + half * 32;
     const bool all = key >= from && key + 32 <= q.n && loaded_ok == 3;
+    // (Of the keys [from, end) each is seen by one of the rows.)
     if (!all && !is_values && lane == 0 &&
-        ((!(loaded_ok & 1) && key < q.n) || (!(loaded_ok & 2) && key + 16 < q.n)))
+        ((!(loaded_ok & 1) && key < end && key + 16 > from) || (!(loaded_ok & 2) && key + 16 < end && key + 32 > from)))
       atomicAdd(p.bad, 1u);
     bool poison = false;
     if (is_values) {

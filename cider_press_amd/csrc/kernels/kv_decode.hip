@@ -616,7 +616,8 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     const int stage = (ti - t0) / kWaves % kStages;
     const int t = base + ti * kTile, oks = ok >> 2 * stage & 3;
     const bool whole = t >= seen_from && t + kTile <= seen_end && oks == 3;
-    if (lane == 0 && ((!(oks & 1) && t < q.n) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
+    // (Of the keys [q.lo, q.n) each is seen by one of the rows.)
+    if (lane == 0 && ((!(oks & 1) && t < q.n && t + 16 > q.lo) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
     const bool poison = R.add(ring, ring + stage * X::kStage, lane, whole, a.scale, t, oks, from, to, q.lo, q.n);
     if (poison) {
       const KvPlaces pl = kv_places(c, blocks[kv_index(t, q.n, bs_shift)], blocks[kv_index(t + 16, q.n, bs_shift)], t,

@@ -523,8 +523,10 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
  * of keys of any sequence, as far as the host knows; max_kv only steers how
  * the work is split, a sequence with more than max_q queries is not computed.
  * Rows past query_starts[n_seqs] are not written.  Such sequences, sequences
- * whose rows pass n_tokens, and blocks past n_blocks or max_blocks (their keys
- * count as masked) are reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.
+ * whose rows pass n_tokens, and blocks past n_blocks or max_blocks of which a
+ * query would see a key (they count as masked) are reported by the next wait as
+ * CPQ_ERR_INVALID_ARGUMENT; entries of blocks behind every query's window may hold
+ * anything.
  * Session scratch holds the partial results where keys are split. */
 typedef struct cpq_kv_attention_args {
   const void* q;

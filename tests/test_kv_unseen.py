@@ -7,6 +7,7 @@ nothing of the others (test_kv_cache.py: Batch).
 import numpy as np
 import pytest
 
+from cider_press_amd import _lib
 from test_kv_cache import GEOMETRIES, NAN, Batch
 
 FILLED = GEOMETRIES + [("bf16", 128, 128, 16), ("f16", 64, 64, 16)]
@@ -41,3 +42,21 @@ def test_places_past_the_end(device, dtype, dim, gs, bs, what):
         b = Batch(rng, device, dtype, dim, gs, bs, 2, 3, q, kv)
         _fill(b, what)
         b.check(b.run(causal, window), causal, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q", [1, 5, 40, 200])
+@pytest.mark.parametrize("window", [16, 33, 70, 300])
+def test_blocks_behind_the_window(device, q, window):
+    """A program that gives blocks back once no query sees them, and clears their
+    entries, has no error; the block of the first key that a query sees is one."""
+    rng = np.random.default_rng(q + window)
+    kv = [q + n for n in (0, 1, 90, 333, 350, 1111)]
+    b = Batch(rng, device, "bf16", 128, 64, 16, 2, 4, [q] * len(kv), kv)
+    for s, n in enumerate(kv):
+        b.table[s, :max(0, n - q + 1 - window) // 16] = 0xFFFFFFFF
+    b.check(b.run(window=window), window=window)
+    first = max(0, kv[-1] - q + 1 - window) // 16
+    b.table[-1, first] = 0xFFFFFFFF
+    with pytest.raises(_lib.InvalidArgument, match="kv_attention"):
+        b.run(window=window)
