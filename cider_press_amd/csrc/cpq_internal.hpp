@@ -22,7 +22,7 @@ struct cpq_device {
   struct cpq_commands* eval_session = nullptr;
 };
 
-constexpr int kStatusWords = 7;  // of cpq_commands::status
+constexpr int kStatusWords = 8;  // of cpq_commands::status
 
 struct cpq_commands {
   cpq_device* dev = nullptr;
@@ -31,8 +31,9 @@ struct cpq_commands {
   // Device-side status words: kernels that can detect bad data count it
   // here ([0] gather rows with out-of-range indices, [1] embed ids out of
   // range, [2] MoE combine positions out of range, [3] blocks that
-  // cpq_kv_release dropped, [4] tokens that cpq_kv_plan did not place, [5]
-  // slots past a key/value cache, [6] what cpq_kv_attention could not compute)
+  // cpq_kv_release dropped, [4] and [5], 64 bits, tokens that cpq_kv_plan did not
+  // place (a caller's lengths may add up to a multiple of 2^32), [6] slots past a
+  // key/value cache, [7] what cpq_kv_attention could not compute)
   // add to it; cpq_commands_wait reads and clears it.
   unsigned int* status = nullptr;
   // Scratch of the split-K reductions and the routing sort: arrival
@@ -316,7 +317,7 @@ hipError_t launch_kv_plan(hipStream_t s, const uint32_t* lens, const uint32_t* n
                           uint32_t n_seqs, uint32_t max_blocks, uint32_t block_size, const uint32_t* free_list,
                           uint32_t free_cap, const uint32_t* free_count, uint32_t* starts, uint32_t* kv_lens,
                           uint32_t* slots, uint32_t* positions, uint32_t cap, uint32_t* free_count_out,
-                          unsigned int* bad);
+                          unsigned long long* bad);
 hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k, size_t k_token, size_t k_head,
                             const void* v, size_t v_token, size_t v_head, const uint32_t* slots, uint32_t n_tokens,
                             unsigned int* bad);

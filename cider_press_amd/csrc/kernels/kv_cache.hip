@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(
     uint32_t max_blocks, int bs_shift, const uint32_t* __restrict__ free_list, uint32_t free_cap,
     const uint32_t* __restrict__ free_count, uint32_t* __restrict__ starts_out, uint32_t* __restrict__ kv_lens,
     uint32_t* __restrict__ slots, uint32_t* __restrict__ positions, uint32_t cap,
-    uint32_t* __restrict__ free_count_out, unsigned int* bad) {
+    uint32_t* __restrict__ free_count_out, unsigned long long* bad) {
   extern __shared__ uint32_t plan_lds[];
   uint32_t* starts = plan_lds;            // [n_seqs + 1]
   uint32_t* first = plan_lds + n_seqs + 1;  // [n_seqs]
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(
         const uint32_t got = have + (top < n_free ? min(need, n_free - top) : 0u);
         const uint64_t room = (uint64_t)got << bs_shift, all = (uint64_t)len + n;
         kv_lens[s] = (uint32_t)(all < room ? all : room);
-        if (want > n) atomicAdd(bad, want - n);
+        if (want > n) atomicAdd(bad, (unsigned long long)(want - n));
       }
     }
   }
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(
     slots[t] = slot;
     positions[t] = pos;
   }
-  if (lost) atomicAdd(bad, lost);
+  if (lost) atomicAdd(bad, (unsigned long long)lost);
 }
 
 // The largest exponent's bits, above which a pattern is an Inf or NaN.
@@ -362,7 +362,7 @@ hipError_t launch_kv_plan(hipStream_t s, const uint32_t* lens, const uint32_t* n
                           uint32_t n_seqs, uint32_t max_blocks, uint32_t block_size, const uint32_t* free_list,
                           uint32_t free_cap, const uint32_t* free_count, uint32_t* starts, uint32_t* kv_lens,
                           uint32_t* slots, uint32_t* positions, uint32_t cap, uint32_t* free_count_out,
-                          unsigned int* bad) {
+                          unsigned long long* bad) {
   const uint32_t grid = std::min(std::max((cap + kPlanThreads - 1) / kPlanThreads, 1u), 256u);
   const size_t lds = (2 * (size_t)n_seqs + 1) * 4;  // at most 64 KiB + 4
   if (lds > 64 * 1024 - 1024) {

@@ -173,7 +173,7 @@ cpq_status cpq_kv_plan(cpq_commands* cmds, const uint32_t* lens, const uint32_t*
   return launched(cpq::launch_kv_plan(cmds->stream, lens, new_lens, block_table, (uint32_t)n_seqs,
                                       (uint32_t)max_blocks, block_size, free_list, (uint32_t)free_cap, free_count,
                                       query_starts, kv_lens, slots, positions, (uint32_t)cap, free_count_out,
-                                      cmds->status + 4),
+                                      reinterpret_cast<unsigned long long*>(cmds->status + 4)),
                   "kv_plan launch");
 }
 
@@ -194,7 +194,7 @@ cpq_status cpq_kv_append(cpq_commands* cmds, const cpq_kv_cache* cache, const vo
   st = check_words(op, w, 1, 0);
   if (st != CPQ_OK) return st;
   return launched(cpq::launch_kv_append(cmds->stream, *cache, k, k_token_stride, k_head_stride, v, v_token_stride,
-                                        v_head_stride, slots, (uint32_t)n_tokens, cmds->status + 5),
+                                        v_head_stride, slots, (uint32_t)n_tokens, cmds->status + 6),
                   "kv_append launch");
 }
 
@@ -210,7 +210,7 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
   const Words w[] = {{"slots", slots, n_rows}};
   st = check_words(op, w, 1, 0);
   if (st != CPQ_OK) return st;
-  return launched(cpq::launch_kv_gather(cmds->stream, *cache, slots, (uint32_t)n_rows, k_out, v_out, cmds->status + 5),
+  return launched(cpq::launch_kv_gather(cmds->stream, *cache, slots, (uint32_t)n_rows, k_out, v_out, cmds->status + 6),
                   "kv_gather launch");
 }
 
@@ -253,7 +253,7 @@ cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const
   cpq_status st = cpq_check_kv_attention_args(cache, args);
   if (st != CPQ_OK) return st;
   if (args->n_tokens == 0 || args->n_seqs == 0) return CPQ_OK;
-  return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 6),
+  return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 7),
                   "kv_attention launch");
 }
 

@@ -276,18 +276,18 @@ cpq_status cpq_commands_wait(cpq_commands* cmds) {
     if (bad[2])
       msg += std::string(msg.empty() ? "" : "; ") + "moe_combine: " + std::to_string(bad[2]) +
              " (token, slot) position(s) outside the expert rows; they contributed 0";
-    const char* const kv[] = {
-        "kv_release: %u block(s) past the free list's capacity; they were dropped",
-        "kv_plan: %u token(s) without a place (past the slots, the block table's rows or the free blocks)",
-        "kv_append / kv_gather: %u slot(s) past the cache; they were skipped, or read as 0",
-        "kv_attention: %u time(s) a sequence's lengths passed max_q or the query rows (not computed), or a block "
-        "the cache or the block table (masked)"};
-    for (int i = 3; i < kStatusWords; ++i) {
-      if (!bad[i]) continue;
-      char text[200];
-      std::snprintf(text, sizeof(text), kv[i - 3], bad[i]);
-      msg += std::string(msg.empty() ? "" : "; ") + text;
+    auto count = [&](unsigned int n, const char* op, const char* what) {
+      if (n) msg += std::string(msg.empty() ? "" : "; ") + op + std::to_string(n) + what;
+    };
+    count(bad[3], "kv_release: ", " block(s) past the free list's capacity; they were dropped");
+    if (bad[4] || bad[5]) {
+      const std::string high = bad[5] ? std::to_string(bad[5]) + " * 2^32" : "", low = bad[4] ? std::to_string(bad[4]) : "";
+      msg += std::string(msg.empty() ? "" : "; ") + "kv_plan: " + high + (bad[4] && bad[5] ? " + " : "") + low +
+             " token(s) without a place (past the slots, the block table's rows or the free blocks)";
     }
+    count(bad[6], "kv_append / kv_gather: ", " slot(s) past the cache; they were skipped, or read as 0");
+    count(bad[7], "kv_attention: ", " time(s) a sequence's lengths passed max_q or the query rows (not computed), or a "
+                                    "block the cache or the block table (masked)");
     return fail(CPQ_ERR_INVALID_ARGUMENT, msg);
   }
   return CPQ_OK;
