@@ -28,7 +28,7 @@
 //   a key that repeats among them doubles it).
 // No maximum is taken on the way: weights are 2^(score - reference), and only
 // where their sums show that one leaves f16's range (the first tile's do) is the
-// maximum of the half tile found, the reference raised to 2^-6 of it and its weights
+// maximum of the half tile found, the reference raised to 2^-10 of it and its weights
 // made again.  The weights of a tile's first 32 keys are made between the matrix
 // instructions of the other 32 keys' scores, theirs between those of the first
 // keys' values (when that came in: head_dim 64 350 -> 337 us, 256 411 -> 354).
@@ -51,8 +51,11 @@ using namespace dev;
 
 constexpr int kKeys = 64;        // of a tile
 constexpr int kMinTiles = 4;     // of a part
-constexpr float kRaise = 6.f;     // log2 of the largest weight when the reference is set
-constexpr float kMost = 32768.f;  // of 16 weights' sum, so that each fits f16
+// log2 of the largest weight when the reference is set: with it one of 2^-24 of the
+// largest keeps 11 bits (beside a key that draws nearly all weight and holds zeros the
+// others make the output).  At 2^6 the reference is set less often: 1 % of the time.
+constexpr float kRaise = 10.f;
+constexpr float kMost = 65504.f;  // of 16 weights' sum, so that each fits f16
 // What a wave publishes of its half of a tile: the exponent (0: all constants so
 // far are zeros), which 16 keys have their block, whether a value constant is not
 // finite.

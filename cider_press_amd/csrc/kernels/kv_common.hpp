@@ -7,7 +7,7 @@
 // with a single rounding.  E, uniform over the wave, keeps the largest constant of
 // the keys (of the values) met so far, max(|b|, 16 |s|), within 2^(E - 5): then
 // s * 2^(24 - E) <= 2^15 fits f16, whatever T's range.  A value is off by at most
-// 2^-12 of itself or, where it lies among f16's subnormals, by its bias's rounding
+// 2^-11 of itself or, where it lies among f16's subnormals, by its bias's rounding
 // and its own, 2^-19 each of that largest.  E rises when a tile brings a larger
 // constant.
 //

@@ -17,8 +17,8 @@
 // in LDS by asynchronous copies, a tile ahead, each lane's 16 bytes as it will
 // read them; no barrier until the waves' results are joined.  The constants of
 // 32 keys' values are turned into f16 once per wave, not once per lane that uses
-// them.  The running maximum moves only when a tile exceeds it by 2^8 (weights
-// stay below 2^8 in f16, sums are fp32).
+// them.  The weights' reference, 2^-12 of the largest, moves only when a tile exceeds
+// that by 2^3 (weights stay below 2^15 in f16, sums are fp32).
 //
 // The workgroups divide the tiles of all sequences evenly, by the lengths on
 // the device.  Where a sequence's keys are split, every part parks its maximum,
@@ -54,7 +54,11 @@ constexpr int kPartTiles = 8, kWholeTiles = 24;
 // 11.7 and 10.0; one of 8001: 15.8 and 13.0).
 constexpr size_t kEightWaves = 64;
 constexpr size_t kScanSeqs = 128;
-constexpr float kSlack = 8.f;  // log2 of how far a weight may pass 1
+// log2 of the largest weight when the reference moves, and of how far one may pass it:
+// up to 2^15 the weights take f16's whole range, so that one of 2^-26 of the largest
+// still keeps 11 bits (beside a key that draws nearly all weight and holds zeros the
+// others make the output).  The reference moves in the first tile and seldom after.
+constexpr float kRaise = 12.f, kSlack = 3.f;
 
 template <int D, int GS>
 struct Geo {
@@ -310,7 +314,7 @@ struct Rows {
       if (__any(m > top[cc] + kSlack)) {
         const float was = ref[cc];
         top[cc] = fmaxf(top[cc], m);
-        ref[cc] = fmaxf(top[cc], -FLT_MAX);
+        ref[cc] = fmaxf(top[cc] - kRaise, -FLT_MAX);
         const float keep = __builtin_amdgcn_exp2f(was - ref[cc]);
         sum[cc] *= keep;
 #pragma unroll

@@ -1,0 +1,36 @@
+"""Attention over the key/value cache: weights far below the largest keep their
+precision (test_kv_cache.py: Batch)."""
+import numpy as np
+import pytest
+
+from cider_press_amd.synthetic import from_bits, to_bits
+from test_kv_cache import Batch, dequantize, quantize
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("q", [1, 5, 60])
+@pytest.mark.parametrize("size", [1.0, 1.5, 1.9296875, 2.1875, 2.25])
+def test_small_weights_beside_sinks(device, dtype, q, size):
+    """Every 32nd key takes nearly all of a row's weight and has zeros for values;
+    the others weigh w = 2^-11.5 to 2^-26 of it and make the output.  A weight is
+    off by half a unit of f16, 2^-11 of itself, and 2^-35 of the row's largest, values
+    by 2^-11, the output by half a unit of T; keys and queries are exact here."""
+    rng = np.random.default_rng(int(size * 64) + q)
+    n = 700
+    b = Batch(rng, device, dtype, 64, 32, 16, 1, 4, [q], [n])
+    sink = np.arange(n) % 32 == 0
+    k = np.where(sink[:, None, None], size, 0.0) * np.ones((n, 1, 64))
+    v = np.where(sink[:, None, None], 0.0, 1.0 + 0.5 * rng.random((n, 1, 64)))
+    parts = [quantize(from_bits(to_bits(x.astype(np.float32), dtype), dtype).astype(np.float32), 32, dtype) for x in (k, v)]
+    b.host.put(b.table[0][np.arange(n) // 16] * 16 + np.arange(n) % 16, *parts)
+    b.k[0], b.v[0] = (dequantize(*p, 32, dtype) for p in parts)
+    b.q_bits = to_bits(np.ones(b.q.shape, np.float32), dtype)
+    b.q = np.ones(b.q.shape)
+    want, _ = b.expect(scale=0.125)
+    got = from_bits(b.run(scale=0.125), dtype).astype(np.float64)
+    w = np.exp(-8.0 * size)  # 64 dimensions of 1 x size, scale 1/8
+    unit = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+    tiny = 2.0 ** -25 if dtype == "f16" else 0.0  # subnormal outputs
+    limit = 1.02 * (unit + 2.0 ** -10 + 2.0 ** -35 / w) * np.abs(want) + tiny
+    assert (np.abs(got - want) <= limit).all(), (np.abs(got - want) / np.abs(want)).max()
