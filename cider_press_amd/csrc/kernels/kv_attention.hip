@@ -37,6 +37,11 @@
 // TFLOP/s (a large f16 product of the library: 1322), with the vector pipes busy for
 // 55% of the cycles, the matrix pipes for 43%, both at once for 18%.
 //
+// A tile whose tokens are too far apart for one exponent is staged and multiplied again
+// for each set of them that goes together (kv_common.hpp), its words loaded once more
+// each time; that, like all that is rare, lies outside the loop's straight line (with it
+// inside the line 7 % were lost).
+//
 // Where there are few row tiles their keys are split, evenly over the resident
 // workgroups by the lengths on the device, and joined, in part order, by the last
 // to arrive.
@@ -58,11 +63,11 @@ constexpr float kRaise = 10.f;
 constexpr float kMost = 65504.f;  // of 16 weights' sum, so that each fits f16
 // What a wave publishes of its half of a tile: the exponent (0: all constants so
 // far are zeros), which 16 keys have their block, whether a value constant is not
-// finite.
-constexpr int kExpBias = 1 << 12, kOkShift = 16, kPoison = 1 << 20;
-// Halves of values whose exponents differ by no more than this are joined by
-// smaller weights, others are dequantized again to the same exponent.
-constexpr int kMostApart = 10;
+// finite, whether its tokens are too far apart for one exponent.
+constexpr int kExpBias = 1 << 12, kOkShift = 16, kPoison = 1 << 20, kApart = 1 << 21;
+// Halves of values whose exponents differ by no more than this are joined by smaller
+// weights; others are too far apart.
+constexpr int kMostApart = 4;
 
 struct TileArgs {
   cpq_kv_cache c;
@@ -131,37 +136,54 @@ __device__ __forceinline__ void load_values(Packed<D>& t, const cpq_kv_cache& c,
   }
 }
 
-// A wave's running exponent for the constants it has met, and the limits that
-// go with it.
-struct Range {
-  int e = 0;
-  uint32_t limits = 0;
-};
-template <typename TT>
-__device__ __forceinline__ void raise(Range& r, float largest_size) {
-  const int e = size_exponent(wave_max(largest_size));
-  if (r.limits == 0 || e > r.e) {
-    r.e = e;
-    r.limits = size_limits<TT>(e);
-  }
+// Exponents of constants as `Packed` has them: of a lane's key (a lane each, both halves the
+// same), of the eight keys that a lane's values are of.
+template <typename TT, int NK>
+__device__ __forceinline__ int key_exponent(const uint32_t* sb) {
+  float f = 0.f;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) f = fmaxf(f, finite_size<TT>(sb[i]));
+  const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(f), __float_as_uint(f), false, false);
+  return size_exponent(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+}
+template <typename TT, int D>
+__device__ __forceinline__ int value_exponent(const u32x4* sb, int e) {
+  float f = 0.f;
+#pragma unroll
+  for (int v = 0; v < Packed<D>::VS; ++v) f = fmaxf(f, finite_size<TT>(sb[2 * v + (e >> 2)][e & 3]));
+  int x = size_exponent(f);  // the largest over the words: 8 or 16 neighbouring lanes
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0xB1, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x4E, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x141, 0xf, 0xf, false));
+  if (D > 64) x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x140, 0xf, 0xf, false));
+  return x;
 }
 
-// 32 keys (key0 .. in the tile) as operands.
-template <typename TT, int D>
-__device__ __forceinline__ void store_keys(const Packed<D>& t, u32x4* lds, int key0, int lane, Range& range,
-                                           bool live) {
+// 32 keys (key0 .. in the tile) as operands.  FIT: the exponent is moved to what they
+// need; returns whether some are too small for it.
+template <typename TT, int D, bool FIT>
+__device__ __forceinline__ bool store_keys(const Packed<D>& t, u32x4* lds, int key0, int lane, KvRange& range, bool live) {
   constexpr int W = D / 8, NK = Packed<D>::NK;
-  uint32_t sb[NK], m = range.limits;
+  bool apart = false;
+  uint32_t sb[NK];
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
-    sb[i] = live ? t.sb[0][i] : 0u;
-    m = sizes(m, sb[i]);
-  }
-  if (__any(m != range.limits)) {
-    float f = 0.f;
+  for (int i = 0; i < NK; ++i) sb[i] = live ? t.sb[0][i] : 0u;
+  if (FIT) {
+    uint32_t m = 0u, l = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) f = fmaxf(f, finite_size<TT>(sb[i]));
-    raise<TT>(range, f);
+    for (int i = 0; i < NK; ++i) {
+      m = sizes(m, sb[i]);
+      l = smallest(l, sb[i]);
+    }
+    if (!live) l = 0xffffffffu;
+    if (__builtin_expect(!__all(range.holds(m, l)), 0)) {
+      if (__all(all_finite<TT>(m))) range.template fit<TT>(max_of_wave(size_exponent(finite_size<TT>(m))));
+      if (!__all(range.holds(m, l))) {
+        const int x = key_exponent<TT, NK>(sb);
+        range.template fit<TT>(max_of_wave(x));
+        apart = __any(!range.takes(x));
+      }
+    }
   }
   const int key = key0 + (lane & 31), half = lane >> 5;
 #pragma unroll
@@ -172,39 +194,68 @@ __device__ __forceinline__ void store_keys(const Packed<D>& t, u32x4* lds, int k
     for (int e = 0; e < 4; ++e)
       lds[key_unit<W>(key, half * (W / 2) + 4 * i + e)] = key_slice(t.q[i][e], s0, s1, b0);
   }
+  return apart;
 }
 
-// 32 keys' values (half k steps ts0 ..) as operands; returns whether a
-// constant was not finite (those count as zeros).
-template <typename TT, int D>
-__device__ __forceinline__ bool store_values(Packed<D>& t, u32x4* lds, int ts0, int lane, Range& range,
-                                             uint32_t live) {
+// 32 keys' values (half k steps ts0 ..) as operands, likewise; `poison`: a constant was
+// not finite (those count as zeros).
+template <typename TT, int D, bool FIT>
+__device__ __forceinline__ bool store_values(const Packed<D>& t, u32x4* lds, int ts0, int lane, KvRange& range,
+                                             uint32_t live, bool& poison) {
   constexpr int W = D / 8, L = W < 16 ? 8 : 16, VS = Packed<D>::VS;
-  uint32_t m = range.limits;
+  bool apart = false;
+  u32x4 sb[2 * VS];
+#pragma unroll
+  for (int i = 0; i < 2 * VS; ++i) sb[i] = t.sb[i];
+  uint32_t out0 = 0u, out1 = 0u;  // of the lane's own two keys: not live
   if (live != 0xffu) {
 #pragma unroll
     for (int i = 0; i < 2 * VS; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) t.sb[i][e] = live >> (4 * (i & 1) + e) & 1 ? t.sb[i][e] : 0u;
+      for (int e = 0; e < 4; ++e) sb[i][e] = live >> (4 * (i & 1) + e) & 1 ? sb[i][e] : 0u;
+    out0 = live >> (lane & 3) & 1 ? 0u : 0xffffffffu;
+    out1 = live >> (4 + (lane & 3)) & 1 ? 0u : 0xffffffffu;
   }
+  // The lanes of a group's words have the same constants: four neighbours look at a
+  // quarter of them each.
+  uint32_t m = 0u, l = 0xffffffffu;
+  if (FIT) {
 #pragma unroll
-  for (int i = 0; i < 2 * VS; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = sizes(m, t.sb[i][e]);
-  bool poison = false;
-  if (__any(m != range.limits)) {
-    float f = 0.f;
+    for (int i = 0; i < 2 * VS; ++i) {
+      const uint32_t a = lane & 1 ? sb[i][1] : sb[i][0], b = lane & 1 ? sb[i][3] : sb[i][2], mine = lane & 2 ? b : a;
+      m = sizes(m, mine);
+      l = smallest(l, mine | (i & 1 ? out1 : out0));
+    }
+  }
+  bool fits = FIT && __all(range.holds(m, l));
+  if (FIT && __builtin_expect(!fits, 0) && __all(all_finite<TT>(m))) {
+    range.template fit<TT>(max_of_wave(size_exponent(finite_size<TT>(m))));
+    fits = __all(range.holds(m, l));
+  }
+  if (!FIT || __builtin_expect(!fits, 0)) {
+    bool bad = false;
 #pragma unroll
     for (int i = 0; i < 2 * VS; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        f = fmaxf(f, finite_size<TT>(t.sb[i][e]));
-        const bool ok = finite(TT::lo(t.sb[i][e])) && finite(TT::hi(t.sb[i][e]));
-        poison |= !ok;
-        t.sb[i][e] = ok ? t.sb[i][e] : 0u;
+        const bool ok = finite(TT::lo(sb[i][e])) && finite(TT::hi(sb[i][e]));
+        bad |= !ok;
+        sb[i][e] = ok ? sb[i][e] : 0u;
       }
-    raise<TT>(range, f);
-    poison = __any(poison);
+    poison = __any(bad);
+    if (FIT) {
+      int x[8], top = kKvNone;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = value_exponent<TT, D>(sb, e);
+        top = max(top, x[e]);
+      }
+      range.template fit<TT>(max_of_wave(top));
+      bool out = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) out |= !range.takes(x[e]);
+      apart = __any(out);
+    }
   }
   const int ts = ts0 + (lane / L & 3);
 #pragma unroll
@@ -212,7 +263,7 @@ __device__ __forceinline__ bool store_values(Packed<D>& t, u32x4* lds, int ts0, 
     uint32_t s0[4], s1[4], b0[4];
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
-      const uint32_t c0 = t.sb[2 * v + (x >> 1)][2 * (x & 1)], c1 = t.sb[2 * v + (x >> 1)][2 * (x & 1) + 1];
+      const uint32_t c0 = sb[2 * v + (x >> 1)][2 * (x & 1)], c1 = sb[2 * v + (x >> 1)][2 * (x & 1) + 1];
       s0[x] = F16::pack2(scaled(TT::lo(c0), 24 - range.e), scaled(TT::lo(c1), 24 - range.e));
       b0[x] = F16::pack2(scaled(TT::hi(c0), -range.e), scaled(TT::hi(c1), -range.e));
       s1[x] = sixteenth(s0[x]);
@@ -236,7 +287,7 @@ __device__ __forceinline__ bool store_values(Packed<D>& t, u32x4* lds, int ts0, 
       lds[value_unit(8 * w + 2 * (y + y0) + 1, ts)] = hi;
     }
   }
-  return poison;
+  return apart;
 }
 
 // What a workgroup does: rows tile `qt` of a sequence, a head, a part of the keys.
@@ -313,6 +364,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
   extern __shared__ u32x4 units[];  // [kBufs][keys, values][kUnits]
   __shared__ int meta[kBufs][4];         // of the halves' keys, then their values
   __shared__ unsigned int arrived;
+  __shared__ int exponents[2][kKeys];    // of tokens too far apart: keys, values
   constexpr int kRows = 32 * kWaves;
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
@@ -373,27 +425,28 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     for (int e = 0; e < 16; ++e) o[j][e] = 0.f;
   float ref = -FLT_MAX, sum = 0.f;
   uint32_t nan_groups = 0;             // groups of dimensions that are NaN in this row
-  int ev = -1000;                      // o, so far zeros, is in units of 2^ev
+  int unit = 0;                        // o is in units of 2^unit
   float cl0 = 0.f, cl1 = 0.f;          // of the halves: log2(e) * scale * 2^(exponents of q and the keys)
-  int d0 = 0, d1 = 0;                  // and the values' exponents less ev
+  int ve = 0, d0 = 0, d1 = 0;          // the values' exponent, and the halves' less that
+  int alike = 0;                       // the rows' units are ve
 
   // Staging: of each four waves two keys and two values of the tile's halves.
   const uint32_t* __restrict__ blocks = a.block_table + (size_t)it.s * a.max_blocks;
   const int team = wave >> 2;
   const bool is_values = ((wave >> 1) ^ team) & 1;  // on each SIMD one wave of either kind
   const int half = wave & 1;
-  Range range;
+  KvRange range;
   Packed<D> packed;
   int loaded_ok = 3;
   // The blocks of this half of 32 tiles, a lane each 16 keys (scalar loads in
   // flight would make every LDS wait a wait for all).
   uint32_t ids = 0;
-  auto load = [&](int t, bool again) {
+  auto load = [&](int t) {
     const int lane = (int)opaque((uint32_t)(tid & 63));
     const int key = t * kKeys + half * 32;
     const int l = 2 * ((t - begin) / kTeams & 31);
-    if (l == 0 || again)
-      ids = blocks[min((t + kTeams * ((lane - l) >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1) >> bs_shift];
+    if (l == 0)
+      ids = blocks[min((t + kTeams * (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1) >> bs_shift];
     const KvPlaces pl = kv_places(c, (uint32_t)__builtin_amdgcn_readlane((int)ids, l),
                                   (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1), min(key, (q.n - 1) & ~15), q.n,
                                   head, bs_shift);
@@ -401,37 +454,45 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     if (is_values) load_values<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
     else load_keys<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
   };
+  // The words of a tile that `load` has taken already.
+  auto load_again = [&](int t) {
+    asm volatile("" : "+s"(t));  // (addresses made here, not ahead of the branch)
+    const int lane = (int)opaque((uint32_t)(tid & 63));
+    const int key = t * kKeys + half * 32;
+    const KvPlaces pl = kv_places(c, blocks[min(key, q.n - 1) >> bs_shift], blocks[min(key + 16, q.n - 1) >> bs_shift],
+                                  min(key, (q.n - 1) & ~15), q.n, head, bs_shift);
+    if (is_values) load_values<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
+    else load_keys<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
+  };
+  // The half's keys of which bit k of `seen` (from key 32 * half on) is set.
+  auto live_values = [&](uint32_t seen, int lane) {
+    const int ts = lane / (W < 16 ? 8 : 16) & 3;
+    seen >>= 16 * (ts >> 1) + 4 * (ts & 1);
+    return (seen & 15u) | (seen >> 4 & 0xf0u);
+  };
   auto store = [&](int t, int buf) {
     // (The lane hidden from the optimiser: addresses made anew each time take a few
     // instructions, kept through the loop they spill registers.)
     const int lane = (int)opaque((uint32_t)(tid & 63));
     u32x4* keys = units + buf * 2 * kUnits;
     const int key = t * kKeys + half * 32;
-    const bool all = key >= from && key + 32 <= q.n && loaded_ok == 3;
+    const bool all = key >= from && key + 32 <= end && loaded_ok == 3;
     // (Of the keys [from, end) each is seen by one of the rows.)
     if (!all && !is_values && lane == 0 &&
         ((!(loaded_ok & 1) && key < end && key + 16 > from) || (!(loaded_ok & 2) && key + 16 < end && key + 32 > from)))
       atomicAdd(p.bad, 1u);
-    bool poison = false;
-    if (is_values) {
-      uint32_t live = 0xff;
-      if (!all) {
-        const int ts = lane / (W < 16 ? 8 : 16) & 3;
-        live = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = key + 16 * (ts >> 1) + 4 * (ts & 1) + (e & 3) + 8 * (e >> 2);
-          live |= (uint32_t)(k >= from && k < q.n && (loaded_ok >> (ts >> 1) & 1)) << e;
-        }
-      }
-      poison = store_values<TT, D>(packed, keys + kUnits, 4 * half, lane, range, live);
-    } else {
-      const int k = key + (lane & 31);
-      const bool live = all || (k >= from && k < q.n && (loaded_ok >> (lane >> 4 & 1) & 1));
-      store_keys<TT, D>(packed, keys, 32 * half, lane, range, live);
-    }
+    const uint32_t seen = all ? 0xffffffffu
+                              : range_bits(from - key, end - key) &
+                                    ((loaded_ok & 1 ? 0xffffu : 0u) | (loaded_ok & 2 ? 0xffff0000u : 0u));
+    bool poison = false, apart;
+    if (is_values)
+      apart = store_values<TT, D, true>(packed, keys + kUnits, 4 * half, lane, range,
+                                        all ? 0xffu : live_values(seen, lane), poison);
+    else
+      apart = store_keys<TT, D, true>(packed, keys, 32 * half, lane, range, all || (seen >> (lane & 31) & 1));
     if (lane == 0)
-      meta[buf][2 * is_values + half] = (range.limits ? range.e + kExpBias : 0) + (loaded_ok << kOkShift) + (poison ? kPoison : 0);
+      meta[buf][2 * is_values + half] = (range.high ? range.e + kExpBias : 0) + (loaded_ok << kOkShift) +
+                                        (poison ? kPoison : 0) + (apart ? kApart : 0);
   };
 
   // Byte offsets of the lane's operands in LDS; the half of LDS in turn is the
@@ -450,58 +511,129 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     return *reinterpret_cast<const u32x4*>(lds + at_value[k] + j * (32 * 8 * 16));
   };
 
-  if (begin + team < stop) load(begin + team, false);
+  if (begin + team < stop) load(begin + team);
   if (begin + team < stop) {
     store(begin + team, team);
-    if (begin + team + kTeams < stop) load(begin + team + kTeams, false);
+    if (begin + team + kTeams < stop) load(begin + team + kTeams);
   }
   __syncthreads();
-  int known = -1, ok = 0;  // the published words that cl, d and ok are of
-  bool poison = false;
-  for (int t = begin; t < stop; ++t) {
-    const int buf = (t - begin) & (kBufs - 1);
-    int news = meta[buf][lane & 3];
-    if (__any(news != known)) {
-      auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
-      auto exponent = [&](int i, int none) { return word(i) & 0xffff ? (word(i) & 0xffff) - kExpBias : none; };
-      const int e = max(ev, max(exponent(2, ev), exponent(3, ev)));  // o's unit: the largest exponent so far
-      const int own = is_values ? e : max(exponent(0, range.e), exponent(1, range.e));
-      if (own > range.e) {  // the keys, and the values, share the largest from here on
-        range.e = own;
-        range.limits = size_limits<TT>(own);
-      }
-      if (e - min(exponent(2, e), exponent(3, e)) > kMostApart) {  // (all waves alike: they read the same words)
-        __syncthreads();
-        if (is_values && (t - begin) % kTeams == team) {
-          load(t, true);
-          store(t, buf);
-          if (t + kTeams < stop) load(t + kTeams, true);
-        }
-        __syncthreads();
-        news = meta[buf][lane & 3];
-      }
-      known = news;
-      poison = (word(2) | word(3)) >= kPoison;
-      ok = (word(0) >> kOkShift & 3) | (word(1) >> kOkShift & 3) << 2;
-      cl0 = fmaxf(scaled(a.scale * kLog2e, exponent(0, 0) + qe), FLT_MIN);
-      cl1 = fmaxf(scaled(a.scale * kLog2e, exponent(1, 0) + qe), FLT_MIN);
-      d0 = exponent(2, e) - e;
-      d1 = exponent(3, e) - e;
-      if (e != ev) {
+  int known = -1;     // the published words that what follows is of
+  uint64_t keep = 0;  // keys that are there
+  int poison = 0, apart = 0;  // (uniform, in scalar registers)
+  // The units of the rows that see some of the tile's keys `keep`.
+  auto rescale = [&](int key0) {
+    asm volatile("" : "+s"(key0));  // (what follows is made here, not kept)
+    const int lo = see_from - key0, hi = see_to - key0;
+    const uint64_t seen = (uint64_t)range_bits(lo, hi) | (uint64_t)range_bits(lo - 32, hi - 32) << 32;
+    if (ref == -FLT_MAX) unit = ve;  // nothing yet
+    int next = seen & keep ? ve : unit;
+    if (__any(next != unit)) {
+      if (__any(next < unit)) {
+        float m = 0.f;
 #pragma unroll
         for (int j = 0; j < ND; ++j)
 #pragma unroll
-          for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], ev - e);
-        ev = e;
+          for (int x = 0; x < 16; ++x) m = fmaxf(m, fabsf(o[j][x]));
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+        m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        next = next < unit ? lower_unit(unit, next, m) : next;
       }
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[j][x] = scaled(o[j][x], unit - next);
+      unit = next;
+    }
+    alike = __builtin_amdgcn_readfirstlane((int)!__any(unit != ve));
+  };
+  for (int t = begin; t < stop; ++t) {
+    const int buf = (t - begin) & (kBufs - 1), key0 = t * kKeys;
+    const int news = meta[buf][lane & 3];
+    if (__builtin_expect(__any(news != known), 0)) {
+      auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
+      auto exponent = [&](int i) { return word(i) & 0xffff ? (word(i) & 0xffff) - kExpBias : kKvNone; };
+      const int k0 = exponent(0), k1 = exponent(1), v0 = exponent(2), v1 = exponent(3);
+      // The keys, and the values, of all waves share the largest where it is near, so
+      // that the words change seldom.
+      const int own = is_values ? max(v0, v1) : max(k0, k1);
+      if (range.high && own > range.e && own <= range.e + kKvKeep) range.set<TT>(own);
+      const int any = word(0) | word(1) | word(2) | word(3);
+      poison = any & kPoison;
+      apart = any & kApart;
+      if (min(v0, v1) != kKvNone && abs(v0 - v1) > kMostApart) apart = kApart;
+      const uint32_t there0 = word(0) >> kOkShift & 3, there1 = word(1) >> kOkShift & 3;
+      keep = (uint64_t)((there0 & 1) * 0xffffu | (there0 >> 1) * 0xffff0000u) |
+             (uint64_t)((there1 & 1) * 0xffffu | (there1 >> 1) * 0xffff0000u) << 32;
+      if (!apart) {
+        cl0 = fmaxf(scaled(a.scale * kLog2e, (k0 == kKvNone ? 0 : k0) + qe), FLT_MIN);
+        cl1 = fmaxf(scaled(a.scale * kLog2e, (k1 == kKvNone ? 0 : k1) + qe), FLT_MIN);
+        if (max(v0, v1) != kKvNone) ve = max(v0, v1);
+        d0 = v0 == kKvNone ? 0 : v0 - ve;
+        d1 = v1 == kKvNone ? 0 : v1 - ve;
+        rescale(key0);
+      }
+      known = alike ? news : -1;  // (else again at the next tile)
     }
     if (t + kTeams < stop && (t - begin) % kTeams == team) {
       store(t + kTeams, (t + kTeams - begin) & (kBufs - 1));
-      if (t + 2 * kTeams < stop) load(t + 2 * kTeams, false);
+      if (t + 2 * kTeams < stop) load(t + 2 * kTeams);
     }
-    const int key0 = t * kKeys;
-    if (key0 < any_to && key0 + kKeys > any_from) {
-      const bool whole = key0 >= all_from && key0 + kKeys <= all_to && ok == 15;
+    uint64_t left = 0;  // keys that some row sees, of a tile whose tokens are taken in passes
+    const bool mine = (t - begin) % kTeams == team;
+    if (__builtin_expect(apart != 0, 0)) {
+      __syncthreads();
+      if (mine) {
+        load_again(t);
+        const int lane = (int)opaque((uint32_t)(tid & 63));
+        if (is_values) {
+          const int ts = lane / (W < 16 ? 8 : 16) & 3;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int x = value_exponent<TT, D>(packed.sb, e);
+            if (lane % (W < 16 ? 8 : 16) == 0)
+              exponents[1][32 * half + 16 * (ts >> 1) + 4 * (ts & 1) + (e & 3) + 8 * (e >> 2)] = x;
+          }
+        } else {
+          uint32_t sb[Packed<D>::NK];
+#pragma unroll
+          for (int i = 0; i < Packed<D>::NK; ++i) sb[i] = packed.sb[0][i];
+          const int x = key_exponent<TT, Packed<D>::NK>(sb);
+          if (lane < 32) exponents[0][32 * half + lane] = x;
+        }
+      }
+      __syncthreads();
+      left = keep & __ballot(key0 + lane >= from && key0 + lane < end);
+    }
+    do {
+      if (__builtin_expect(apart != 0, 0)) {
+        const int kx = exponents[0][lane], vx = exponents[1][lane];
+        KvRange kr, vr;
+        bool in = left >> lane & 1;
+        vr.fit<TT>(max_of_wave(in ? vx : kKvNone));
+        in = in && vr.takes(vx);
+        kr.fit<TT>(max_of_wave(in ? kx : kKvNone));
+        keep = __ballot(in && kr.takes(kx));
+        left &= ~keep;
+        __syncthreads();  // (the reads of the pass before)
+        if (mine) {
+          load_again(t);
+          const int lane = (int)opaque((uint32_t)(tid & 63));
+          u32x4* keys = units + buf * 2 * kUnits;
+          const uint32_t seen = (uint32_t)(keep >> (32 * half));
+          bool bad;
+          if (is_values)
+            store_values<TT, D, false>(packed, keys + kUnits, 4 * half, lane, vr, live_values(seen, lane), bad);
+          else
+            store_keys<TT, D, false>(packed, keys, 32 * half, lane, kr, seen >> (lane & 31) & 1);
+        }
+        __syncthreads();
+        cl0 = cl1 = fmaxf(scaled(a.scale * kLog2e, kr.e + qe), FLT_MIN);
+        if (vr.high) ve = vr.e;
+        d0 = d1 = 0;
+        rescale(key0);
+      }
+      if (key0 >= any_to || key0 + kKeys <= any_from) continue;
+      const bool whole = key0 >= all_from && key0 + kKeys <= all_to && keep == ~0ull;
       // Operands are read a step ahead of the matrix instructions that take them, and
       // the weights of one half of the keys are made between those of the other.
       f32x16 sc[2];
@@ -509,16 +641,14 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       u32x4 op[kAhead], pw[kKeys / 16], vop[2][ND];
       float add[2] = {0.f, 0.f};
       auto mask = [&](int u) {
-        if (whole) return;
-        // Of the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
+        if (__builtin_expect(whole, 1)) return;
+        // From the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
         // the scalar registers and every tile selects.)
-        int lo = see_from - key0 - 4 * h, hi = see_to - key0 - 4 * h;
-        asm volatile("" : "+v"(lo), "+v"(hi));
+        int at = key0 + 32 * u;
+        asm volatile("" : "+s"(at));
+        const uint32_t seen = (range_bits(see_from - at, see_to - at) & (uint32_t)(keep >> (32 * u))) >> (4 * h);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int k = 32 * u + 8 * (x >> 2) + (x & 3);
-          sc[u][x] = k >= lo && k < hi && (ok >> (2 * u + (x >> 3)) & 1) ? sc[u][x] : -INFINITY;
-        }
+        for (int x = 0; x < 16; ++x) sc[u][x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? sc[u][x] : -INFINITY;
       };
       auto weights = [&](int u, float rel, int i) {  // two of a half's
         const float cl = u ? cl1 : cl0;
@@ -531,7 +661,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       // Where a weight of half u left f16's range: a new reference, the weights again.
       auto settle = [&](int u) {
         const uint64_t redo = __ballot(!(add[u] < kMost));
-        if (redo) {
+        if (__builtin_expect(redo != 0, 0)) {
           const float cl = u ? cl1 : cl0;
           float mine = sc[u][0];
 #pragma unroll
@@ -552,6 +682,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
           for (int i = 0; i < 8; ++i) weights(u, rel, i);
         }
         sum += scaled(add[u], u ? -d1 : -d0);
+        // (A row whose sums are beyond these values by all that fp32 holds leaves them out.)
+        if (__builtin_expect(!alike, 0)) {
+          uint32_t with = unit == ve ? 0xffffffffu : 0u;
+          asm volatile("" : "+v"(with));  // (a branch, not selections in every tile)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            pw[2 * u][x] &= with;
+            pw[2 * u + 1][x] &= with;
+          }
+        }
       };
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) op[i] = key_operand(i / NS, i % NS);
@@ -596,12 +736,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
           fence();
         }
       }
-      if (poison) {
+    } while (__builtin_expect(left != 0, 0));
+    if (__builtin_expect(poison != 0, 0) && key0 < any_to && key0 + kKeys > any_from) {
 #pragma clang loop unroll(disable)
-        for (int k = 0; k < kKeys && key0 + k < q.n; k += 16)
-          nan_groups |= poisoned_groups<TT>(c, kv_place(c, blocks[(key0 + k) >> bs_shift], key0 + k, head, bs_shift),
-                                            key0 + k, W >> gw_shift, see_from, see_to);
-      }
+      for (int k = 0; k < kKeys && key0 + k < q.n; k += 16)
+        nan_groups |= poisoned_groups<TT>(c, kv_place(c, blocks[(key0 + k) >> bs_shift], key0 + k, head, bs_shift),
+                                          key0 + k, W >> gw_shift, see_from, see_to);
+    }
+    if (__builtin_expect(apart != 0, 0)) {
+      known = -1;
+      if (mine && t + 2 * kTeams < stop) load_again(t + 2 * kTeams);
     }
     const uint32_t next = kTeams > 1 && (t - begin) % kTeams ? 3 * kHalf : kHalf;
 #pragma unroll
@@ -637,8 +781,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       for (int j = 0; j < ND; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          put(4 * j + x, f32x4{scaled(o[j][4 * x], ev), scaled(o[j][4 * x + 1], ev),
-                               scaled(o[j][4 * x + 2], ev), scaled(o[j][4 * x + 3], ev)});
+          put(4 * j + x, f32x4{scaled(o[j][4 * x], unit), scaled(o[j][4 * x + 1], unit),
+                               scaled(o[j][4 * x + 2], unit), scaled(o[j][4 * x + 3], unit)});
       put(D / 8, f32x4{ref, sum, 0.f, 0.f});
     }
     __builtin_amdgcn_s_waitcnt(0);
@@ -650,7 +794,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     const int joined = idle ? 0 : parts;
     for (int k = 0; k < joined; ++k) m = fmaxf(m, get(k, D / 8)[0]);
     sum = 0.f;
-    ev = 0;
+    unit = 0;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
@@ -684,8 +828,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
 #pragma unroll
     for (int x = 0; x < 4; ++x)
       *reinterpret_cast<u32x2*>(out + 32 * j + 8 * x) =
-          u32x2{TT::pack2(scaled(o[j][4 * x] * inv, ev), scaled(o[j][4 * x + 1] * inv, ev)),
-                TT::pack2(scaled(o[j][4 * x + 2] * inv, ev), scaled(o[j][4 * x + 3] * inv, ev))};
+          u32x2{TT::pack2(scaled(o[j][4 * x] * inv, unit), scaled(o[j][4 * x + 1] * inv, unit)),
+                TT::pack2(scaled(o[j][4 * x + 2] * inv, unit), scaled(o[j][4 * x + 3] * inv, unit))};
 }
 
 template <typename TT, int D, int kWaves>

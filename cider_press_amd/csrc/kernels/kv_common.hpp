@@ -4,12 +4,17 @@
 // a 16-bit half reads as the f16 subnormal q * 2^-24 (q * 2^-20), so one AND
 // extracts two of them and one v_pk_fma_f16 makes two values
 //   (s * 2^(24 - E)) * (q * 2^-24) + b * 2^-E = (s q + b) * 2^-E
-// with a single rounding.  E, uniform over the wave, keeps the largest constant of
-// the keys (of the values) met so far, max(|b|, 16 |s|), within 2^(E - 5): then
+// with a single rounding.  E, the same for the keys (the values) of one product, is
+// chosen by the largest constant among them, max(|b|, 16 |s|) within 2^(E - 5): then
 // s * 2^(24 - E) <= 2^15 fits f16, whatever T's range.  A value is off by at most
 // 2^-11 of itself or, where it lies among f16's subnormals, by its bias's rounding
-// and its own, 2^-19 each of that largest.  E rises when a tile brings a larger
-// constant.
+// and its own, 2^-19 each of 2^(E - 5).
+//
+// Tokens whose constants are far apart do not share a product, or the largest would
+// take the others' bits, also from rows that do not see it.  E stays from tile to tile
+// while it holds every token (their largest constants within (2^(E - 12), 2^(E - 5)]),
+// so any of them is off by 2^-11 of its largest at most; else the tile's tokens are taken in
+// passes, the largest first (a softmax takes its keys in any portions).  A row's sums change their unit where a product that it sees has another.
 //
 // fp32 operands would run the matrix instructions at a sixteenth of the rate.  What
 // one rounding each of keys, values and weights costs: nothing at T = bf16, where
@@ -28,7 +33,10 @@
 namespace cpq {
 namespace dev {
 
-constexpr int kKvTop = 5;  // constants stay below 2^(E - kKvTop)
+constexpr int kKvTop = 5;    // constants stay below 2^(E - kKvTop)
+constexpr int kKvBand = 6;   // exponents of tokens are E - kKvBand .. E
+constexpr int kKvKeep = 2;   // E stays while it is at most this much more than a tile needs
+constexpr int kKvNone = -1000;  // the exponent of a token whose constants are zero: fits all
 constexpr float kLog2e = 1.44269504088896340736f;
 
 __device__ __forceinline__ f16x2 as_f16x2(uint32_t v) { return __builtin_bit_cast(f16x2, v); }
@@ -46,11 +54,15 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 
 // The largest |scale| and |bias| of constants as T patterns in one word (both
 // types order like integers; Inf and NaN come last).
-__device__ __forceinline__ uint32_t sizes(uint32_t m, uint32_t sb) {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
-                                                                __builtin_bit_cast(u16x2, sb & 0x7fff7fffu)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
+__device__ __forceinline__ uint32_t pk_min(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ uint32_t sizes(uint32_t m, uint32_t sb) { return pk_max(m, sb & 0x7fff7fffu); }
+__device__ __forceinline__ uint32_t smallest(uint32_t m, uint32_t sb) { return pk_min(m, sb & 0x7fff7fffu); }
 // What `sizes` may reach at exponent E: scales 2^(E - 9), biases 2^(E - 5), finite.
 template <typename TT>
 __device__ __forceinline__ uint32_t size_limits(int e) {
@@ -58,17 +70,54 @@ __device__ __forceinline__ uint32_t size_limits(int e) {
   const uint32_t s = TT::from_f32(scaled(1.f, e - kKvTop - 4)), b = TT::from_f32(scaled(1.f, e - kKvTop));
   return min(s, top) | min(b, top) << 16;
 }
+// Whether `sizes` of constants has none that is not finite.
+template <typename TT>
+__device__ __forceinline__ bool all_finite(uint32_t m) {
+  return finite(TT::lo(m)) && finite(TT::hi(m));
+}
 // max(|b|, 16 |s|) of a constant, 0 where it is not finite.
 template <typename TT>
 __device__ __forceinline__ float finite_size(uint32_t sb) {
   const float s = fabsf(TT::lo(sb)), b = fabsf(TT::hi(sb));
   return s <= FLT_MAX && b <= FLT_MAX ? fminf(fmaxf(b, 16.f * s), FLT_MAX) : 0.f;
 }
-// The exponent for constants up to m.
-__device__ __forceinline__ int size_exponent(float m) { return max(exponent_above(m), -110) + kKvTop; }
+// The exponent for constants up to m; none for zeros.
+__device__ __forceinline__ int size_exponent(float m) {
+  return m > 0.f ? max(exponent_above(m), -110) + kKvTop : kKvNone;
+}
+// An exponent E with what goes with it: the limits of sizes that it holds, and sizes
+// at or below which a token may be too small for it.
+struct KvRange {
+  int e = 0;
+  uint32_t high = 0, low = 0;
+  // m, l: `sizes` and `smallest` of constants.  False where one may not fit (a small
+  // bias of one and a small scale of another look like a small token).
+  __device__ __forceinline__ bool holds(uint32_t m, uint32_t l) const {
+    return (pk_max(m, high) == high) & (pk_max(l, low) != low);
+  }
+  template <typename TT>
+  __device__ __forceinline__ void set(int to) {
+    e = to;
+    high = size_limits<TT>(to);
+    low = size_limits<TT>(to - kKvBand - 1);
+  }
+  // For tokens whose largest exponent is `need`; takes(x): those it holds.
+  template <typename TT>
+  __device__ __forceinline__ void fit(int need) {
+    if (need != kKvNone && (high == 0 || need > e || need < e - kKvKeep)) set<TT>(need);
+  }
+  __device__ __forceinline__ bool takes(int x) const { return x == kKvNone || (x <= e && x >= e - kKvBand); }
+};
 
 // Until the wave's LDS reads and writes are done.
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14)); }
+
+// Bits [lo, hi) of 32 keys.
+__device__ __forceinline__ uint32_t range_bits(int lo, int hi) {
+  lo = min(max(lo, 0), 32);
+  hi = min(max(hi, 0), 32);
+  return (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
+}
 
 // Over the lanes that differ in bits 4 and 5 (16 columns are left).
 template <typename F>
@@ -82,10 +131,32 @@ __device__ __forceinline__ float over_rows(float v, F f) {
 }
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+// The exponent of the unit that a row's sums take, of which `largest_sum` in units of 2^was
+// is the largest, where a product comes in units of 2^to below that: not beyond what
+// fp32 holds.
+__device__ __forceinline__ int lower_unit(int was, int to, float largest_sum) {
+  return largest_sum > 0.f ? min(max(to, was + exponent_above(largest_sum) - 120), was) : to;
+}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
+}
+
+// The largest of 16 columns' values that the wave's rows share, in a scalar register.
+__device__ __forceinline__ int max_of_columns(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x128, 0xf, 0xf, false));  // row_ror 8, 4, 2, 1
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x124, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x122, 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x121, 0xf, 0xf, false));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+__device__ __forceinline__ int max_of_wave(int v) {
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max_of_columns(max((int)b[0], (int)b[1]));
 }
 
 // Inclusive sum over the wave: within rows of 16 lanes, then from row to row.

@@ -134,7 +134,7 @@ __device__ __forceinline__ void start_tile(const cpq_kv_cache& c, size_t row_a, 
   }
 }
 
-// A wave's running result: o in units of 2^ev, relative to 2^ref per row.
+// A wave's running result, relative to 2^ref per row.
 template <typename TT, int D, int GS, int NC>
 struct Rows {
   using X = Geo<D, GS>;
@@ -147,44 +147,75 @@ struct Rows {
   u32x4 qs[NC][X::WL];
   u32x4 qsum[NC];  // sums over a lane's words of each group, in units of 2^6: high and low part
   int qe[NC];    // exponents of the query rows
-  float cl[NC];  // log2(e) * scale * 2^(qe + ek)
+  float cl[NC];  // log2(e) * scale * 2^(qe + keys.e)
   f32x4 o[X::VS][X::NJ][NC];
   float top[NC], ref[NC], sum[NC];
-  int ek = 0, ev = 0;  // exponents of keys and values; zeros alone fit them so far
-  uint32_t klim = 0, vlim = 0;
+  int unit[NC];         // of a row's sums o: 2^unit
+  KvRange keys, values;  // of the operands
+  bool alike = false;   // every row's unit is the values' exponent
 
-  // Raises the exponents to a tile's constants.
-  __device__ __forceinline__ void raise(float km, float vm, float scale) {
-    km = wave_max(km);
-    vm = wave_max(vm);
-    if (klim == 0 || size_exponent(km) > ek) {
-      ek = size_exponent(km);
-      klim = size_limits<TT>(ek);
+  // Chooses the keys of one pass among `left` (bit k: key k of the tile is seen by a
+  // row and not yet taken) and sets the exponents to them.
+  __device__ __forceinline__ uint32_t choose(const uint32_t (&ksb)[2][X::NG], const uint32_t* vc, int lane, uint32_t left) {
+    const int i = lane & 15, h = lane >> 4;
+    int kx[2], vx[2];  // of keys i and 16 + i
 #pragma unroll
-      for (int cc = 0; cc < NC; ++cc) cl[cc] = fmaxf(scaled(scale * kLog2e, ek + qe[cc]), FLT_MIN);
+    for (int u = 0; u < 2; ++u) {
+      float k = 0.f, v = 0.f;
+#pragma unroll
+      for (int g = 0; g < X::NG; ++g) k = fmaxf(k, finite_size<TT>(ksb[u][g]));
+#pragma unroll
+      for (int g = 0; g < X::G; g += 4)
+        v = fmaxf(v, finite_size<TT>(vc[(4 * u + (i >> 2)) * 4 * X::G + 4 * min(g + h, X::G - 1) + (i & 3)]));
+      const bool live = left >> (16 * u + i) & 1;
+      kx[u] = live ? size_exponent(over_rows(k, max_of)) : kKvNone;
+      vx[u] = live ? size_exponent(over_rows(v, max_of)) : kKvNone;
     }
-    if (vlim == 0 || size_exponent(vm) > ev) {
-      const int e = size_exponent(vm);
+    values.template fit<TT>(max_of_columns(max(vx[0], vx[1])));
+    const bool in0 = (left >> i & 1) && values.takes(vx[0]), in1 = (left >> (16 + i) & 1) && values.takes(vx[1]);
+    keys.template fit<TT>(max_of_columns(max(in0 ? kx[0] : kKvNone, in1 ? kx[1] : kKvNone)));
+    const uint32_t taken = ((uint32_t)__ballot(in0 && keys.takes(kx[0])) & 0xffffu) |
+                           (uint32_t)__ballot(in1 && keys.takes(kx[1])) << 16;
+    return taken;
+  }
+  // The units of the rows that see one of the keys `taken`.
+  __device__ __forceinline__ void rescale(float scale, int t, uint32_t taken, const int (&from)[NC], const int (&to)[NC]) {
+    alike = true;
 #pragma unroll
-      for (int v = 0; v < X::VS; ++v)
+    for (int cc = 0; cc < NC; ++cc) {
+      cl[cc] = fmaxf(scaled(scale * kLog2e, keys.e + qe[cc]), FLT_MIN);
+      const bool sees = range_bits(from[cc] - t, to[cc] - t) & taken;
+      if (top[cc] == -INFINITY) unit[cc] = values.e;  // nothing yet
+      int next = sees ? values.e : unit[cc];
+      if (__any(next != unit[cc])) {
+        if (__any(next < unit[cc])) {
+          float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < X::NJ; ++j)
+          for (int v = 0; v < X::VS; ++v)
 #pragma unroll
-          for (int cc = 0; cc < NC; ++cc)
+            for (int j = 0; j < X::NJ; ++j)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[v][j][cc][x] = scaled(o[v][j][cc][x], ev - e);
-      ev = e;
-      vlim = size_limits<TT>(ev);
+              for (int x = 0; x < 4; ++x) m = fmaxf(m, fabsf(o[v][j][cc][x]));
+          m = over_rows(m, max_of);
+          next = next < unit[cc] ? lower_unit(unit[cc], next, m) : next;
+        }
+#pragma unroll
+        for (int v = 0; v < X::VS; ++v)
+#pragma unroll
+          for (int j = 0; j < X::NJ; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[v][j][cc][x] = scaled(o[v][j][cc][x], unit[cc] - next);
+        unit[cc] = next;
+      }
+      alike = alike && !__any(next != values.e);
     }
   }
 
-  // One tile in `stage`, keys t on.  whole: all rows see all of it; else rows see
-  // keys [from, to) of theirs in the 16-key halves whose bit in `oks` is set, and
-  // none any outside [any_from, any_to).  Returns whether a value's constants were
-  // not finite (they count as zeros).
+  // One pass over the tile in `stage`, keys t on: those of `left` (bit k: key k is seen by
+  // a row) that go together; `left` loses them.  Rows see keys [from, to) of theirs.
+  // Returns whether a value's constants were not finite (they count as zeros).
   __device__ __forceinline__ bool add(unsigned char* wave_lds, const unsigned char* stage, int lane, bool whole,
-                                      float scale, int t, int oks, const int (&from)[NC], const int (&to)[NC],
-                                      int any_from, int any_to) {
+                                      float scale, int t, uint32_t& left, const int (&from)[NC], const int (&to)[NC]) {
     const int i = lane & 15, h = lane >> 4;
     const uint32_t* kc = reinterpret_cast<const uint32_t*>(stage + X::kKc);
     const uint32_t* vc = reinterpret_cast<const uint32_t*>(stage + X::kVc);
@@ -192,50 +223,72 @@ struct Rows {
 
     // Constants: whether they fit the exponents (and are finite).
     uint32_t ksb[2][X::NG], vsb[X::NL];
-    uint32_t ks = klim, vs = vlim;
+    uint32_t ks = 0u, vs = 0u, kl = 0xffffffffu, vl = 0xffffffffu;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int g = 0; g < X::NG; ++g) {
         ksb[u][g] = kc[(16 * u + i) * X::G + h * X::WL / X::GW + g];
         ks = sizes(ks, ksb[u][g]);
+        kl = smallest(kl, ksb[u][g]);
       }
 #pragma unroll
     for (int q = 0; q < X::NL; ++q) {
       vsb[q] = vc[64 * q + lane];
       vs = sizes(vs, vsb[q]);
+      vl = smallest(vl, vsb[q]);
     }
-    auto any = [&](int k) { return t + k >= any_from && t + k < any_to && (oks >> (k >> 4) & 1); };
-    const bool careful = !whole || __any(ks != klim || vs != vlim);
+    uint32_t taken = left;
     bool poison = false;
-    if (careful) {  // what no row sees counts as zeros, as do values that are not finite
-      float km = 0.f, vm = 0.f;
+    // The key of a tile's value constant e.  (One group a head: 32 constants, and the lanes
+    // after them hold copies of the last.)
+    auto key_of = [](int e) { return X::G > 1 ? e / (4 * X::G) * 4 + (e & 3) : min(e, 31); };
+    const bool fit = __all(keys.holds(ks, kl) & values.holds(vs, vl));
+    whole = whole & (left == 0xffffffffu);
+    if (__builtin_expect(!(whole & alike & fit), 0)) {
+      ks = vs = 0u;
+      kl = vl = 0xffffffffu;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int g = 0; g < X::NG; ++g)
-          km = fmaxf(km, any(16 * u + i) ? finite_size<TT>(ksb[u][g]) : 0.f);
+        for (int g = 0; g < X::NG; ++g) {
+          const bool live = left >> (16 * u + i) & 1;
+          ks = sizes(ks, live ? ksb[u][g] : 0u);
+          kl = smallest(kl, live ? ksb[u][g] : 0xffffffffu);
+        }
 #pragma unroll
       for (int q = 0; q < X::NL; ++q) {
-        const int e = 64 * q + lane, key = e / (4 * X::G) * 4 + (e & 3) & 31;
-        // (One group a head: 32 constants, the lanes after them hold copies of the last.)
-        const bool live = (X::G > 1 || lane < 32) && any(key);
+        const bool live = left >> key_of(64 * q + lane) & 1;
+        vs = sizes(vs, live ? vsb[q] : 0u);
+        vl = smallest(vl, live ? vsb[q] : 0xffffffffu);
+      }
+      bool together = __all(all_finite<TT>(ks) & all_finite<TT>(vs));
+      if (together) {  // nearly always: one exponent holds all
+        keys.template fit<TT>(max_of_wave(size_exponent(finite_size<TT>(ks))));
+        values.template fit<TT>(max_of_wave(size_exponent(finite_size<TT>(vs))));
+        together = __all(keys.holds(ks, kl) & values.holds(vs, vl));
+      }
+      if (!together) taken = choose(ksb, vc, lane, left);
+      rescale(scale, t, taken, from, to);
+      whole = whole && taken == 0xffffffffu;
+#pragma unroll
+      for (int q = 0; q < X::NL; ++q) {  // what is not taken counts as zeros, as do values that are not finite
+        const bool live = taken >> key_of(64 * q + lane) & 1;
         const bool ok = finite(TT::lo(vsb[q])) && finite(TT::hi(vsb[q]));
         poison |= live && !ok;
         vsb[q] = live && ok ? vsb[q] : 0u;
-        vm = fmaxf(vm, finite_size<TT>(vsb[q]));
       }
-      raise(km, vm, scale);
       poison = __any(poison);
     }
+    left &= ~taken;
     // The values' constants in f16, each once: [group][key].
     wave_lds_order();
 #pragma unroll
     for (int q = 0; q < X::NL; ++q) {
       const int e = 64 * q + lane, at = e / 4 % X::G * 32 + e / (4 * X::G) * 4 + (e & 3);
       if (X::G > 1 || lane < 32) {
-        cs[at] = F16::from_f32(scaled(TT::lo(vsb[q]), 24 - ev));
-        cs[32 * X::G + at] = F16::from_f32(scaled(TT::hi(vsb[q]), -ev));
+        cs[at] = F16::from_f32(scaled(TT::lo(vsb[q]), 24 - values.e));
+        cs[32 * X::G + at] = F16::from_f32(scaled(TT::hi(vsb[q]), -values.e));
       }
     }
     wave_lds_order();
@@ -246,7 +299,7 @@ struct Rows {
       uint32_t s0[X::NG], s1[X::NG], bb[X::NG], r0[X::NG], r1[X::NG];
 #pragma unroll
       for (int g = 0; g < X::NG; ++g) {
-        const float sv = scaled(TT::lo(ksb[u][g]), 24 - ek), bv = scaled(TT::hi(ksb[u][g]), (kExact ? 6 : 0) - ek);
+        const float sv = scaled(TT::lo(ksb[u][g]), 24 - keys.e), bv = scaled(TT::hi(ksb[u][g]), (kExact ? 6 : 0) - keys.e);
         s0[g] = F16::pack2(sv, sv);
         bb[g] = F16::pack2(bv, bv);
         if constexpr (kExact) {  // 7 bits and the other 4
@@ -299,19 +352,16 @@ struct Rows {
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
       if (!whole) {
-        const int lo = from[cc] - t - 4 * h, hi = to[cc] - t - 4 * h;  // of the lane's first key
+        const uint32_t seen = (range_bits(from[cc] - t, to[cc] - t) & taken) >> (4 * h);  // from the lane's first key
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = 16 * u + e;
-            sc[u][cc][e] = k >= lo && k < hi && (oks >> u & 1) ? sc[u][cc][e] : -INFINITY;
-          }
+          for (int e = 0; e < 4; ++e) sc[u][cc][e] = seen >> (16 * u + e) & 1 ? sc[u][cc][e] : -INFINITY;
       }
       float m = fmaxf(fmaxf(fmaxf(sc[0][cc][0], sc[0][cc][1]), fmaxf(sc[0][cc][2], sc[0][cc][3])),
                       fmaxf(fmaxf(sc[1][cc][0], sc[1][cc][1]), fmaxf(sc[1][cc][2], sc[1][cc][3])));
       m = over_rows(m, max_of) * cl[cc];
-      if (__any(m > top[cc] + kSlack)) {
+      if (__builtin_expect(__any(m > top[cc] + kSlack), 0)) {
         const float was = ref[cc];
         top[cc] = fmaxf(top[cc], m);
         ref[cc] = fmaxf(top[cc] - kRaise, -FLT_MAX);
@@ -333,6 +383,11 @@ struct Rows {
         pw[cc][x] = F16::pack2(w[2 * x], w[2 * x + 1]);
         if constexpr (kExact)
           lost[cc][x] = F16::pack2(w[2 * x] - F16::lo(pw[cc][x]), w[2 * x + 1] - F16::hi(pw[cc][x]));
+      }
+      // (A row whose sums are beyond these values by all that fp32 holds leaves them out.)
+      if (__builtin_expect(!alike, 0) && unit[cc] != values.e) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) pw[cc][x] = lost[cc][x] = 0u;
       }
     }
 
@@ -585,6 +640,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     R.top[cc] = -INFINITY;
     R.ref[cc] = -FLT_MAX;
     R.sum[cc] = 0.f;
+    R.unit[cc] = 0;
 #pragma unroll
     for (int v = 0; v < X::VS; ++v)
 #pragma unroll
@@ -622,8 +678,16 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     const bool whole = t >= seen_from && t + kTile <= seen_end && oks == 3;
     // (Of the keys [q.lo, q.n) each is seen by one of the rows.)
     if (lane == 0 && ((!(oks & 1) && t < q.n && t + 16 > q.lo) || (!(oks & 2) && t + 16 < q.n))) atomicAdd(p.bad, 1u);
-    const bool poison = R.add(ring, ring + stage * X::kStage, lane, whole, a.scale, t, oks, from, to, q.lo, q.n);
-    if (poison) {
+    uint32_t left = 0xffffffffu;  // keys that some row sees
+    if (!whole)
+      left = range_bits(q.lo - t, q.n - t) & ((oks & 1 ? 0xffffu : 0u) | (oks & 2 ? 0xffff0000u : 0u));
+    bool poison = false;
+    if (left) {
+      do {
+        poison |= R.add(ring, ring + stage * X::kStage, lane, whole, a.scale, t, left, from, to);
+      } while (__builtin_expect(left != 0, 0));
+    }
+    if (__builtin_expect(poison, 0)) {
       const KvPlaces pl = kv_places(c, blocks[kv_index(t, q.n, bs_shift)], blocks[kv_index(t + 16, q.n, bs_shift)], t,
                                     q.n, head, bs_shift);
 #pragma unroll
@@ -654,7 +718,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
           for (int x = 0; x < 4; ++x) {
             const int w = 4 * h + x;  // of 16: word, or word and half of its dimensions
             const int d = D == 64 ? 8 * (w & 7) + 4 * (w >> 3) + j : 8 * (16 * v + w) + j;
-            dst[d] = nan_groups[cc] >> (d / GS) & 1 ? NAN : scaled(R.o[v][j][cc][x], R.ev);
+            dst[d] = nan_groups[cc] >> (d / GS) & 1 ? NAN : scaled(R.o[v][j][cc][x], R.unit[cc]);
           }
       if (h == 0) {
         wmax[wave * rows + r] = R.ref[cc];
