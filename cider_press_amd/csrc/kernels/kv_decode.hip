@@ -949,7 +949,7 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.rows_max = rows_max;
   p.report = report;
   const size_t reach = a.window ? std::min<size_t>(a.max_kv, (size_t)a.window + a.max_q) : a.max_kv;
-  const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : most_tiles / kPartTiles;
+  const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : (most_tiles + kPartTiles - 1) / kPartTiles;
   const bool fits = c.head_dim < 256 || c.group_size > 32;  // the rings of eight waves in LDS
   p.waves = fits && p.rows_max <= 16 && most_tiles > 9 && most_tiles <= kEightWaves &&
                     a.n_seqs * c.n_kv_heads * most_parts <= (size_t)ex.cu_count
