@@ -13,7 +13,9 @@ namespace {
 using namespace dev;
 
 constexpr int kPlanThreads = 1024;
-// Heads to a thread of the gather where that leaves enough workgroups.
+// Heads to a thread of the gather where that leaves enough workgroups (with one head
+// instead: 12000 rows of 8 heads of 128, 3000 workgroups of four heads, 13.8 us for
+// 10.1; 2000 workgroups 10.5 for 9.3; up to 1500 no difference, the launch's time).
 constexpr uint32_t kHeads = 4, kEnough = 1024;
 
 // ceil(n / block) bounded by a table row's blocks.

@@ -39,7 +39,7 @@ namespace {
 
 using namespace dev;
 
-constexpr int kStages = 2;  // of a wave's ring
+constexpr int kStages = 2;  // of a wave's ring: a tile is copied while one is worked on
 constexpr int kTile = 32;
 constexpr int kMaxParts = 256;
 // Least tiles of a part, and most that are one part all the same where parts are
@@ -49,10 +49,11 @@ constexpr int kMaxParts = 256;
 constexpr int kPartTiles = 8, kWholeTiles = 24;
 // Eight waves a workgroup instead of four halve what a wave goes over, but are
 // slower to start and leave one workgroup to a CU.  They are taken where that is
-// enough and a sequence is more than a tile a wave and at most this many tiles (16
-// requests of 701 tokens, 8 heads: 12.1 us, with four waves 13.9; 32 requests of 251:
+// enough and a sequence is more than a tile a wave (one request of 290 tokens: 9.3 us,
+// with four waves 10.6; of 250 no difference) and at most this many tiles (16
+// requests of 701 tokens, 8 heads: 12.5 us, with four waves 14.8; 32 requests of 251:
 // 11.7 and 10.0; one of 8001: 15.8 and 13.0).
-constexpr size_t kEightWaves = 64;
+constexpr size_t kFewTiles = 9, kEightWaves = 64;
 constexpr size_t kScanSeqs = 128;
 // log2 of the largest weight when the reference moves, and of how far one may pass it:
 // up to 2^15 the weights take f16's whole range, so that one of 2^-26 of the largest
@@ -87,7 +88,6 @@ struct DecodeArgs {
   int rows_max;    // sequences of more rows are another kernel's
   int target;      // workgroups to divide the tiles over
   int report;      // this launch counts what is wrong with the sequences
-  int waves;       // of a workgroup: 4 or 8
   int joined;      // the parts are joined by kv_join_kernel, not by the last to arrive
   unsigned int* counters;  // per (sequence, head)
   float* partial;          // [workgroup][rows_max][D + 4]: rows, then maximum and sum
@@ -667,8 +667,6 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     if (ti + (kStages - 1) * kWaves < last) {
       start(ti + (kStages - 1) * kWaves);
       wait_vmcnt<(kStages - 1) * X::kLoads>();
-    } else if (kStages > 2 && ti + kWaves < last) {
-      wait_vmcnt<X::kLoads>();
     } else {
       wait_vmcnt<0>();
     }
@@ -951,7 +949,7 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   const size_t reach = a.window ? std::min<size_t>(a.max_kv, (size_t)a.window + a.max_q) : a.max_kv;
   const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : (most_tiles + kPartTiles - 1) / kPartTiles;
   const bool fits = c.head_dim < 256 || c.group_size > 32;  // the rings of eight waves in LDS
-  p.waves = fits && p.rows_max <= 16 && most_tiles > 9 && most_tiles <= kEightWaves &&
+  const int waves = fits && p.rows_max <= 16 && most_tiles > kFewTiles && most_tiles <= kEightWaves &&
                     a.n_seqs * c.n_kv_heads * most_parts <= (size_t)ex.cu_count
                 ? 8
                 : 4;
@@ -985,7 +983,7 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   const size_t grid = pairs + target;
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   if (p.rows_max > 16) return bf16 ? launch_d<BF16, 2, 4>(ex.stream, p, grid) : launch_d<F16, 2, 4>(ex.stream, p, grid);
-  if (p.waves == 8) return bf16 ? launch_d<BF16, 1, 8>(ex.stream, p, grid) : launch_d<F16, 1, 8>(ex.stream, p, grid);
+  if (waves == 8) return bf16 ? launch_d<BF16, 1, 8>(ex.stream, p, grid) : launch_d<F16, 1, 8>(ex.stream, p, grid);
   return bf16 ? launch_d<BF16, 1, 4>(ex.stream, p, grid) : launch_d<F16, 1, 4>(ex.stream, p, grid);
 }
 
