@@ -565,8 +565,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       keep = (uint64_t)((there0 & 1) * 0xffffu | (there0 >> 1) * 0xffff0000u) |
              (uint64_t)((there1 & 1) * 0xffffu | (there1 >> 1) * 0xffff0000u) << 32;
       if (!apart) {
-        cl0 = fmaxf(scaled(a.scale * kLog2e, (k0 == kKvNone ? 0 : k0) + qe), FLT_MIN);
-        cl1 = fmaxf(scaled(a.scale * kLog2e, (k1 == kKvNone ? 0 : k1) + qe), FLT_MIN);
+        cl0 = fmaxf(scaled(a.scale, (k0 == kKvNone ? 0 : k0) + qe) * kLog2e, FLT_MIN);
+        cl1 = fmaxf(scaled(a.scale, (k1 == kKvNone ? 0 : k1) + qe) * kLog2e, FLT_MIN);
         if (max(v0, v1) != kKvNone) ve = max(v0, v1);
         d0 = v0 == kKvNone ? 0 : v0 - ve;
         d1 = v1 == kKvNone ? 0 : v1 - ve;
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
             store_keys<TT, D, false>(packed, keys, 32 * half, lane, kr, seen >> (lane & 31) & 1);
         }
         __syncthreads();
-        cl0 = cl1 = fmaxf(scaled(a.scale * kLog2e, kr.e + qe), FLT_MIN);
+        cl0 = cl1 = fmaxf(scaled(a.scale, kr.e + qe) * kLog2e, FLT_MIN);
         if (vr.high) ve = vr.e;
         d0 = d1 = 0;
         rescale(key0);

@@ -183,7 +183,7 @@ struct Rows {
     alike = true;
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-      cl[cc] = fmaxf(scaled(scale * kLog2e, keys.e + qe[cc]), FLT_MIN);
+      cl[cc] = fmaxf(scaled(scale, keys.e + qe[cc]) * kLog2e, FLT_MIN);
       const bool sees = range_bits(from[cc] - t, to[cc] - t) & taken;
       if (top[cc] == -INFINITY) unit[cc] = values.e;  // nothing yet
       int next = sees ? values.e : unit[cc];
@@ -636,7 +636,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
         R.qsum[cc][g] = F16::pack2(high, all - high);
       }
     }
-    R.cl[cc] = fmaxf(scaled(a.scale * kLog2e, R.qe[cc]), FLT_MIN);
+    R.cl[cc] = fmaxf(scaled(a.scale, R.qe[cc]) * kLog2e, FLT_MIN);
     R.top[cc] = -INFINITY;
     R.ref[cc] = -FLT_MAX;
     R.sum[cc] = 0.f;

@@ -34,3 +34,19 @@ def test_small_weights_beside_sinks(device, dtype, q, size):
     tiny = 2.0 ** -25 if dtype == "f16" else 0.0  # subnormal outputs
     limit = 1.02 * (unit + 2.0 ** -10 + 2.0 ** -35 / w) * np.abs(want) + tiny
     assert (np.abs(got - want) <= limit).all(), (np.abs(got - want) / np.abs(want)).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q", [1, 40])
+def test_largest_scales(device, q):
+    """Scales up to the largest accepted, whose product with log2(e) no float holds:
+    the logits are ordinary."""
+    rng = np.random.default_rng(q)
+    n = 200
+    b = Batch(rng, device, "bf16", 64, 32, 16, 1, 2, [q], [n], sharp=1e-33)
+    x = from_bits(to_bits((rng.standard_normal((n, 1, 64)) * 1e-6).astype(np.float32), "bf16"), "bf16").astype(np.float32)
+    v = from_bits(to_bits(rng.standard_normal((n, 1, 64)).astype(np.float32), "bf16"), "bf16").astype(np.float32)
+    parts = [quantize(a, 32, "bf16") for a in (x, v)]
+    b.host.put(b.table[0][np.arange(n) // 16] * 16 + np.arange(n) % 16, *parts)
+    b.k[0], b.v[0] = (dequantize(*p, 32, "bf16") for p in parts)
+    b.check(b.run(scale=3.3e38), scale=3.3e38)
