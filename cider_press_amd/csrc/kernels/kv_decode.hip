@@ -88,6 +88,7 @@ struct DecodeArgs {
   int rows_max;    // sequences of more rows are another kernel's
   int target;      // workgroups to divide the tiles over
   int report;      // this launch counts what is wrong with the sequences
+  int whole;       // sequences of up to kWholeTiles are one part whatever the others' size
   int joined;      // the parts are joined by kv_join_kernel, not by the last to arrive
   unsigned int* counters;  // per (sequence, head)
   float* partial;          // [workgroup][rows_max][D + 4]: rows, then maximum and sum
@@ -457,7 +458,7 @@ __device__ __forceinline__ int part_of(const DecodeArgs& p, int total) {
   return max(kPartTiles, p.target ? (int)(((long)total * (int)p.c.n_kv_heads + p.target - 1) / p.target) : 0x3fffffff);
 }
 __device__ __forceinline__ int parts_of(const DecodeArgs& p, int own, int per) {
-  return per == kPartTiles && own <= kWholeTiles ? min(own, 1) : min((own + per - 1) / per, kMaxParts);
+  return (per == kPartTiles || p.whole) && own <= kWholeTiles ? min(own, 1) : min((own + per - 1) / per, kMaxParts);
 }
 // The item of workgroup b where kv_starts_kernel has run: two steps of a search
 // 64 wide (more past 4096 sequences).
@@ -947,7 +948,7 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   p.rows_max = rows_max;
   p.report = report;
   const size_t reach = a.window ? std::min<size_t>(a.max_kv, (size_t)a.window + a.max_q) : a.max_kv;
-  const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : (most_tiles + kPartTiles - 1) / kPartTiles;
+  const size_t most_tiles = (reach + kTile - 1) / kTile + 1, most_parts = most_tiles <= kWholeTiles ? 1 : most_tiles / kPartTiles;
   const bool fits = c.head_dim < 256 || c.group_size > 32;  // the rings of eight waves in LDS
   const int waves = fits && p.rows_max <= 16 && most_tiles > kFewTiles && most_tiles <= kEightWaves &&
                     a.n_seqs * c.n_kv_heads * most_parts <= (size_t)ex.cu_count
@@ -960,9 +961,12 @@ hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_
   // (up to 600 keys each: 700 sequences 67 us, 117 without; 100 sequences 18 and 16).
   const size_t starts = a.n_seqs > kScanSeqs ? (a.n_seqs + 4) / 4 * 16 : 0;
   const size_t room = left > starts ? (left - starts) / slab : 0;
-  // As many parts as workgroups are resident; each (sequence, head) rounds its
-  // own up, by half a part on average.
-  const size_t resident = (size_t)(c.head_dim == 256 || p.rows_max > 16 ? 2 : 3) * ex.cu_count;
+  // As many parts as workgroups are resident (of eight waves one to a CU: 64 pairs of 33
+  // tiles made 320 parts by the others' count, a second round: 19.3 us, now 13.4; f16 in
+  // groups of 32 20.4 and 14.2); each (sequence, head) rounds its own up, by half a part
+  // on average.
+  p.whole = waves == 8;
+  const size_t resident = (size_t)(waves == 8 ? 1 : c.head_dim == 256 || p.rows_max > 16 ? 2 : 3) * ex.cu_count;
   size_t target = std::max(resident - std::min(resident, pairs / 2), resident / 4);
   if (pairs * sizeof(unsigned int) > kWideCounterBytes || room <= pairs) target = 0;
   else target = std::min(target, room - pairs);

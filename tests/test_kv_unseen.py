@@ -207,3 +207,32 @@ def test_large_tokens_of_many_prompts(device, dtype, gs):
     got = b.run()
     _rows_close(b, got, rows)
     assert np.array_equal(b.run(), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim,gs,bs", FILLED)
+@pytest.mark.parametrize("q", [3, 50])
+def test_not_finite_beside_large(device, dtype, dim, gs, bs, q):
+    """Rows whose queries are Inf or NaN, a token of NaN and one far larger than the
+    others behind the rows looked at: those stay as they are."""
+    rng = np.random.default_rng(dim + q)
+    n = q + 80
+    b = Batch(rng, device, dtype, dim, gs, bs, 1, 3, [q], [n])
+    _put(b, 0, n - 1, 50.0, BIG[dtype][-1])
+    slot = int(b.table[0, (n - 2) // bs]) * bs + (n - 2) % bs
+    b.host.v_sb[slot // bs, :, slot % bs // 4, :, slot % 4] = NAN[dtype] * 0x10001
+    b.host.k_sb[slot // bs, :, slot % bs] = NAN[dtype] * 0x10001
+    inf = 0x7F80 if dtype == "bf16" else 0x7C00
+    b.q_bits[0, 0, 5], b.q_bits[0, 1, dim - 1] = inf, NAN[dtype]
+    got = b.run()
+    rows = np.arange(q) < q - 2
+    rows[0] = False
+    if rows.any():
+        _rows_close(b, got, rows)
+    # Of the first row's heads the third's query is finite.
+    want, bound = b.expect()
+    first = from_bits(got, dtype).astype(np.float64)[0]
+    unit = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+    assert not np.isfinite(first[:2]).any()
+    assert (np.abs(first[2] - want[0, 2]) <= unit * np.abs(want[0, 2]) + bound[0, 2] + 1e-7).all()
+    assert np.isnan(from_bits(got[-2:], dtype)).all()
