@@ -69,6 +69,9 @@ constexpr int kExpBias = 1 << 12, kOkShift = 16, kPoison = 1 << 20, kApart = 1 <
 // weights; others are too far apart.
 constexpr int kMostApart = 4;
 
+// At T = f16 queries' sums over a group enter a product as 2^-kSumShift of them.
+constexpr int kSumShift = 7;
+
 struct TileArgs {
   cpq_kv_cache c;
   cpq_kv_attention_args a;
@@ -195,6 +198,28 @@ __device__ __forceinline__ bool store_keys(const Packed<D>& t, u32x4* lds, int k
       lds[key_unit<W>(key, half * (W / 2) + 4 * i + e)] = key_slice(t.q[i][e], s0, s1, b0);
   }
   return apart;
+}
+
+// 32 keys for T = f16: their words as integers (a nibble's f16 subnormals, q * 2^-24 and
+// q * 2^-20 in turn), scales and biases beside them.
+template <int D>
+__device__ __forceinline__ void store_whole_keys(const Packed<D>& t, u32x4* lds, float* scales, uint32_t* biases,
+                                                 int key0, int lane, int gw_shift) {
+  constexpr int W = D / 8, NK = Packed<D>::NK;
+  const int key = key0 + (lane & 31), half = lane >> 5;
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    const uint32_t sb = t.sb[0][i];
+    const int g = (half * (W / 2) + 4 * i) >> gw_shift;
+    scales[g * kKeys + key] = scaled(F16::lo(sb), 24 - kSumShift);
+    biases[key * 8 + g] = __builtin_amdgcn_perm(sb, sb, 0x03020302u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t w = t.q[i][e], w8 = w >> 8;
+      lds[key_unit<W>(key, half * (W / 2) + 4 * i + e)] =
+          u32x4{w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+    }
+  }
 }
 
 // 32 keys' values (half k steps ts0 ..) as operands, likewise; `poison`: a constant was
@@ -357,20 +382,30 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
   return false;
 }
 
-template <typename TT, int D, int kWaves>
-__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void kv_tile_kernel(TileArgs p) {
+// GS: the group size at T = f16, 0 (any) at bf16.
+template <typename TT, int D, int kWaves, int GS>
+__global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
   constexpr int kTeams = kWaves / 4, kBufs = 2 * kTeams;
   extern __shared__ u32x4 units[];  // [kBufs][keys, values][kUnits]
   __shared__ int meta[kBufs][4];         // of the halves' keys, then their values
   __shared__ unsigned int arrived;
   __shared__ int exponents[2][kKeys];    // of tokens too far apart: keys, values
+  // At T = f16 one rounding of keys and weights would show (off by 0.0005 to 0.0007 from 64
+  // bits, 0.0003 now): keys enter as integers, their scales by an fma after the product
+  // over a group, their biases by a product with the queries' sums, a weight with what its
+  // rounding took.  A step of 13 requests 54 us instead of 48, a prompt of 2048 over 2048
+  // in groups of 64 219 instead of 154, in groups of 32 232.
+  constexpr bool kExact = !Sig16<TT>::bf16;
+  constexpr int kGroups = kExact ? D / (GS ? GS : 1) : 1;
+  __shared__ __align__(16) float key_scales[kExact ? kBufs : 1][kGroups][kExact ? kKeys : 4];
+  __shared__ __align__(16) uint32_t key_biases[kExact ? kBufs : 1][kExact ? kKeys : 1][8];  // of group g, twice
   constexpr int kRows = 32 * kWaves;
   const cpq_kv_cache& c = p.c;
   const cpq_kv_attention_args& a = p.a;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, h = lane >> 5;
-  const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(c.group_size);
+  const int bs_shift = 31 - __builtin_clz(c.block_size), gw_shift = 28 - __builtin_clz(GS ? GS : c.group_size);
   const int group = (int)a.n_heads / (int)c.n_kv_heads;
   Item it{};
   if (!find_item(p, blockIdx.x, group, bs_shift, kRows, it)) return;
@@ -407,6 +442,32 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     qe = query_exponent(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
 #pragma unroll
     for (int i = 0; i < NS; ++i) qs[i] = query_slice<TT>(qs[i], qe);
+  }
+  u32x4 qsum{0u, 0u, 0u, 0u};  // of groups 4 h .. 4 h + 3: high and low part
+  if constexpr (kExact) {
+    // (Groups that there are not; the waves that stage write the others after this.)
+    for (int e = tid; e < kBufs * kKeys * 8; e += kWaves * 64) (&key_biases[0][0][0])[e] = 0u;
+    __syncthreads();
+    float all[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      all[g] = 0.f;
+#pragma unroll
+      for (int i = g * NS / kGroups; i < (g + 1) * NS / kGroups; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) all[g] = F16::dot2(qs[i][e], 0x3c003c00u, all[g]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(all[g]), __float_as_uint(all[g]), false, false);
+      all[g] = scaled(__uint_as_float(sw[0]) + __uint_as_float(sw[1]), -kSumShift);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float v = h ? (4 + g < kGroups ? all[(4 + g) % kGroups] : 0.f) : g < kGroups ? all[g % kGroups] : 0.f;
+      const float high = F16::lo(F16::pack2(v, 0.f));
+      qsum[g] = F16::pack2(high, v - high);
+    }
+    // The words' second and fourth pairs are in units 16 times as large.
+#pragma unroll
+    for (int i = 0; i < NS; ++i) qs[i] = u32x4{qs[i][0], sixteenth(qs[i][1]), qs[i][2], sixteenth(qs[i][3])};
   }
   const int see_to = a.causal ? min(qpos + 1, q.n) : q.n;  // keys [see_from, see_to) of this row
   const int see_from = a.window ? (int)max((int64_t)qpos + 1 - (int64_t)a.window, (int64_t)0) : 0;
@@ -488,6 +549,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     if (is_values)
       apart = store_values<TT, D, true>(packed, keys + kUnits, 4 * half, lane, range,
                                         all ? 0xffu : live_values(seen, lane), poison);
+    else if constexpr (kExact)
+      apart = false, store_whole_keys<D>(packed, keys, &key_scales[buf][0][0], &key_biases[buf][0][0], 32 * half, lane, gw_shift);
     else
       apart = store_keys<TT, D, true>(packed, keys, 32 * half, lane, range, all || (seen >> (lane & 31) & 1));
     if (lane == 0)
@@ -565,8 +628,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       keep = (uint64_t)((there0 & 1) * 0xffffu | (there0 >> 1) * 0xffff0000u) |
              (uint64_t)((there1 & 1) * 0xffffu | (there1 >> 1) * 0xffff0000u) << 32;
       if (!apart) {
-        cl0 = fmaxf(scaled(a.scale, (k0 == kKvNone ? 0 : k0) + qe) * kLog2e, FLT_MIN);
-        cl1 = fmaxf(scaled(a.scale, (k1 == kKvNone ? 0 : k1) + qe) * kLog2e, FLT_MIN);
+        cl0 = fmaxf(scaled(a.scale, (kExact ? kSumShift : k0 == kKvNone ? 0 : k0) + qe) * kLog2e, FLT_MIN);
+        cl1 = fmaxf(scaled(a.scale, (kExact ? kSumShift : k1 == kKvNone ? 0 : k1) + qe) * kLog2e, FLT_MIN);
         if (max(v0, v1) != kKvNone) ve = max(v0, v1);
         d0 = v0 == kKvNone ? 0 : v0 - ve;
         d1 = v1 == kKvNone ? 0 : v1 - ve;
@@ -606,7 +669,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
     }
     do {
       if (__builtin_expect(apart != 0, 0)) {
-        const int kx = exponents[0][lane], vx = exponents[1][lane];
+        const int kx = kExact ? kKvNone : exponents[0][lane], vx = exponents[1][lane];
         KvRange kr, vr;
         bool in = left >> lane & 1;
         vr.fit<TT>(max_of_wave(in ? vx : kKvNone));
@@ -623,11 +686,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
           bool bad;
           if (is_values)
             store_values<TT, D, false>(packed, keys + kUnits, 4 * half, lane, vr, live_values(seen, lane), bad);
-          else
+          else if constexpr (!kExact)
             store_keys<TT, D, false>(packed, keys, 32 * half, lane, kr, seen >> (lane & 31) & 1);
         }
         __syncthreads();
-        cl0 = cl1 = fmaxf(scaled(a.scale, kr.e + qe) * kLog2e, FLT_MIN);
+        cl0 = cl1 = fmaxf(scaled(a.scale, (kExact ? kSumShift : kr.e) + qe) * kLog2e, FLT_MIN);
         if (vr.high) ve = vr.e;
         d0 = d1 = 0;
         rescale(key0);
@@ -638,7 +701,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       // the weights of one half of the keys are made between those of the other.
       f32x16 sc[2];
       constexpr int kAhead = 4;
-      u32x4 op[kAhead], pw[kKeys / 16], vop[2][ND];
+      u32x4 op[kAhead], pw[kKeys / 16], lost[kExact ? kKeys / 16 : 1], vop[2][kExact ? 1 : ND];
       float add[2] = {0.f, 0.f};
       auto mask = [&](int u) {
         if (__builtin_expect(whole, 1)) return;
@@ -652,11 +715,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
       };
       auto weights = [&](int u, float rel, int i) {  // two of a half's
         const float cl = u ? cl1 : cl0;
-        const uint32_t w = F16::pack2(__builtin_amdgcn_exp2f(fmaf(sc[u][2 * i], cl, rel)),
-                                      __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i + 1], cl, rel)));
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i], cl, rel));
+        const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i + 1], cl, rel));
+        const uint32_t w = F16::pack2(w0, w1);
         pw[2 * u + (i >> 2)][i & 3] = w;
         // The sum is of the rounded weights, two at a time.
         add[u] = F16::dot2(w, 0x3c003c00u, add[u]);
+        if constexpr (kExact) {
+          lost[2 * u + (i >> 2)][i & 3] = F16::pack2(w0 - F16::lo(w), w1 - F16::hi(w));
+          add[u] = F16::dot2(lost[2 * u + (i >> 2)][i & 3], 0x3c003c00u, add[u]);
+        }
       };
       // Where a weight of half u left f16's range: a new reference, the weights again.
       auto settle = [&](int u) {
@@ -690,50 +758,101 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
           for (int x = 0; x < 4; ++x) {
             pw[2 * u][x] &= with;
             pw[2 * u + 1][x] &= with;
+            if constexpr (kExact) {
+              lost[2 * u][x] &= with;
+              lost[2 * u + 1][x] &= with;
+            }
           }
         }
       };
+      if constexpr (kExact) {
+        // One half of the keys after the other: what both would hold exceeds the registers.
+        constexpr int kSteps = NS / kGroups;  // of a group
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) op[i] = key_operand(i / NS, i % NS);
-      fence();
+        for (int u = 0; u < 2; ++u) {
+          const f32x16 none{};
+          sc[u] = mma(*reinterpret_cast<const u32x4*>(&key_biases[buf][32 * u + col][4 * h]), qsum, none);
 #pragma unroll
-      for (int x = 0; x < 16; ++x) sc[0][x] = sc[1][x] = 0.f;
-      auto score = [&](int i) {
-        sc[i / NS] = mma(op[i % kAhead], qs[i % NS], sc[i / NS]);
-        if (i + kAhead < 2 * NS) op[i % kAhead] = key_operand((i + kAhead) / NS, (i + kAhead) % NS);
-      };
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        score(i);
-        fence();
-      }
-#pragma unroll
-      for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
-      fence();
-      mask(0);
-      const float rel0 = (float)d0 - ref;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        score(NS + i);
-#pragma unroll
-        for (int x = i * 8 / NS; x < (i + 1) * 8 / NS; ++x) weights(0, rel0, x);
-        fence();
-      }
-      settle(0);
-      mask(1);
-      const float rel1 = (float)d1 - ref;
-#pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k) {
-        if (k == 2) settle(1);
-#pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = value_operand(j, k + 1);
-          o[j] = mma(vop[k & 1][j], pw[k], o[j]);
-          if (k < 2) {
-#pragma unroll
-            for (int x = (k * ND + j) * 4 / ND; x < (k * ND + j + 1) * 4 / ND; ++x) weights(1, rel1, x);
-          }
+          for (int i = 0; i < kAhead; ++i) op[i] = key_operand(u, i);
           fence();
+          f32x16 run;  // the integers' product over a group so far
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            const bool ends = i % kSteps == kSteps - 1;
+            f32x4 by[4];
+            if (ends) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                by[x] = *reinterpret_cast<const f32x4*>(&key_scales[buf][i / kSteps][32 * u + 8 * x + 4 * h]);
+            }
+            run = mma(op[i % kAhead], qs[i], i % kSteps ? run : none);
+            if (i + kAhead < NS) op[i % kAhead] = key_operand(u, i + kAhead);
+            fence();
+            if (!ends) continue;
+#pragma unroll
+            for (int x = 0; x < 16; ++x) sc[u][x] = fmaf(run[x], by[x >> 2][x & 3], sc[u][x]);
+            fence();
+          }
+          mask(u);
+          const float rel = (float)(u ? d1 : d0) - ref;
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) op[i] = value_operand(i % ND, 2 * u + i / ND);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) weights(u, rel, i);
+          settle(u);
+          fence();
+#pragma unroll
+          for (int n = 0; n < 2 * ND; ++n) {
+            const int k = 2 * u + n / ND, j = n % ND;
+            o[j] = mma(op[n % kAhead], pw[k], o[j]);
+            o[j] = mma(op[n % kAhead], lost[k], o[j]);
+            if (n + kAhead < 2 * ND) op[n % kAhead] = value_operand((n + kAhead) % ND, 2 * u + (n + kAhead) / ND);
+            fence();
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) op[i] = key_operand(i / NS, i % NS);
+        fence();
+#pragma unroll
+        for (int x = 0; x < 16; ++x) sc[0][x] = sc[1][x] = 0.f;
+        auto score = [&](int i) {
+          sc[i / NS] = mma(op[i % kAhead], qs[i % NS], sc[i / NS]);
+          if (i + kAhead < 2 * NS) op[i % kAhead] = key_operand((i + kAhead) / NS, (i + kAhead) % NS);
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          score(i);
+          fence();
+        }
+#pragma unroll
+        for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
+        fence();
+        mask(0);
+        const float rel0 = (float)d0 - ref;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          score(NS + i);
+#pragma unroll
+          for (int x = i * 8 / NS; x < (i + 1) * 8 / NS; ++x) weights(0, rel0, x);
+          fence();
+        }
+        settle(0);
+        mask(1);
+        const float rel1 = (float)d1 - ref;
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k) {
+          if (k == 2) settle(1);
+#pragma unroll
+          for (int j = 0; j < ND; ++j) {
+            if (k + 1 < kKeys / 16) vop[(k + 1) & 1][j] = value_operand(j, k + 1);
+            o[j] = mma(vop[k & 1][j], pw[k], o[j]);
+            if (k < 2) {
+#pragma unroll
+              for (int x = (k * ND + j) * 4 / ND; x < (k * ND + j + 1) * 4 / ND; ++x) weights(1, rel1, x);
+            }
+            fence();
+          }
         }
       }
     } while (__builtin_expect(left != 0, 0));
@@ -832,15 +951,26 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 ? 3 : 2) void k
                 TT::pack2(scaled(o[j][4 * x + 2] * inv, unit), scaled(o[j][4 * x + 3] * inv, unit))};
 }
 
-template <typename TT, int D, int kWaves>
+template <typename TT, int D, int kWaves, int GS>
 hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
   const size_t lds = (size_t)(kWaves / 2) * 2 * kKeys * (D / 8) * 16;
-  auto kernel = kv_tile_kernel<TT, D, kWaves>;
+  auto kernel = kv_tile_kernel<TT, D, kWaves, GS>;
   static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return raised;
   hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), lds, s, p);
   return hipGetLastError();
+}
+template <int D, int kWaves>
+hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
+  if (p.c.dtype == CPQ_DTYPE_BF16) return launch_tiles<BF16, D, kWaves, 0>(s, p, grid);
+  switch (p.c.group_size) {
+    case 32: return launch_tiles<F16, D, kWaves, 32>(s, p, grid);
+    case 64: return launch_tiles<F16, D, kWaves, 64>(s, p, grid);
+    case 128:
+      if constexpr (D >= 128) return launch_tiles<F16, D, kWaves, 128>(s, p, grid);
+    default: return hipErrorInvalidValue;
+  }
 }
 
 }  // namespace
@@ -880,18 +1010,16 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
   // as far as the scratch goes.
   const size_t slab = waves * (c.head_dim / 8 + 1) * 64 * 16;
   const size_t room = ex.scratch_bytes > kWideCounterBytes ? (ex.scratch_bytes - kWideCounterBytes) / slab : 0;
-  const size_t target = (size_t)(c.head_dim == 64 ? 3 : c.head_dim == 128 && waves == 4 ? 2 : 1) * ex.cu_count;
+  const bool three = c.head_dim == 64 && c.dtype == CPQ_DTYPE_BF16;
+  const size_t target = (size_t)(three ? 3 : c.head_dim == 64 || (c.head_dim == 128 && waves == 4) ? 2 : 1) * ex.cu_count;
   p.target = wgs < room && wgs < target ? (int)std::min(target, room - wgs) : 0;
   p.counters = static_cast<unsigned int*>(ex.scratch);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
   const dim3 grid((uint32_t)(wgs + p.target));
-  const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
   switch (c.head_dim) {
-    case 64: return bf16 ? launch_tiles<BF16, 64, 4>(ex.stream, p, grid) : launch_tiles<F16, 64, 4>(ex.stream, p, grid);
-    case 128:
-      if (waves == 4) return bf16 ? launch_tiles<BF16, 128, 4>(ex.stream, p, grid) : launch_tiles<F16, 128, 4>(ex.stream, p, grid);
-      return bf16 ? launch_tiles<BF16, 128, 8>(ex.stream, p, grid) : launch_tiles<F16, 128, 8>(ex.stream, p, grid);
-    case 256: return bf16 ? launch_tiles<BF16, 256, 4>(ex.stream, p, grid) : launch_tiles<F16, 256, 4>(ex.stream, p, grid);
+    case 64: return launch_tiles<64, 4>(ex.stream, p, grid);
+    case 128: return waves == 4 ? launch_tiles<128, 4>(ex.stream, p, grid) : launch_tiles<128, 8>(ex.stream, p, grid);
+    case 256: return launch_tiles<256, 4>(ex.stream, p, grid);
     default: return hipErrorInvalidValue;
   }
 }

@@ -17,12 +17,12 @@
 // passes, the largest first (a softmax takes its keys in any portions).  A row's sums change their unit where a product that it sees has another.
 //
 // fp32 operands would run the matrix instructions at a sixteenth of the rate.  What
-// one rounding each of keys, values and weights costs: nothing at T = bf16, where
-// the output's own is eight times coarser (2-norm 0.0017 against 64 bits either
-// way).  At T = f16 outputs would be off by 0.0004 to 0.0013, most of it the keys',
-// where the output's rounding alone is 0.0002: for few rows keys and weights are
-// kept whole there (kv_decode.hip), for many, which the matrix instructions bound,
-// they are not (0.0005).
+// one rounding each of keys, values and weights costs at T = bf16: for few rows
+// nothing (2-norm 0.0017 against 64 bits either way, the output's own rounding), for
+// prompts 0.0018 where a form in 32 bits has 0.0016.  At T = f16, where the output's
+// rounding alone is 0.0002, outputs would be off by 0.0004 to 0.0013, most of it the
+// keys': keys and weights are kept whole there and the values' one rounding is left
+// (0.0003; kv_decode.hip and kv_attention.hip say how).
 #pragma once
 
 #include <cfloat>

@@ -514,9 +514,9 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
  * with scores, softmax and sums in fp32; keys, values and weights enter the
  * matrix products as f16 for either T, each rounded once: a weight is off by 2^-11 of
  * itself and 2^-31 of its row's largest, a key or value by 2^-11 of itself and of the
- * largest constant of its own token and head (at T = f16, for sequences of few rows,
- * keys and weights keep what that rounding takes); out is rounded to T once.  A row
- * without keys is zero.  Else masked keys and values are not seen, whatever they hold.
+ * largest constant of its own token and head (at T = f16 keys and weights keep what
+ * that rounding takes); out is rounded to T once.  A row without keys is zero.  Else
+ * masked keys and values are not seen, whatever they hold.
  * q, out: T, [n_tokens, n_heads, head_dim] at token and head strides in
  * elements (multiples of 8), 16-byte aligned.  block_table [n_seqs][max_blocks]
  * as cpq_kv_plan keeps it.  max_q, max_kv: the largest number of queries and

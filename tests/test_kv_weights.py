@@ -50,3 +50,16 @@ def test_largest_scales(device, q):
     b.host.put(b.table[0][np.arange(n) // 16] * 16 + np.arange(n) % 16, *parts)
     b.k[0], b.v[0] = (dequantize(*p, 32, "bf16") for p in parts)
     b.check(b.run(scale=3.3e38), scale=3.3e38)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,gs", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128)])
+@pytest.mark.parametrize("q,causal,window", [(1, True, 0), (130, True, 0), (70, False, 0), (200, True, 150)])
+def test_f16_keeps_keys_and_weights(device, dim, gs, q, causal, window):
+    """At T = f16 no more is lost than the output's rounding and the values' (a
+    root mean square of 2.07e-4 of each, 2.9e-4 of both), for few rows and many."""
+    rng = np.random.default_rng(dim + gs + q)
+    b = Batch(rng, device, "f16", dim, gs, 16, 2, 4, [q, q + 1], [800, q + 1], sharp=2.0)
+    want, _ = b.expect(causal, window)
+    got = from_bits(b.run(causal, window), "f16").astype(np.float64)
+    assert np.linalg.norm(got - want) <= 3.2e-4 * np.linalg.norm(want)
