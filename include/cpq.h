@@ -494,9 +494,10 @@ cpq_status cpq_kv_plan(cpq_commands* cmds, const uint32_t* lens, const uint32_t*
  * holds an Inf or NaN, or whose range overflows, is stored as q = 0, scale = 0,
  * bias = NaN.  A scale that RNE_T rounds up can carry the highest value of a group
  * past T's own range: it is read back as Inf (f16: lowest -65504 and highest 65504,
- * scale 8736, 65536), while cpq_kv_attention takes scale * q + bias as it is.  Slots that are none are skipped; slots past the cache are skipped
- * and reported by the next wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one
- * slot: either wins, word by word. */
+ * scale 8736, 65536), while cpq_kv_attention takes scale * q + bias as it is.
+ * Slots that are none are skipped; slots past the cache are skipped and reported by
+ * the next wait as CPQ_ERR_INVALID_ARGUMENT.  Two tokens in one slot: either wins,
+ * word by word. */
 cpq_status cpq_kv_append(cpq_commands* cmds, const cpq_kv_cache* cache, const void* k, size_t k_token_stride,
                          size_t k_head_stride, const void* v, size_t v_token_stride, size_t v_head_stride,
                          const uint32_t* slots, size_t n_tokens);
@@ -523,12 +524,12 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
  * elements (multiples of 8), 16-byte aligned.  block_table [n_seqs][max_blocks]
  * as cpq_kv_plan keeps it.  max_q, max_kv: the largest number of queries and
  * of keys of any sequence, as far as the host knows; max_kv only steers how
- * the work is split, a sequence with more than max_q queries is not computed.
- * out must not overlap the inputs.  Rows past query_starts[n_seqs] are not written.  Such sequences, sequences
- * whose rows pass n_tokens, and blocks past n_blocks or max_blocks of which a
- * query would see a key (they count as masked) are reported by the next wait as
- * CPQ_ERR_INVALID_ARGUMENT; entries of blocks behind every query's window may hold
- * anything.
+ * the work is split.  out must not overlap the inputs.  Rows past
+ * query_starts[n_seqs] are not written.  The next wait reports, as
+ * CPQ_ERR_INVALID_ARGUMENT, sequences with more than max_q queries and sequences
+ * whose rows pass n_tokens (they are not computed), and blocks past n_blocks or
+ * max_blocks of which a query would see a key (they count as masked); entries of blocks
+ * behind every query's window may hold anything.
  * Session scratch holds the partial results where keys are split. */
 typedef struct cpq_kv_attention_args {
   const void* q;
