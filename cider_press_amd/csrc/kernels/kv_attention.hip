@@ -19,9 +19,10 @@
 // the registers), at 64 (three workgroups share a CU) and where eight waves a
 // workgroup would leave CUs without one, it has one team, two tiles of LDS and a
 // barrier every tile.  The packed words of a team's next tile are in
-// flight meanwhile.  (4096 queries of 32 heads over 8192 keys of 8: head_dim 128 429
-// us, 470 with a barrier every tile, 607 with four waves a workgroup; head_dim 64
-// 344 us, 429 with eight.)
+// flight meanwhile.  (4096 queries of 32 heads over 8192 keys of 8, back to back until
+// the clock has settled: head_dim 128 442 us, 64 370, 256 1434; when each was chosen:
+// a barrier every tile 470 us for 429, four waves a workgroup 607; head_dim 64 with
+// eight waves 429 us for 344.)
 //   LDS image: 16-byte units, a key's word (8 dimensions) or a dimension's 8
 //   keys of a k step, XORed so that neighbouring lanes' b128 reads and writes meet
 //   in different banks (measured: 8 lanes are served at a time, 8 cycles a read;
@@ -31,11 +32,12 @@
 // maximum of the half tile found, the reference raised to 2^-10 of it and its weights
 // made again.  The weights of a tile's first 32 keys are made between the matrix
 // instructions of the other 32 keys' scores, theirs between those of the first
-// keys' values (when that came in: head_dim 64 350 -> 337 us, 256 411 -> 354).
+// keys' values (when that came in: head_dim 64 350 -> 337 us).
 //
-// Bound by its instructions: 4096 queries over 8192 keys at head_dim 128 run at 960
+// Bound by its instructions: 4096 queries over 8192 keys at head_dim 128 run at 933
 // TFLOP/s (a large f16 product of the library: 1322), with the vector pipes busy for
-// 55% of the cycles, the matrix pipes for 43%, both at once for 18%.
+// 55% of the cycles, the matrix pipes for 42%, both at once for 17%.  The first twenty
+// calls after a pause take 520 us, not 442: the clock.
 //
 // A tile whose tokens are too far apart for one exponent is staged and multiplied again
 // for each set of them that goes together (kv_common.hpp), its words loaded once more
@@ -95,7 +97,8 @@ __device__ __forceinline__ int key_unit(int key, int w) {
 }
 // Unit of a dimension's keys of half k step ts (2 * step + h): read at
 // neighbouring dimensions, written at dimensions 8 apart (two of eight lanes
-// meet there).  Dimensions 32 apart have the same place in their rows.
+// meet there: the bank conflicts that are left, 16 cycles a wave's tile, 2.6% of the
+// busy ones).  Dimensions 32 apart have the same place in their rows.
 __device__ __forceinline__ int value_unit(int d, int ts) { return d * 8 + (ts ^ ((d ^ (d >> 3 & 3)) & 7)); }
 
 // The packed words of one wave's 32 keys: as keys, lane (key, half of the
@@ -394,8 +397,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
   // At T = f16 one rounding of keys and weights would show (off by 0.0005 to 0.0007 from 64
   // bits, 0.0003 now): keys enter as integers, their scales by an fma after the product
   // over a group, their biases by a product with the queries' sums, a weight with what its
-  // rounding took.  A step of 13 requests 54 us instead of 48, a prompt of 2048 over 2048
-  // in groups of 64 219 instead of 154, in groups of 32 232.
+  // rounding took.  A step of 13 requests 51 us instead of 46, 4096 queries over 8192 keys
+  // in groups of 64 668 instead of 446, in groups of 32 726.
   constexpr bool kExact = !Sig16<TT>::bf16;
   constexpr int kGroups = kExact ? D / (GS ? GS : 1) : 1;
   __shared__ __align__(16) float key_scales[kExact ? kBufs : 1][kGroups][kExact ? kKeys : 4];

@@ -26,10 +26,10 @@
 // in part order, or a kernel after this one where there are many.
 //
 // Bound by HBM where the keys are long (64 requests of 4097 tokens, 8 heads of 128 in
-// groups of 64: 65 us, 4.7 TB/s), at T = f16 by its instructions too (three requests
-// of 120002 tokens, groups of 32: 105 us, 4.4 TB/s), by fixed
+// groups of 64: 63 us, 4.8 TB/s; three of 120002 in groups of 32 93 us, 5.0 TB/s), at
+// T = f16 by its instructions too (the same three: 110 us, 4.2 TB/s), by fixed
 // phases of 9 us where they are not: launch, search, first tile, join (48 requests of
-// up to 8193 tokens: 25 us, 2.9 TB/s; one of 391 tokens, 2 heads of 64: 10.3 us).
+// up to 8193 tokens: 27 us, 2.6 TB/s; one of 391 tokens, 2 heads of 64: 8.6 us).
 #include <algorithm>
 
 #include "kv_common.hpp"
@@ -44,8 +44,8 @@ constexpr int kTile = 32;
 constexpr int kMaxParts = 256;
 // Least tiles of a part, and most that are one part all the same where parts are
 // that small: a join costs 3 us, a wave's tile 1.1 us while its SIMD has no other.
-// (One request of 4001 tokens, 8 heads: 12.6 us at 8 tiles a part, 14.4 at 16; one
-// of 391 tokens, 2 heads: 11.4 us as one part, 13.1 as two.)
+// (When chosen: one request of 4001 tokens, 8 heads, 12.6 us at 8 tiles a part, 14.4 at
+// 16; one of 391 tokens, 2 heads, 11.4 us as one part, 13.1 as two.)
 constexpr int kPartTiles = 8, kWholeTiles = 24;
 // Eight waves a workgroup instead of four halve what a wave goes over, but are
 // slower to start and leave one workgroup to a CU.  They are taken where that is
@@ -142,8 +142,8 @@ struct Rows {
   // At T = f16 a key's and a weight's one rounding to f16 would show in the output: a
   // scale enters in two parts whose products with a nibble are exact, the biases by
   // a product of their own with the queries' sums, a weight with what it lost.
-  // (Three requests of 120002 tokens: off by 0.0002 to 0.0003 from 64 bits instead of
-  // 0.0006 to 0.0013, in 105 us instead of 92.)
+  // (Three requests of 120002 tokens: off by 0.0003 from 64 bits instead of 0.0006 to
+  // 0.0013, in 110 us instead of 93.)
   static constexpr bool kExact = !Sig16<TT>::bf16;
   u32x4 qs[NC][X::WL];
   u32x4 qsum[NC];  // sums over a lane's words of each group, in units of 2^6: high and low part
