@@ -1,7 +1,7 @@
 #!/usr/bin/env python3
 """Benchmark of the MI355X quantized-matmul path (one GPU).
 
-Headline metric (BASELINE.json): qmv HBM GB/s at K=4096 x N=12288, 4-bit gs64,
+Headline metric: qmv HBM GB/s at K=4096 x N=12288, 4-bit gs64,
 bf16 (config 2a) -> `value`; qmm TFLOP/s at M=512, N=K=4096 (config 3a) -> the
 `qmm` object.  A "step" is one kernel call over one batch of synthetic input
 already resident in HBM.
