@@ -37,6 +37,7 @@ SOURCES = [
     "kernels/moe.hip",
     "kernels/stream_read.hip",
     "kv.cpp", "kernels/kv_cache.hip", "kernels/kv_attention.hip", "kernels/kv_decode.hip",
+    "kernels/kv_attention_scored.hip", "kernels/kv_decode_scored.hip",
 ]
 
 ARCH = "gfx950"

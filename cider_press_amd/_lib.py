@@ -182,6 +182,8 @@ SIGNATURES = {
     "cpq_embed_tokens": (_st, [_vp, _int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _sz, _sz, _vp, _sz, _u32, _u32]),
     "cpq_tensor_embed_tokens": (_st, [_vp, _vp, _pp]),
     "cpq_moe_route": (_st, [_vp, _int, _vp, _sz, _sz, _u32, _int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cpq_check_moe_route_grouped_args": (_st, [_int, _sz, _sz, _u32, _vp]),
+    "cpq_moe_route_grouped": (_st, [_vp, _int, _vp, _sz, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cpq_moe_combine": (_st, [_vp, _int, _vp, _sz, _vp, _vp, _sz, _u32, _sz, _vp, _sz]),
     "cpq_kv_cache_words": (_st, [_vp, _psz, _psz]),
     "cpq_check_kv_cache": (_st, [_vp]),
@@ -191,6 +193,10 @@ SIGNATURES = {
     "cpq_kv_append": (_st, [_vp, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz]),
     "cpq_kv_gather": (_st, [_vp, _vp, _vp, _sz, _vp, _vp]),
     "cpq_kv_attention": (_st, [_vp, _vp, _vp]),
+    "cpq_check_kv_attention_scored_args": (_st, [_vp, _vp, _vp]),
+    "cpq_kv_attention_scored": (_st, [_vp, _vp, _vp, _vp]),
+    "cpq_check_kv_append_rotary_args": (_st, [_vp, _vp]),
+    "cpq_kv_append_rotary": (_st, [_vp, _vp, _vp]),
     "cpq_check_gather_args": (_st, [_int, _sz, _sz, _sz, _sz, _int, _sz, _sz, _sz, _sz, _sz, _u32, _u32]),
     "cpq_qweight_from_bytes": (_st, [_vp, _int, _sz, _sz, _sz, _u32, _u32, _vp, _sz, _vp, _sz, _vp, _sz, _pp]),
     "cpq_qweight_release": (None, [_vp]),

@@ -144,6 +144,12 @@ bool moe_route_sort_fits(int tokens);
 hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
                                  int top_k, int normalize, uint32_t* experts, float* scores, uint32_t* lhs,
                                  uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
+hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
+                                    int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores);
+hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens,
+                                         int n_experts, int top_k, const cpq_moe_router& r, uint32_t* experts,
+                                         float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
+                                         uint32_t* offsets);
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,
                            uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
 hipError_t launch_moe_combine(hipStream_t s, int dtype, const void* y, const float* scores, const uint32_t* inv,
@@ -223,8 +229,8 @@ struct ExecCtx {
   size_t scratch_bytes;
 };
 ExecCtx session_ctx(const cpq_commands* cmds);
-// Attention over the key/value cache (kernels/kv_attention.hip) and its kernel
-// for few query rows per sequence (kernels/kv_decode.hip): sequences of up to
+// Attention over the key/value cache (kernels/kv_attention.hpp) and its kernel
+// for few query rows per sequence (kernels/kv_decode.hpp): sequences of up to
 // rows_max <= kKvDecodeRows rows of one key/value head; `report` counts sequences
 // whose lengths are wrong.
 constexpr size_t kKvDecodeRows = 32;
@@ -232,6 +238,19 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
                                unsigned int* bad);
 hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a, int rows_max,
                             bool report, unsigned int* bad);
+// The same with scores that are capped (cap * log2(e), 2 / cap; 0: not) or fall with
+// distance ([n_heads] or null), and prefixes ([n_seqs] or null).
+constexpr float kKvMostCap = 1024.f;
+struct KvScore {
+  float cap = 0.f;
+  float per_cap = 0.f;
+  const float* slopes = nullptr;
+  const uint32_t* prefix_lens = nullptr;
+};
+hipError_t launch_kv_attention_scored(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                      const KvScore& score, unsigned int* bad);
+hipError_t launch_kv_decode_scored(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                   const KvScore& score, int rows_max, bool report, unsigned int* bad);
 // Y = X . W^T with the kernel chosen by M (small-M kernels, else the prefill
 // plan), as affine_qmm_t and the runtime node run it.
 hipError_t launch_matmul(const ExecCtx& ex, const QuantArgs& q, const void* x, void* y, int m, int n, int k);
@@ -321,6 +340,8 @@ hipError_t launch_kv_plan(hipStream_t s, const uint32_t* lens, const uint32_t* n
 hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k, size_t k_token, size_t k_head,
                             const void* v, size_t v_token, size_t v_head, const uint32_t* slots, uint32_t n_tokens,
                             unsigned int* bad);
+hipError_t launch_kv_append_rotary(hipStream_t s, const cpq_kv_cache& c, const cpq_kv_append_rotary_args& a,
+                                   unsigned int* bad);
 hipError_t launch_kv_gather(hipStream_t s, const cpq_kv_cache& c, const uint32_t* slots, uint32_t n_rows, void* k_out,
                             void* v_out, unsigned int* bad);
 // Whether the small-M kernel's per-slab constants fit in LDS at this K and

@@ -220,31 +220,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return o;
 }
 
-// A workgroup takes consecutive tokens of one head, keys or values: thread =
-// one word (8 values) of one token, so a group is 4, 8 or 16 adjacent lanes
-// and the words of four tokens in adjacent slots, which the value layout
-// interleaves, come from one wave (head_dim 128).  Bound by its instructions, 183 a
-// wave of 512 values: 8191 tokens of 8 heads of 128 in 14.5 us (3.0 TB/s; with
-// IEEE divisions 17.4).  Four heads to a thread, as in the gather: no faster.
+// Eight values of T, word wi of a token's row, quantized into their place in the cache.
+// The `lanes` words of a group are adjacent lanes, all of them here.
 template <typename TT>
-__global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const uint16_t* __restrict__ k,
-                                                        size_t k_token, size_t k_head,
-                                                        const uint16_t* __restrict__ v, size_t v_token,
-                                                        size_t v_head, const uint32_t* __restrict__ slots,
-                                                        uint32_t n_tokens, int w_shift, int lanes, unsigned int* bad) {
-  const uint32_t wi = threadIdx.x & ((1u << w_shift) - 1), t = blockIdx.x * (256u >> w_shift) + (threadIdx.x >> w_shift);
-  const uint32_t head = blockIdx.y;
-  const bool values = blockIdx.z;
-  if (t >= n_tokens) return;
-  const uint32_t slot = slots[t];
-  const uint32_t bs = c.block_size, bs_shift = 31 - __builtin_clz(bs);
-  const uint32_t block = slot >> bs_shift, off = slot & (bs - 1);
-  if (block >= c.n_blocks) {
-    if (slot != CPQ_KV_NO_SLOT && wi == 0 && head == 0 && !values) atomicAdd(bad, 1u);
-    return;
-  }
-  const uint16_t* src = values ? v + t * v_token + head * v_head : k + t * k_token + head * k_head;
-  const u32x4 raw = *reinterpret_cast<const u32x4*>(src + wi * 8);
+__device__ __forceinline__ void append_word(const cpq_kv_cache& c, u32x4 raw, uint32_t block, uint32_t off,
+                                            uint32_t head, bool values, uint32_t wi, int w_shift, int lanes) {
+  const uint32_t bs = c.block_size;
   float x[8];
   uint32_t most = 0;
 #pragma unroll
@@ -292,6 +273,107 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
   } else {
     c.k_q[(row + off) * w + wi] = word;
     if (wi % lanes == 0) c.k_sb[(row + off) * g + gi] = sb;
+  }
+}
+
+// A workgroup takes consecutive tokens of one head, keys or values: thread =
+// one word (8 values) of one token, so a group is 4, 8 or 16 adjacent lanes
+// and the words of four tokens in adjacent slots, which the value layout
+// interleaves, come from one wave (head_dim 128).  Bound by its instructions, 183 a
+// wave of 512 values: 8191 tokens of 8 heads of 128 in 14.5 us (3.0 TB/s; with
+// IEEE divisions 17.4).  Four heads to a thread, as in the gather: no faster.
+template <typename TT>
+__global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const uint16_t* __restrict__ k,
+                                                        size_t k_token, size_t k_head,
+                                                        const uint16_t* __restrict__ v, size_t v_token,
+                                                        size_t v_head, const uint32_t* __restrict__ slots,
+                                                        uint32_t n_tokens, int w_shift, int lanes, unsigned int* bad) {
+  const uint32_t wi = threadIdx.x & ((1u << w_shift) - 1), t = blockIdx.x * (256u >> w_shift) + (threadIdx.x >> w_shift);
+  const uint32_t head = blockIdx.y;
+  const bool values = blockIdx.z;
+  if (t >= n_tokens) return;
+  const uint32_t slot = slots[t];
+  const uint32_t bs = c.block_size, bs_shift = 31 - __builtin_clz(bs);
+  const uint32_t block = slot >> bs_shift, off = slot & (bs - 1);
+  if (block >= c.n_blocks) {
+    if (slot != CPQ_KV_NO_SLOT && wi == 0 && head == 0 && !values) atomicAdd(bad, 1u);
+    return;
+  }
+  const uint16_t* src = values ? v + t * v_token + head * v_head : k + t * k_token + head * k_head;
+  const u32x4 raw = *reinterpret_cast<const u32x4*>(src + wi * 8);
+  append_word<TT>(c, raw, block, off, head, values, wi, w_shift, lanes);
+}
+
+// Rotation and append.  A workgroup takes 256 / W consecutive tokens (thread = one word of
+// one token, as above) and `rows` of their rows: keys, values, then queries.  The cosines
+// and sines of its tokens are made once, in LDS, and kept in registers over the rows; a
+// rotated word takes its partner's word besides its own (from the cache: a lane nearby
+// loads it too).  In fp64, whose fma runs at fp32's rate here: which of 16 steps a key's
+// value falls on is a whole number, so that a rotation in fp32 would store other steps than
+// an append of keys that were rotated exactly.
+constexpr uint32_t kRotaryEnough = 2048;  // workgroups
+template <typename TT, bool PAIRS>
+__global__ __launch_bounds__(256) void kv_append_rotary_kernel(cpq_kv_cache c, cpq_kv_append_rotary_args a, int w_shift,
+                                                               int lanes, uint32_t rows, unsigned int* bad) {
+  __shared__ double2 turns[1024];  // [j][token][word]: cosine and sine of its j-th
+  constexpr uint32_t kTurns = PAIRS ? 4 : 8;  // of a word
+  const uint32_t w = 1u << w_shift, tokens = 256u >> w_shift, t0 = blockIdx.x * tokens;
+  const uint32_t wi = threadIdx.x & (w - 1), tl = threadIdx.x >> w_shift, t = t0 + tl;
+  const uint32_t n_tokens = (uint32_t)a.n_tokens, kv_heads = c.n_kv_heads;
+  const uint32_t all = 2 * kv_heads + (uint32_t)a.n_heads, r0 = blockIdx.y * rows, r1 = min(r0 + rows, all);
+  const uint32_t half = a.rotary_dim / 2, words = half / kTurns;  // words of distinct turns
+  for (uint32_t e = threadIdx.x; e < half << (8 - w_shift); e += 256) {
+    const uint32_t tt = e / half, i = e - tt * half;
+    if (t0 + tt >= n_tokens) break;
+    double si, co;
+    sincos((double)a.positions[t0 + tt] * (double)a.frequencies[i], &si, &co);
+    turns[(i % kTurns * tokens + tt) * words + i / kTurns] = double2{co * a.magnitude, si * a.magnitude};
+  }
+  __syncthreads();
+  if (t >= n_tokens) return;
+  const uint32_t slot = a.slots[t];
+  const uint32_t bs = c.block_size, bs_shift = 31 - __builtin_clz(bs);
+  const uint32_t block = slot >> bs_shift, off = slot & (bs - 1);
+  if (block >= c.n_blocks) {
+    if (slot != CPQ_KV_NO_SLOT && wi == 0 && r0 == 0) atomicAdd(bad, 1u);
+    return;
+  }
+  const bool turned = wi < a.rotary_dim / 8, second = !PAIRS && wi >= words;
+  const uint32_t partner = !turned || PAIRS ? wi : second ? wi - words : wi + words;
+  double co[kTurns], si[kTurns];
+  if (turned) {
+#pragma unroll
+    for (uint32_t j = 0; j < kTurns; ++j) {
+      const double2 v = turns[(j * tokens + tl) * words + (second ? wi - words : wi)];
+      co[j] = v.x;
+      si[j] = PAIRS || second ? v.y : -v.y;
+    }
+  }
+  for (uint32_t r = r0; r < r1; ++r) {
+    const bool key = r < kv_heads, value = !key && r < 2 * kv_heads;
+    const uint32_t head = key ? r : value ? r - kv_heads : r - 2 * kv_heads;
+    const uint16_t* src = static_cast<const uint16_t*>(key ? a.k : value ? a.v : a.q) +
+                          t * (key ? a.k_token_stride : value ? a.v_token_stride : a.q_token_stride) +
+                          head * (key ? a.k_head_stride : value ? a.v_head_stride : a.q_head_stride);
+    u32x4 raw = *reinterpret_cast<const u32x4*>(src + wi * 8);
+    if (!value && turned) {
+      const u32x4 other = *reinterpret_cast<const u32x4*>(src + partner * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double x = TT::lo(raw[i]), y = TT::hi(raw[i]);
+        if constexpr (PAIRS) {
+          raw[i] = TT::pack2((float)fma(x, co[i], -(y * si[i])), (float)fma(y, co[i], x * si[i]));
+        } else {
+          raw[i] = TT::pack2((float)fma(x, co[2 * i], (double)TT::lo(other[i]) * si[2 * i]),
+                             (float)fma(y, co[2 * i + 1], (double)TT::hi(other[i]) * si[2 * i + 1]));
+        }
+      }
+    }
+    if (r < 2 * kv_heads)
+      append_word<TT>(c, raw, block, off, head, value, wi, w_shift, lanes);
+    else
+      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_token_stride +
+                                head * a.q_out_head_stride + wi * 8) = raw;
   }
 }
 
@@ -389,6 +471,22 @@ hipError_t launch_kv_append(hipStream_t s, const cpq_kv_cache& c, const void* k,
     return hipGetLastError();
   };
   return c.dtype == CPQ_DTYPE_BF16 ? run(kv_append_kernel<BF16>) : run(kv_append_kernel<F16>);
+}
+
+hipError_t launch_kv_append_rotary(hipStream_t s, const cpq_kv_cache& c, const cpq_kv_append_rotary_args& a,
+                                   unsigned int* bad) {
+  const int w_shift = log2_of(c.head_dim / 8), lanes = (int)c.group_size / 8;
+  const uint32_t per = 256u >> w_shift, blocks = ((uint32_t)a.n_tokens + per - 1) / per;
+  const uint32_t all = 2 * c.n_kv_heads + (uint32_t)a.n_heads;
+  const uint32_t rows = (uint32_t)std::max<size_t>((size_t)all * blocks / kRotaryEnough, 1);
+  const dim3 grid(blocks, (all + rows - 1) / rows);
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, c, a, w_shift, lanes, rows, bad);
+    return hipGetLastError();
+  };
+  if (a.interleaved)
+    return c.dtype == CPQ_DTYPE_BF16 ? run(kv_append_rotary_kernel<BF16, true>) : run(kv_append_rotary_kernel<F16, true>);
+  return c.dtype == CPQ_DTYPE_BF16 ? run(kv_append_rotary_kernel<BF16, false>) : run(kv_append_rotary_kernel<F16, false>);
 }
 
 hipError_t launch_kv_gather(hipStream_t s, const cpq_kv_cache& c, const uint32_t* slots, uint32_t n_rows, void* k_out,

@@ -22,7 +22,7 @@
 // prompts 0.0018 where a form in 32 bits has 0.0016.  At T = f16, where the output's
 // rounding alone is 0.0002, outputs would be off by 0.0004 to 0.0013, most of it the
 // keys': keys and weights are kept whole there and the values' one rounding is left
-// (0.0003; kv_decode.hip and kv_attention.hip say how).
+// (0.0003; kv_decode.hpp and kv_attention.hpp say how).
 #pragma once
 
 #include <cfloat>
@@ -214,6 +214,43 @@ __device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, i
   q.pos = q.n - q.n_q;
   q.lo = a.window && (uint64_t)(q.pos + 1 > 0 ? q.pos + 1 : 0) > a.window ? q.pos + 1 - (int)a.window : 0;
   return q;
+}
+
+// What scores become, in units of log2(e) (cpq_kv_attention_scored).  With a cap
+//   cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)),
+// whose error is one of cap, 2^-23 of it, where s itself is small: caps are limited to
+// kKvMostCap, which leaves a weight off by 2^-12 of itself at most.  Both ends of the
+// exponential's range come out as they should, +-cap.
+constexpr float kKvMostSlope = 0x1p96f;  // times any distance finite
+struct KvRowScore {
+  float slope = 0.f;  // times log2(e)
+  int anchor = 0;     // distances are from here: of the keys that a row sees the one of the largest bias, so
+                      // that sums with it lose nothing (a softmax takes any constant)
+  float base = 0.f;   // bias, and with a cap the cap, of the key that `at` was given
+  float by = 0.f;     // of a score as the product has it: to log2(e), with a cap to the exponential's argument
+  __device__ __forceinline__ void head(const KvScore& k, int hh, int from, int to) {
+    if (!k.slopes) return;
+    const float s = k.slopes[hh];
+    slope = (fabsf(s) > kKvMostSlope ? copysignf(kKvMostSlope, s) : s) * kLog2e;
+    anchor = slope < 0.f ? from : to - 1;
+  }
+  // For keys from `key` on, products in units of cl (positive, maybe infinite).
+  __device__ __forceinline__ void at(const KvScore& k, int key, float cl) {
+    base = fmaf(slope, (float)(key - anchor), k.cap);
+    by = k.cap > 0.f ? fminf(cl * k.per_cap, FLT_MAX) : cl;
+  }
+  // Of the product of key `key` + x.
+  template <typename X>
+  __device__ __forceinline__ float of(const KvScore& k, float product, X x) const {
+    const float plus = fmaf(slope, (float)x, base);
+    if (k.cap > 0.f)
+      return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * by)), -2.f * k.cap, plus);
+    return fmaf(product, by, plus);
+  }
+};
+// The prefix of sequence s that all its queries see, of n keys.
+__device__ __forceinline__ int kv_prefix(const KvScore& k, int s, int n) {
+  return k.prefix_lens ? (int)min(k.prefix_lens[s], (uint32_t)max(n, 0)) : 0;
 }
 
 // A block table's row, read through the scalar cache: nothing writes it while

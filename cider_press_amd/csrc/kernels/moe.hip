@@ -20,6 +20,8 @@
 //            fp32, j ascending.
 // All three are tiny next to the expert matmuls (bytes: T*E logits;
 // 16*T*k of indices; (k + 1)*T*N*sizeof(T) for the combine).
+#include <type_traits>
+
 #include "../cpq_internal.hpp"
 #include "common.hpp"
 
@@ -108,17 +110,141 @@ __device__ __forceinline__ void route_token(const void* logits, size_t row, int 
   score = normalize ? my_p / psum : my_p;
 }
 
+// The kinds of routers: a token by one wave, lane j < top_k returns pick j and its score.
+struct SoftmaxRouter {
+  int normalize;
+  template <int L, int NV>
+  __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
+                                        float& score) const {
+    route_token<L, NV>(logits, row, n_experts, top_k, normalize, pick, score);
+  }
+};
+
+// moe_route_grouped, in fp64: a choice is a whole number, which near scores must not
+// change with the order of a sum.
+struct GroupedRouter {
+  cpq_moe_router r;
+  // Orders like the values, NaN below all of them; 0: no choice.
+  static __device__ __forceinline__ unsigned long long key_of(double v) {
+    const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+    return v != v ? 1ull : b >> 63 ? ~b : b | 1ull << 63;
+  }
+  static __device__ __forceinline__ double value_of(unsigned long long key) {
+    return key == 1ull ? NAN : __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key));
+  }
+  // The largest key of the wave and its lowest expert; the owner's is struck out.
+  template <int NV>
+  static __device__ __forceinline__ unsigned long long take(unsigned long long (&key)[NV], const bool (&among)[NV],
+                                                            int& expert) {
+    unsigned long long best = 0ull;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) best = among[i] && key[i] > best ? key[i] : best;
+    best = __ockl_wfred_max_u64(best);
+    expert = -1;
+#pragma unroll
+    for (int i = NV - 1; i >= 0; --i) {
+      const uint64_t who = __ballot(among[i] && key[i] == best);
+      if (who) expert = 64 * i + __builtin_ctzll(who);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (expert == (int)(threadIdx.x & 63) + 64 * i) key[i] = 0ull;
+    return best;
+  }
+  template <int L, int NV>
+  __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
+                                        float& score) const {
+    const int lane = threadIdx.x & 63;
+    double s[NV];
+    unsigned long long key[NV];
+    bool live[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int e = lane + 64 * i;
+      live[i] = e < n_experts;
+      s[i] = live[i] ? (double)logit_at<L>(logits, row + e) : -INFINITY;
+    }
+    if (r.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) s[i] = 1.0 / (1.0 + exp(-s[i]));
+    } else {
+      double m = s[0], sum = 0.0;
+#pragma unroll
+      for (int i = 1; i < NV; ++i) m = fmax(m, s[i]);
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) m = fmax(m, __shfl_xor(m, o, 64));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        s[i] = live[i] ? exp(s[i] - m) : 0.0;
+        sum += s[i];
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) s[i] /= sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      key[i] = live[i] ? key_of(r.bias ? s[i] + (double)r.bias[lane + 64 * i] : s[i]) : 0ull;
+    int e;
+    if (r.n_groups > 1 && r.top_groups < r.n_groups) {
+      const int size = n_experts / (int)r.n_groups;
+      int group[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) group[i] = (lane + 64 * i) / size;
+      unsigned long long mine = 0ull;  // of group `lane`
+      for (int g = 0; g < (int)r.n_groups; ++g) {
+        bool in[NV];
+        unsigned long long rest[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          in[i] = live[i] && group[i] == g;
+          rest[i] = key[i];
+        }
+        unsigned long long best = take<NV>(rest, in, e);
+        if (r.group_best > 1) best = key_of(value_of(best) + value_of(take<NV>(rest, in, e)));
+        if (lane == g) mine = best;
+      }
+      int before = 0;  // groups ahead of this lane's
+      for (int g = 0; g < (int)r.n_groups; ++g) {
+        const unsigned long long other = __shfl(mine, g, 64);
+        before += other > mine || (other == mine && g < lane);
+      }
+      const uint64_t kept = __ballot(lane < (int)r.n_groups && before < (int)r.top_groups);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (live[i] && !(kept >> group[i] & 1)) key[i] = 0ull;
+    }
+    double mine = 0.0, sum = 0.0;
+    pick = 0;
+    for (int j = 0; j < top_k; ++j) {
+      take<NV>(key, live, e);
+      double all = s[0];
+#pragma unroll
+      for (int i = 1; i < NV; ++i) all = e >> 6 == i ? s[i] : all;
+      all = __shfl(all, e & 63, 64);
+      sum += all;
+      if (lane == j) {
+        mine = all;
+        pick = e;
+      }
+    }
+    if (r.normalize) mine = sum == 0.0 ? 0.0 : mine / sum;
+    score = (float)(mine * (double)r.scale);
+  }
+};
+
 // One wave per token.
-template <int L, int NV>
+template <int L, int NV, typename Router>
 __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ logits, int tokens, int n_experts,
-                                                    int top_k, int normalize, uint32_t* __restrict__ experts,
+                                                    int top_k, Router router, uint32_t* __restrict__ experts,
                                                     float* __restrict__ scores) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= tokens) return;  // whole waves leave together
   int pick;
   float score;
-  route_token<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, normalize, pick, score);
+  router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
   if (lane < top_k) {
     experts[(size_t)t * top_k + lane] = (uint32_t)pick;
     scores[(size_t)t * top_k + lane] = score;
@@ -146,9 +272,9 @@ __device__ __forceinline__ void lane_rank(uint32_t e, uint32_t& rank, uint32_t& 
 // counts of expert e, a scan over the experts gives the starts, and each row's
 // position is its expert's start, the earlier waves' counts and its rank.
 constexpr int kFusedTokens = 32;
-template <int L, int NV>
+template <int L, int NV, typename Router>
 __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict__ logits, int tokens, int n_experts,
-                                                          int top_k, int normalize, uint32_t* __restrict__ experts,
+                                                          int top_k, Router router, uint32_t* __restrict__ experts,
                                                           float* __restrict__ scores, uint32_t* __restrict__ lhs,
                                                           uint32_t* __restrict__ rhs, uint32_t* __restrict__ inv,
                                                           uint32_t* __restrict__ offsets) {
@@ -163,7 +289,7 @@ __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict
   for (int t = wave; t < tokens; t += 16) {
     int pick;
     float score;
-    route_token<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, normalize, pick, score);
+    router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
     if (lane < top_k) {
       const int r = t * top_k + lane;
       pick_of[r] = (uint32_t)pick;
@@ -325,64 +451,70 @@ size_t moe_sort_scratch_bytes(int rows, int n_experts) {
   return blocks * (size_t)n_experts * 4;
 }
 
-template <int L>
-hipError_t launch_route_nv(hipStream_t s, const void* logits, int tokens, int n_experts, int top_k, int normalize,
-                           uint32_t* experts, float* scores) {
-  const unsigned grid = (unsigned)((tokens + 3) / 4);
+// run(L, NV) as types of integral constants: the logits' type and their number a lane.
+template <typename F>
+hipError_t with_logits(int logits_dtype, int n_experts, F run) {
   const int nv = (n_experts + 63) / 64;
-#define CPQ_ROUTE(NVV) \
-  hipLaunchKernelGGL((route_kernel<L, NVV>), dim3(grid), dim3(256), 0, s, logits, tokens, n_experts, top_k, \
-                     normalize, experts, scores)
-  if (nv <= 1) CPQ_ROUTE(1);
-  else if (nv <= 2) CPQ_ROUTE(2);
-  else if (nv <= 4) CPQ_ROUTE(4);
-  else if (nv <= 8) CPQ_ROUTE(8);
-  else CPQ_ROUTE(16);
-#undef CPQ_ROUTE
-  return hipGetLastError();
+  auto typed = [&](auto l) {
+    if (nv <= 1) run(l, std::integral_constant<int, 1>{});
+    else if (nv <= 2) run(l, std::integral_constant<int, 2>{});
+    else if (nv <= 4) run(l, std::integral_constant<int, 4>{});
+    else if (nv <= 8) run(l, std::integral_constant<int, 8>{});
+    else run(l, std::integral_constant<int, 16>{});
+    return hipGetLastError();
+  };
+  if (logits_dtype == CPQ_DTYPE_F32) return typed(std::integral_constant<int, 0>{});
+  if (logits_dtype == CPQ_DTYPE_F16) return typed(std::integral_constant<int, 1>{});
+  return typed(std::integral_constant<int, 2>{});
 }
 
-template <int L>
-hipError_t launch_route_sort_nv(hipStream_t s, const void* logits, int tokens, int n_experts, int top_k, int normalize,
-                                uint32_t* experts, float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
-                                uint32_t* offsets) {
-  const int nv = (n_experts + 63) / 64;
-#define CPQ_ROUTE(NVV)                                                                                               \
-  hipLaunchKernelGGL((route_sort_kernel<L, NVV>), dim3(1), dim3(1024), 0, s, logits, tokens, n_experts, top_k, normalize, \
-                     experts, scores, lhs, rhs, inv, offsets)
-  if (nv <= 1) CPQ_ROUTE(1);
-  else if (nv <= 2) CPQ_ROUTE(2);
-  else if (nv <= 4) CPQ_ROUTE(4);
-  else if (nv <= 8) CPQ_ROUTE(8);
-  else CPQ_ROUTE(16);
-#undef CPQ_ROUTE
-  return hipGetLastError();
+template <typename Router>
+hipError_t launch_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
+                        const Router& router, uint32_t* experts, float* scores) {
+  if (tokens == 0) return hipSuccess;
+  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    hipLaunchKernelGGL((route_kernel<decltype(l)::value, decltype(nv)::value, Router>),
+                       dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, logits, tokens, n_experts, top_k, router,
+                       experts, scores);
+  });
+}
+
+template <typename Router>
+hipError_t launch_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
+                             const Router& router, uint32_t* experts, float* scores, uint32_t* lhs, uint32_t* rhs,
+                             uint32_t* inv, uint32_t* offsets) {
+  if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
+  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    hipLaunchKernelGGL((route_sort_kernel<decltype(l)::value, decltype(nv)::value, Router>), dim3(1), dim3(1024), 0, s,
+                       logits, tokens, n_experts, top_k, router, experts, scores, lhs, rhs, inv, offsets);
+  });
 }
 
 bool moe_route_sort_fits(int tokens) { return tokens >= 1 && tokens <= kFusedTokens; }
 
+hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
+                            int normalize, uint32_t* experts, float* scores) {
+  return launch_route(s, logits_dtype, logits, tokens, n_experts, top_k, SoftmaxRouter{normalize}, experts, scores);
+}
+
 hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
                                  int top_k, int normalize, uint32_t* experts, float* scores, uint32_t* lhs,
                                  uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
-  if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
-  if (logits_dtype == CPQ_DTYPE_F32)
-    return launch_route_sort_nv<0>(s, logits, tokens, n_experts, top_k, normalize, experts, scores, lhs, rhs, inv,
-                                   offsets);
-  if (logits_dtype == CPQ_DTYPE_F16)
-    return launch_route_sort_nv<1>(s, logits, tokens, n_experts, top_k, normalize, experts, scores, lhs, rhs, inv,
-                                   offsets);
-  return launch_route_sort_nv<2>(s, logits, tokens, n_experts, top_k, normalize, experts, scores, lhs, rhs, inv,
-                                 offsets);
+  return launch_route_sort(s, logits_dtype, logits, tokens, n_experts, top_k, SoftmaxRouter{normalize}, experts, scores,
+                           lhs, rhs, inv, offsets);
 }
 
-hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
-                            int normalize, uint32_t* experts, float* scores) {
-  if (tokens == 0) return hipSuccess;
-  if (logits_dtype == CPQ_DTYPE_F32)
-    return launch_route_nv<0>(s, logits, tokens, n_experts, top_k, normalize, experts, scores);
-  if (logits_dtype == CPQ_DTYPE_F16)
-    return launch_route_nv<1>(s, logits, tokens, n_experts, top_k, normalize, experts, scores);
-  return launch_route_nv<2>(s, logits, tokens, n_experts, top_k, normalize, experts, scores);
+hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
+                                    int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores) {
+  return launch_route(s, logits_dtype, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts, scores);
+}
+
+hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens,
+                                         int n_experts, int top_k, const cpq_moe_router& r, uint32_t* experts,
+                                         float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
+                                         uint32_t* offsets) {
+  return launch_route_sort(s, logits_dtype, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts, scores, lhs,
+                           rhs, inv, offsets);
 }
 
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,

@@ -1,6 +1,7 @@
 // Entry points of the 4-bit key/value cache (cpq_kv_*): argument validation
 // and launch.  No reference counterpart; semantics in cpq.h.
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -77,6 +78,14 @@ cpq_status check_strided(const char* op, const char* name, const void* p, size_t
   return CPQ_OK;
 }
 
+// No two rows of [tokens, heads, dim] share elements: heads within a token's row, or
+// tokens within a head's.
+bool rows_apart(size_t tokens, size_t heads, size_t d, size_t t, size_t h) {
+  const bool inner_heads = (heads == 1 || h >= d) && (tokens == 1 || t >= (heads - 1) * h + d);
+  const bool inner_tokens = (tokens == 1 || t >= d) && (heads == 1 || h >= (tokens - 1) * t + d);
+  return inner_heads || inner_tokens;
+}
+
 bool overlap(const void* a, size_t a_words, const void* b, size_t b_words) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
   return a_words && b_words && x < y + 4 * b_words && y < x + 4 * a_words;
@@ -84,11 +93,11 @@ bool overlap(const void* a, size_t a_words, const void* b, size_t b_words) {
 
 struct Words {
   const char* name;
-  const void* p;
+  const void* p;  // of 32-bit values
   size_t n;
 };
 
-// u32 arrays of one call: not NULL, 4-byte aligned, and no output (the last
+// 32-bit arrays of one call: not NULL, 4-byte aligned, and no output (the last
 // n_out of them) over another.
 cpq_status check_words(const char* op, const Words* w, int n, int n_out) {
   for (int i = 0; i < n; ++i) {
@@ -214,8 +223,7 @@ cpq_status cpq_kv_gather(cpq_commands* cmds, const cpq_kv_cache* cache, const ui
                   "kv_gather launch");
 }
 
-cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* a) {
-  const char* op = "kv_attention";
+static cpq_status check_attention(const char* op, const cpq_kv_cache* cache, const cpq_kv_attention_args* a) {
   cpq_status st = check_cache(op, cache);
   if (st != CPQ_OK) return st;
   if (!a) return invalid(op, "NULL arguments");
@@ -237,15 +245,16 @@ cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_a
   st = check_strided(op, "out", a->out, a->n_tokens, a->n_heads, cache->head_dim, a->out_token_stride,
                      a->out_head_stride);
   if (st != CPQ_OK) return st;
-  // No two output rows share elements: heads within a token's row, or tokens within a head's.
-  const size_t d = cache->head_dim, t = a->out_token_stride, h = a->out_head_stride;
-  const bool inner_heads = (a->n_heads == 1 || h >= d) && (a->n_tokens == 1 || t >= (a->n_heads - 1) * h + d);
-  const bool inner_tokens = (a->n_tokens == 1 || t >= d) && (a->n_heads == 1 || h >= (a->n_tokens - 1) * t + d);
-  if (!inner_heads && !inner_tokens) return invalid(op, "out rows overlap at these strides");
+  if (!rows_apart(a->n_tokens, a->n_heads, cache->head_dim, a->out_token_stride, a->out_head_stride))
+    return invalid(op, "out rows overlap at these strides");
   const Words w[] = {{"block_table", a->block_table, entries},
                      {"query_starts", a->query_starts, a->n_seqs + 1},
                      {"kv_lens", a->kv_lens, a->n_seqs}};
   return check_words(op, w, 3, 0);
+}
+
+cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* a) {
+  return check_attention("kv_attention", cache, a);
 }
 
 cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_attention_args* args) {
@@ -255,6 +264,80 @@ cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const
   if (args->n_tokens == 0 || args->n_seqs == 0) return CPQ_OK;
   return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 7),
                   "kv_attention launch");
+}
+
+cpq_status cpq_check_kv_attention_scored_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* a,
+                                              const cpq_kv_scores* scores) {
+  const char* op = "kv_attention_scored";
+  cpq_status st = check_attention(op, cache, a);
+  if (st != CPQ_OK) return st;
+  if (!scores) return invalid(op, "NULL scores");
+  if (!(scores->softcap >= 0.f) || scores->softcap > cpq::kKvMostCap)
+    return invalid(op, "softcap outside 0..=" + std::to_string((int)cpq::kKvMostCap));
+  if (!aligned(scores->slopes, 4) || !aligned(scores->prefix_lens, 4))
+    return invalid(op, "slopes and prefix_lens must be 4-byte aligned");
+  return CPQ_OK;
+}
+
+cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_attention_args* args,
+                                   const cpq_kv_scores* scores) {
+  if (!cmds) return invalid("kv_attention_scored", "NULL command session");
+  cpq_status st = cpq_check_kv_attention_scored_args(cache, args, scores);
+  if (st != CPQ_OK) return st;
+  if (args->n_tokens == 0 || args->n_seqs == 0) return CPQ_OK;
+  const float cap = scores->softcap;
+  const cpq::KvScore score{cap * 1.44269504088896340736f, cap > 0.f ? 2.f / cap : 0.f, scores->slopes,
+                           args->causal ? scores->prefix_lens : nullptr};
+  if (!(score.cap > 0.f) && !score.slopes && !score.prefix_lens)
+    return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 7),
+                    "kv_attention_scored launch");
+  return launched(cpq::launch_kv_attention_scored(cpq::session_ctx(cmds), *cache, *args, score, cmds->status + 7),
+                  "kv_attention_scored launch");
+}
+
+cpq_status cpq_check_kv_append_rotary_args(const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* a) {
+  const char* op = "kv_append_rotary";
+  cpq_status st = check_cache(op, cache);
+  if (st != CPQ_OK) return st;
+  if (!a) return invalid(op, "NULL arguments");
+  if (a->n_tokens > (size_t)INT_MAX) return invalid(op, "n_tokens must fit in i32");
+  if (a->n_heads > 65535) return invalid(op, "n_heads outside 0..=65535");
+  if (a->rotary_dim == 0 || a->rotary_dim % 16 != 0 || a->rotary_dim > cache->head_dim)
+    return invalid(op, "rotary_dim (" + std::to_string(a->rotary_dim) + ") must be a multiple of 16 up to head_dim (" +
+                           std::to_string(cache->head_dim) + ")");
+  if (!std::isfinite(a->magnitude)) return invalid(op, "magnitude must be finite");
+  if (a->n_tokens == 0) return CPQ_OK;
+  const size_t d = cache->head_dim, heads = cache->n_kv_heads;
+  st = check_strided(op, "k", a->k, a->n_tokens, heads, d, a->k_token_stride, a->k_head_stride);
+  if (st != CPQ_OK) return st;
+  st = check_strided(op, "v", a->v, a->n_tokens, heads, d, a->v_token_stride, a->v_head_stride);
+  if (st != CPQ_OK) return st;
+  if (a->n_heads) {
+    st = check_strided(op, "q", a->q, a->n_tokens, a->n_heads, d, a->q_token_stride, a->q_head_stride);
+    if (st != CPQ_OK) return st;
+    st = check_strided(op, "q_out", a->q_out, a->n_tokens, a->n_heads, d, a->q_out_token_stride,
+                       a->q_out_head_stride);
+    if (st != CPQ_OK) return st;
+    if (!rows_apart(a->n_tokens, a->n_heads, d, a->q_out_token_stride, a->q_out_head_stride))
+      return invalid(op, "q_out rows overlap at these strides");
+    if (a->q == a->q_out &&
+        ((a->n_tokens > 1 && a->q_token_stride != a->q_out_token_stride) ||
+         (a->n_heads > 1 && a->q_head_stride != a->q_out_head_stride)))
+      return invalid(op, "q_out is q at other strides");
+  }
+  const Words w[] = {{"slots", a->slots, a->n_tokens},
+                     {"positions", a->positions, a->n_tokens},
+                     {"frequencies", a->frequencies, a->rotary_dim / 2}};
+  return check_words(op, w, 3, 0);
+}
+
+cpq_status cpq_kv_append_rotary(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* args) {
+  if (!cmds) return invalid("kv_append_rotary", "NULL command session");
+  cpq_status st = cpq_check_kv_append_rotary_args(cache, args);
+  if (st != CPQ_OK) return st;
+  if (args->n_tokens == 0) return CPQ_OK;
+  return launched(cpq::launch_kv_append_rotary(cmds->stream, *cache, *args, cmds->status + 6),
+                  "kv_append_rotary launch");
 }
 
 }  // extern "C"

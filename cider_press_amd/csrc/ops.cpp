@@ -84,6 +84,41 @@ bool mul_ok(size_t a, size_t b, size_t* out) {
   return true;
 }
 
+// What moe_route and moe_route_grouped check alike: sizes; then buffers, and the sort's
+// histograms in the session's scratch.
+cpq_status check_route_sizes(const char* op, cpq_dtype logits_dtype, size_t tokens, size_t n_experts, uint32_t top_k,
+                             size_t* rows) {
+  cpq_status st = check_dtype(op, logits_dtype);
+  if (st != CPQ_OK) return st;
+  if (n_experts == 0 || n_experts > 1024)
+    return fail(CPQ_ERR_INVALID_ARGUMENT,
+                std::string(op) + ": n_experts=" + std::to_string(n_experts) + " outside 1..=1024");
+  if (top_k == 0 || top_k > 16 || top_k > n_experts)
+    return fail(CPQ_ERR_INVALID_ARGUMENT,
+                std::string(op) + ": top_k=" + std::to_string(top_k) + " outside 1..=min(16, n_experts)");
+  if (!mul_ok(tokens, top_k, rows) || *rows >= (1ull << 31) || tokens * n_experts / n_experts != tokens)
+    return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": tokens*top_k beyond 32-bit indexing");
+  return CPQ_OK;
+}
+cpq_status check_route_buffers(const char* op, const cpq_commands* cmds, size_t tokens, size_t rows, size_t n_experts,
+                               const void* logits, const void* experts, const void* scores, const void* lhs,
+                               const void* rhs, const void* inv, const void* offsets, uint32_t** hist) {
+  if (!offsets) return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": NULL offsets");
+  if (tokens && (!logits || !experts || !scores || !lhs || !rhs || !inv))
+    return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": NULL buffer");
+  void* scratch = nullptr;
+  const size_t need = kWideCounterBytes + moe_sort_scratch_bytes((int)rows, (int)n_experts);
+  if (!session_scratch(cmds, need, &scratch))
+    return fail(CPQ_ERR_BUFFER_TOO_LARGE, std::string(op) + ": the sort needs " + std::to_string(need) +
+                                              " bytes of session scratch; the session holds " +
+                                              std::to_string(cmds->scratch_bytes) +
+                                              " (CPQ_SESSION_SCRATCH_MB sets it when the session is made)");
+  // The scratch head holds the prefill kernel's arrival counters; the sort's
+  // block histograms go after it.
+  *hist = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + kWideCounterBytes);
+  return CPQ_OK;
+}
+
 }  // namespace
 }  // namespace cpq
 
@@ -828,35 +863,20 @@ cpq_status cpq_embed_tokens(cpq_commands* cmds, cpq_dtype dtype, const uint32_t*
 cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void* logits, size_t tokens,
                          size_t n_experts, uint32_t top_k, int normalize, uint32_t* experts, float* scores,
                          uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
+  const char* op = "moe_route";
   if (!cmds) return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: NULL command session");
-  cpq_status st = cpq::check_dtype("moe_route", logits_dtype);
-  if (st != CPQ_OK) return st;
-  if (n_experts == 0 || n_experts > 1024)
-    return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: n_experts=" + std::to_string(n_experts) + " outside 1..=1024");
-  if (top_k == 0 || top_k > 16 || top_k > n_experts)
-    return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: top_k=" + std::to_string(top_k) +
-                                              " outside 1..=min(16, n_experts)");
   size_t rows;
-  if (!cpq::mul_ok(tokens, top_k, &rows) || rows >= (1ull << 31) || tokens * n_experts / n_experts != tokens)
-    return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: tokens*top_k beyond 32-bit indexing");
-  if (!offsets) return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: NULL offsets");
-  if (tokens && (!logits || !experts || !scores || !lhs || !rhs || !inv))
-    return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route: NULL buffer");
-  void* scratch = nullptr;
-  const size_t need = cpq::kWideCounterBytes + cpq::moe_sort_scratch_bytes((int)rows, (int)n_experts);
-  if (!cpq::session_scratch(cmds, need, &scratch))
-    return fail(CPQ_ERR_BUFFER_TOO_LARGE, "moe_route: the sort needs " + std::to_string(need) +
-                                              " bytes of session scratch; the session holds " +
-                                              std::to_string(cmds->scratch_bytes) +
-                                              " (CPQ_SESSION_SCRATCH_MB sets it when the session is made)");
+  cpq_status st = cpq::check_route_sizes(op, logits_dtype, tokens, n_experts, top_k, &rows);
+  if (st != CPQ_OK) return st;
+  uint32_t* hist;
+  st = cpq::check_route_buffers(op, cmds, tokens, rows, n_experts, logits, experts, scores, lhs, rhs, inv, offsets,
+                                &hist);
+  if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))
     return cpq::launched(cpq::launch_moe_route_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,
                                                     (int)n_experts, (int)top_k, normalize, experts, scores, lhs, rhs,
                                                     inv, offsets),
                          "moe_route launch");
-  // The scratch head holds the prefill kernel's arrival counters; the sort's
-  // block histograms go after it.
-  uint32_t* hist = reinterpret_cast<uint32_t*>(static_cast<char*>(scratch) + cpq::kWideCounterBytes);
   st = cpq::launched(cpq::launch_moe_route(cmds->stream, (int)logits_dtype, logits, (int)tokens, (int)n_experts,
                                            (int)top_k, normalize, experts, scores),
                      "moe_route launch");
@@ -864,6 +884,54 @@ cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void*
   return cpq::launched(cpq::launch_moe_sort(cmds->stream, experts, (int)rows, (int)top_k, (int)n_experts, hist, lhs,
                                             rhs, inv, offsets),
                        "moe_route sort launch");
+}
+
+cpq_status cpq_check_moe_route_grouped_args(cpq_dtype logits_dtype, size_t tokens, size_t n_experts, uint32_t top_k,
+                                            const cpq_moe_router* r) {
+  const char* op = "moe_route_grouped";
+  size_t rows;
+  cpq_status st = cpq::check_route_sizes(op, logits_dtype, tokens, n_experts, top_k, &rows);
+  if (st != CPQ_OK) return st;
+  auto invalid = [&](const std::string& what) { return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what); };
+  if (!r) return invalid("NULL router");
+  if (r->n_groups == 0 || r->n_groups > 64 || n_experts % r->n_groups != 0)
+    return invalid("n_groups=" + std::to_string(r->n_groups) + " outside 1..=64 or no divisor of n_experts=" +
+                   std::to_string(n_experts));
+  const size_t size = n_experts / r->n_groups;
+  if (r->top_groups == 0 || r->top_groups > r->n_groups)
+    return invalid("top_groups=" + std::to_string(r->top_groups) + " outside 1..=n_groups");
+  if (r->group_best == 0 || r->group_best > 2 || r->group_best > size)
+    return invalid("group_best=" + std::to_string(r->group_best) + " outside 1..=min(2, experts of a group)");
+  if (top_k > size * r->top_groups) return invalid("top_k exceeds the experts of top_groups groups");
+  if (!std::isfinite(r->scale)) return invalid("scale must be finite");
+  if (reinterpret_cast<uintptr_t>(r->bias) & 3u) return invalid("bias must be 4-byte aligned");
+  return CPQ_OK;
+}
+
+cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, const void* logits, size_t tokens,
+                                 size_t n_experts, uint32_t top_k, const cpq_moe_router* router, uint32_t* experts,
+                                 float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
+  const char* op = "moe_route_grouped";
+  if (!cmds) return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route_grouped: NULL command session");
+  cpq_status st = cpq_check_moe_route_grouped_args(logits_dtype, tokens, n_experts, top_k, router);
+  if (st != CPQ_OK) return st;
+  const size_t rows = tokens * top_k;
+  uint32_t* hist;
+  st = cpq::check_route_buffers(op, cmds, tokens, rows, n_experts, logits, experts, scores, lhs, rhs, inv, offsets,
+                                &hist);
+  if (st != CPQ_OK) return st;
+  if (cpq::moe_route_sort_fits((int)tokens))
+    return cpq::launched(cpq::launch_moe_route_grouped_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,
+                                                            (int)n_experts, (int)top_k, *router, experts, scores, lhs,
+                                                            rhs, inv, offsets),
+                         "moe_route_grouped launch");
+  st = cpq::launched(cpq::launch_moe_route_grouped(cmds->stream, (int)logits_dtype, logits, (int)tokens,
+                                                   (int)n_experts, (int)top_k, *router, experts, scores),
+                     "moe_route_grouped launch");
+  if (st != CPQ_OK) return st;
+  return cpq::launched(cpq::launch_moe_sort(cmds->stream, experts, (int)rows, (int)top_k, (int)n_experts, hist, lhs,
+                                            rhs, inv, offsets),
+                       "moe_route_grouped sort launch");
 }
 
 cpq_status cpq_moe_combine(cpq_commands* cmds, cpq_dtype dtype, const void* y, size_t y_len, const float* scores,

@@ -1,5 +1,6 @@
 """Key/value cache in 4 bits: block tables and slots from request lengths, the
-quantizing append, the dequantizing gather, and attention over the cache.
+quantizing append (with the position rotation on the way), the dequantizing
+gather, and attention over the cache (with capped or biased scores).
 
 No reference counterpart: its KV cache (crates/cider-press-runtime/src/
 kv_cache.rs) holds dense T.  Layouts and semantics are stated in
@@ -36,6 +37,18 @@ def _attention_args(*fields) -> bytes:
         return _ATTENTION_ARGS.pack(*fields)
     except struct.error as e:  # a negative or too large count
         raise _lib.InvalidArgument(f"kv_attention: {e}") from None
+
+
+# cpq_kv_scores and cpq_kv_append_rotary_args, likewise.
+_SCORES = struct.Struct("@fPP")
+_ROTARY_ARGS = struct.Struct("@PNNPNNNPNNPNNPPNPIif0P")
+
+
+def _pack(op: str, fields: struct.Struct, *values) -> bytes:
+    try:
+        return fields.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise _lib.InvalidArgument(f"{op}: {e}") from None
 
 
 class KvCache:
@@ -120,6 +133,29 @@ def kv_append(commands: Commands, cache: KvCache, k: Buffer, v: Buffer, slots: B
                                         tokens))
 
 
+def kv_append_rotary(commands: Commands, cache: KvCache, q, k: Buffer, v: Buffer, slots: Buffer, positions: Buffer,
+                     frequencies: Buffer, q_out, tokens: int, n_heads: int, interleaved: bool = False,
+                     magnitude: float = 1.0, q_strides=None, k_strides=None, v_strides=None,
+                     q_out_strides=None) -> None:
+    """kv_append with the position rotation of keys on the way, queries rotated
+    into q_out; the first 2 * len(frequencies) dimensions rotate, as pairs
+    (i, i + len(frequencies)) or, interleaved, (2 i, 2 i + 1), by positions[t] *
+    frequencies[i], cosines and sines times magnitude.  n_heads = 0 with q and
+    q_out None: keys and values only.  Encodes only."""
+    op = "kv_append_rotary"
+    _need(op, "u32", (slots, tokens), (positions, tokens))
+    _need(op, "f32", (frequencies, 0))
+    kt, kh = _strides(op, cache.dtype, k_strides, k, tokens, cache.n_kv_heads, cache.head_dim)
+    vt, vh = _strides(op, cache.dtype, v_strides, v, tokens, cache.n_kv_heads, cache.head_dim)
+    qt = qh = ot = oh = 0
+    if n_heads:
+        qt, qh = _strides(op, cache.dtype, q_strides, q, tokens, n_heads, cache.head_dim)
+        ot, oh = _strides(op, cache.dtype, q_out_strides, q_out, tokens, n_heads, cache.head_dim)
+    args = _pack(op, _ROTARY_ARGS, _ptr(q) or 0, qt, qh, _ptr(q_out) or 0, ot, oh, n_heads, k.ptr, kt, kh, v.ptr, vt, vh,
+                 slots.ptr, positions.ptr, tokens, frequencies.ptr, 2 * frequencies._len, bool(interleaved), magnitude)
+    _lib.check(_lib.lib().cpq_kv_append_rotary(commands.handle, cache._ref, args))
+
+
 def kv_gather(commands: Commands, cache: KvCache, slots: Buffer, rows: int, k_out=None, v_out=None) -> None:
     """Cached keys and values of `rows` slots as dense T [rows, n_kv_heads,
     head_dim]; either output may be None.  Encodes only."""
@@ -143,3 +179,24 @@ def kv_attention(commands: Commands, cache: KvCache, q: Buffer, block_table: Buf
     args = _attention_args(q.ptr, qt, qh, out.ptr, ot, oh, tokens, n_heads, block_table.ptr, max_blocks,
                            query_starts.ptr, kv_lens.ptr, n_seqs, max_q, max_kv, scale, bool(causal), window)
     _lib.check(_lib.lib().cpq_kv_attention(commands.handle, cache._ref, args))
+
+
+def kv_attention_scored(commands: Commands, cache: KvCache, q: Buffer, block_table: Buffer, max_blocks: int,
+                        query_starts: Buffer, kv_lens: Buffer, out: Buffer, tokens: int, n_heads: int, n_seqs: int,
+                        max_q: int, max_kv: int, scale: float, causal: bool = True, window: int = 0,
+                        softcap: float = 0.0, slopes=None, prefix_lens=None, q_strides=None, out_strides=None) -> None:
+    """kv_attention whose scores t become softcap * tanh(t / softcap) (softcap >
+    0), plus slopes[h] * (key's position - query's), and whose first
+    prefix_lens[s] keys every query of sequence s sees.  Encodes only."""
+    op = "kv_attention_scored"
+    _need(op, "u32", (block_table, n_seqs * max_blocks), (query_starts, n_seqs + 1), (kv_lens, n_seqs))
+    if slopes is not None:
+        _need(op, "f32", (slopes, n_heads))
+    if prefix_lens is not None:
+        _need(op, "u32", (prefix_lens, n_seqs))
+    qt, qh = _strides(op, cache.dtype, q_strides, q, tokens, n_heads, cache.head_dim)
+    ot, oh = _strides(op, cache.dtype, out_strides, out, tokens, n_heads, cache.head_dim)
+    args = _pack(op, _ATTENTION_ARGS, q.ptr, qt, qh, out.ptr, ot, oh, tokens, n_heads, block_table.ptr, max_blocks,
+                 query_starts.ptr, kv_lens.ptr, n_seqs, max_q, max_kv, scale, bool(causal), window)
+    scores = _pack(op, _SCORES, softcap, _ptr(slopes) or 0, _ptr(prefix_lens) or 0)
+    _lib.check(_lib.lib().cpq_kv_attention_scored(commands.handle, cache._ref, args, scores))

@@ -402,6 +402,35 @@ cpq_status cpq_embed_tokens(cpq_commands* cmds, cpq_dtype dtype, const uint32_t*
 cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void* logits, size_t tokens,
                          size_t n_experts, uint32_t top_k, int normalize, uint32_t* experts, float* scores,
                          uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
+/* moe_route with other scores, a bias and groups.  Per token, in fp64:
+ *   s = softmax(logits) or, sigmoid, 1 / (1 + e^-logits);  c = s + bias (f32
+ *   [n_experts] on the device, or NULL: c = s)
+ *   n_groups > 1: of the n_groups runs of n_experts / n_groups experts the top_groups with
+ *   the highest score are kept (ties: lower group), a group's score being its largest c
+ *   (group_best 1) or the sum of its two largest (2)
+ *   experts: among the kept, the top_k largest c in descending order (ties: lower expert)
+ *   scores: s of these, divided by their sum when `normalize`, times scale; rounded to
+ *   fp32 once.  (A sum of 0 gives 0.)
+ * A c that is NaN counts as lower than every number (its s is kept as it is).  Choices
+ * are made in fp64 because they are whole numbers: in fp32 near scores would change
+ * places with the order of a sum.  Then the sort, as moe_route.  n_experts <= 1024, top_k
+ * <= min(16, n_experts / n_groups * top_groups), n_groups <= 64 divides n_experts,
+ * group_best <= n_experts / n_groups.  Uses session scratch. */
+typedef struct cpq_moe_router {
+  int sigmoid;
+  const float* bias;
+  uint32_t n_groups;
+  uint32_t top_groups;
+  uint32_t group_best;
+  int normalize;
+  float scale;
+} cpq_moe_router;
+cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, const void* logits, size_t tokens,
+                                 size_t n_experts, uint32_t top_k, const cpq_moe_router* router, uint32_t* experts,
+                                 float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
+/* Host-only argument validator of the above (callable without a GPU). */
+cpq_status cpq_check_moe_route_grouped_args(cpq_dtype logits_dtype, size_t tokens, size_t n_experts, uint32_t top_k,
+                                            const cpq_moe_router* router);
 /* moe_combine: out[t, :] = RNE_T(sum_j scores[t*k + j] * y[inv[t*k + j], :]),
  * fp32 accumulation in j order; y is the [tokens*k, N] expert output in
  * sorted row order.  A position outside the rows contributes nothing and is
@@ -553,10 +582,69 @@ typedef struct cpq_kv_attention_args {
 } cpq_kv_attention_args;
 cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_attention_args* args);
 
+/* cpq_kv_attention with scores that are capped or fall with distance, and with
+ * prefixes.  In its notation, t = scale * <q, k_j> becomes
+ *   softcap > 0:  softcap * tanh(t / softcap)
+ *   slopes:       that + slopes[h] * (j - p) for query head h ([n_heads], f32 on the
+ *                 device; magnitudes past 2^96 count as 2^96)
+ * and, if causal, keys j < prefix_lens[s] are seen from every position too ([n_seqs]; a
+ * window hides them as it hides others; past kv_lens[s]: all keys).  softcap up to
+ * 1024: a weight is off by 2^-22 * softcap of itself besides.  NULL or 0: not that; with
+ * none of them this is cpq_kv_attention.  All else as there. */
+typedef struct cpq_kv_scores {
+  float softcap;
+  const float* slopes;
+  const uint32_t* prefix_lens;
+} cpq_kv_scores;
+cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_attention_args* args,
+                                   const cpq_kv_scores* scores);
+
+/* Position rotation and append in one pass.  For each token t with a slot: the first
+ * rotary_dim dimensions of its queries and keys are rotated by its position,
+ *   angle = positions[t] * frequencies[i],  c, s = magnitude * cos, sin (angle)
+ *   (a, b) becomes (a c - b s, b c + a s)
+ * over the pairs (i, i + rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), i <
+ * rotary_dim / 2, the other dimensions stay; with the arithmetic in fp64, rounded to fp32
+ * and then to T.  Queries are written to q_out (which may be q at the same strides, and
+ * else must not overlap an input); keys, rotated, and values go into the cache as
+ * cpq_kv_append puts them there, bit for bit.  Tokens whose slot is none are skipped,
+ * their rows of q_out too; so are slots past the cache, which are reported as by
+ * cpq_kv_append.
+ * q, q_out [n_tokens, n_heads, head_dim], k, v [n_tokens, n_kv_heads, head_dim] at token
+ * and head strides in elements (multiples of 8), 16-byte aligned; n_heads = 0: keys and
+ * values only.  rotary_dim: a multiple of 16, up to head_dim.  frequencies: f32
+ * [rotary_dim / 2], radians a position.  magnitude: finite. */
+typedef struct cpq_kv_append_rotary_args {
+  const void* q;
+  size_t q_token_stride;
+  size_t q_head_stride;
+  void* q_out;
+  size_t q_out_token_stride;
+  size_t q_out_head_stride;
+  size_t n_heads;
+  const void* k;
+  size_t k_token_stride;
+  size_t k_head_stride;
+  const void* v;
+  size_t v_token_stride;
+  size_t v_head_stride;
+  const uint32_t* slots;
+  const uint32_t* positions;
+  size_t n_tokens;
+  const float* frequencies;
+  uint32_t rotary_dim;
+  int interleaved;
+  float magnitude; /* 1: none */
+} cpq_kv_append_rotary_args;
+cpq_status cpq_kv_append_rotary(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* args);
+
 /* Host-only argument validators of the above (callable without a GPU; of the
- * pointers only NULL and alignment are looked at). */
+ * pointers only NULL, alignment and overlap are looked at). */
 cpq_status cpq_check_kv_cache(const cpq_kv_cache* cache);
 cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* args);
+cpq_status cpq_check_kv_attention_scored_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* args,
+                                              const cpq_kv_scores* scores);
+cpq_status cpq_check_kv_append_rotary_args(const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* args);
 
 /* ------------------------------------------------------------------ */
 /* Runtime node (runtime/src/{quantized,tensor,eval}.rs)                 */
