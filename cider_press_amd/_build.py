@@ -37,7 +37,8 @@ SOURCES = [
     "kernels/moe.hip",
     "kernels/stream_read.hip",
     "kv.cpp", "kernels/kv_cache.hip", "kernels/kv_attention.hip", "kernels/kv_decode.hip",
-    "kernels/kv_attention_scored.hip", "kernels/kv_decode_scored.hip",
+    "kernels/kv_attention_biased.hip", "kernels/kv_attention_capped.hip",
+    "kernels/kv_decode_biased.hip", "kernels/kv_decode_capped.hip",
 ]
 
 ARCH = "gfx950"

@@ -247,9 +247,13 @@ struct KvScore {
   const float* slopes = nullptr;
   const uint32_t* prefix_lens = nullptr;
 };
-hipError_t launch_kv_attention_scored(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+hipError_t launch_kv_attention_biased(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                       const KvScore& score, unsigned int* bad);
-hipError_t launch_kv_decode_scored(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+hipError_t launch_kv_decode_biased(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                   const KvScore& score, int rows_max, bool report, unsigned int* bad);
+hipError_t launch_kv_attention_capped(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                      const KvScore& score, unsigned int* bad);
+hipError_t launch_kv_decode_capped(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                    const KvScore& score, int rows_max, bool report, unsigned int* bad);
 // Y = X . W^T with the kernel chosen by M (small-M kernels, else the prefill
 // plan), as affine_qmm_t and the runtime node run it.

@@ -1,5 +1,5 @@
 // Attention of a step's queries over the 4-bit key/value cache (semantics:
-// cpq_kv_attention and, SCORED, cpq_kv_attention_scored in cpq.h): the kernel for many
+// cpq_kv_attention and, scored, cpq_kv_attention_scored in cpq.h): the kernel for many
 // query rows per sequence, and the choice between it and kv_decode.hpp.
 //
 // A workgroup takes 32 query rows a wave of one key/value head (rows run over the
@@ -389,7 +389,7 @@ __device__ __forceinline__ bool find_item(const TileArgs& p, int b, int group, i
 }
 
 // GS: the group size at T = f16, 0 (any) at bf16.
-template <typename TT, int D, int kWaves, int GS, bool SCORED>
+template <typename TT, int D, int kWaves, int GS, Scores SCORES>
 __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2) void kv_tile_kernel(TileArgs p) {
   constexpr int W = D / 8, NS = D / 16, ND = D / 32, kUnits = kKeys * W;
   constexpr int kTeams = kWaves / 4, kBufs = 2 * kTeams;
@@ -423,7 +423,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
 
   // Keys that any of the rows sees, in tiles; this part's.
   const int pos0 = q.pos + row0 / group, pos1 = q.pos + (row1 - 1) / group;
-  const int prefix = SCORED ? kv_prefix(p.score, it.s, q.n) : 0;
+  constexpr bool kScored = SCORES != Scores::kPlain;
+  const int prefix = kScored ? kv_prefix(p.score, it.s, q.n) : 0;
   const int end = max(a.causal ? min(max(pos1 + 1, prefix), q.n) : q.n, 0);
   const int from = a.window ? (int)max((int64_t)pos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
   const int first = from / kKeys, tiles = max((end + kKeys - 1) / kKeys - first, 0);
@@ -487,8 +488,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
   const int any_from = a.window ? (int)max((int64_t)wpos0 + 1 - (int64_t)a.window, (int64_t)0) : 0;
   const int all_from = a.window ? (int)max((int64_t)wpos1 + 1 - (int64_t)a.window, (int64_t)0) : 0;
 
-  KvRowScore score;
-  if constexpr (SCORED) score.head(p.score, hh, see_from, see_to);
+  KvRowScore<SCORES> score;
+  if constexpr (kScored) score.head(p.score, hh, see_from, see_to);
 
   f32x16 o[ND];
 #pragma unroll
@@ -714,28 +715,55 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
       constexpr int kAhead = 4;
       u32x4 op[kAhead], pw[kKeys / 16], lost[kExact ? kKeys / 16 : 1], vop[2][kExact ? 1 : ND];
       float add[2] = {0.f, 0.f};
-      // From here on the scores of half u are what they become.
-      auto become = [&](int u) {
-        if constexpr (SCORED) {
-          score.at(p.score, key0 + 32 * u + 4 * h, u ? cl1 : cl0);
-#pragma unroll
-          for (int x = 0; x < 16; ++x) sc[u][x] = score.of(p.score, sc[u][x], 8 * (x >> 2) + (x & 3));
-        }
-      };
-      auto mask = [&](int u) {
-        if (__builtin_expect(whole, 1)) return;
-        // From the lane's first key. (Kept inside the branch: hoisted, the comparisons fill
-        // the scalar registers and every tile selects.)
+      // Bits of half u's keys that the row sees, from the lane's first key.
+      auto seen_of = [&](int u) {
+        // (Kept inside the branch: hoisted, the comparisons fill the scalar registers and
+        // every tile selects.)
         int at = key0 + 32 * u;
         asm volatile("" : "+s"(at));
-        const uint32_t seen = (range_bits(see_from - at, see_to - at) & (uint32_t)(keep >> (32 * u))) >> (4 * h);
+        return (range_bits(see_from - at, see_to - at) & (uint32_t)(keep >> (32 * u))) >> (4 * h);
+      };
+      uint32_t seen[2];  // where not all are (scored)
+      // What the scores become (apart from `sc`, whose 16 registers stay one operand).
+      float z[kScored ? 2 : 1][16];
+      auto logit = [&](int u, int x) { return kScored ? z[u][x] : sc[u][x]; };
+      // Before a half's weights.
+      auto mask = [&](int u) {
+        if constexpr (kScored) {
+          // (What has no side effects is otherwise made where it is used, after the fences: the
+          // operands of all sixteen scores stay in registers, 50 of them.)
+          if constexpr (kExact) asm volatile("" : "+v"(sc[u]));
+          score.at(p.score, key0 + 32 * u + 4 * h, u ? cl1 : cl0);
+        }
+        if (__builtin_expect(whole, 1)) return;
+        const uint32_t bits = seen_of(u);
+        if constexpr (kScored) {
+          seen[u] = bits;
+          return;
+        }
 #pragma unroll
-        for (int x = 0; x < 16; ++x) sc[u][x] = seen >> (8 * (x >> 2) + (x & 3)) & 1 ? sc[u][x] : -INFINITY;
+        for (int x = 0; x < 16; ++x) sc[u][x] = bits >> (8 * (x >> 2) + (x & 3)) & 1 ? sc[u][x] : -INFINITY;
+      };
+      // Scored: two of a half's scores become what they are to be, then are masked.  In order:
+      // `base` goes on to the next two keys.
+      auto become = [&](int u, int i) {
+        if constexpr (kScored) {
+          const float next = score.base + score.slope;
+          z[u][2 * i] = score.of(p.score, sc[u][2 * i], score.base);
+          z[u][2 * i + 1] = score.of(p.score, sc[u][2 * i + 1], next);
+          score.base = fmaf(score.slope, i & 1 ? 6.f : 2.f, score.base);
+          asm volatile("" : "+v"(z[u][2 * i]), "+v"(z[u][2 * i + 1]), "+v"(score.base));
+          if (__builtin_expect(!whole, 0)) {
+            const int x = 8 * (i >> 1) + 2 * (i & 1);
+            z[u][2 * i] = seen[u] >> x & 1 ? z[u][2 * i] : -INFINITY;
+            z[u][2 * i + 1] = seen[u] >> (x + 1) & 1 ? z[u][2 * i + 1] : -INFINITY;
+          }
+        }
       };
       auto weights = [&](int u, float rel, int i) {  // two of a half's
-        const float cl = SCORED ? 1.f : u ? cl1 : cl0;
-        const float w0 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i], cl, rel));
-        const float w1 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * i + 1], cl, rel));
+        const float cl = kScored ? 1.f : u ? cl1 : cl0;
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(logit(u, 2 * i), cl, rel));
+        const float w1 = __builtin_amdgcn_exp2f(fmaf(logit(u, 2 * i + 1), cl, rel));
         const uint32_t w = F16::pack2(w0, w1);
         pw[2 * u + (i >> 2)][i & 3] = w;
         // The sum is of the rounded weights, two at a time.
@@ -749,10 +777,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
       auto settle = [&](int u) {
         const uint64_t redo = __ballot(!(add[u] < kMost));
         if (__builtin_expect(redo != 0, 0)) {
-          const float cl = SCORED ? 1.f : u ? cl1 : cl0;
-          float mine = sc[u][0];
+          const float cl = kScored ? 1.f : u ? cl1 : cl0;
+          float mine = logit(u, 0);
 #pragma unroll
-          for (int x = 1; x < 16; ++x) mine = fmaxf(mine, sc[u][x]);
+          for (int x = 1; x < 16; ++x) mine = fmaxf(mine, logit(u, x));
           mine *= cl;
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
           const float was = ref;
@@ -812,13 +840,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
             for (int x = 0; x < 16; ++x) sc[u][x] = fmaf(run[x], by[x >> 2][x & 3], sc[u][x]);
             fence();
           }
-          become(u);
           mask(u);
           const float rel = (float)(u ? d1 : d0) - ref;
 #pragma unroll
           for (int i = 0; i < kAhead; ++i) op[i] = value_operand(i % ND, 2 * u + i / ND);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) weights(u, rel, i);
+          for (int i = 0; i < 8; ++i) {
+            become(u, i);
+            weights(u, rel, i);
+            if (kScored) fence();
+          }
           settle(u);
           fence();
 #pragma unroll
@@ -848,18 +879,19 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
 #pragma unroll
         for (int j = 0; j < ND; ++j) vop[0][j] = value_operand(j, 0);
         fence();
-        become(0);
         mask(0);
         const float rel0 = (float)d0 - ref;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           score(NS + i);
 #pragma unroll
-          for (int x = i * 8 / NS; x < (i + 1) * 8 / NS; ++x) weights(0, rel0, x);
+          for (int x = i * 8 / NS; x < (i + 1) * 8 / NS; ++x) {
+            become(0, x);
+            weights(0, rel0, x);
+          }
           fence();
         }
         settle(0);
-        become(1);
         mask(1);
         const float rel1 = (float)d1 - ref;
 #pragma unroll
@@ -871,7 +903,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
             o[j] = mma(vop[k & 1][j], pw[k], o[j]);
             if (k < 2) {
 #pragma unroll
-              for (int x = (k * ND + j) * 4 / ND; x < (k * ND + j + 1) * 4 / ND; ++x) weights(1, rel1, x);
+              for (int x = (k * ND + j) * 4 / ND; x < (k * ND + j + 1) * 4 / ND; ++x) {
+                become(1, x);
+                weights(1, rel1, x);
+              }
             }
             fence();
           }
@@ -973,30 +1008,30 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
                 TT::pack2(scaled(o[j][4 * x + 2] * inv, unit), scaled(o[j][4 * x + 3] * inv, unit))};
 }
 
-template <typename TT, int D, int kWaves, int GS, bool SCORED>
+template <typename TT, int D, int kWaves, int GS, Scores SCORES>
 hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
   const size_t lds = (size_t)(kWaves / 2) * 2 * kKeys * (D / 8) * 16;
-  auto kernel = kv_tile_kernel<TT, D, kWaves, GS, SCORED>;
+  auto kernel = kv_tile_kernel<TT, D, kWaves, GS, SCORES>;
   static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (raised != hipSuccess) return raised;
   hipLaunchKernelGGL(kernel, grid, dim3(kWaves * 64), lds, s, p);
   return hipGetLastError();
 }
-template <int D, int kWaves, bool SCORED>
+template <int D, int kWaves, Scores SCORES>
 hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
-  if (p.c.dtype == CPQ_DTYPE_BF16) return launch_tiles<BF16, D, kWaves, 0, SCORED>(s, p, grid);
+  if (p.c.dtype == CPQ_DTYPE_BF16) return launch_tiles<BF16, D, kWaves, 0, SCORES>(s, p, grid);
   switch (p.c.group_size) {
-    case 32: return launch_tiles<F16, D, kWaves, 32, SCORED>(s, p, grid);
-    case 64: return launch_tiles<F16, D, kWaves, 64, SCORED>(s, p, grid);
+    case 32: return launch_tiles<F16, D, kWaves, 32, SCORES>(s, p, grid);
+    case 64: return launch_tiles<F16, D, kWaves, 64, SCORES>(s, p, grid);
     case 128:
-      if constexpr (D >= 128) return launch_tiles<F16, D, kWaves, 128, SCORED>(s, p, grid);
+      if constexpr (D >= 128) return launch_tiles<F16, D, kWaves, 128, SCORES>(s, p, grid);
     default: return hipErrorInvalidValue;
   }
 }
 
 // `decode`: launch_kv_decode or launch_kv_decode_scored.
-template <bool SCORED, typename Decode>
+template <Scores SCORES, typename Decode>
 hipError_t run_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& given,
                          const KvScore& score, unsigned int* bad, Decode decode) {
   // Bounds past what a sequence can have mean no more than that, and would wrap.
@@ -1040,9 +1075,9 @@ hipError_t run_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_
   p.partial = reinterpret_cast<float*>(static_cast<char*>(ex.scratch) + kWideCounterBytes);
   const dim3 grid((uint32_t)(wgs + p.target));
   switch (c.head_dim) {
-    case 64: return launch_tiles<64, 4, SCORED>(ex.stream, p, grid);
-    case 128: return waves == 4 ? launch_tiles<128, 4, SCORED>(ex.stream, p, grid) : launch_tiles<128, 8, SCORED>(ex.stream, p, grid);
-    case 256: return launch_tiles<256, 4, SCORED>(ex.stream, p, grid);
+    case 64: return launch_tiles<64, 4, SCORES>(ex.stream, p, grid);
+    case 128: return waves == 4 ? launch_tiles<128, 4, SCORES>(ex.stream, p, grid) : launch_tiles<128, 8, SCORES>(ex.stream, p, grid);
+    case 256: return launch_tiles<256, 4, SCORES>(ex.stream, p, grid);
     default: return hipErrorInvalidValue;
   }
 }

@@ -216,12 +216,15 @@ __device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, i
   return q;
 }
 
-// What scores become, in units of log2(e) (cpq_kv_attention_scored).  With a cap
+// What scores become, in units of log2(e) (cpq_kv_attention_scored): nothing else, plus a
+// bias, capped and plus a bias.  With a cap
 //   cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)),
 // whose error is one of cap, 2^-23 of it, where s itself is small: caps are limited to
 // kKvMostCap, which leaves a weight off by 2^-12 of itself at most.  Both ends of the
 // exponential's range come out as they should, +-cap.
+enum class Scores { kPlain, kBiased, kCapped };
 constexpr float kKvMostSlope = 0x1p96f;  // times any distance finite
+template <Scores SCORES>
 struct KvRowScore {
   float slope = 0.f;  // times log2(e)
   int anchor = 0;     // distances are from here: of the keys that a row sees the one of the largest bias, so
@@ -236,16 +239,16 @@ struct KvRowScore {
   }
   // For keys from `key` on, products in units of cl (positive, maybe infinite).
   __device__ __forceinline__ void at(const KvScore& k, int key, float cl) {
-    base = fmaf(slope, (float)(key - anchor), k.cap);
-    by = k.cap > 0.f ? fminf(cl * k.per_cap, FLT_MAX) : cl;
+    base = fmaf(slope, (float)(key - anchor), SCORES == Scores::kCapped ? k.cap : 0.f);
+    by = SCORES == Scores::kCapped ? fminf(cl * k.per_cap, FLT_MAX) : cl;
   }
-  // Of the product of key `key` + x.
-  template <typename X>
-  __device__ __forceinline__ float of(const KvScore& k, float product, X x) const {
-    const float plus = fmaf(slope, (float)x, base);
-    if (k.cap > 0.f)
+  // Of a product, `plus` being its key's base: base + slope * (key - `at`'s).  (Callers step
+  // from key to key: with distances as factors their sixteen constants fill registers.)
+  __device__ __forceinline__ float of(const KvScore& k, float product, float plus) const {
+    if constexpr (SCORES == Scores::kCapped)
       return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * by)), -2.f * k.cap, plus);
-    return fmaf(product, by, plus);
+    else
+      return fmaf(product, by, plus);
   }
 };
 // The prefix of sequence s that all its queries see, of n keys.

@@ -1,5 +1,5 @@
 // Attention over the 4-bit key/value cache for few query rows per sequence
-// (kernels/kv_attention.hpp chooses; semantics: cpq_kv_attention and, SCORED,
+// (kernels/kv_attention.hpp chooses; semantics: cpq_kv_attention and, scored,
 // cpq_kv_attention_scored in cpq.h).
 //
 // The query rows of one key/value head (n_q queries times the heads of its
@@ -140,7 +140,7 @@ __device__ __forceinline__ void start_tile(const cpq_kv_cache& c, size_t row_a, 
 }
 
 // A wave's running result, relative to 2^ref per row.
-template <typename TT, int D, int GS, int NC, bool SCORED>
+template <typename TT, int D, int GS, int NC, Scores SCORES>
 struct Rows {
   using X = Geo<D, GS>;
   // At T = f16 a key's and a weight's one rounding to f16 would show in the output: a
@@ -158,7 +158,8 @@ struct Rows {
   int unit[NC];         // of a row's sums o: 2^unit
   KvRange keys, values;  // of the operands
   bool alike = false;   // every row's unit is the values' exponent
-  KvRowScore score[SCORED ? NC : 1];
+  static constexpr bool kScored = SCORES != Scores::kPlain;
+  KvRowScore<SCORES> score[kScored ? NC : 1];
 
   // Chooses the keys of one pass among `left` (bit k: key k of the tile is seen by a
   // row and not yet taken) and sets the exponents to them.
@@ -358,14 +359,19 @@ struct Rows {
     u32x4 pw[NC], lost[NC];
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc) {
-      if constexpr (SCORED) {
+      if constexpr (kScored) {
         score[cc].at(k, t + 4 * h, cl[cc]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < 2; ++u) {
+          float plus = fmaf(score[cc].slope, 16.f * u, score[cc].base);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[u][cc][e] = score[cc].of(k, sc[u][cc][e], 16 * u + e);
+          for (int e = 0; e < 4; ++e) {
+            sc[u][cc][e] = score[cc].of(k, sc[u][cc][e], plus);
+            plus += score[cc].slope;
+          }
+        }
       }
-      const float cl = SCORED ? 1.f : this->cl[cc];
+      const float cl = kScored ? 1.f : this->cl[cc];
       if (!whole) {
         const uint32_t seen = (range_bits(from[cc] - t, to[cc] - t) & taken) >> (4 * h);  // from the lane's first key
 #pragma unroll
@@ -574,7 +580,7 @@ __global__ __launch_bounds__(kStartsThreads) void kv_starts_kernel(DecodeArgs p)
   if (tid == 0) p.starts[n_seqs] = at;
 }
 
-template <typename TT, int D, int GS, int NC, int kWaves, bool SCORED>
+template <typename TT, int D, int GS, int NC, int kWaves, Scores SCORES>
 __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>)) void kv_decode_kernel(DecodeArgs p) {
   using X = Geo<D, GS>;
   extern __shared__ __align__(16) unsigned char lds_bytes[];  // the waves' rings; then the join
@@ -612,8 +618,8 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
   look(t0);
   // Query rows: column n = lane % 16 of tile cc is row r = 16 cc + n, query r / group, head r % group.
   // Their loads, the first tile's blocks and its copies are under way together.
-  Rows<TT, D, GS, NC, SCORED> R;
-  const int prefix = SCORED ? kv_prefix(p.score, it.s, q.n) : 0;
+  Rows<TT, D, GS, NC, SCORES> R;
+  const int prefix = R.kScored ? kv_prefix(p.score, it.s, q.n) : 0;
   int from[NC], to[NC];  // keys that a row sees
 #pragma unroll
   for (int cc = 0; cc < NC; ++cc) {
@@ -625,7 +631,7 @@ __global__ __launch_bounds__(kWaves * 64, (Geo<D, GS>::template kOccupancy<NC>))
     const int pos = q.pos + qi;
     from[cc] = a.window ? (int)max((int64_t)pos + 1 - (int64_t)a.window, (int64_t)0) : 0;
     to[cc] = a.causal ? min(max(pos + 1, prefix), q.n) : q.n;
-    if constexpr (SCORED) R.score[cc].head(p.score, hh, from[cc], to[cc]);
+    if constexpr (R.kScored) R.score[cc].head(p.score, hh, from[cc], to[cc]);
   }
 #pragma unroll
   for (int st = 0; st < kStages - 1; ++st)
@@ -917,13 +923,13 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(DecodeArgs p) {
   *reinterpret_cast<u32x2*>(out) = u32x2{TT::pack2(acc[0], acc[1]), TT::pack2(acc[2], acc[3])};
 }
 
-template <typename TT, int D, int GS, int NC, int kWaves, bool SCORED>
+template <typename TT, int D, int GS, int NC, int kWaves, Scores SCORES>
 hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
   const size_t ring = (size_t)kWaves * Geo<D, GS>::kWave;
   const size_t waves = (size_t)kWaves * p.rows_max * (D + 4 + 2) * sizeof(float);
   const size_t join = ((size_t)p.rows_max * (kMaxParts + 1) + 4 + (size_t)kWaves * 64 * 4) * sizeof(float);
   const size_t lds = std::max(ring, std::max(waves, p.target ? join : 0));
-  auto kernel = kv_decode_kernel<TT, D, GS, NC, kWaves, SCORED>;
+  auto kernel = kv_decode_kernel<TT, D, GS, NC, kWaves, SCORES>;
   if (lds > 60 * 1024) {
     static const hipError_t raised = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                          hipFuncAttributeMaxDynamicSharedMemorySize, 156 * 1024);
@@ -938,22 +944,22 @@ hipError_t launch(hipStream_t s, const DecodeArgs& p, size_t grid) {
   return hipGetLastError();
 }
 
-template <typename TT, int NC, int kWaves, bool SCORED>
+template <typename TT, int NC, int kWaves, Scores SCORES>
 hipError_t launch_d(hipStream_t s, const DecodeArgs& p, size_t grid) {
   switch (p.c.head_dim * 1000 + p.c.group_size) {
-    case 64032: return launch<TT, 64, 32, NC, kWaves, SCORED>(s, p, grid);
-    case 64064: return launch<TT, 64, 64, NC, kWaves, SCORED>(s, p, grid);
-    case 128032: return launch<TT, 128, 32, NC, kWaves, SCORED>(s, p, grid);
-    case 128064: return launch<TT, 128, 64, NC, kWaves, SCORED>(s, p, grid);
-    case 128128: return launch<TT, 128, 128, NC, kWaves, SCORED>(s, p, grid);
-    case 256032: return launch<TT, 256, 32, NC, 4, SCORED>(s, p, grid);
-    case 256064: return launch<TT, 256, 64, NC, kWaves, SCORED>(s, p, grid);
-    case 256128: return launch<TT, 256, 128, NC, kWaves, SCORED>(s, p, grid);
+    case 64032: return launch<TT, 64, 32, NC, kWaves, SCORES>(s, p, grid);
+    case 64064: return launch<TT, 64, 64, NC, kWaves, SCORES>(s, p, grid);
+    case 128032: return launch<TT, 128, 32, NC, kWaves, SCORES>(s, p, grid);
+    case 128064: return launch<TT, 128, 64, NC, kWaves, SCORES>(s, p, grid);
+    case 128128: return launch<TT, 128, 128, NC, kWaves, SCORES>(s, p, grid);
+    case 256032: return launch<TT, 256, 32, NC, 4, SCORES>(s, p, grid);
+    case 256064: return launch<TT, 256, 64, NC, kWaves, SCORES>(s, p, grid);
+    case 256128: return launch<TT, 256, 128, NC, kWaves, SCORES>(s, p, grid);
     default: return hipErrorInvalidValue;
   }
 }
 
-template <bool SCORED>
+template <Scores SCORES>
 hipError_t run_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a, const KvScore& score,
                       int rows_max, bool report, unsigned int* bad) {
   DecodeArgs p{};
@@ -1002,9 +1008,9 @@ hipError_t run_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_att
   p.partial = reinterpret_cast<float*>(rest);
   const size_t grid = pairs + target;
   const bool bf16 = c.dtype == CPQ_DTYPE_BF16;
-  if (p.rows_max > 16) return bf16 ? launch_d<BF16, 2, 4, SCORED>(ex.stream, p, grid) : launch_d<F16, 2, 4, SCORED>(ex.stream, p, grid);
-  if (waves == 8) return bf16 ? launch_d<BF16, 1, 8, SCORED>(ex.stream, p, grid) : launch_d<F16, 1, 8, SCORED>(ex.stream, p, grid);
-  return bf16 ? launch_d<BF16, 1, 4, SCORED>(ex.stream, p, grid) : launch_d<F16, 1, 4, SCORED>(ex.stream, p, grid);
+  if (p.rows_max > 16) return bf16 ? launch_d<BF16, 2, 4, SCORES>(ex.stream, p, grid) : launch_d<F16, 2, 4, SCORES>(ex.stream, p, grid);
+  if (waves == 8) return bf16 ? launch_d<BF16, 1, 8, SCORES>(ex.stream, p, grid) : launch_d<F16, 1, 8, SCORES>(ex.stream, p, grid);
+  return bf16 ? launch_d<BF16, 1, 4, SCORES>(ex.stream, p, grid) : launch_d<F16, 1, 4, SCORES>(ex.stream, p, grid);
 }
 
 }  // namespace

@@ -1,12 +1,12 @@
 // Attention over the 4-bit key/value cache for few query rows per sequence, scores
-// capped or biased, prefixes seen.
+// capped, prefixes seen.
 #include "kv_decode.hpp"
 
 namespace cpq {
 
-hipError_t launch_kv_decode_scored(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+hipError_t launch_kv_decode_capped(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
                                    const KvScore& score, int rows_max, bool report, unsigned int* bad) {
-  return run_decode<true>(ex, c, a, score, rows_max, report, bad);
+  return run_decode<dev::Scores::kCapped>(ex, c, a, score, rows_max, report, bad);
 }
 
 }  // namespace cpq

@@ -288,11 +288,13 @@ cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache
   const float cap = scores->softcap;
   const cpq::KvScore score{cap * 1.44269504088896340736f, cap > 0.f ? 2.f / cap : 0.f, scores->slopes,
                            args->causal ? scores->prefix_lens : nullptr};
-  if (!(score.cap > 0.f) && !score.slopes && !score.prefix_lens)
-    return launched(cpq::launch_kv_attention(cpq::session_ctx(cmds), *cache, *args, cmds->status + 7),
-                    "kv_attention_scored launch");
-  return launched(cpq::launch_kv_attention_scored(cpq::session_ctx(cmds), *cache, *args, score, cmds->status + 7),
-                  "kv_attention_scored launch");
+  const cpq::ExecCtx ex = cpq::session_ctx(cmds);
+  unsigned int* bad = cmds->status + 7;
+  const hipError_t e = score.cap > 0.f ? cpq::launch_kv_attention_capped(ex, *cache, *args, score, bad)
+                       : score.slopes || score.prefix_lens
+                           ? cpq::launch_kv_attention_biased(ex, *cache, *args, score, bad)
+                           : cpq::launch_kv_attention(ex, *cache, *args, bad);
+  return launched(e, "kv_attention_scored launch");
 }
 
 cpq_status cpq_check_kv_append_rotary_args(const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* a) {
