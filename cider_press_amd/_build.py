@@ -37,8 +37,8 @@ SOURCES = [
     "kernels/moe.hip",
     "kernels/stream_read.hip",
     "kv.cpp", "kernels/kv_cache.hip", "kernels/kv_attention.hip", "kernels/kv_decode.hip",
-    "kernels/kv_attention_biased.hip", "kernels/kv_attention_capped.hip",
-    "kernels/kv_decode_biased.hip", "kernels/kv_decode_capped.hip",
+    "kernels/kv_attention_biased.hip", "kernels/kv_attention_capped.hip", "kernels/kv_attention_both.hip",
+    "kernels/kv_decode_biased.hip", "kernels/kv_decode_capped.hip", "kernels/kv_decode_both.hip",
 ]
 
 ARCH = "gfx950"

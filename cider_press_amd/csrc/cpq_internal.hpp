@@ -238,8 +238,8 @@ hipError_t launch_kv_attention(const ExecCtx& ex, const cpq_kv_cache& c, const c
                                unsigned int* bad);
 hipError_t launch_kv_decode(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a, int rows_max,
                             bool report, unsigned int* bad);
-// The same with scores that are capped (cap * log2(e), 2 / cap; 0: not) or fall with
-// distance ([n_heads] or null), and prefixes ([n_seqs] or null).
+// The same with scores that are capped (cap * log2(e), 2 / cap; 0: not), fall with
+// distance ([n_heads] or null) or both, and prefixes ([n_seqs] or null).
 constexpr float kKvMostCap = 1024.f;
 struct KvScore {
   float cap = 0.f;
@@ -248,13 +248,17 @@ struct KvScore {
   const uint32_t* prefix_lens = nullptr;
 };
 hipError_t launch_kv_attention_biased(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                                      const KvScore& score, unsigned int* bad);
+                                   const KvScore& score, unsigned int* bad);
 hipError_t launch_kv_decode_biased(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                                   const KvScore& score, int rows_max, bool report, unsigned int* bad);
+                                const KvScore& score, int rows_max, bool report, unsigned int* bad);
 hipError_t launch_kv_attention_capped(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                                      const KvScore& score, unsigned int* bad);
+                                   const KvScore& score, unsigned int* bad);
 hipError_t launch_kv_decode_capped(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
-                                   const KvScore& score, int rows_max, bool report, unsigned int* bad);
+                                const KvScore& score, int rows_max, bool report, unsigned int* bad);
+hipError_t launch_kv_attention_both(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                   const KvScore& score, unsigned int* bad);
+hipError_t launch_kv_decode_both(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& a,
+                                const KvScore& score, int rows_max, bool report, unsigned int* bad);
 // Y = X . W^T with the kernel chosen by M (small-M kernels, else the prefill
 // plan), as affine_qmm_t and the runtime node run it.
 hipError_t launch_matmul(const ExecCtx& ex, const QuantArgs& q, const void* x, void* y, int m, int n, int k);

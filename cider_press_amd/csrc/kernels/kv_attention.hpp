@@ -514,12 +514,19 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
   // The blocks of this half of 32 tiles, a lane each 16 keys (scalar loads in
   // flight would make every LDS wait a wait for all).
   uint32_t ids = 0;
+  // The first key of the t-th tile of `begin` to `stop`.  With biases, which mostly fall
+  // with distance, the last keys come first: forward the weights of most heads grow from tile
+  // to tile, and with each the reference is raised and weights are made twice (4096 queries
+  // over 8192 keys 667 us; so 483.  Slopes below 0 still have it).
+  auto key_of = [&](int t) { return (biased(SCORES) ? begin + stop - 1 - t : t) * kKeys; };
   auto load = [&](int t) {
     const int lane = (int)opaque((uint32_t)(tid & 63));
-    const int key = t * kKeys + half * 32;
+    const int key = key_of(t) + half * 32;
     const int l = 2 * ((t - begin) / kTeams & 31);
-    if (l == 0)
-      ids = blocks[min((t + kTeams * (lane >> 1)) * kKeys + half * 32 + 16 * (lane & 1), q.n - 1) >> bs_shift];
+    if (l == 0) {
+      const int ahead = key_of(t + kTeams * (lane >> 1)) + half * 32 + 16 * (lane & 1);
+      ids = blocks[min(biased(SCORES) ? max(ahead, 0) : ahead, q.n - 1) >> bs_shift];
+    }
     const KvPlaces pl = kv_places(c, (uint32_t)__builtin_amdgcn_readlane((int)ids, l),
                                   (uint32_t)__builtin_amdgcn_readlane((int)ids, l + 1), min(key, (q.n - 1) & ~15), q.n,
                                   head, bs_shift);
@@ -531,7 +538,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
   auto load_again = [&](int t) {
     asm volatile("" : "+s"(t));  // (addresses made here, not ahead of the branch)
     const int lane = (int)opaque((uint32_t)(tid & 63));
-    const int key = t * kKeys + half * 32;
+    const int key = key_of(t) + half * 32;
     const KvPlaces pl = kv_places(c, blocks[min(key, q.n - 1) >> bs_shift], blocks[min(key + 16, q.n - 1) >> bs_shift],
                                   min(key, (q.n - 1) & ~15), q.n, head, bs_shift);
     if (is_values) load_values<D>(packed, c, pl.a.row, pl.b.row, lane, gw_shift);
@@ -548,7 +555,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
     // instructions, kept through the loop they spill registers.)
     const int lane = (int)opaque((uint32_t)(tid & 63));
     u32x4* keys = units + buf * 2 * kUnits;
-    const int key = t * kKeys + half * 32;
+    const int key = key_of(t) + half * 32;
     const bool all = key >= from && key + 32 <= end && loaded_ok == 3;
     // (Of the keys [from, end) each is seen by one of the rows.)
     if (!all && !is_values && lane == 0 &&
@@ -622,7 +629,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
     alike = __builtin_amdgcn_readfirstlane((int)!__any(unit != ve));
   };
   for (int t = begin; t < stop; ++t) {
-    const int buf = (t - begin) & (kBufs - 1), key0 = t * kKeys;
+    const int buf = (t - begin) & (kBufs - 1), key0 = key_of(t);
     const int news = meta[buf][lane & 3];
     if (__builtin_expect(__any(news != known), 0)) {
       auto word = [&](int i) { return __builtin_amdgcn_readlane(news, i); };
@@ -724,16 +731,21 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
         return (range_bits(see_from - at, see_to - at) & (uint32_t)(keep >> (32 * u))) >> (4 * h);
       };
       uint32_t seen[2];  // where not all are (scored)
-      // What the scores become (apart from `sc`, whose 16 registers stay one operand).
+      // What the scores become (apart from `sc`, whose 16 registers stay one operand).  Caps
+      // bound how far they lie from the reference, which is subtracted on the way then (574
+      // us instead of 580); with biases it would take their last bits where it jumps.
+      constexpr bool kFolded = SCORES == Scores::kCapped;
+      float rel[2];  // what `z` holds besides
       float z[kScored ? 2 : 1][16];
       auto logit = [&](int u, int x) { return kScored ? z[u][x] : sc[u][x]; };
       // Before a half's weights.
       auto mask = [&](int u) {
         if constexpr (kScored) {
+          if constexpr (kFolded) rel[u] = ref == -FLT_MAX ? 0.f : (float)(u ? d1 : d0) - ref;
           // (What has no side effects is otherwise made where it is used, after the fences: the
           // operands of all sixteen scores stay in registers, 50 of them.)
           if constexpr (kExact) asm volatile("" : "+v"(sc[u]));
-          score.at(p.score, key0 + 32 * u + 4 * h, u ? cl1 : cl0);
+          score.at(p.score, key0 + 32 * u + 4 * h, u ? cl1 : cl0, kFolded ? rel[u] : 0.f);
         }
         if (__builtin_expect(whole, 1)) return;
         const uint32_t bits = seen_of(u);
@@ -748,10 +760,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
       // `base` goes on to the next two keys.
       auto become = [&](int u, int i) {
         if constexpr (kScored) {
-          const float next = score.base + score.slope;
+          const float next = score.step(score.base, 1.f);
           z[u][2 * i] = score.of(p.score, sc[u][2 * i], score.base);
           z[u][2 * i + 1] = score.of(p.score, sc[u][2 * i + 1], next);
-          score.base = fmaf(score.slope, i & 1 ? 6.f : 2.f, score.base);
+          score.base = score.step(score.base, i & 1 ? 6.f : 2.f);
           asm volatile("" : "+v"(z[u][2 * i]), "+v"(z[u][2 * i + 1]), "+v"(score.base));
           if (__builtin_expect(!whole, 0)) {
             const int x = 8 * (i >> 1) + 2 * (i & 1);
@@ -761,9 +773,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
         }
       };
       auto weights = [&](int u, float rel, int i) {  // two of a half's
-        const float cl = kScored ? 1.f : u ? cl1 : cl0;
-        const float w0 = __builtin_amdgcn_exp2f(fmaf(logit(u, 2 * i), cl, rel));
-        const float w1 = __builtin_amdgcn_exp2f(fmaf(logit(u, 2 * i + 1), cl, rel));
+        const float cl = u ? cl1 : cl0;
+        const float w0 = __builtin_amdgcn_exp2f(kFolded   ? z[u][2 * i]
+                                                : kScored ? z[u][2 * i] + rel
+                                                          : fmaf(sc[u][2 * i], cl, rel));
+        const float w1 = __builtin_amdgcn_exp2f(kFolded   ? z[u][2 * i + 1]
+                                                : kScored ? z[u][2 * i + 1] + rel
+                                                          : fmaf(sc[u][2 * i + 1], cl, rel));
         const uint32_t w = F16::pack2(w0, w1);
         pw[2 * u + (i >> 2)][i & 3] = w;
         // The sum is of the rounded weights, two at a time.
@@ -775,9 +791,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
       };
       // Where a weight of half u left f16's range: a new reference, the weights again.
       auto settle = [&](int u) {
-        const uint64_t redo = __ballot(!(add[u] < kMost));
+        const uint64_t redo = __ballot(!(add[u] < kMost) || (kFolded && ref == -FLT_MAX));
         if (__builtin_expect(redo != 0, 0)) {
           const float cl = kScored ? 1.f : u ? cl1 : cl0;
+          if constexpr (kFolded) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) z[u][x] -= rel[u];
+          }
           float mine = logit(u, 0);
 #pragma unroll
           for (int x = 1; x < 16; ++x) mine = fmaxf(mine, logit(u, x));
@@ -792,9 +812,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
 #pragma unroll
           for (int j = 0; j < ND; ++j) o[j] *= keep;
           add[u] = 0.f;
-          const float rel = (float)(u ? d1 : d0) - ref;
+          const float to = (float)(u ? d1 : d0) - ref;
+          if constexpr (kFolded) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) weights(u, rel, i);
+            for (int x = 0; x < 16; ++x) z[u][x] += to;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) weights(u, to, i);
         }
         sum += scaled(add[u], u ? -d1 : -d0);
         // (A row whose sums are beyond these values by all that fp32 holds leaves them out.)
@@ -1062,7 +1086,11 @@ hipError_t run_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_
   // leaves compute units without one, workgroups of four, two to a CU (a step of 13
   // requests, 590 and 115 tokens of prompts: 46.6 us, 52.6 with eight; 1024 queries
   // of 48 heads on one key/value head: 75 and 87; 4096 of 32 on 8: 502 and 432).
-  const size_t waves = c.head_dim == 128 && row_tiles(8) >= (size_t)ex.cu_count ? 8 : 4;
+  // (With scores the rows that there are count, not the most row tiles that sequences may
+  // round up to: a step of 13 requests, 850, 690, 270 and 115 tokens of prompts, 78 us, 103
+  // with eight.)
+  const size_t full = SCORES == Scores::kPlain ? row_tiles(8) : a.n_tokens * a.n_heads / 256;
+  const size_t waves = c.head_dim == 128 && full >= (size_t)ex.cu_count ? 8 : 4;
   const size_t wgs = row_tiles(waves);
   // As many parts as workgroups are resident where there are fewer tiles than that,
   // as far as the scratch goes.

@@ -217,12 +217,15 @@ __device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, i
 }
 
 // What scores become, in units of log2(e) (cpq_kv_attention_scored): nothing else, plus a
-// bias, capped and plus a bias.  With a cap
+// bias, capped, both.  (A bias costs an addition a score: 4096 capped queries over 8192 keys
+// 571 us without, 589 with.)  With a cap
 //   cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)),
-// whose error is one of cap, 2^-23 of it, where s itself is small: caps are limited to
-// kKvMostCap, which leaves a weight off by 2^-12 of itself at most.  Both ends of the
+// whose error is one of cap, 2^-22 of it, where s itself is small: caps are limited to
+// kKvMostCap, which leaves a weight off by 2^-11 of itself at most.  Both ends of the
 // exponential's range come out as they should, +-cap.
-enum class Scores { kPlain, kBiased, kCapped };
+enum class Scores { kPlain, kBiased, kCapped, kBoth };
+constexpr bool biased(Scores s) { return s == Scores::kBiased || s == Scores::kBoth; }
+constexpr bool capped(Scores s) { return s == Scores::kCapped || s == Scores::kBoth; }
 constexpr float kKvMostSlope = 0x1p96f;  // times any distance finite
 template <Scores SCORES>
 struct KvRowScore {
@@ -232,20 +235,24 @@ struct KvRowScore {
   float base = 0.f;   // bias, and with a cap the cap, of the key that `at` was given
   float by = 0.f;     // of a score as the product has it: to log2(e), with a cap to the exponential's argument
   __device__ __forceinline__ void head(const KvScore& k, int hh, int from, int to) {
-    if (!k.slopes) return;
+    if (!biased(SCORES) || !k.slopes) return;
     const float s = k.slopes[hh];
     slope = (fabsf(s) > kKvMostSlope ? copysignf(kKvMostSlope, s) : s) * kLog2e;
     anchor = slope < 0.f ? from : to - 1;
   }
-  // For keys from `key` on, products in units of cl (positive, maybe infinite).
-  __device__ __forceinline__ void at(const KvScore& k, int key, float cl) {
-    base = fmaf(slope, (float)(key - anchor), SCORES == Scores::kCapped ? k.cap : 0.f);
-    by = SCORES == Scores::kCapped ? fminf(cl * k.per_cap, FLT_MAX) : cl;
+  // For keys from `key` on, products in units of cl (positive, maybe infinite); `plus`
+  // comes on top.
+  __device__ __forceinline__ void at(const KvScore& k, int key, float cl, float plus = 0.f) {
+    base = capped(SCORES) ? k.cap + plus : plus;
+    if (biased(SCORES)) base = fmaf(slope, (float)(key - anchor), base);
+    by = capped(SCORES) ? fminf(cl * k.per_cap, FLT_MAX) : cl;
   }
+  // From one key's base to that of the key x on.
+  __device__ __forceinline__ float step(float from, float x) const { return biased(SCORES) ? fmaf(slope, x, from) : from; }
   // Of a product, `plus` being its key's base: base + slope * (key - `at`'s).  (Callers step
   // from key to key: with distances as factors their sixteen constants fill registers.)
   __device__ __forceinline__ float of(const KvScore& k, float product, float plus) const {
-    if constexpr (SCORES == Scores::kCapped)
+    if constexpr (capped(SCORES))
       return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(product * by)), -2.f * k.cap, plus);
     else
       return fmaf(product, by, plus);

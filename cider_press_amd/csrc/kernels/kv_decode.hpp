@@ -363,11 +363,11 @@ struct Rows {
         score[cc].at(k, t + 4 * h, cl[cc]);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          float plus = fmaf(score[cc].slope, 16.f * u, score[cc].base);
+          float plus = score[cc].step(score[cc].base, 16.f * u);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             sc[u][cc][e] = score[cc].of(k, sc[u][cc][e], plus);
-            plus += score[cc].slope;
+            plus = score[cc].step(plus, 1.f);
           }
         }
       }

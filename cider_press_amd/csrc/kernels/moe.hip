@@ -20,6 +20,7 @@
 //            fp32, j ascending.
 // All three are tiny next to the expert matmuls (bytes: T*E logits;
 // 16*T*k of indices; (k + 1)*T*N*sizeof(T) for the combine).
+#include <algorithm>
 #include <type_traits>
 
 #include "../cpq_internal.hpp"
@@ -120,8 +121,34 @@ struct SoftmaxRouter {
   }
 };
 
+// Over the wave by DPP: rows of 16 lanes, then from row to row; uniform.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_u32(uint32_t v, F f) {
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// Of 64-bit keys the high words first, then the low words of those that have it.
+__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long key) {
+  auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  const uint32_t high = wave_u32((uint32_t)(key >> 32), larger);
+  const uint32_t low = wave_u32((uint32_t)(key >> 32) == high ? (uint32_t)key : 0u, larger);
+  return (unsigned long long)high << 32 | low;
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+  const unsigned long long b = (unsigned long long)__double_as_longlong(v);
+  return __longlong_as_double((long long)((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), lane) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane)));
+}
+
 // moe_route_grouped, in fp64: a choice is a whole number, which near scores must not
-// change with the order of a sum.
+// change with the order of a sum.  Lane l holds experts NV l .. NV l + NV - 1, so that a
+// group is a run of lanes (where it is not, the wave goes over the groups one by one).  Bound
+// by its instructions, about XXX a wave: 8191 tokens of 256 experts XXX us.
 struct GroupedRouter {
   cpq_moe_router r;
   // Orders like the values, NaN below all of them; 0: no choice.
@@ -132,105 +159,141 @@ struct GroupedRouter {
   static __device__ __forceinline__ double value_of(unsigned long long key) {
     return key == 1ull ? NAN : __longlong_as_double((long long)(key >> 63 ? key & ~(1ull << 63) : ~key));
   }
-  // The largest key of the wave and its lowest expert; the owner's is struck out.
+  // A group's key by its two largest.
+  __device__ __forceinline__ unsigned long long group_key(unsigned long long first, unsigned long long second) const {
+    return r.group_best > 1 ? key_of(value_of(first) + value_of(second)) : first;
+  }
+  // The larger two of two pairs, each in order.
+  static __device__ __forceinline__ void merge(unsigned long long& first, unsigned long long& second,
+                                               unsigned long long a, unsigned long long b) {
+    const unsigned long long low = first < a ? first : a, high = first < a ? b : second;
+    first = first < a ? a : first;
+    second = low > high ? low : high;
+  }
+  // The first of a lane's largest keys.
   template <int NV>
-  static __device__ __forceinline__ unsigned long long take(unsigned long long (&key)[NV], const bool (&among)[NV],
-                                                            int& expert) {
-    unsigned long long best = 0ull;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) best = among[i] && key[i] > best ? key[i] : best;
-    best = __ockl_wfred_max_u64(best);
-    expert = -1;
-#pragma unroll
-    for (int i = NV - 1; i >= 0; --i) {
-      const uint64_t who = __ballot(among[i] && key[i] == best);
-      if (who) expert = 64 * i + __builtin_ctzll(who);
-    }
+  static __device__ __forceinline__ void head_of(const unsigned long long (&key)[NV], unsigned long long& head, int& at) {
+    head = 0ull;
+    at = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (expert == (int)(threadIdx.x & 63) + 64 * i) key[i] = 0ull;
+      if (key[i] > head) {
+        head = key[i];
+        at = i;
+      }
+  }
+  // The wave's largest key, at its lowest expert, which is taken out.
+  template <int NV>
+  static __device__ __forceinline__ unsigned long long take(unsigned long long (&key)[NV], unsigned long long& head,
+                                                            int& at, int& expert) {
+    const unsigned long long best = wave_max_key(head);
+    const int owner = __builtin_ctzll(__ballot(head == best));
+    expert = owner * NV + __builtin_amdgcn_readlane(at, owner);
+    const bool mine = (int)(threadIdx.x & 63) == owner;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) key[i] = mine && at == i ? 0ull : key[i];
+    head_of<NV>(key, head, at);
     return best;
+  }
+  // Keys of groups that are not kept become 0.
+  template <int NV>
+  __device__ __forceinline__ void keep_groups(unsigned long long (&key)[NV], int n_experts) const {
+    const int lane = threadIdx.x & 63, groups = (int)r.n_groups, size = n_experts / groups;
+    if (size % NV == 0) {
+      const int lanes = size / NV, group = lane / lanes, at = lane - group * lanes;
+      unsigned long long first = 0ull, second = 0ull;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) merge(first, second, key[i], 0ull);
+      for (int d = 1; d < lanes; d <<= 1) {  // over lanes at .. at + 2 d - 1 of the group
+        const unsigned long long a = __shfl(first, (lane + d) & 63, 64), b = __shfl(second, (lane + d) & 63, 64);
+        if (at + d < lanes) merge(first, second, a, b);
+      }
+      const unsigned long long of_group = group_key(first, second);  // in its first lane
+      const unsigned long long mine = __shfl(of_group, (lane - at) & 63, 64);
+      int before = 0;
+      for (int g = 0; g < groups; ++g) {
+        const unsigned long long other =
+            (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(of_group >> 32), g * lanes) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)of_group, g * lanes);
+        before += other > mine || (other == mine && g < group);
+      }
+#pragma unroll
+      for (int i = 0; i < NV; ++i) key[i] = before < (int)r.top_groups ? key[i] : 0ull;
+      return;
+    }
+    unsigned long long mine = 0ull;  // of group `lane`
+    for (int g = 0; g < groups; ++g) {
+      unsigned long long part[NV], head;
+      int at, e;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) part[i] = (lane * NV + i) / size == g ? key[i] : 0ull;
+      head_of<NV>(part, head, at);
+      const unsigned long long first = take<NV>(part, head, at, e);
+      const unsigned long long both = group_key(first, wave_max_key(head));
+      mine = lane == g ? both : mine;
+    }
+    int before = 0;  // groups ahead of this lane's
+    for (int g = 0; g < groups; ++g) {
+      const unsigned long long other = __shfl(mine, g, 64);
+      before += other > mine || (other == mine && g < lane);
+    }
+    const uint64_t kept = __ballot(lane < groups && before < (int)r.top_groups);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int group = (lane * NV + i) / size;
+      if (group >= groups || !(kept >> group & 1)) key[i] = 0ull;
+    }
   }
   template <int L, int NV>
   __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
                                         float& score) const {
     const int lane = threadIdx.x & 63;
-    double s[NV];
+    float x[NV];
     unsigned long long key[NV];
-    bool live[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = lane + 64 * i;
-      live[i] = e < n_experts;
-      s[i] = live[i] ? (double)logit_at<L>(logits, row + e) : -INFINITY;
+      const int e = lane * NV + i;
+      x[i] = e < n_experts ? logit_at<L>(logits, row + e) : -INFINITY;
     }
-    if (r.sigmoid) {
+    double most = 0.0, total = 1.0;  // of a softmax
+    if (!r.sigmoid) {
+      float m = x[0];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) s[i] = 1.0 / (1.0 + exp(-s[i]));
-    } else {
-      double m = s[0], sum = 0.0;
+      for (int i = 1; i < NV; ++i) m = fmaxf(m, x[i]);
+      most = (double)__ockl_wfred_max_f32(m);
+      double sum = 0.0;
 #pragma unroll
-      for (int i = 1; i < NV; ++i) m = fmax(m, s[i]);
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) m = fmax(m, __shfl_xor(m, o, 64));
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        s[i] = live[i] ? exp(s[i] - m) : 0.0;
-        sum += s[i];
-      }
+      for (int i = 0; i < NV; ++i) sum += lane * NV + i < n_experts ? exp((double)x[i] - most) : 0.0;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) s[i] /= sum;
+      total = sum;
     }
+    auto score_of = [&](float v) {
+      return r.sigmoid ? 1.0 / (1.0 + exp(-(double)v)) : exp((double)v - most) / total;
+    };
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      key[i] = live[i] ? key_of(r.bias ? s[i] + (double)r.bias[lane + 64 * i] : s[i]) : 0ull;
-    int e;
-    if (r.n_groups > 1 && r.top_groups < r.n_groups) {
-      const int size = n_experts / (int)r.n_groups;
-      int group[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) group[i] = (lane + 64 * i) / size;
-      unsigned long long mine = 0ull;  // of group `lane`
-      for (int g = 0; g < (int)r.n_groups; ++g) {
-        bool in[NV];
-        unsigned long long rest[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          in[i] = live[i] && group[i] == g;
-          rest[i] = key[i];
-        }
-        unsigned long long best = take<NV>(rest, in, e);
-        if (r.group_best > 1) best = key_of(value_of(best) + value_of(take<NV>(rest, in, e)));
-        if (lane == g) mine = best;
-      }
-      int before = 0;  // groups ahead of this lane's
-      for (int g = 0; g < (int)r.n_groups; ++g) {
-        const unsigned long long other = __shfl(mine, g, 64);
-        before += other > mine || (other == mine && g < lane);
-      }
-      const uint64_t kept = __ballot(lane < (int)r.n_groups && before < (int)r.top_groups);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (live[i] && !(kept >> group[i] & 1)) key[i] = 0ull;
+    for (int i = 0; i < NV; ++i) {
+      const int e = lane * NV + i;
+      const double s = score_of(x[i]);
+      key[i] = e < n_experts ? key_of(r.bias ? s + (double)r.bias[e] : s) : 0ull;
     }
-    double mine = 0.0, sum = 0.0;
+    if (r.n_groups > 1 && r.top_groups < r.n_groups) keep_groups<NV>(key, n_experts);
+    unsigned long long head;
+    int at, e;
+    head_of<NV>(key, head, at);
     pick = 0;
     for (int j = 0; j < top_k; ++j) {
-      take<NV>(key, live, e);
-      double all = s[0];
-#pragma unroll
-      for (int i = 1; i < NV; ++i) all = e >> 6 == i ? s[i] : all;
-      all = __shfl(all, e & 63, 64);
-      sum += all;
-      if (lane == j) {
-        mine = all;
-        pick = e;
-      }
+      take<NV>(key, head, at, e);
+      if (lane == j) pick = e;
     }
-    if (r.normalize) mine = sum == 0.0 ? 0.0 : mine / sum;
-    score = (float)(mine * (double)r.scale);
+    // Lane j's pick again, cheaper than every expert's score kept until here.
+    double s = lane < top_k ? score_of(logit_at<L>(logits, row + pick)) : 0.0;
+    if (r.normalize) {
+      double sum = 0.0;
+      for (int j = 0; j < top_k; ++j) sum += lane_f64(s, j);
+      s = sum == 0.0 ? 0.0 : s / sum;
+    }
+    score = (float)(s * (double)r.scale);
   }
 };
 
@@ -345,62 +408,90 @@ __global__ __launch_bounds__(64) void sort_count_kernel(const uint32_t* __restri
   for (int e = threadIdx.x; e < n_experts; e += 64) counts[(size_t)blockIdx.x * n_experts + e] = h[e];
 }
 
-// Thread e turns the histograms into per-(block, expert) start positions
-// (expert-major, block order within an expert) and writes offsets[e];
-// thread E-1 also writes offsets[E].  One block of 1024 threads.
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t* __restrict__ counts, int blocks, int n_experts,
-                                                         uint32_t* __restrict__ offsets) {
-  __shared__ uint32_t tot[kMaxExperts];
-  const int e = threadIdx.x;
-  uint32_t s = 0;
+// Turns the histograms of kScanExperts experts a workgroup into each block's first position
+// within its expert, and writes their totals behind the histograms.  A thread sums a
+// sixteenth of the blocks, 16 neighbouring lanes the experts of one.  (One thread an expert
+// over all blocks, by one workgroup: 65528 rows of 256 experts 26 us; so XXX.)
+constexpr int kScanExperts = 16, kScanSlices = 16;
+__global__ __launch_bounds__(kScanExperts * kScanSlices) void sort_scan_kernel(uint32_t* __restrict__ counts, int blocks,
+                                                                              int n_experts) {
+  __shared__ uint32_t sums[kScanSlices][kScanExperts];
+  const int el = threadIdx.x % kScanExperts, slice = threadIdx.x / kScanExperts;
+  const int e = blockIdx.x * kScanExperts + el;
+  const int per = (blocks + kScanSlices - 1) / kScanSlices, b0 = slice * per, b1 = min(b0 + per, blocks);
+  uint32_t sum = 0;
   if (e < n_experts) {
-#pragma unroll 8
-    for (int b = 0; b < blocks; ++b) s += counts[(size_t)b * n_experts + e];
+#pragma unroll 16
+    for (int b = b0; b < b1; ++b) sum += counts[(size_t)b * n_experts + e];
   }
-  tot[e] = e < n_experts ? s : 0u;
+  sums[slice][el] = sum;
   __syncthreads();
-  // Exclusive prefix over experts (Hillis-Steele in LDS; E <= 1024).
-  for (int d = 1; d < kMaxExperts; d <<= 1) {
-    const uint32_t add = e >= d ? tot[e - d] : 0u;
-    __syncthreads();
-    tot[e] += add;
-    __syncthreads();
+  if (e >= n_experts) return;
+  uint32_t start = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kScanSlices; ++i) {
+    start += i < slice ? sums[i][el] : 0u;
+    total += sums[i][el];
   }
-  if (e < n_experts) {
-    uint32_t start = tot[e] - s;  // exclusive
-    offsets[e] = start;
-#pragma unroll 8
-    for (int b = 0; b < blocks; ++b) {
-      const uint32_t c = counts[(size_t)b * n_experts + e];
-      counts[(size_t)b * n_experts + e] = start;
-      start += c;
-    }
-    if (e == n_experts - 1) offsets[n_experts] = start;
+  if (slice == 0) counts[(size_t)blocks * n_experts + e] = total;
+#pragma unroll 16
+  for (int b = b0; b < b1; ++b) {
+    const uint32_t c = counts[(size_t)b * n_experts + e];
+    counts[(size_t)b * n_experts + e] = start;
+    start += c;
   }
 }
 
 // Four waves per block of kSortRows rows, wave w on rows 64w .. 64w+63 of
 // the block; the last lane of each (wave, expert) run publishes the run's
-// length, and a lane's sorted position is its block's start for the expert, plus
-// the counts of the earlier waves, plus its rank -- so equal experts keep row
-// order.
+// length, and a lane's sorted position is its expert's start (every workgroup sums the
+// experts' totals), plus its block's within the expert, plus the counts of the earlier waves,
+// plus its rank -- so equal experts keep row order.
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows, int top_k,
                                                            int n_experts, const uint32_t* __restrict__ starts,
+                                                           const uint32_t* __restrict__ totals,
                                                            uint32_t* __restrict__ lhs, uint32_t* __restrict__ rhs,
-                                                           uint32_t* __restrict__ inv) {
+                                                           uint32_t* __restrict__ inv, uint32_t* __restrict__ offsets) {
   __shared__ uint32_t cnt[4][kMaxExperts];
-  const int wave = threadIdx.x >> 6;
+  __shared__ uint32_t first[kMaxExperts];
+  __shared__ uint32_t wave_total[4];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int i = threadIdx.x; i < 4 * kMaxExperts; i += 256) (&cnt[0][0])[i] = 0u;
   const int r = blockIdx.x * kSortRows + threadIdx.x;
   const bool live = r < rows;
   const uint32_t e = live ? experts[r] : 0xffffffffu;
+  // Thread t sums experts 4 t .. 4 t + 3.
+  uint32_t t4[4], sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * (int)threadIdx.x + i;
+    t4[i] = at < n_experts ? totals[at] : 0u;
+    sum += t4[i];
+  }
+  uint32_t upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(upto, d, 64);
+    upto += lane >= d ? o : 0u;
+  }
+  if (lane == 63) wave_total[wave] = upto;
   uint32_t rank, same;
   lane_rank(e, rank, same);
-  __syncthreads();  // cnt cleared
+  __syncthreads();  // cnt cleared, waves' totals
+  uint32_t before = upto - sum;
+  for (int w = 0; w < wave; ++w) before += wave_total[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * (int)threadIdx.x + i;
+    first[at] = before;
+    if (blockIdx.x == 0 && at < n_experts) offsets[at] = before;
+    before += t4[i];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 255) offsets[n_experts] = before;
   if (live && rank + 1 == same) cnt[wave][e] = same;
   __syncthreads();
   if (live) {
-    uint32_t pos = starts[(size_t)blockIdx.x * n_experts + e] + rank;
+    uint32_t pos = first[e] + starts[(size_t)blockIdx.x * n_experts + e] + rank;
     for (int w = 0; w < wave; ++w) pos += cnt[w][e];
     lhs[pos] = (uint32_t)(r / top_k);
     rhs[pos] = e;
@@ -448,7 +539,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict
 
 size_t moe_sort_scratch_bytes(int rows, int n_experts) {
   const size_t blocks = (size_t)(rows + kSortRows - 1) / kSortRows;
-  return blocks * (size_t)n_experts * 4;
+  return (blocks + 1) * (size_t)n_experts * 4;  // histograms, totals
 }
 
 // run(L, NV) as types of integral constants: the logits' type and their number a lane.
@@ -520,18 +611,18 @@ hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const 
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,
                            uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   const int blocks = (rows + kSortRows - 1) / kSortRows;
-  if (blocks == 0) {
-    hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, scratch, 0, n_experts, offsets);
-    return hipGetLastError();
+  hipError_t e = hipSuccess;
+  if (blocks) {
+    hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)blocks), dim3(64), 0, s, experts, rows, n_experts, scratch);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)blocks), dim3(64), 0, s, experts, rows, n_experts, scratch);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sort_scan_kernel, dim3(1), dim3(1024), 0, s, scratch, blocks, n_experts, offsets);
+  hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)((n_experts + kScanExperts - 1) / kScanExperts)),
+                     dim3(kScanExperts * kScanSlices), 0, s, scratch, blocks, n_experts);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)blocks), dim3(256), 0, s, experts, rows, top_k, n_experts,
-                     scratch, lhs, rhs, inv);
+  hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows, top_k,
+                     n_experts, scratch, scratch + (size_t)blocks * n_experts, lhs, rhs, inv, offsets);
   return hipGetLastError();
 }
 

@@ -290,9 +290,10 @@ cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache
                            args->causal ? scores->prefix_lens : nullptr};
   const cpq::ExecCtx ex = cpq::session_ctx(cmds);
   unsigned int* bad = cmds->status + 7;
-  const hipError_t e = score.cap > 0.f ? cpq::launch_kv_attention_capped(ex, *cache, *args, score, bad)
-                       : score.slopes || score.prefix_lens
-                           ? cpq::launch_kv_attention_biased(ex, *cache, *args, score, bad)
+  const auto launch = score.cap > 0.f ? score.slopes ? cpq::launch_kv_attention_both : cpq::launch_kv_attention_capped
+                                      : cpq::launch_kv_attention_biased;
+  const hipError_t e = score.cap > 0.f || score.slopes || score.prefix_lens
+                           ? launch(ex, *cache, *args, score, bad)
                            : cpq::launch_kv_attention(ex, *cache, *args, bad);
   return launched(e, "kv_attention_scored launch");
 }

@@ -589,7 +589,7 @@ cpq_status cpq_kv_attention(cpq_commands* cmds, const cpq_kv_cache* cache, const
  *                 device; magnitudes past 2^96 count as 2^96)
  * and, if causal, keys j < prefix_lens[s] are seen from every position too ([n_seqs]; a
  * window hides them as it hides others; past kv_lens[s]: all keys).  softcap up to
- * 1024: a weight is off by 2^-22 * softcap of itself besides.  NULL or 0: not that; with
+ * 1024: a weight is off by 2^-21 * softcap of itself besides.  NULL or 0: not that; with
  * none of them this is cpq_kv_attention.  All else as there. */
 typedef struct cpq_kv_scores {
   float softcap;
