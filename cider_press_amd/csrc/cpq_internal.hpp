@@ -149,7 +149,7 @@ hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void*
 hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens,
                                          int n_experts, int top_k, const cpq_moe_router& r, uint32_t* experts,
                                          float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
-                                         uint32_t* offsets);
+                                         uint32_t* offsets, unsigned int* counter);
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,
                            uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
 hipError_t launch_moe_combine(hipStream_t s, int dtype, const void* y, const float* scores, const uint32_t* inv,

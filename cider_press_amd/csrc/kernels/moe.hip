@@ -132,11 +132,20 @@ __device__ __forceinline__ uint32_t wave_u32(uint32_t v, F f) {
   v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// Of 64-bit keys the high words first, then the low words of those that have it.
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long key) {
+// The largest of 64-bit keys and the lanes that have it: the high words first, the low
+// words where several lanes share that.
+__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long key, uint64_t& who) {
   auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
   const uint32_t high = wave_u32((uint32_t)(key >> 32), larger);
-  const uint32_t low = wave_u32((uint32_t)(key >> 32) == high ? (uint32_t)key : 0u, larger);
+  who = __ballot((uint32_t)(key >> 32) == high);
+  uint32_t low;
+  if ((who & (who - 1)) == 0) {
+    low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, __builtin_ctzll(who));
+  } else {
+    const bool in = who >> (threadIdx.x & 63) & 1;
+    low = wave_u32(in ? (uint32_t)key : 0u, larger);
+    who = __ballot(in && (uint32_t)key == low);
+  }
   return (unsigned long long)high << 32 | low;
 }
 __device__ __forceinline__ double lane_f64(double v, int lane) {
@@ -170,40 +179,86 @@ struct GroupedRouter {
     first = first < a ? a : first;
     second = low > high ? low : high;
   }
-  // The first of a lane's largest keys.
+  // A lane's keys with the places of their experts.  Up to four are in order (descending,
+  // lower places first), so that the next is the first; of more the largest is looked for
+  // (8191 tokens of 256 experts: XXX us, looked for XXX).
   template <int NV>
-  static __device__ __forceinline__ void head_of(const unsigned long long (&key)[NV], unsigned long long& head, int& at) {
-    head = 0ull;
-    at = 0;
+  struct Keys {
+    static constexpr bool kSorted = NV <= 4;
+    unsigned long long key[NV];
+    int place[NV];
+    unsigned long long head;
+    int at;
+    __device__ __forceinline__ void order(int i, int j) {
+      const bool swap = key[i] < key[j] || (key[i] == key[j] && place[i] > place[j]);
+      const unsigned long long k = key[i];
+      const int p = place[i];
+      key[i] = swap ? key[j] : k;
+      place[i] = swap ? place[j] : p;
+      key[j] = swap ? k : key[j];
+      place[j] = swap ? p : place[j];
+    }
+    __device__ __forceinline__ void find() {
+      if constexpr (kSorted) {
+        head = key[0];
+        at = place[0];
+      } else {
+        head = 0ull;
+        at = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (key[i] > head) {
-        head = key[i];
-        at = i;
+        for (int i = 0; i < NV; ++i)
+          if (key[i] > head) {
+            head = key[i];
+            at = i;
+          }
       }
-  }
-  // The wave's largest key, at its lowest expert, which is taken out.
-  template <int NV>
-  static __device__ __forceinline__ unsigned long long take(unsigned long long (&key)[NV], unsigned long long& head,
-                                                            int& at, int& expert) {
-    const unsigned long long best = wave_max_key(head);
-    const int owner = __builtin_ctzll(__ballot(head == best));
-    expert = owner * NV + __builtin_amdgcn_readlane(at, owner);
-    const bool mine = (int)(threadIdx.x & 63) == owner;
+    }
+    // Of keys at their own places.
+    __device__ __forceinline__ void start() {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) key[i] = mine && at == i ? 0ull : key[i];
-    head_of<NV>(key, head, at);
-    return best;
-  }
+      for (int i = 0; i < NV; ++i) place[i] = i;
+      if constexpr (NV == 2) order(0, 1);
+      if constexpr (NV == 4) {
+        order(0, 1);
+        order(2, 3);
+        order(0, 2);
+        order(1, 3);
+        order(1, 2);
+      }
+      find();
+    }
+    // The wave's largest key, at its lowest expert, which is taken out.
+    __device__ __forceinline__ unsigned long long take(int& expert) {
+      uint64_t who;
+      const unsigned long long best = wave_max_key(head, who);
+      const int owner = __builtin_ctzll(who);
+      expert = owner * NV + __builtin_amdgcn_readlane(at, owner);
+      const bool mine = (int)(threadIdx.x & 63) == owner;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if constexpr (kSorted) {
+          key[i] = mine ? i + 1 < NV ? key[(i + 1) % NV] : 0ull : key[i];
+          place[i] = mine && i + 1 < NV ? place[(i + 1) % NV] : place[i];
+        } else {
+          key[i] = mine && at == i ? 0ull : key[i];
+        }
+      }
+      find();
+      return best;
+    }
+  };
   // Keys of groups that are not kept become 0.
   template <int NV>
-  __device__ __forceinline__ void keep_groups(unsigned long long (&key)[NV], int n_experts) const {
+  __device__ __forceinline__ void keep_groups(Keys<NV>& k, int n_experts) const {
     const int lane = threadIdx.x & 63, groups = (int)r.n_groups, size = n_experts / groups;
     if (size % NV == 0) {
       const int lanes = size / NV, group = lane / lanes, at = lane - group * lanes;
-      unsigned long long first = 0ull, second = 0ull;
+      unsigned long long first = k.key[0], second = NV > 1 ? k.key[NV > 1] : 0ull;
+      if constexpr (!Keys<NV>::kSorted) {
+        first = second = 0ull;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) merge(first, second, key[i], 0ull);
+        for (int i = 0; i < NV; ++i) merge(first, second, k.key[i], 0ull);
+      }
       for (int d = 1; d < lanes; d <<= 1) {  // over lanes at .. at + 2 d - 1 of the group
         const unsigned long long a = __shfl(first, (lane + d) & 63, 64), b = __shfl(second, (lane + d) & 63, 64);
         if (at + d < lanes) merge(first, second, a, b);
@@ -218,38 +273,54 @@ struct GroupedRouter {
         before += other > mine || (other == mine && g < group);
       }
 #pragma unroll
-      for (int i = 0; i < NV; ++i) key[i] = before < (int)r.top_groups ? key[i] : 0ull;
-      return;
-    }
-    unsigned long long mine = 0ull;  // of group `lane`
-    for (int g = 0; g < groups; ++g) {
-      unsigned long long part[NV], head;
-      int at, e;
+      for (int i = 0; i < NV; ++i) k.key[i] = before < (int)r.top_groups ? k.key[i] : 0ull;
+    } else {
+      unsigned long long mine = 0ull;  // of group `lane`
+      for (int g = 0; g < groups; ++g) {
+        Keys<NV> part = k;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) part[i] = (lane * NV + i) / size == g ? key[i] : 0ull;
-      head_of<NV>(part, head, at);
-      const unsigned long long first = take<NV>(part, head, at, e);
-      const unsigned long long both = group_key(first, wave_max_key(head));
-      mine = lane == g ? both : mine;
-    }
-    int before = 0;  // groups ahead of this lane's
-    for (int g = 0; g < groups; ++g) {
-      const unsigned long long other = __shfl(mine, g, 64);
-      before += other > mine || (other == mine && g < lane);
-    }
-    const uint64_t kept = __ballot(lane < groups && before < (int)r.top_groups);
+        for (int i = 0; i < NV; ++i) part.key[i] = (lane * NV + k.place[i]) / size == g ? k.key[i] : 0ull;
+        part.start();  // (which place is taken does not matter)
+        int e;
+        uint64_t who;
+        const unsigned long long first = part.take(e);
+        const unsigned long long both = group_key(first, wave_max_key(part.head, who));
+        mine = lane == g ? both : mine;
+      }
+      int before = 0;  // groups ahead of this lane's
+      for (int g = 0; g < groups; ++g) {
+        const unsigned long long other = __shfl(mine, g, 64);
+        before += other > mine || (other == mine && g < lane);
+      }
+      const uint64_t kept = __ballot(lane < groups && before < (int)r.top_groups);
+      bool some = false;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int group = (lane * NV + i) / size;
-      if (group >= groups || !(kept >> group & 1)) key[i] = 0ull;
+      for (int i = 0; i < NV; ++i) {
+        const int group = (lane * NV + k.place[i]) / size;
+        const bool in = group < groups && (kept >> group & 1);
+        k.key[i] = in ? k.key[i] : 0ull;
+        some |= !in;
+      }
+      if constexpr (Keys<NV>::kSorted && NV > 1) {  // in order again
+        if (some) {
+          k.order(0, 1);
+          if constexpr (NV == 4) {
+            k.order(2, 3);
+            k.order(0, 2);
+            k.order(1, 3);
+            k.order(1, 2);
+          }
+        }
+      }
     }
+    k.find();
   }
   template <int L, int NV>
   __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
                                         float& score) const {
     const int lane = threadIdx.x & 63;
     float x[NV];
-    unsigned long long key[NV];
+    Keys<NV> k;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int e = lane * NV + i;
@@ -275,15 +346,14 @@ struct GroupedRouter {
     for (int i = 0; i < NV; ++i) {
       const int e = lane * NV + i;
       const double s = score_of(x[i]);
-      key[i] = e < n_experts ? key_of(r.bias ? s + (double)r.bias[e] : s) : 0ull;
+      k.key[i] = e < n_experts ? key_of(r.bias ? s + (double)r.bias[e] : s) : 0ull;
     }
-    if (r.n_groups > 1 && r.top_groups < r.n_groups) keep_groups<NV>(key, n_experts);
-    unsigned long long head;
-    int at, e;
-    head_of<NV>(key, head, at);
+    k.start();
+    if (r.n_groups > 1 && r.top_groups < r.n_groups) keep_groups<NV>(k, n_experts);
     pick = 0;
     for (int j = 0; j < top_k; ++j) {
-      take<NV>(key, head, at, e);
+      int e;
+      k.take(e);
       if (lane == j) pick = e;
     }
     // Lane j's pick again, cheaper than every expert's score kept until here.
@@ -335,9 +405,9 @@ __device__ __forceinline__ void lane_rank(uint32_t e, uint32_t& rank, uint32_t& 
 // counts of expert e, a scan over the experts gives the starts, and each row's
 // position is its expert's start, the earlier waves' counts and its rank.
 constexpr int kFusedTokens = 32;
-template <int L, int NV, typename Router>
+template <int L, int NV>
 __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict__ logits, int tokens, int n_experts,
-                                                          int top_k, Router router, uint32_t* __restrict__ experts,
+                                                          int top_k, int normalize, uint32_t* __restrict__ experts,
                                                           float* __restrict__ scores, uint32_t* __restrict__ lhs,
                                                           uint32_t* __restrict__ rhs, uint32_t* __restrict__ inv,
                                                           uint32_t* __restrict__ offsets) {
@@ -352,7 +422,7 @@ __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict
   for (int t = wave; t < tokens; t += 16) {
     int pick;
     float score;
-    router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
+    route_token<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, normalize, pick, score);
     if (lane < top_k) {
       const int r = t * top_k + lane;
       pick_of[r] = (uint32_t)pick;
@@ -393,6 +463,98 @@ __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict
     lhs[pos] = (uint32_t)(tid / top_k);
     rhs[pos] = e;
     inv[tid] = pos;
+  }
+}
+
+// The same for the grouped router, whose thousand instructions a token are spread over the
+// chip: four tokens a workgroup, and the last workgroup to arrive sorts (16 tokens of 256
+// experts XXX us, by one workgroup of 16 waves 13.6).  Picks go through to the memory side
+// and come back from it; `counter` is zero between launches.
+template <int L, int NV>
+__global__ __launch_bounds__(256) void route_grouped_sort_kernel(const void* __restrict__ logits, int tokens,
+                                                                 int n_experts, int top_k, GroupedRouter router,
+                                                                 uint32_t* experts, float* __restrict__ scores,
+                                                                 uint32_t* __restrict__ lhs, uint32_t* __restrict__ rhs,
+                                                                 uint32_t* __restrict__ inv,
+                                                                 uint32_t* __restrict__ offsets,
+                                                                 unsigned int* counter) {
+  constexpr int ROWS = kFusedTokens * kMaxTopK, RW = ROWS / 64, RT = ROWS / 256;
+  __shared__ uint32_t start[kMaxExperts];
+  __shared__ uint32_t wave_total[4];
+  __shared__ unsigned int arrived;
+  __shared__ __attribute__((aligned(4))) uint8_t cnt[RW][kMaxExperts];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int rows = tokens * top_k, t = blockIdx.x * 4 + wave;
+  for (int i = tid; i < RW * kMaxExperts / 4; i += 256) reinterpret_cast<uint32_t*>(&cnt[0][0])[i] = 0u;
+  if (t < tokens) {
+    int pick;
+    float score;
+    router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
+    if (lane < top_k) {
+      __hip_atomic_store(experts + t * top_k + lane, (uint32_t)pick, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      scores[t * top_k + lane] = score;
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();  // the workgroup's picks are there, cnt cleared
+  if (gridDim.x > 1) {
+    if (tid == 0) arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != gridDim.x - 1) return;
+    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  // Wave w ranks rows 64 w .. and 64 (w + 4) ..
+  uint32_t e[RT], rank[RT];
+#pragma unroll
+  for (int h = 0; h < RT; ++h) {
+    const int r = 256 * h + tid;
+    e[h] = r < rows ? __hip_atomic_load(experts + r, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0xffffffffu;
+  }
+#pragma unroll
+  for (int h = 0; h < RT; ++h) {
+    if (256 * h + 64 * wave >= rows) break;
+    uint32_t same;
+    lane_rank(e[h], rank[h], same);
+    if (256 * h + tid < rows && rank[h] + 1 == same) cnt[4 * h + wave][e[h]] = (uint8_t)same;
+  }
+  __syncthreads();
+  // Thread t sums experts 4 t .. 4 t + 3.
+  uint32_t t4[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int w = 0; w < RW; ++w) {
+    const uint32_t c = reinterpret_cast<const uint32_t*>(cnt[w])[tid];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t4[i] += c >> (8 * i) & 255u;
+  }
+  const uint32_t sum = t4[0] + t4[1] + t4[2] + t4[3];
+  uint32_t upto = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t o = __shfl_up(upto, d, 64);
+    upto += lane >= d ? o : 0u;
+  }
+  if (lane == 63) wave_total[wave] = upto;
+  __syncthreads();
+  uint32_t before = upto - sum;
+  for (int w = 0; w < wave; ++w) before += wave_total[w];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = 4 * tid + i;
+    start[at] = before;
+    if (at < n_experts) offsets[at] = before;
+    before += t4[i];
+  }
+  if (tid == 255) offsets[n_experts] = (uint32_t)rows;
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < RT; ++h) {
+    const int r = 256 * h + tid;
+    if (r >= rows) break;
+    uint32_t pos = start[e[h]] + rank[h];
+    for (int w = 0; w < 4 * h + wave; ++w) pos += cnt[w][e[h]];
+    lhs[pos] = (uint32_t)(r / top_k);
+    rhs[pos] = e[h];
+    inv[r] = pos;
   }
 }
 
@@ -570,17 +732,6 @@ hipError_t launch_route(hipStream_t s, int logits_dtype, const void* logits, int
   });
 }
 
-template <typename Router>
-hipError_t launch_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
-                             const Router& router, uint32_t* experts, float* scores, uint32_t* lhs, uint32_t* rhs,
-                             uint32_t* inv, uint32_t* offsets) {
-  if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
-  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
-    hipLaunchKernelGGL((route_sort_kernel<decltype(l)::value, decltype(nv)::value, Router>), dim3(1), dim3(1024), 0, s,
-                       logits, tokens, n_experts, top_k, router, experts, scores, lhs, rhs, inv, offsets);
-  });
-}
-
 bool moe_route_sort_fits(int tokens) { return tokens >= 1 && tokens <= kFusedTokens; }
 
 hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
@@ -591,8 +742,11 @@ hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits,
 hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
                                  int top_k, int normalize, uint32_t* experts, float* scores, uint32_t* lhs,
                                  uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
-  return launch_route_sort(s, logits_dtype, logits, tokens, n_experts, top_k, SoftmaxRouter{normalize}, experts, scores,
-                           lhs, rhs, inv, offsets);
+  if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
+  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    hipLaunchKernelGGL((route_sort_kernel<decltype(l)::value, decltype(nv)::value>), dim3(1), dim3(1024), 0, s, logits,
+                       tokens, n_experts, top_k, normalize, experts, scores, lhs, rhs, inv, offsets);
+  });
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
@@ -602,10 +756,14 @@ hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void*
 
 hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens,
                                          int n_experts, int top_k, const cpq_moe_router& r, uint32_t* experts,
-                                         float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
-                                         uint32_t* offsets) {
-  return launch_route_sort(s, logits_dtype, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts, scores, lhs,
-                           rhs, inv, offsets);
+                                         float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets,
+                                         unsigned int* counter) {
+  if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
+  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    hipLaunchKernelGGL((route_grouped_sort_kernel<decltype(l)::value, decltype(nv)::value>),
+                       dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, logits, tokens, n_experts, top_k,
+                       GroupedRouter{r}, experts, scores, lhs, rhs, inv, offsets, counter);
+  });
 }
 
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,

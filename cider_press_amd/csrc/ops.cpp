@@ -923,7 +923,8 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
   if (cpq::moe_route_sort_fits((int)tokens))
     return cpq::launched(cpq::launch_moe_route_grouped_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,
                                                             (int)n_experts, (int)top_k, *router, experts, scores, lhs,
-                                                            rhs, inv, offsets),
+                                                            rhs, inv, offsets,
+                                                            static_cast<unsigned int*>(cmds->scratch)),
                          "moe_route_grouped launch");
   st = cpq::launched(cpq::launch_moe_route_grouped(cmds->stream, (int)logits_dtype, logits, (int)tokens,
                                                    (int)n_experts, (int)top_k, *router, experts, scores),
