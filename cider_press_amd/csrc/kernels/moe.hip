@@ -111,16 +111,6 @@ __device__ __forceinline__ void route_token(const void* logits, size_t row, int 
   score = normalize ? my_p / psum : my_p;
 }
 
-// The kinds of routers: a token by one wave, lane j < top_k returns pick j and its score.
-struct SoftmaxRouter {
-  int normalize;
-  template <int L, int NV>
-  __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
-                                        float& score) const {
-    route_token<L, NV>(logits, row, n_experts, top_k, normalize, pick, score);
-  }
-};
-
 // Over the wave by DPP: rows of 16 lanes, then from row to row; uniform.
 template <typename F>
 __device__ __forceinline__ uint32_t wave_u32(uint32_t v, F f) {
@@ -157,7 +147,8 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
 // moe_route_grouped, in fp64: a choice is a whole number, which near scores must not
 // change with the order of a sum.  Lane l holds experts NV l .. NV l + NV - 1, so that a
 // group is a run of lanes (where it is not, the wave goes over the groups one by one).  Bound
-// by its instructions, about XXX a wave: 8191 tokens of 256 experts XXX us.
+// by its instructions, a quarter of them five exponentials, half the picks: 8191 tokens of
+// 256 experts 17 us of the 26 that the call takes, the chip's vector pipes busy for 75 %.
 struct GroupedRouter {
   cpq_moe_router r;
   // Orders like the values, NaN below all of them; 0: no choice.
@@ -180,8 +171,8 @@ struct GroupedRouter {
     second = low > high ? low : high;
   }
   // A lane's keys with the places of their experts.  Up to four are in order (descending,
-  // lower places first), so that the next is the first; of more the largest is looked for
-  // (8191 tokens of 256 experts: XXX us, looked for XXX).
+  // lower places first), so that the next is the first (8191 tokens of 256 experts: 27.4 us,
+  // looked for each time 29.4); of more the largest is looked for, ordering them takes longer.
   template <int NV>
   struct Keys {
     static constexpr bool kSorted = NV <= 4;
@@ -368,20 +359,54 @@ struct GroupedRouter {
 };
 
 // One wave per token.
-template <int L, int NV, typename Router>
+template <int L, int NV>
 __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ logits, int tokens, int n_experts,
-                                                    int top_k, Router router, uint32_t* __restrict__ experts,
+                                                    int top_k, int normalize, uint32_t* __restrict__ experts,
                                                     float* __restrict__ scores) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= tokens) return;  // whole waves leave together
   int pick;
   float score;
-  router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
+  route_token<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, normalize, pick, score);
   if (lane < top_k) {
     experts[(size_t)t * top_k + lane] = (uint32_t)pick;
     scores[(size_t)t * top_k + lane] = score;
   }
+}
+
+// The grouped router, a token to a wave, with the histogram of the workgroup's tokens, which
+// the sort starts from (a launch less: 8191 tokens of 256 experts 26.0 us instead of 27.4).
+// Workgroups of 16 tokens leave CUs idle, those of four make four times the histograms and the
+// sort's workgroups (1500 tokens of 160 experts: 18.5 us, 21.6 with four; 200 tokens of 256:
+// 16.0 and 14.9).
+constexpr int kFewBlocks = 64;
+constexpr int most_tokens(int nv) { return nv > 8 ? 8 : 16; }  // by the registers of a wave
+inline int grouped_tokens(int tokens, int n_experts) {
+  int per = 4;
+  while (per < most_tokens((n_experts + 63) / 64) && tokens > kFewBlocks * per) per *= 2;
+  return per;
+}
+template <int L, int NV>
+__global__ __launch_bounds__(most_tokens(NV) * 64) void route_grouped_kernel(
+    const void* __restrict__ logits, int tokens, int n_experts, int top_k, GroupedRouter router,
+    uint32_t* __restrict__ experts, float* __restrict__ scores, uint32_t* __restrict__ counts) {
+  __shared__ uint32_t h[kMaxExperts];
+  const int lane = threadIdx.x & 63, t = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 6);
+  for (int e = threadIdx.x; e < n_experts; e += blockDim.x) h[e] = 0u;
+  __syncthreads();
+  if (t < tokens) {
+    int pick;
+    float score;
+    router.template route<L, NV>(logits, (size_t)t * n_experts, n_experts, top_k, pick, score);
+    if (lane < top_k) {
+      experts[(size_t)t * top_k + lane] = (uint32_t)pick;
+      scores[(size_t)t * top_k + lane] = score;
+      atomicAdd(&h[pick], 1u);
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_experts; e += blockDim.x) counts[(size_t)blockIdx.x * n_experts + e] = h[e];
 }
 
 // Rank of a lane among the earlier lanes of its wave with the same value, and
@@ -468,7 +493,7 @@ __global__ __launch_bounds__(1024) void route_sort_kernel(const void* __restrict
 
 // The same for the grouped router, whose thousand instructions a token are spread over the
 // chip: four tokens a workgroup, and the last workgroup to arrive sorts (16 tokens of 256
-// experts XXX us, by one workgroup of 16 waves 13.6).  Picks go through to the memory side
+// experts 9.6 us, by one workgroup of 16 waves 13.6).  Picks go through to the memory side
 // and come back from it; `counter` is zero between launches.
 template <int L, int NV>
 __global__ __launch_bounds__(256) void route_grouped_sort_kernel(const void* __restrict__ logits, int tokens,
@@ -573,7 +598,7 @@ __global__ __launch_bounds__(64) void sort_count_kernel(const uint32_t* __restri
 // Turns the histograms of kScanExperts experts a workgroup into each block's first position
 // within its expert, and writes their totals behind the histograms.  A thread sums a
 // sixteenth of the blocks, 16 neighbouring lanes the experts of one.  (One thread an expert
-// over all blocks, by one workgroup: 65528 rows of 256 experts 26 us; so XXX.)
+// over all blocks, by one workgroup: 65528 rows of 256 experts 26 us; so 4.)
 constexpr int kScanExperts = 16, kScanSlices = 16;
 __global__ __launch_bounds__(kScanExperts * kScanSlices) void sort_scan_kernel(uint32_t* __restrict__ counts, int blocks,
                                                                               int n_experts) {
@@ -604,13 +629,13 @@ __global__ __launch_bounds__(kScanExperts * kScanSlices) void sort_scan_kernel(u
   }
 }
 
-// Four waves per block of kSortRows rows, wave w on rows 64w .. 64w+63 of
+// Four waves per block of up to kSortRows rows, wave w on rows 64w .. 64w+63 of
 // the block; the last lane of each (wave, expert) run publishes the run's
 // length, and a lane's sorted position is its expert's start (every workgroup sums the
 // experts' totals), plus its block's within the expert, plus the counts of the earlier waves,
 // plus its rank -- so equal experts keep row order.
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows, int top_k,
-                                                           int n_experts, const uint32_t* __restrict__ starts,
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows,
+                                                           int block_rows, int top_k, int n_experts, const uint32_t* __restrict__ starts,
                                                            const uint32_t* __restrict__ totals,
                                                            uint32_t* __restrict__ lhs, uint32_t* __restrict__ rhs,
                                                            uint32_t* __restrict__ inv, uint32_t* __restrict__ offsets) {
@@ -619,8 +644,8 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
   __shared__ uint32_t wave_total[4];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int i = threadIdx.x; i < 4 * kMaxExperts; i += 256) (&cnt[0][0])[i] = 0u;
-  const int r = blockIdx.x * kSortRows + threadIdx.x;
-  const bool live = r < rows;
+  const int r = blockIdx.x * block_rows + threadIdx.x;
+  const bool live = (int)threadIdx.x < block_rows && r < rows;
   const uint32_t e = live ? experts[r] : 0xffffffffu;
   // Thread t sums experts 4 t .. 4 t + 3.
   uint32_t t4[4], sum = 0;
@@ -721,22 +746,15 @@ hipError_t with_logits(int logits_dtype, int n_experts, F run) {
   return typed(std::integral_constant<int, 2>{});
 }
 
-template <typename Router>
-hipError_t launch_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
-                        const Router& router, uint32_t* experts, float* scores) {
-  if (tokens == 0) return hipSuccess;
-  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
-    hipLaunchKernelGGL((route_kernel<decltype(l)::value, decltype(nv)::value, Router>),
-                       dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, logits, tokens, n_experts, top_k, router,
-                       experts, scores);
-  });
-}
-
 bool moe_route_sort_fits(int tokens) { return tokens >= 1 && tokens <= kFusedTokens; }
 
 hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
                             int normalize, uint32_t* experts, float* scores) {
-  return launch_route(s, logits_dtype, logits, tokens, n_experts, top_k, SoftmaxRouter{normalize}, experts, scores);
+  if (tokens == 0) return hipSuccess;
+  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    hipLaunchKernelGGL((route_kernel<decltype(l)::value, decltype(nv)::value>), dim3((unsigned)((tokens + 3) / 4)),
+                       dim3(256), 0, s, logits, tokens, n_experts, top_k, normalize, experts, scores);
+  });
 }
 
 hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
@@ -749,9 +767,39 @@ hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* lo
   });
 }
 
+// From the histograms of blocks of block_rows rows to the sorted rows.
+static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, int block_rows, int blocks, int top_k,
+                              int n_experts, uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv,
+                              uint32_t* offsets) {
+  hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)((n_experts + kScanExperts - 1) / kScanExperts)),
+                     dim3(kScanExperts * kScanSlices), 0, s, scratch, blocks, n_experts);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows,
+                     block_rows, top_k, n_experts, scratch, scratch + (size_t)blocks * n_experts, lhs, rhs, inv,
+                     offsets);
+  return hipGetLastError();
+}
+
+size_t moe_grouped_scratch_bytes(int tokens, int n_experts) {
+  const size_t per = (size_t)grouped_tokens(tokens, n_experts);
+  return ((tokens + per - 1) / per + 1) * (size_t)n_experts * 4;
+}
+
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
-                                    int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores) {
-  return launch_route(s, logits_dtype, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts, scores);
+                                    int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores,
+                                    uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
+  const int per = grouped_tokens(tokens, n_experts), blocks = (tokens + per - 1) / per;
+  if (blocks) {
+    const hipError_t e = with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+      constexpr int NV = decltype(nv)::value;
+      hipLaunchKernelGGL((route_grouped_kernel<decltype(l)::value, NV>), dim3((unsigned)blocks),
+                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts,
+                         scores, scratch);
+    });
+    if (e != hipSuccess) return e;
+  }
+  return sort_blocks(s, experts, tokens * top_k, per * top_k, blocks, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
 }
 
 hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const void* logits, int tokens,
@@ -769,19 +817,12 @@ hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const 
 hipError_t launch_moe_sort(hipStream_t s, const uint32_t* experts, int rows, int top_k, int n_experts,
                            uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   const int blocks = (rows + kSortRows - 1) / kSortRows;
-  hipError_t e = hipSuccess;
   if (blocks) {
     hipLaunchKernelGGL(sort_count_kernel, dim3((unsigned)blocks), dim3(64), 0, s, experts, rows, n_experts, scratch);
-    e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)((n_experts + kScanExperts - 1) / kScanExperts)),
-                     dim3(kScanExperts * kScanSlices), 0, s, scratch, blocks, n_experts);
-  e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows, top_k,
-                     n_experts, scratch, scratch + (size_t)blocks * n_experts, lhs, rhs, inv, offsets);
-  return hipGetLastError();
+  return sort_blocks(s, experts, rows, kSortRows, blocks, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
 }
 
 hipError_t launch_moe_combine(hipStream_t s, int dtype, const void* y, const float* scores, const uint32_t* inv,

@@ -100,14 +100,14 @@ cpq_status check_route_sizes(const char* op, cpq_dtype logits_dtype, size_t toke
     return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": tokens*top_k beyond 32-bit indexing");
   return CPQ_OK;
 }
-cpq_status check_route_buffers(const char* op, const cpq_commands* cmds, size_t tokens, size_t rows, size_t n_experts,
+cpq_status check_route_buffers(const char* op, const cpq_commands* cmds, size_t tokens, size_t sort_bytes,
                                const void* logits, const void* experts, const void* scores, const void* lhs,
                                const void* rhs, const void* inv, const void* offsets, uint32_t** hist) {
   if (!offsets) return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": NULL offsets");
   if (tokens && (!logits || !experts || !scores || !lhs || !rhs || !inv))
     return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": NULL buffer");
   void* scratch = nullptr;
-  const size_t need = kWideCounterBytes + moe_sort_scratch_bytes((int)rows, (int)n_experts);
+  const size_t need = kWideCounterBytes + sort_bytes;
   if (!session_scratch(cmds, need, &scratch))
     return fail(CPQ_ERR_BUFFER_TOO_LARGE, std::string(op) + ": the sort needs " + std::to_string(need) +
                                               " bytes of session scratch; the session holds " +
@@ -869,8 +869,8 @@ cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void*
   cpq_status st = cpq::check_route_sizes(op, logits_dtype, tokens, n_experts, top_k, &rows);
   if (st != CPQ_OK) return st;
   uint32_t* hist;
-  st = cpq::check_route_buffers(op, cmds, tokens, rows, n_experts, logits, experts, scores, lhs, rhs, inv, offsets,
-                                &hist);
+  st = cpq::check_route_buffers(op, cmds, tokens, cpq::moe_sort_scratch_bytes((int)rows, (int)n_experts), logits,
+                                experts, scores, lhs, rhs, inv, offsets, &hist);
   if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))
     return cpq::launched(cpq::launch_moe_route_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,
@@ -915,10 +915,9 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
   if (!cmds) return fail(CPQ_ERR_INVALID_ARGUMENT, "moe_route_grouped: NULL command session");
   cpq_status st = cpq_check_moe_route_grouped_args(logits_dtype, tokens, n_experts, top_k, router);
   if (st != CPQ_OK) return st;
-  const size_t rows = tokens * top_k;
   uint32_t* hist;
-  st = cpq::check_route_buffers(op, cmds, tokens, rows, n_experts, logits, experts, scores, lhs, rhs, inv, offsets,
-                                &hist);
+  st = cpq::check_route_buffers(op, cmds, tokens, cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts), logits,
+                                experts, scores, lhs, rhs, inv, offsets, &hist);
   if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))
     return cpq::launched(cpq::launch_moe_route_grouped_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,
@@ -926,13 +925,10 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
                                                             rhs, inv, offsets,
                                                             static_cast<unsigned int*>(cmds->scratch)),
                          "moe_route_grouped launch");
-  st = cpq::launched(cpq::launch_moe_route_grouped(cmds->stream, (int)logits_dtype, logits, (int)tokens,
-                                                   (int)n_experts, (int)top_k, *router, experts, scores),
-                     "moe_route_grouped launch");
-  if (st != CPQ_OK) return st;
-  return cpq::launched(cpq::launch_moe_sort(cmds->stream, experts, (int)rows, (int)top_k, (int)n_experts, hist, lhs,
-                                            rhs, inv, offsets),
-                       "moe_route_grouped sort launch");
+  return cpq::launched(cpq::launch_moe_route_grouped(cmds->stream, (int)logits_dtype, logits, (int)tokens,
+                                                     (int)n_experts, (int)top_k, *router, experts, scores, hist, lhs,
+                                                     rhs, inv, offsets),
+                       "moe_route_grouped launch");
 }
 
 cpq_status cpq_moe_combine(cpq_commands* cmds, cpq_dtype dtype, const void* y, size_t y_len, const float* scores,
