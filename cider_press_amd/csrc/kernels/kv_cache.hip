@@ -304,6 +304,58 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
   append_word<TT>(c, raw, block, off, head, values, wi, w_shift, lanes);
 }
 
+// Cosine and sine of an angle, off by 2^-52.  The angle less the nearest multiple of a
+// quarter turn (in two parts, pi / 2 = kHigh + kLow + 2^-109: up to 2^32 quarters nothing else
+// is lost), then Taylor's series about 0, whose next terms are below 2^-54 at an eighth of
+// a turn.  A third of the library's instructions; it takes what is larger or not finite.
+__device__ __forceinline__ void cos_sin(double angle, double& c, double& s) {
+  constexpr double kQuarters = 0x1.45f306dc9c883p-1;  // 2 / pi
+  constexpr double kWhole = 0x1.8p52;
+  constexpr double kHigh = 0x1.921fb54442d18p+0, kLow = 0x1.1a62633145c07p-54;
+  if (!(fabs(angle) < 0x1p32)) {
+    sincos(angle, &s, &c);
+    return;
+  }
+  const double whole = fma(angle, kQuarters, kWhole), k = whole - kWhole;  // rounded, its low bits at the end
+  const double r = fma(-k, kLow, fma(-k, kHigh, angle)), z = r * r;
+  double p = -1.0 / 1307674368000.0, q = 1.0 / 20922789888000.0;  // -1 / 15!, 1 / 16!
+  p = fma(p, z, 1.0 / 6227020800.0);
+  p = fma(p, z, -1.0 / 39916800.0);
+  p = fma(p, z, 1.0 / 362880.0);
+  p = fma(p, z, -1.0 / 5040.0);
+  p = fma(p, z, 1.0 / 120.0);
+  p = fma(p, z, -1.0 / 6.0);
+  p = fma(p * z, r, r);
+  q = fma(q, z, -1.0 / 87178291200.0);
+  q = fma(q, z, 1.0 / 479001600.0);
+  q = fma(q, z, -1.0 / 3628800.0);
+  q = fma(q, z, 1.0 / 40320.0);
+  q = fma(q, z, -1.0 / 720.0);
+  q = fma(q, z, 1.0 / 24.0);
+  q = fma(q, z, -0.5);
+  q = fma(q, z, 1.0);
+  const uint32_t quarter = (uint32_t)(unsigned long long)__double_as_longlong(whole);
+  const double x = quarter & 1 ? p : q, y = quarter & 1 ? q : p;
+  c = (quarter + 1) & 2 ? -x : x;
+  s = quarter & 2 ? -y : y;
+}
+
+// Eight values rotated: pairs within the word, or with those of `other`.
+template <typename TT, bool PAIRS, int N>
+__device__ __forceinline__ u32x4 turn(u32x4 raw, u32x4 other, const double (&co)[N], const double (&si)[N]) {
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const double x = TT::lo(raw[i]), y = TT::hi(raw[i]);
+    if constexpr (PAIRS)
+      out[i] = TT::pack2((float)fma(x, co[i], -(y * si[i])), (float)fma(y, co[i], x * si[i]));
+    else
+      out[i] = TT::pack2((float)fma(x, co[2 * i], (double)TT::lo(other[i]) * si[2 * i]),
+                         (float)fma(y, co[2 * i + 1], (double)TT::hi(other[i]) * si[2 * i + 1]));
+  }
+  return out;
+}
+
 // Rotation and append.  A workgroup takes 256 / W consecutive tokens (thread = one word of
 // one token, as above) and `rows` of their rows: keys, values, then queries.  The cosines
 // and sines of its tokens are made once, in LDS, and kept in registers over the rows; a
@@ -311,7 +363,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
 // loads it too).  In fp64, whose fma runs at fp32's rate here: which of 16 steps a key's
 // value falls on is a whole number, so that a rotation in fp32 would store other steps than
 // an append of keys that were rotated exactly.
-constexpr uint32_t kRotaryEnough = 2048;  // workgroups
+// Bound by HBM, and by its instructions where it is not: 8191 tokens of 32 + 8 + 8 heads of
+// 128, 178 MB that no cache holds, 45.7 us, 3.9 TB/s (a copy 4.7); with the library's sine and
+// rows addressed one by one 60.  1500 tokens of 16 + 4 + 4 heads of 256 9.3 us.
+// Workgroups that many rows are divided over: with twice as many the cosines are made twice
+// as often (50 us), half leave CUs idle towards the end (51 us).
+constexpr uint32_t kRotaryEnough = 1024;
 template <typename TT, bool PAIRS>
 __global__ __launch_bounds__(256) void kv_append_rotary_kernel(cpq_kv_cache c, cpq_kv_append_rotary_args a, int w_shift,
                                                                int lanes, uint32_t rows, unsigned int* bad) {
@@ -325,8 +382,8 @@ __global__ __launch_bounds__(256) void kv_append_rotary_kernel(cpq_kv_cache c, c
   for (uint32_t e = threadIdx.x; e < half << (8 - w_shift); e += 256) {
     const uint32_t tt = e / half, i = e - tt * half;
     if (t0 + tt >= n_tokens) break;
-    double si, co;
-    sincos((double)a.positions[t0 + tt] * (double)a.frequencies[i], &si, &co);
+    double co, si;
+    cos_sin((double)a.positions[t0 + tt] * (double)a.frequencies[i], co, si);
     turns[(i % kTurns * tokens + tt) * words + i / kTurns] = double2{co * a.magnitude, si * a.magnitude};
   }
   __syncthreads();
@@ -339,7 +396,7 @@ __global__ __launch_bounds__(256) void kv_append_rotary_kernel(cpq_kv_cache c, c
     return;
   }
   const bool turned = wi < a.rotary_dim / 8, second = !PAIRS && wi >= words;
-  const uint32_t partner = !turned || PAIRS ? wi : second ? wi - words : wi + words;
+  const int partner = !turned || PAIRS ? 0 : second ? -(int)words * 8 : (int)words * 8;  // from the own word
   double co[kTurns], si[kTurns];
   if (turned) {
 #pragma unroll
@@ -349,31 +406,40 @@ __global__ __launch_bounds__(256) void kv_append_rotary_kernel(cpq_kv_cache c, c
       si[j] = PAIRS || second ? v.y : -v.y;
     }
   }
-  for (uint32_t r = r0; r < r1; ++r) {
-    const bool key = r < kv_heads, value = !key && r < 2 * kv_heads;
-    const uint32_t head = key ? r : value ? r - kv_heads : r - 2 * kv_heads;
-    const uint16_t* src = static_cast<const uint16_t*>(key ? a.k : value ? a.v : a.q) +
-                          t * (key ? a.k_token_stride : value ? a.v_token_stride : a.q_token_stride) +
-                          head * (key ? a.k_head_stride : value ? a.v_head_stride : a.q_head_stride);
-    u32x4 raw = *reinterpret_cast<const u32x4*>(src + wi * 8);
-    if (!value && turned) {
-      const u32x4 other = *reinterpret_cast<const u32x4*>(src + partner * 8);
+  auto load = [](const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); };
+  uint32_t head = min(r0, kv_heads), end = min(r1, kv_heads);
+  const uint16_t* src = static_cast<const uint16_t*>(a.k) + t * a.k_token_stride + head * a.k_head_stride + wi * 8;
+  for (; head < end; ++head, src += a.k_head_stride) {
+    u32x4 raw = load(src);
+    if (turned) raw = turn<TT, PAIRS>(raw, load(src + partner), co, si);
+    append_word<TT>(c, raw, block, off, head, false, wi, w_shift, lanes);
+  }
+  head = max(r0, kv_heads) - kv_heads;
+  end = max(min(r1, 2 * kv_heads), kv_heads) - kv_heads;
+  src = static_cast<const uint16_t*>(a.v) + t * a.v_token_stride + head * a.v_head_stride + wi * 8;
+  for (; head < end; ++head, src += a.v_head_stride)
+    append_word<TT>(c, load(src), block, off, head, true, wi, w_shift, lanes);
+  // Queries, U rows' loads in flight together (four: no faster).
+  constexpr uint32_t U = 2;
+  head = max(r0, 2 * kv_heads) - 2 * kv_heads;
+  end = max(r1, 2 * kv_heads) - 2 * kv_heads;
+  src = static_cast<const uint16_t*>(a.q) + t * a.q_token_stride + head * a.q_head_stride + wi * 8;
+  uint16_t* dst = static_cast<uint16_t*>(a.q_out) + t * a.q_out_token_stride + head * a.q_out_head_stride + wi * 8;
+  for (; head < end; head += U) {
+    u32x4 raw[U], other[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double x = TT::lo(raw[i]), y = TT::hi(raw[i]);
-        if constexpr (PAIRS) {
-          raw[i] = TT::pack2((float)fma(x, co[i], -(y * si[i])), (float)fma(y, co[i], x * si[i]));
-        } else {
-          raw[i] = TT::pack2((float)fma(x, co[2 * i], (double)TT::lo(other[i]) * si[2 * i]),
-                             (float)fma(y, co[2 * i + 1], (double)TT::hi(other[i]) * si[2 * i + 1]));
-        }
-      }
+    for (uint32_t u = 0; u < U; ++u) {
+      raw[u] = load(src);
+      if (!PAIRS) other[u] = load(src + partner);
+      if (head + u + 1 < end) src += a.q_head_stride;  // (the last one's again)
     }
-    if (r < 2 * kv_heads)
-      append_word<TT>(c, raw, block, off, head, value, wi, w_shift, lanes);
-    else
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.q_out) + t * a.q_out_token_stride +
-                                head * a.q_out_head_stride + wi * 8) = raw;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      if (head + u >= end) break;
+      if (turned) raw[u] = turn<TT, PAIRS>(raw[u], other[u], co, si);
+      *reinterpret_cast<u32x4*>(dst) = raw[u];
+      dst += a.q_out_head_stride;
+    }
   }
 }
 
