@@ -544,7 +544,8 @@ hipError_t launch_kv_append_rotary(hipStream_t s, const cpq_kv_cache& c, const c
   const int w_shift = log2_of(c.head_dim / 8), lanes = (int)c.group_size / 8;
   const uint32_t per = 256u >> w_shift, blocks = ((uint32_t)a.n_tokens + per - 1) / per;
   const uint32_t all = 2 * c.n_kv_heads + (uint32_t)a.n_heads;
-  const uint32_t rows = (uint32_t)std::max<size_t>((size_t)all * blocks / kRotaryEnough, 1);
+  // (At most 65535 workgroups along the rows.)
+  const uint32_t rows = (uint32_t)std::max<size_t>((size_t)all * blocks / kRotaryEnough, (all + 65534) / 65535);
   const dim3 grid(blocks, (all + rows - 1) / rows);
   auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, c, a, w_shift, lanes, rows, bad);

@@ -595,8 +595,8 @@ __global__ __launch_bounds__(64) void sort_count_kernel(const uint32_t* __restri
   for (int e = threadIdx.x; e < n_experts; e += 64) counts[(size_t)blockIdx.x * n_experts + e] = h[e];
 }
 
-// Turns the histograms of kScanExperts experts a workgroup into each block's first position
-// within its expert, and writes their totals behind the histograms.  A thread sums a
+// Turns the histograms of kScanExperts experts a workgroup into where each block's rows end
+// within their expert (the last block's are the totals).  A thread sums a
 // sixteenth of the blocks, 16 neighbouring lanes the experts of one.  (One thread an expert
 // over all blocks, by one workgroup: 65528 rows of 256 experts 26 us; so 4.)
 constexpr int kScanExperts = 16, kScanSlices = 16;
@@ -614,29 +614,30 @@ __global__ __launch_bounds__(kScanExperts * kScanSlices) void sort_scan_kernel(u
   sums[slice][el] = sum;
   __syncthreads();
   if (e >= n_experts) return;
-  uint32_t start = 0, total = 0;
+  uint32_t end = 0;
 #pragma unroll
-  for (int i = 0; i < kScanSlices; ++i) {
-    start += i < slice ? sums[i][el] : 0u;
-    total += sums[i][el];
-  }
-  if (slice == 0) counts[(size_t)blocks * n_experts + e] = total;
-#pragma unroll 16
-  for (int b = b0; b < b1; ++b) {
-    const uint32_t c = counts[(size_t)b * n_experts + e];
-    counts[(size_t)b * n_experts + e] = start;
-    start += c;
+  for (int i = 0; i < kScanSlices; ++i) end += i < slice ? sums[i][el] : 0u;
+  constexpr int U = 16;  // loads in flight, which the stores between them would keep apart
+  for (int b = b0; b < b1; b += U) {
+    uint32_t c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u] = b + u < b1 ? counts[(size_t)(b + u) * n_experts + e] : 0u;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      end += c[u];
+      if (b + u < b1) counts[(size_t)(b + u) * n_experts + e] = end;
+    }
   }
 }
 
 // Four waves per block of up to kSortRows rows, wave w on rows 64w .. 64w+63 of
 // the block; the last lane of each (wave, expert) run publishes the run's
 // length, and a lane's sorted position is its expert's start (every workgroup sums the
-// experts' totals), plus its block's within the expert, plus the counts of the earlier waves,
-// plus its rank -- so equal experts keep row order.
+// experts' totals), plus the end of the block before within the expert, plus the counts of
+// the earlier waves, plus its rank -- so equal experts keep row order.
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows,
-                                                           int block_rows, int top_k, int n_experts, const uint32_t* __restrict__ starts,
-                                                           const uint32_t* __restrict__ totals,
+                                                           int block_rows, int blocks, int top_k, int n_experts,
+                                                           const uint32_t* __restrict__ ends,
                                                            uint32_t* __restrict__ lhs, uint32_t* __restrict__ rhs,
                                                            uint32_t* __restrict__ inv, uint32_t* __restrict__ offsets) {
   __shared__ uint32_t cnt[4][kMaxExperts];
@@ -652,7 +653,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = 4 * (int)threadIdx.x + i;
-    t4[i] = at < n_experts ? totals[at] : 0u;
+    t4[i] = at < n_experts && blocks ? ends[(size_t)(blocks - 1) * n_experts + at] : 0u;
     sum += t4[i];
   }
   uint32_t upto = sum;
@@ -678,7 +679,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
   if (live && rank + 1 == same) cnt[wave][e] = same;
   __syncthreads();
   if (live) {
-    uint32_t pos = first[e] + starts[(size_t)blockIdx.x * n_experts + e] + rank;
+    uint32_t pos = first[e] + (blockIdx.x ? ends[(size_t)(blockIdx.x - 1) * n_experts + e] : 0u) + rank;
     for (int w = 0; w < wave; ++w) pos += cnt[w][e];
     lhs[pos] = (uint32_t)(r / top_k);
     rhs[pos] = e;
@@ -726,7 +727,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const uint16_t* __restrict
 
 size_t moe_sort_scratch_bytes(int rows, int n_experts) {
   const size_t blocks = (size_t)(rows + kSortRows - 1) / kSortRows;
-  return (blocks + 1) * (size_t)n_experts * 4;  // histograms, totals
+  return blocks * (size_t)n_experts * 4;
 }
 
 // run(L, NV) as types of integral constants: the logits' type and their number a lane.
@@ -776,14 +777,13 @@ static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, 
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows,
-                     block_rows, top_k, n_experts, scratch, scratch + (size_t)blocks * n_experts, lhs, rhs, inv,
-                     offsets);
+                     block_rows, blocks, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
   return hipGetLastError();
 }
 
 size_t moe_grouped_scratch_bytes(int tokens, int n_experts) {
   const size_t per = (size_t)grouped_tokens(tokens, n_experts);
-  return ((tokens + per - 1) / per + 1) * (size_t)n_experts * 4;
+  return (tokens + per - 1) / per * (size_t)n_experts * 4;
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,

@@ -90,7 +90,9 @@ def _strides(op: str, dtype: str, strides, b: Buffer, tokens: int, heads: int, d
     token, head = strides if strides is not None else (heads * dim, dim)
     if token < 0 or head < 0:
         raise _lib.InvalidArgument(f"{op}: negative strides")
-    _need(op, dtype, (b, (tokens - 1) * token + (heads - 1) * head + dim if tokens > 0 and heads > 0 else 0))
+    n = (tokens - 1) * token + (heads - 1) * head + dim if tokens > 0 and heads > 0 else 0
+    if b.dtype != dtype or b._len < n:
+        _need(op, dtype, (b, n))
     return token, head
 
 
@@ -142,17 +144,18 @@ def kv_append_rotary(commands: Commands, cache: KvCache, q, k: Buffer, v: Buffer
     (i, i + len(frequencies)) or, interleaved, (2 i, 2 i + 1), by positions[t] *
     frequencies[i], cosines and sines times magnitude.  n_heads = 0 with q and
     q_out None: keys and values only.  Encodes only."""
-    op = "kv_append_rotary"
+    op, dtype, heads, dim = "kv_append_rotary", cache.dtype, cache.n_kv_heads, cache.head_dim
     _need(op, "u32", (slots, tokens), (positions, tokens))
     _need(op, "f32", (frequencies, 0))
-    kt, kh = _strides(op, cache.dtype, k_strides, k, tokens, cache.n_kv_heads, cache.head_dim)
-    vt, vh = _strides(op, cache.dtype, v_strides, v, tokens, cache.n_kv_heads, cache.head_dim)
-    qt = qh = ot = oh = 0
+    kt, kh = _strides(op, dtype, k_strides, k, tokens, heads, dim)
+    vt, vh = _strides(op, dtype, v_strides, v, tokens, heads, dim)
+    q_ptr = out_ptr = qt = qh = ot = oh = 0
     if n_heads:
-        qt, qh = _strides(op, cache.dtype, q_strides, q, tokens, n_heads, cache.head_dim)
-        ot, oh = _strides(op, cache.dtype, q_out_strides, q_out, tokens, n_heads, cache.head_dim)
-    args = _pack(op, _ROTARY_ARGS, _ptr(q) or 0, qt, qh, _ptr(q_out) or 0, ot, oh, n_heads, k.ptr, kt, kh, v.ptr, vt, vh,
-                 slots.ptr, positions.ptr, tokens, frequencies.ptr, 2 * frequencies._len, bool(interleaved), magnitude)
+        qt, qh = _strides(op, dtype, q_strides, q, tokens, n_heads, dim)
+        ot, oh = _strides(op, dtype, q_out_strides, q_out, tokens, n_heads, dim)
+        q_ptr, out_ptr = q.ptr, q_out.ptr
+    args = _pack(op, _ROTARY_ARGS, q_ptr, qt, qh, out_ptr, ot, oh, n_heads, k.ptr, kt, kh, v.ptr, vt, vh, slots.ptr,
+                 positions.ptr, tokens, frequencies.ptr, 2 * frequencies._len, interleaved, magnitude)
     _lib.check(_lib.lib().cpq_kv_append_rotary(commands.handle, cache._ref, args))
 
 

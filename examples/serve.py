@@ -6,9 +6,10 @@ decoder (random weights in 4 bits), requests that arrive, grow and end.
 A step takes any mixture of prompts and single tokens.  On the device, in order:
 blocks of ended requests go back (kv_release), the step's block table, slots and
 lengths follow from the requests' lengths (kv_plan), the embedding and the fused
-projection of the step's tokens (embed_tokens, quantized_matmul), their keys and
-values into the cache (kv_append), attention over it (kv_attention), the output
-projection and the tied head.  The host knows only lengths and token ids.
+projection of the step's tokens (embed_tokens, quantized_matmul), their queries and keys
+rotated by their positions, keys and values into the cache (kv_append_rotary), attention
+over it (kv_attention), the output projection and the tied head.  The host knows only
+lengths and token ids.
 """
 import sys
 
@@ -40,6 +41,7 @@ class Server:
         self.table = self._u32(np.full((seqs, max_blocks), kv.NO_SLOT))
         self.free, self.free_count = self._u32(np.arange(n_blocks)), self._u32([n_blocks])
         self.lens = self._u32(np.zeros(seqs))
+        self.frequencies = device.upload((1e6 ** -(np.arange(0, dim, 2) / dim)).astype(np.float32), "f32")
 
     def _u32(self, a):
         return self.device.upload(np.asarray(a, np.uint32).reshape(-1), "u32")
@@ -58,17 +60,19 @@ class Server:
         kv.kv_plan(cmds, lens, self._u32(new), *shape, self.free, count, starts, lengths, slots, positions, left)
 
         rows = (self.heads + 2 * self.kv_heads) * self.dim
-        x, qkv, a, y, logits = (d.alloc_buffer(n * k, DTYPE) for k in
-                                (self.hidden, rows, self.heads * self.dim, self.hidden, self.vocab))
+        x, qkv, q, a, y, logits = (d.alloc_buffer(n * k, DTYPE) for k in
+                                   (self.hidden, rows, self.heads * self.dim, self.heads * self.dim, self.hidden,
+                                    self.vocab))
         ids = self._u32(np.concatenate([np.asarray(tokens[r]) for r in sorted(tokens)]))
         embed.embed_tokens(cmds, self.library, *self.table_w, ids, x, self.vocab, self.hidden, 64, 4)
         qmm.quantized_matmul(cmds, *self.qkv_w, x, qkv, n, rows, self.hidden, 64, 4)
         # Queries, keys and values are slices of the fused rows.
         k_at, v_at, strides = self.heads * self.dim, (self.heads + self.kv_heads) * self.dim, (rows, self.dim)
-        kv.kv_append(cmds, self.cache, qkv.slice(k_at, len(qkv) - k_at), qkv.slice(v_at, len(qkv) - v_at), slots, n,
-                     k_strides=strides, v_strides=strides)
-        kv.kv_attention(cmds, self.cache, qkv, self.table, self.max_blocks, starts, lengths, a, n, self.heads, self.seqs,
-                        max(new), self.max_blocks * self.block_size, self.dim ** -0.5, q_strides=strides)
+        kv.kv_append_rotary(cmds, self.cache, qkv, qkv.slice(k_at, len(qkv) - k_at), qkv.slice(v_at, len(qkv) - v_at),
+                            slots, positions, self.frequencies, q, n, self.heads, q_strides=strides, k_strides=strides,
+                            v_strides=strides)
+        kv.kv_attention(cmds, self.cache, q, self.table, self.max_blocks, starts, lengths, a, n, self.heads, self.seqs,
+                        max(new), self.max_blocks * self.block_size, self.dim ** -0.5)
         qmm.quantized_matmul(cmds, *self.out_w, a, y, n, self.hidden, self.heads * self.dim, 64, 4)
         qmm.quantized_matmul(cmds, *self.table_w, y, logits, n, self.vocab, self.hidden, 64, 4)
         cmds.commit_and_wait()

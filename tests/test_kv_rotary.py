@@ -160,6 +160,13 @@ def test_many_tokens(device):
 
 
 @pytest.mark.gpu
+def test_many_heads(device):
+    """More rows than a grid's second dimension holds."""
+    s = Step(np.random.default_rng(2), device, "bf16", 64, 64, 16, 1, 65535, 9)
+    s.check(frequencies_of(64))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_positions_and_frequencies(device, interleaved):
     """Positions up to their type's end; angles next to multiples of a quarter turn, of any size; frequencies of 0, below
