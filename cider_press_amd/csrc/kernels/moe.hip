@@ -122,21 +122,16 @@ __device__ __forceinline__ uint32_t wave_u32(uint32_t v, F f) {
   v = f(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-// The largest of 64-bit keys and the lanes that have it: the high words first, the low
-// words where several lanes share that.
-__device__ __forceinline__ unsigned long long wave_max_key(unsigned long long key, uint64_t& who) {
+// The lanes that have the largest of 64-bit keys: of the high words, and of the low words where
+// several lanes share that.
+__device__ __forceinline__ uint64_t wave_max_key(unsigned long long key) {
   auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
   const uint32_t high = wave_u32((uint32_t)(key >> 32), larger);
-  who = __ballot((uint32_t)(key >> 32) == high);
-  uint32_t low;
-  if ((who & (who - 1)) == 0) {
-    low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, __builtin_ctzll(who));
-  } else {
-    const bool in = who >> (threadIdx.x & 63) & 1;
-    low = wave_u32(in ? (uint32_t)key : 0u, larger);
-    who = __ballot(in && (uint32_t)key == low);
-  }
-  return (unsigned long long)high << 32 | low;
+  const uint64_t who = __ballot((uint32_t)(key >> 32) == high);
+  if ((who & (who - 1)) == 0) return who;
+  const bool in = who >> (threadIdx.x & 63) & 1;
+  const uint32_t low = wave_u32(in ? (uint32_t)key : 0u, larger);
+  return __ballot(in && (uint32_t)key == low);
 }
 __device__ __forceinline__ double lane_f64(double v, int lane) {
   const unsigned long long b = (unsigned long long)__double_as_longlong(v);
@@ -145,12 +140,21 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
 }
 
 // moe_route_grouped, in fp64: a choice is a whole number, which near scores must not
-// change with the order of a sum.  Lane l holds experts NV l .. NV l + NV - 1, so that a
-// group is a run of lanes (where it is not, the wave goes over the groups one by one).  Bound
+// change with the order of a sum.  A group has `lanes` neighbouring lanes, each of them
+// `per` neighbouring experts, up to NV, so that what lies before is the lower expert.  Bound
 // by its instructions, a quarter of them five exponentials, half the picks: 8191 tokens of
 // 256 experts 17 us of the 26 that the call takes, the chip's vector pipes busy for 75 %.
 struct GroupedRouter {
   cpq_moe_router r;
+  bool chosen;           // of the groups some are left out
+  int size, lanes, per;  // experts of a group (of all where none is left out), its lanes, experts of a lane
+  GroupedRouter(const cpq_moe_router& router, int n_experts) : r(router) {
+    chosen = r.top_groups < r.n_groups;
+    const int groups = chosen ? (int)r.n_groups : 1;
+    size = n_experts / groups;
+    lanes = 64 / groups;
+    per = (size + lanes - 1) / lanes;  // 33 lanes or more have experts: up to 32
+  }
   // Orders like the values, NaN below all of them; 0: no choice.
   static __device__ __forceinline__ unsigned long long key_of(double v) {
     const unsigned long long b = (unsigned long long)__double_as_longlong(v);
@@ -218,12 +222,10 @@ struct GroupedRouter {
       }
       find();
     }
-    // The wave's largest key, at its lowest expert, which is taken out.
-    __device__ __forceinline__ unsigned long long take(int& expert) {
-      uint64_t who;
-      const unsigned long long best = wave_max_key(head, who);
-      const int owner = __builtin_ctzll(who);
-      expert = owner * NV + __builtin_amdgcn_readlane(at, owner);
+    // The lowest expert of the wave's largest key, which is taken out (`base`: a lane's first).
+    __device__ __forceinline__ int take(int base) {
+      const int owner = __builtin_ctzll(wave_max_key(head));
+      const int expert = __builtin_amdgcn_readlane(base + at, owner);
       const bool mine = (int)(threadIdx.x & 63) == owner;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -235,88 +237,47 @@ struct GroupedRouter {
         }
       }
       find();
-      return best;
+      return expert;
     }
   };
-  // Keys of groups that are not kept become 0.
+  // Keys of groups that are not kept become 0; this lane is the at-th of `group`.
   template <int NV>
-  __device__ __forceinline__ void keep_groups(Keys<NV>& k, int n_experts) const {
-    const int lane = threadIdx.x & 63, groups = (int)r.n_groups, size = n_experts / groups;
-    if (size % NV == 0) {
-      const int lanes = size / NV, group = lane / lanes, at = lane - group * lanes;
-      unsigned long long first = k.key[0], second = NV > 1 ? k.key[NV > 1] : 0ull;
-      if constexpr (!Keys<NV>::kSorted) {
-        first = second = 0ull;
+  __device__ __forceinline__ void keep_groups(Keys<NV>& k, int group, int at) const {
+    const int lane = threadIdx.x & 63;
+    unsigned long long first = k.key[0], second = NV > 1 ? k.key[NV > 1] : 0ull;
+    if constexpr (!Keys<NV>::kSorted) {
+      first = second = 0ull;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) merge(first, second, k.key[i], 0ull);
-      }
-      for (int d = 1; d < lanes; d <<= 1) {  // over lanes at .. at + 2 d - 1 of the group
-        const unsigned long long a = __shfl(first, (lane + d) & 63, 64), b = __shfl(second, (lane + d) & 63, 64);
-        if (at + d < lanes) merge(first, second, a, b);
-      }
-      const unsigned long long of_group = group_key(first, second);  // in its first lane
-      const unsigned long long mine = __shfl(of_group, (lane - at) & 63, 64);
-      int before = 0;
-      for (int g = 0; g < groups; ++g) {
-        const unsigned long long other =
-            (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(of_group >> 32), g * lanes) << 32 |
-            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)of_group, g * lanes);
-        before += other > mine || (other == mine && g < group);
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) k.key[i] = before < (int)r.top_groups ? k.key[i] : 0ull;
-    } else {
-      unsigned long long mine = 0ull;  // of group `lane`
-      for (int g = 0; g < groups; ++g) {
-        Keys<NV> part = k;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) part.key[i] = (lane * NV + k.place[i]) / size == g ? k.key[i] : 0ull;
-        part.start();  // (which place is taken does not matter)
-        int e;
-        uint64_t who;
-        const unsigned long long first = part.take(e);
-        const unsigned long long both = group_key(first, wave_max_key(part.head, who));
-        mine = lane == g ? both : mine;
-      }
-      int before = 0;  // groups ahead of this lane's
-      for (int g = 0; g < groups; ++g) {
-        const unsigned long long other = __shfl(mine, g, 64);
-        before += other > mine || (other == mine && g < lane);
-      }
-      const uint64_t kept = __ballot(lane < groups && before < (int)r.top_groups);
-      bool some = false;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int group = (lane * NV + k.place[i]) / size;
-        const bool in = group < groups && (kept >> group & 1);
-        k.key[i] = in ? k.key[i] : 0ull;
-        some |= !in;
-      }
-      if constexpr (Keys<NV>::kSorted && NV > 1) {  // in order again
-        if (some) {
-          k.order(0, 1);
-          if constexpr (NV == 4) {
-            k.order(2, 3);
-            k.order(0, 2);
-            k.order(1, 3);
-            k.order(1, 2);
-          }
-        }
-      }
+      for (int i = 0; i < NV; ++i) merge(first, second, k.key[i], 0ull);
     }
+    for (int d = 1; d < lanes; d <<= 1) {  // over lanes at .. at + 2 d - 1 of the group
+      const unsigned long long a = __shfl(first, (lane + d) & 63, 64), b = __shfl(second, (lane + d) & 63, 64);
+      if (at + d < lanes) merge(first, second, a, b);
+    }
+    const unsigned long long of_group = group_key(first, second);  // in its first lane
+    const unsigned long long mine = __shfl(of_group, (lane - at) & 63, 64);
+    int before = 0;
+    for (int g = 0; g < (int)r.n_groups; ++g) {
+      const unsigned long long other =
+          (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(of_group >> 32), g * lanes) << 32 |
+          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)of_group, g * lanes);
+      before += other > mine || (other == mine && g < group);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) k.key[i] = before < (int)r.top_groups ? k.key[i] : 0ull;
     k.find();
   }
   template <int L, int NV>
   __device__ __forceinline__ void route(const void* logits, size_t row, int n_experts, int top_k, int& pick,
                                         float& score) const {
     const int lane = threadIdx.x & 63;
+    const int group = lane / lanes, at = lane - group * lanes, first = at * per, base = group * size + first;
+    // Experts that a lane has: none past the groups' lanes.
+    const int own = (group + 1) * size <= n_experts ? min(size - first, per) : 0;
     float x[NV];
     Keys<NV> k;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = lane * NV + i;
-      x[i] = e < n_experts ? logit_at<L>(logits, row + e) : -INFINITY;
-    }
+    for (int i = 0; i < NV; ++i) x[i] = i < own ? logit_at<L>(logits, row + base + i) : -INFINITY;
     double most = 0.0, total = 1.0;  // of a softmax
     if (!r.sigmoid) {
       float m = x[0];
@@ -325,7 +286,7 @@ struct GroupedRouter {
       most = (double)__ockl_wfred_max_f32(m);
       double sum = 0.0;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) sum += lane * NV + i < n_experts ? exp((double)x[i] - most) : 0.0;
+      for (int i = 0; i < NV; ++i) sum += i < own ? exp((double)x[i] - most) : 0.0;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
       total = sum;
@@ -335,16 +296,14 @@ struct GroupedRouter {
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int e = lane * NV + i;
       const double s = score_of(x[i]);
-      k.key[i] = e < n_experts ? key_of(r.bias ? s + (double)r.bias[e] : s) : 0ull;
+      k.key[i] = i < own ? key_of(r.bias ? s + (double)r.bias[base + i] : s) : 0ull;
     }
     k.start();
-    if (r.n_groups > 1 && r.top_groups < r.n_groups) keep_groups<NV>(k, n_experts);
+    if (chosen) keep_groups<NV>(k, group, at);
     pick = 0;
     for (int j = 0; j < top_k; ++j) {
-      int e;
-      k.take(e);
+      const int e = k.take(base);
       if (lane == j) pick = e;
     }
     // Lane j's pick again, cheaper than every expert's score kept until here.
@@ -382,9 +341,9 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
 // 16.0 and 14.9).
 constexpr int kFewBlocks = 64;
 constexpr int most_tokens(int nv) { return nv > 8 ? 8 : 16; }  // by the registers of a wave
-inline int grouped_tokens(int tokens, int n_experts) {
+inline int grouped_tokens(int tokens, int nv) {
   int per = 4;
-  while (per < most_tokens((n_experts + 63) / 64) && tokens > kFewBlocks * per) per *= 2;
+  while (per < most_tokens(nv) && tokens > kFewBlocks * per) per *= 2;
   return per;
 }
 template <int L, int NV>
@@ -730,16 +689,16 @@ size_t moe_sort_scratch_bytes(int rows, int n_experts) {
   return blocks * (size_t)n_experts * 4;
 }
 
-// run(L, NV) as types of integral constants: the logits' type and their number a lane.
-template <typename F>
-hipError_t with_logits(int logits_dtype, int n_experts, F run) {
-  const int nv = (n_experts + 63) / 64;
+// run(L, NV) as types of integral constants: the logits' type and at least nv of them a lane.
+template <int MOST = 16, typename F>
+hipError_t with_logits(int logits_dtype, int nv, F run) {
   auto typed = [&](auto l) {
     if (nv <= 1) run(l, std::integral_constant<int, 1>{});
     else if (nv <= 2) run(l, std::integral_constant<int, 2>{});
     else if (nv <= 4) run(l, std::integral_constant<int, 4>{});
     else if (nv <= 8) run(l, std::integral_constant<int, 8>{});
-    else run(l, std::integral_constant<int, 16>{});
+    else if (MOST == 16 || nv <= 16) run(l, std::integral_constant<int, 16>{});
+    else run(l, std::integral_constant<int, MOST>{});
     return hipGetLastError();
   };
   if (logits_dtype == CPQ_DTYPE_F32) return typed(std::integral_constant<int, 0>{});
@@ -752,7 +711,7 @@ bool moe_route_sort_fits(int tokens) { return tokens >= 1 && tokens <= kFusedTok
 hipError_t launch_moe_route(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts, int top_k,
                             int normalize, uint32_t* experts, float* scores) {
   if (tokens == 0) return hipSuccess;
-  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+  return with_logits(logits_dtype, (n_experts + 63) / 64, [&](auto l, auto nv) {
     hipLaunchKernelGGL((route_kernel<decltype(l)::value, decltype(nv)::value>), dim3((unsigned)((tokens + 3) / 4)),
                        dim3(256), 0, s, logits, tokens, n_experts, top_k, normalize, experts, scores);
   });
@@ -762,7 +721,7 @@ hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* lo
                                  int top_k, int normalize, uint32_t* experts, float* scores, uint32_t* lhs,
                                  uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
-  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+  return with_logits(logits_dtype, (n_experts + 63) / 64, [&](auto l, auto nv) {
     hipLaunchKernelGGL((route_sort_kernel<decltype(l)::value, decltype(nv)::value>), dim3(1), dim3(1024), 0, s, logits,
                        tokens, n_experts, top_k, normalize, experts, scores, lhs, rhs, inv, offsets);
   });
@@ -781,21 +740,21 @@ static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, 
   return hipGetLastError();
 }
 
-size_t moe_grouped_scratch_bytes(int tokens, int n_experts) {
-  const size_t per = (size_t)grouped_tokens(tokens, n_experts);
+size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r) {
+  const size_t per = (size_t)grouped_tokens(tokens, GroupedRouter(r, n_experts).per);
   return (tokens + per - 1) / per * (size_t)n_experts * 4;
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
                                     int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores,
                                     uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
-  const int per = grouped_tokens(tokens, n_experts), blocks = (tokens + per - 1) / per;
+  const GroupedRouter router(r, n_experts);
+  const int per = grouped_tokens(tokens, router.per), blocks = (tokens + per - 1) / per;
   if (blocks) {
-    const hipError_t e = with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+    const hipError_t e = with_logits<32>(logits_dtype, router.per, [&](auto l, auto nv) {
       constexpr int NV = decltype(nv)::value;
       hipLaunchKernelGGL((route_grouped_kernel<decltype(l)::value, NV>), dim3((unsigned)blocks),
-                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, GroupedRouter{r}, experts,
-                         scores, scratch);
+                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, router, experts, scores, scratch);
     });
     if (e != hipSuccess) return e;
   }
@@ -807,10 +766,11 @@ hipError_t launch_moe_route_grouped_sort(hipStream_t s, int logits_dtype, const 
                                          float* scores, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets,
                                          unsigned int* counter) {
   if (!moe_route_sort_fits(tokens)) return hipErrorInvalidValue;
-  return with_logits(logits_dtype, n_experts, [&](auto l, auto nv) {
+  const GroupedRouter router(r, n_experts);
+  return with_logits<32>(logits_dtype, router.per, [&](auto l, auto nv) {
     hipLaunchKernelGGL((route_grouped_sort_kernel<decltype(l)::value, decltype(nv)::value>),
                        dim3((unsigned)((tokens + 3) / 4)), dim3(256), 0, s, logits, tokens, n_experts, top_k,
-                       GroupedRouter{r}, experts, scores, lhs, rhs, inv, offsets, counter);
+                       router, experts, scores, lhs, rhs, inv, offsets, counter);
   });
 }
 

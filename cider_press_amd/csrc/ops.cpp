@@ -916,8 +916,9 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
   cpq_status st = cpq_check_moe_route_grouped_args(logits_dtype, tokens, n_experts, top_k, router);
   if (st != CPQ_OK) return st;
   uint32_t* hist;
-  st = cpq::check_route_buffers(op, cmds, tokens, cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts), logits,
-                                experts, scores, lhs, rhs, inv, offsets, &hist);
+  st = cpq::check_route_buffers(op, cmds, tokens,
+                                cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts, *router), logits, experts,
+                                scores, lhs, rhs, inv, offsets, &hist);
   if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))
     return cpq::launched(cpq::launch_moe_route_grouped_sort(cmds->stream, (int)logits_dtype, logits, (int)tokens,

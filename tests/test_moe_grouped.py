@@ -124,7 +124,8 @@ SHAPES = [  # tokens, experts, k, groups, top_groups, group_best
     (16, 256, 8, 8, 4, 2), (1, 256, 8, 8, 4, 2), (33, 160, 6, 8, 3, 1), (700, 60, 4, 1, 1, 1), (40, 1024, 16, 64, 5, 2),
     (5, 1000, 16, 50, 3, 2), (300, 12, 2, 6, 2, 2), (2100, 64, 8, 4, 4, 2), (31, 4, 4, 1, 1, 2), (1, 1, 1, 1, 1, 1),
     (90, 65, 5, 13, 2, 1), (64, 512, 1, 64, 1, 1), (32, 48, 12, 16, 4, 2), (77, 320, 10, 5, 2, 2), (50, 130, 3, 2, 1, 2),
-    (45, 64, 3, 64, 3, 1),
+    (45, 64, 3, 64, 3, 1), (40, 990, 16, 33, 4, 2), (20, 1000, 7, 10, 3, 2), (100, 320, 13, 16, 8, 2), (37, 208, 9, 16, 5, 1),
+    (60, 1023, 5, 3, 2, 2),
 ]
 
 
