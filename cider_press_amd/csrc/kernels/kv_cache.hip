@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(cpq_kv_cache c, const ui
 // Cosine and sine of an angle, off by 2^-52.  The angle less the nearest multiple of a
 // quarter turn (in two parts, pi / 2 = kHigh + kLow + 2^-109: up to 2^32 quarters nothing else
 // is lost), then Taylor's series about 0, whose next terms are below 2^-54 at an eighth of
-// a turn.  A third of the library's instructions; it takes what is larger or not finite.
+// a turn.  The library's takes what is larger or not finite.
 __device__ __forceinline__ void cos_sin(double angle, double& c, double& s) {
   constexpr double kQuarters = 0x1.45f306dc9c883p-1;  // 2 / pi
   constexpr double kWhole = 0x1.8p52;
