@@ -304,6 +304,8 @@ cpq_status cpq_check_kv_append_rotary_args(const cpq_kv_cache* cache, const cpq_
   if (st != CPQ_OK) return st;
   if (!a) return invalid(op, "NULL arguments");
   if (a->n_tokens > (size_t)INT_MAX) return invalid(op, "n_tokens must fit in i32");
+  // A thread takes eight dimensions, and a grid counts its threads in 32 bits.
+  if (a->n_tokens * (cache->head_dim / 8) > 0xFFFFFF00ull) return invalid(op, "n_tokens * head_dim past 2^35");
   if (a->n_heads > 65535) return invalid(op, "n_heads outside 0..=65535");
   if (a->rotary_dim == 0 || a->rotary_dim % 16 != 0 || a->rotary_dim > cache->head_dim)
     return invalid(op, "rotary_dim (" + std::to_string(a->rotary_dim) + ") must be a multiple of 16 up to head_dim (" +

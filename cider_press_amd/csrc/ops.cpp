@@ -894,6 +894,8 @@ cpq_status cpq_check_moe_route_grouped_args(cpq_dtype logits_dtype, size_t token
   if (st != CPQ_OK) return st;
   auto invalid = [&](const std::string& what) { return fail(CPQ_ERR_INVALID_ARGUMENT, std::string(op) + ": " + what); };
   if (!r) return invalid("NULL router");
+  // A token is a wave, and a grid counts its threads in 32 bits.
+  if (tokens > (1u << 25)) return invalid("tokens=" + std::to_string(tokens) + " past 2^25");
   if (r->n_groups == 0 || r->n_groups > 64 || n_experts % r->n_groups != 0)
     return invalid("n_groups=" + std::to_string(r->n_groups) + " outside 1..=64 or no divisor of n_experts=" +
                    std::to_string(n_experts));

@@ -155,7 +155,7 @@ def kv_append_rotary(commands: Commands, cache: KvCache, q, k: Buffer, v: Buffer
         ot, oh = _strides(op, dtype, q_out_strides, q_out, tokens, n_heads, dim)
         q_ptr, out_ptr = q.ptr, q_out.ptr
     args = _pack(op, _ROTARY_ARGS, q_ptr, qt, qh, out_ptr, ot, oh, n_heads, k.ptr, kt, kh, v.ptr, vt, vh, slots.ptr,
-                 positions.ptr, tokens, frequencies.ptr, 2 * frequencies._len, interleaved, magnitude)
+                 positions.ptr, tokens, frequencies.ptr, 2 * frequencies._len, bool(interleaved), magnitude)
     _lib.check(_lib.lib().cpq_kv_append_rotary(commands.handle, cache._ref, args))
 
 

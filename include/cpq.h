@@ -115,7 +115,9 @@ void cpq_commands_release(cpq_commands* cmds);
 
 /* HIP graph capture of a session's stream: everything encoded between begin
  * and end is recorded (not run) and replayed by cpq_graph_launch.  No op of
- * this library records a memset, so captured graphs replay identically.  No
+ * this library records a memset, so captured graphs replay identically.  A graph
+ * keeps to the scratch of the session that it was captured in: replay it in that
+ * session's stream, or while neither that session nor another of its graphs runs.  No
  * counterpart in the reference (Metal command buffers are re-encoded per
  * call); used for decode loops and for launch-overhead-free timing. */
 typedef struct cpq_graph cpq_graph;
@@ -415,7 +417,7 @@ cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void*
  * are made in fp64 because they are whole numbers: in fp32 near scores would change
  * places with the order of a sum.  Then the sort, as moe_route.  n_experts <= 1024, top_k
  * <= min(16, n_experts / n_groups * top_groups), n_groups <= 64 divides n_experts,
- * group_best <= n_experts / n_groups.  Uses session scratch. */
+ * group_best <= n_experts / n_groups, tokens <= 2^25.  Uses session scratch. */
 typedef struct cpq_moe_router {
   int sigmoid;
   const float* bias;
@@ -612,7 +614,7 @@ cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache
  * cpq_kv_append.
  * q, q_out [n_tokens, n_heads, head_dim], k, v [n_tokens, n_kv_heads, head_dim] at token
  * and head strides in elements (multiples of 8), 16-byte aligned; n_heads = 0: keys and
- * values only.  rotary_dim: a multiple of 16, up to head_dim.  frequencies: f32
+ * values only; n_tokens * head_dim < 2^35.  rotary_dim: a multiple of 16, up to head_dim.  frequencies: f32
  * [rotary_dim / 2], radians a position.  magnitude: finite. */
 typedef struct cpq_kv_append_rotary_args {
   const void* q;

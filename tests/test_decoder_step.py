@@ -13,7 +13,7 @@ from cider_press_amd.kernels import moe as kmoe
 from cider_press_amd.synthetic import from_bits, make_weight, to_bits
 from test_kv_cache import NONE, _rows
 from test_kv_rotary import frequencies_of, rotate
-from test_kv_scores import standard_slopes
+from test_kv_scores import make, standard_slopes
 from test_moe_grouped import route
 
 pytestmark = pytest.mark.gpu
@@ -111,7 +111,7 @@ def test_steps(device, library, oracle):
             assert positions[at:at + m].tolist() == list(range(t - m, t))
             want = attend(q, K, V, np.arange(t - m, t), prefix[r], cap, slopes)
             got = from_bits(got_a[at:at + m], DTYPE).astype(np.float64)
-            # The gathered rows are rounded to T (2^-9 each), which the cache's values are not; scores through a cap of
+            # The gathered rows are rounded to T (2^-8 each), which the cache's values are not; scores through a cap of
             # slope 1 at most.
             for h in range(HEADS):
                 size = (np.abs(q[:, h]) @ np.abs(K[:, h // GROUP]).T * DIM ** -0.5).max(1, keepdims=True)
@@ -128,3 +128,42 @@ def test_steps(device, library, oracle):
         # Each expert's row is rounded to T, on either side from sums in another order (one unit), then the sum is.
         assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -7 * (weight[:, :, None] * np.abs(dense)).sum(1)).all()
         lens, count = kv, left
+
+
+def test_graphs_of_one_session(device):
+    """Graphs that share a session's scratch (arrival counters, histograms, parts of split keys), replayed in turn."""
+    rng = np.random.default_rng(6)
+    cmds = device.commands()
+    few, many, b = _router(device, rng, cmds, 20), _router(device, rng, cmds, 300), make(
+        rng, device, (DTYPE, DIM, GS, BS, KV_HEADS, GROUP), [1, 1], [900, 4000], cap=6.0, slopes=True)
+    want = b.run(cmds=cmds)
+    b.check(want)
+    graphs = []
+    for encode in (few[0], lambda: b.encode(cmds), many[0]):
+        cmds.begin_capture()
+        encode()
+        graphs.append(cmds.end_capture())
+    for _ in range(3):
+        for _, out, _ in (few, many):
+            out.write(np.zeros(len(out), np.uint32))
+        b.keep[5].write(np.zeros(len(b.keep[5]), np.uint16))
+        for graph in graphs + graphs[::-1]:
+            graph.launch(cmds)
+        cmds.wait()
+        for _, out, picks in (few, many):
+            assert np.array_equal(out.to_numpy(), picks)
+        assert np.array_equal(b.keep[5].to_numpy().reshape(want.shape), want)
+        few[0]()
+        cmds.wait()
+        assert np.array_equal(few[1].to_numpy(), few[2])
+
+
+def _router(device, rng, cmds, tokens):
+    """(encode, buffer of experts, what belongs there)"""
+    logits = rng.standard_normal((tokens, EXPERTS)).astype(np.float32)
+    L, rows = device.upload(logits.reshape(-1), "f32"), tokens * TOP_K
+    out = [device.alloc_buffer(rows, t) for t in ("u32", "f32", "u32", "u32", "u32")] + \
+        [device.alloc_buffer(EXPERTS + 1, "u32")]
+    kw = dict(sigmoid=True, n_groups=4, top_groups=2, group_best=2)
+    return (lambda: kmoe.moe_route_grouped(cmds, L, tokens, EXPERTS, TOP_K, True, *out, **kw), out[0],
+            route(logits, TOP_K, **kw)[0].reshape(-1))

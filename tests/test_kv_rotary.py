@@ -63,7 +63,7 @@ def test_refusals():
                 dict(qo=None), dict(k=None), dict(v=None), dict(slots=None), dict(positions=None),
                 dict(frequencies=None), dict(frequencies=4098), dict(positions=4097), dict(slots=4098), dict(q=4104),
                 dict(qo=4104), dict(k=4098), dict(v=4100), dict(qt=513), dict(oh=4), dict(kt=100), dict(vh=1),
-                dict(tokens=2**31), dict(ot=128), dict(oh=64), dict(qo=4096, ot=1024), dict(kt=2**62)):
+                dict(tokens=2**31), dict(tokens=2**28), dict(ot=128), dict(oh=64), dict(qo=4096, ot=1024), dict(kt=2**62)):
         assert run(**bad) == _lib.INVALID_ARGUMENT, bad
     assert _lib.lib().cpq_kv_append_rotary(None, None, None) == _lib.INVALID_ARGUMENT
     # The packed form is the C structure's.

@@ -60,6 +60,10 @@ def standard_slopes(heads):
     return (2.0 ** (-8.0 * np.arange(1, heads + 1) / heads)).astype(np.float32)
 
 
+# What a value is off by, relative, when rounded to 8 or 11 bits: half a unit of the last one.
+ROUNDING = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+
+
 class Scored(Batch):
     """cap, slopes ([heads] or None), prefix ([sequences] or None) on top of a Batch."""
 
@@ -84,6 +88,17 @@ class Scored(Batch):
         self.encode(cmds, causal, window, **kw)
         cmds.commit_and_wait()
         return out.to_numpy().reshape(self.tokens, self.heads, self.dim)
+
+    def check(self, bits, causal=True, window=0, scale=None):
+        """The result is rounded once, from what `bound` says."""
+        want, bound = self.expect(causal, window, scale)
+        got = from_bits(bits, self.dtype).astype(np.float64)
+        assert np.isfinite(got).all()
+        u, err = ROUNDING[self.dtype], np.abs(got - want)
+        assert (err <= u * np.abs(want) + (1 + u) * bound + 1e-7).all(), (err - u * np.abs(want) - bound).max()
+        # A rounding's root mean square is 0.58 of half a step, over a power of two 0.0015 of the values' in bf16 and
+        # 0.0002 in f16; the operands' (2^-12 each) add to that.
+        assert np.linalg.norm(err) <= (2.2e-3 if self.dtype == "bf16" else 9e-4) * np.linalg.norm(want) + 1e-7
 
     def expect(self, causal=True, window=0, scale=None):
         """As Batch's.  A cap's slope is at most 1, so what a score is off by stays that at most; the cap adds 2^-22 of
@@ -348,4 +363,4 @@ def test_distances_past_24_bits(device):
     b.kv_lens, b.q_lens = [tail * bs - 7], [1]
     b.k, b.v = [np.tile(k, (tail, 1, 1))[:-7]], [np.tile(v, (tail, 1, 1))[:-7]]
     want, bound = b.expect()
-    assert (np.abs(got - want) <= 2.0 ** -9 * 1.02 * np.abs(want) + bound + 1e-7).all()
+    assert (np.abs(got - want) <= ROUNDING["bf16"] * np.abs(want) + bound + 1e-7).all()

@@ -100,7 +100,8 @@ def test_refusals():
     for bad in (dict(dtype="u32"), dict(experts=0), dict(experts=1025), dict(k=0), dict(k=17), dict(experts=4, groups=1, top=1, k=5),
                 dict(groups=0), dict(groups=7), dict(groups=65, experts=650), dict(top=0), dict(top=9), dict(best=0),
                 dict(best=3), dict(groups=64, top=64, best=2), dict(k=9, top=1), dict(bias=4098),
-                dict(scale=float("nan")), dict(scale=float("inf")), dict(tokens=2**28, k=8), dict(tokens=2**62)):
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(tokens=2**28, k=8), dict(tokens=2**62),
+                dict(tokens=2**25 + 1, k=1)):
         assert args(**bad) == _lib.INVALID_ARGUMENT, bad
     assert check_args(0, 5, 64, 8, None) == _lib.INVALID_ARGUMENT
     assert _lib.lib().cpq_moe_route_grouped(None, 0, None, 0, 4, 1, None, *[None] * 6) == _lib.INVALID_ARGUMENT
