@@ -1054,7 +1054,7 @@ hipError_t launch_tiles(hipStream_t s, const TileArgs& p, dim3 grid) {
   }
 }
 
-// `decode`: launch_kv_decode or launch_kv_decode_scored.
+// `decode`: launch_kv_decode of the same form.
 template <Scores SCORES, typename Decode>
 hipError_t run_attention(const ExecCtx& ex, const cpq_kv_cache& c, const cpq_kv_attention_args& given,
                          const KvScore& score, unsigned int* bad, Decode decode) {
