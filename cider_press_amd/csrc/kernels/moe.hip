@@ -143,7 +143,7 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {
 // change with the order of a sum.  A group has `lanes` neighbouring lanes, each of them
 // `per` neighbouring experts, up to NV, so that what lies before is the lower expert.  Bound
 // by its instructions, a quarter of them five exponentials, a third the picks: 8191 tokens of
-// 256 experts 15.5 us of the 24.8 that the call takes, the chip's vector pipes busy for 84 %.
+// 256 experts 15.5 us of the 22.7 that the call takes, the chip's vector pipes busy for 84 %.
 struct GroupedRouter {
   cpq_moe_router r;
   bool chosen;           // of the groups some are left out
@@ -294,8 +294,8 @@ struct GroupedRouter {
       most = (double)__ockl_wfred_max_f32(m);
     }
     // Four at a time, own or not: in one block they share their exponentials' constants and
-    // hide each other's latency (8191 tokens of 256 experts 24.8 us, one by one 25.6; 1500 of
-    // 160 16.5 and 17.9).
+    // hide each other's latency (8191 tokens of 256 experts 0.8 us less than one by one, 1500
+    // of 160 1.4).
     constexpr int F = NV < 4 ? NV : 4;
     double v[NV], sum = 0.0;
 #pragma unroll
@@ -366,23 +366,27 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
 
 // The grouped router, a token to a wave, with the histogram of the workgroup's tokens, which
 // the sort starts from (a launch less: 8191 tokens of 256 experts 26.0 us instead of 27.4).
-// Workgroups of 16 tokens leave CUs idle, those of four make four times the histograms and the
-// sort's workgroups (1500 tokens of 160 experts: 18.5 us, 21.6 with four; 200 tokens of 256:
-// 16.0 and 14.9).
-constexpr int kFewBlocks = 64;
+// Small workgroups make more histograms, large ones leave CUs idle: four tokens each while that
+// is one for a CU, then eight, then 16 (256 experts, 1000 tokens 13.4 us, 15.5 with 16 each; 1500
+// 14.0, 15.6 with 16; 4000, in 16s either way, 16.2).
+constexpr int kFewBlocks = 256;
 constexpr int most_tokens(int nv) { return nv > 8 ? 8 : 16; }  // by the registers of a wave
 inline int grouped_tokens(int tokens, int nv) {
   int per = 4;
   while (per < most_tokens(nv) && tokens > kFewBlocks * per) per *= 2;
   return per;
 }
+// A histogram's rows of bytes (a token picks an expert once, so counts are at most 16), where the
+// sort takes them so: whole groups of 16.
+constexpr int byte_row(int n_experts) { return (n_experts + 15) & ~15; }
 template <int L, int NV>
 __global__ __launch_bounds__(most_tokens(NV) * 64) void route_grouped_kernel(
     const void* __restrict__ logits, int tokens, int n_experts, int top_k, GroupedRouter router,
-    uint32_t* __restrict__ experts, float* __restrict__ scores, uint32_t* __restrict__ counts) {
+    uint32_t* __restrict__ experts, float* __restrict__ scores, uint32_t* __restrict__ counts, int bytes) {
   __shared__ uint32_t h[kMaxExperts];
   const int lane = threadIdx.x & 63, t = (int)((blockIdx.x * blockDim.x + threadIdx.x) >> 6);
-  for (int e = threadIdx.x; e < n_experts; e += blockDim.x) h[e] = 0u;
+  const int row = byte_row(n_experts);
+  for (int e = threadIdx.x; e < row; e += blockDim.x) h[e] = 0u;
   __syncthreads();
   if (t < tokens) {
     int pick;
@@ -395,6 +399,11 @@ __global__ __launch_bounds__(most_tokens(NV) * 64) void route_grouped_kernel(
     }
   }
   __syncthreads();
+  if (bytes) {
+    for (int i = threadIdx.x; i < row / 4; i += blockDim.x)
+      counts[(size_t)blockIdx.x * (row / 4) + i] = h[4 * i] | h[4 * i + 1] << 8 | h[4 * i + 2] << 16 | h[4 * i + 3] << 24;
+    return;
+  }
   for (int e = threadIdx.x; e < n_experts; e += blockDim.x) counts[(size_t)blockIdx.x * n_experts + e] = h[e];
 }
 
@@ -619,30 +628,104 @@ __global__ __launch_bounds__(kScanExperts * kScanSlices) void sort_scan_kernel(u
   }
 }
 
+// Histograms of bytes that a workgroup sums itself: of experts 16 c .. 16 c + 15 a thread of
+// column c takes every row of its slice, eight at a time in bytes (8 * 16 < 256), then in pairs
+// of 16 bits, which go into LDS.  Pair 2 j + p of a column holds its experts 4 j + p and
+// 4 j + p + 2.
+struct ByteSums {
+  uint32_t of[kMaxExperts / 2];
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kMaxExperts / 2; i += blockDim.x) of[i] = 0u;
+  }
+  __device__ __forceinline__ uint32_t get(int e, int columns) const {
+    const int k = e & 15;
+    return of[(k >> 2 << 1 | (k & 1)) * columns + (e >> 4)] >> (k & 2 ? 16 : 0) & 0xffffu;
+  }
+  __device__ __forceinline__ void add(const uint32_t (&pairs)[8], int column, int columns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) atomicAdd(&of[i * columns + column], pairs[i]);
+  }
+};
+template <int U>  // loads in flight, summed by eight
+__device__ __forceinline__ void sum_bytes(const u32x4* __restrict__ counts, int column, int columns, int b0, int b1,
+                                          uint32_t (&pairs)[8]) {
+  for (int b = b0; b < b1; b += U) {
+    u32x4 c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      c[u] = b + u < b1 ? counts[(size_t)(b + u) * columns + column] : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int h = 0; h < U; h += 8) {
+#pragma unroll
+      for (int u = 1; u < 8; ++u) c[h] += c[h + u];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pairs[2 * j] += c[h][j] & 0x00ff00ffu;
+        pairs[2 * j + 1] += c[h][j] >> 8 & 0x00ff00ffu;
+      }
+    }
+  }
+}
+// Up to here (and below 65536 tokens) it does, which saves the scan's launch; past it the scan
+// reads less (of 256 experts 8191 tokens 22.7 us, 24.8 with the scan; 16000 38.7 and 44.2; 24000,
+// 375 KB, 59.1 and 59.3; 32000 78.3 and 74.1).
+constexpr size_t kByteSums = 320 * 1024;
+inline bool sums_bytes(int tokens, int blocks, int n_experts) {
+  return tokens < 65536 && (size_t)blocks * byte_row(n_experts) <= kByteSums;
+}
+
 // Four waves per block of up to kSortRows rows, wave w on rows 64w .. 64w+63 of
 // the block; the last lane of each (wave, expert) run publishes the run's
 // length, and a lane's sorted position is its expert's start (every workgroup sums the
 // experts' totals), plus the end of the block before within the expert, plus the counts of
-// the earlier waves, plus its rank -- so equal experts keep row order.
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows,
-                                                           int block_rows, int blocks, int top_k, int n_experts,
-                                                           const uint32_t* __restrict__ ends,
+// the earlier waves, plus its rank -- so equal experts keep row order.  SUMS: `ends` are
+// histograms of bytes yet, `blocks` in all and `per` of a workgroup's rows.
+constexpr int kSumThreads = 512;  // (8191 tokens of 256 experts 22.7 us; 256 threads 23.3, 1024 23.8)
+template <bool SUMS>
+__global__ __launch_bounds__(SUMS ? kSumThreads : 256) void sort_scatter_kernel(const uint32_t* __restrict__ experts, int rows,
+                                                           int block_rows, int blocks, int per, int top_k,
+                                                           int n_experts, const uint32_t* __restrict__ ends,
                                                            uint32_t* __restrict__ lhs, uint32_t* __restrict__ rhs,
                                                            uint32_t* __restrict__ inv, uint32_t* __restrict__ offsets) {
   __shared__ uint32_t cnt[4][kMaxExperts];
   __shared__ uint32_t first[kMaxExperts];
-  __shared__ uint32_t wave_total[4];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int i = threadIdx.x; i < 4 * kMaxExperts; i += 256) (&cnt[0][0])[i] = 0u;
+  constexpr int THREADS = SUMS ? kSumThreads : 256;
+  __shared__ uint32_t wave_total[THREADS / 64];
+  __shared__ ByteSums before_of, after_of;  // this workgroup's rows, and from them on
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, columns = byte_row(n_experts) / 16;
+  for (int i = threadIdx.x; i < 4 * kMaxExperts; i += THREADS) (&cnt[0][0])[i] = 0u;
   const int r = blockIdx.x * block_rows + threadIdx.x;
   const bool live = (int)threadIdx.x < block_rows && r < rows;
   const uint32_t e = live ? experts[r] : 0xffffffffu;
+  if constexpr (SUMS) {
+    before_of.clear();
+    after_of.clear();
+    __syncthreads();
+    const int slices = THREADS / columns, slice = threadIdx.x / columns, column = threadIdx.x - slice * columns;
+    const int n = (blocks + slices - 1) / slices, mine = min((int)blockIdx.x * per, blocks);
+    const int b0 = min(slice * n, blocks), b1 = slice < slices ? min(b0 + n, blocks) : b0;
+    const u32x4* rows_of = reinterpret_cast<const u32x4*>(ends);
+    uint32_t early[8] = {}, late[8] = {};
+    if (n > 8) {
+      sum_bytes<16>(rows_of, column, columns, b0, min(b1, mine), early);
+      sum_bytes<16>(rows_of, column, columns, max(b0, mine), b1, late);
+    } else {
+      sum_bytes<8>(rows_of, column, columns, b0, min(b1, mine), early);
+      sum_bytes<8>(rows_of, column, columns, max(b0, mine), b1, late);
+    }
+    if (b0 < min(b1, mine)) before_of.add(early, column, columns);
+    if (max(b0, mine) < b1) after_of.add(late, column, columns);
+    __syncthreads();
+  }
   // Thread t sums experts 4 t .. 4 t + 3.
   uint32_t t4[4], sum = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = 4 * (int)threadIdx.x + i;
-    t4[i] = at < n_experts && blocks ? ends[(size_t)(blocks - 1) * n_experts + at] : 0u;
+    if constexpr (SUMS)
+      t4[i] = at < n_experts ? before_of.get(at, columns) + after_of.get(at, columns) : 0u;
+    else
+      t4[i] = at < n_experts && blocks ? ends[(size_t)(blocks - 1) * n_experts + at] : 0u;
     sum += t4[i];
   }
   uint32_t upto = sum;
@@ -660,7 +743,7 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int at = 4 * (int)threadIdx.x + i;
-    first[at] = before;
+    if (at < kMaxExperts) first[at] = before;
     if (blockIdx.x == 0 && at < n_experts) offsets[at] = before;
     before += t4[i];
   }
@@ -668,7 +751,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const uint32_t* __res
   if (live && rank + 1 == same) cnt[wave][e] = same;
   __syncthreads();
   if (live) {
-    uint32_t pos = first[e] + (blockIdx.x ? ends[(size_t)(blockIdx.x - 1) * n_experts + e] : 0u) + rank;
+    uint32_t pos = first[e] + rank;
+    if constexpr (SUMS) pos += before_of.get((int)e, columns);
+    else pos += blockIdx.x ? ends[(size_t)(blockIdx.x - 1) * n_experts + e] : 0u;
     for (int w = 0; w < wave; ++w) pos += cnt[w][e];
     lhs[pos] = (uint32_t)(r / top_k);
     rhs[pos] = e;
@@ -765,14 +850,14 @@ static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, 
                      dim3(kScanExperts * kScanSlices), 0, s, scratch, blocks, n_experts);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sort_scatter_kernel, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows,
-                     block_rows, blocks, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
+  hipLaunchKernelGGL(sort_scatter_kernel<false>, dim3((unsigned)std::max(blocks, 1)), dim3(256), 0, s, experts, rows,
+                     block_rows, blocks, 1, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
   return hipGetLastError();
 }
 
 size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r) {
-  const size_t per = (size_t)grouped_tokens(tokens, GroupedRouter(r, n_experts).per);
-  return (tokens + per - 1) / per * (size_t)n_experts * 4;
+  const int per = grouped_tokens(tokens, GroupedRouter(r, n_experts).per), blocks = (tokens + per - 1) / per;
+  return (size_t)blocks * (sums_bytes(tokens, blocks, n_experts) ? (size_t)byte_row(n_experts) : (size_t)n_experts * 4);
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
@@ -780,13 +865,22 @@ hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void*
                                     uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   const GroupedRouter router(r, n_experts);
   const int per = grouped_tokens(tokens, router.per), blocks = (tokens + per - 1) / per;
+  const bool bytes = sums_bytes(tokens, blocks, n_experts);
   if (blocks) {
     const hipError_t e = with_logits<32>(logits_dtype, router.per, [&](auto l, auto nv) {
       constexpr int NV = decltype(nv)::value;
       hipLaunchKernelGGL((route_grouped_kernel<decltype(l)::value, NV>), dim3((unsigned)blocks),
-                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, router, experts, scores, scratch);
+                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, router, experts, scores, scratch,
+                         (int)bytes);
     });
     if (e != hipSuccess) return e;
+  }
+  if (bytes) {
+    const int rows = per * top_k, together = std::max(kSortRows / rows, 1);
+    hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3((unsigned)std::max((blocks + together - 1) / together, 1)),
+                       dim3(kSumThreads), 0, s, experts, tokens * top_k, together * rows, blocks, together, top_k, n_experts,
+                       scratch, lhs, rhs, inv, offsets);
+    return hipGetLastError();
   }
   return sort_blocks(s, experts, tokens * top_k, per * top_k, blocks, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
 }

@@ -145,6 +145,22 @@ def test_route(device, shape, sigmoid, biased, normalize, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,experts,k,groups,top,best", [
+    (8192, 256, 8, 8, 4, 2), (8193, 256, 3, 8, 4, 2), (2560, 1024, 8, 8, 2, 2), (2561, 1024, 8, 8, 2, 2), (65535, 32, 1, 4, 1, 1), (65536, 32, 1, 4, 1, 1), (70001, 2, 2, 2, 2, 1),
+    (2100, 1024, 5, 1, 1, 1), (1100, 1000, 16, 10, 4, 2), (40000, 17, 3, 1, 1, 1), (65535, 1, 1, 1, 1, 1)])
+def test_many_tokens(device, tokens, experts, k, groups, top, best):
+    """On either side of where the sort scans its histograms; all tokens with one expert, too."""
+    rng = np.random.default_rng(tokens)
+    logits = rng.standard_normal((tokens, experts)).astype(np.float32)
+    kw = dict(sigmoid=True, n_groups=groups, top_groups=top, group_best=best)
+    check(device, logits, "f32", k, **kw)
+    rows = rng.permutation(tokens)[:300]
+    logits[:] = np.linspace(3.0, -3.0, experts)  # the same picks for all but a few
+    logits[rows] = logits[rows, ::-1]
+    check(device, logits, "f32", k, **kw)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [3, 50])
 @pytest.mark.parametrize("sigmoid", [True, False])
 def test_ties(device, tokens, sigmoid):
