@@ -794,17 +794,14 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
         const uint64_t redo = __ballot(!(add[u] < kMost) || (kFolded && ref == -FLT_MAX));
         if (__builtin_expect(redo != 0, 0)) {
           const float cl = kScored ? 1.f : u ? cl1 : cl0;
-          if constexpr (kFolded) {
-#pragma unroll
-            for (int x = 0; x < 16; ++x) z[u][x] -= rel[u];
-          }
           float mine = logit(u, 0);
 #pragma unroll
           for (int x = 1; x < 16; ++x) mine = fmaxf(mine, logit(u, x));
           mine *= cl;
+          if constexpr (kFolded) mine -= rel[u];
           const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mine), __float_as_uint(mine), false, false);
           const float was = ref;
-          // (Rows that need none keep theirs: a row's result is its own.)
+          // (Rows that need none keep theirs, and their weights: a row's result is its own.)
           if ((redo | redo >> 32) >> col & 1)
             ref = fmaxf(ref, fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kRaise);
           const float keep = __builtin_amdgcn_exp2f(was - ref);
@@ -814,8 +811,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
           add[u] = 0.f;
           const float to = (float)(u ? d1 : d0) - ref;
           if constexpr (kFolded) {
+            const float by = to - rel[u];  // (0 where the reference stays)
 #pragma unroll
-            for (int x = 0; x < 16; ++x) z[u][x] += to;
+            for (int x = 0; x < 16; ++x) z[u][x] += by;
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) weights(u, to, i);
