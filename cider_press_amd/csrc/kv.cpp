@@ -1,5 +1,6 @@
 // Entry points of the 4-bit key/value cache (cpq_kv_*): argument validation
 // and launch.  No reference counterpart; semantics in cpq.h.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -84,6 +85,50 @@ bool rows_apart(size_t tokens, size_t heads, size_t d, size_t t, size_t h) {
   const bool inner_heads = (heads == 1 || h >= d) && (tokens == 1 || t >= (heads - 1) * h + d);
   const bool inner_tokens = (tokens == 1 || t >= d) && (heads == 1 || h >= (tokens - 1) * t + d);
   return inner_heads || inner_tokens;
+}
+
+// [tokens][heads] pieces of `bytes` bytes, `token` and `head` bytes apart.
+struct Rows {
+  const char* name;
+  const void* p;
+  size_t tokens, heads, token, head, bytes;
+};
+Rows rows_of(const char* name, const void* p, size_t tokens, size_t heads, size_t dim, size_t token, size_t head) {
+  return {name, p, tokens, heads, 2 * token, 2 * head, 2 * dim};  // strides and dim in elements of T
+}
+
+// Whether any two of their pieces share a byte.  Exact where tokens are equally far apart, as
+// slices of one fused buffer are (by the distances between heads that there are); others that
+// lie among each other count as sharing, and so do more than 2^16 pairs of differently spaced
+// heads.
+bool meet(const Rows& a, const Rows& b) {
+  auto extent = [](const Rows& r) { return (r.tokens - 1) * r.token + (r.heads - 1) * r.head + r.bytes; };
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+  if (!a.tokens || !b.tokens || !a.heads || !b.heads || !a.bytes || !b.bytes) return false;
+  if (x >= y + extent(b) || y >= x + extent(a)) return false;
+  if (a.tokens > 1 && b.tokens > 1 && a.token != b.token) return true;
+  const int64_t step = (int64_t)(a.tokens > 1 ? a.token : b.token);
+  const int64_t lo = -(int64_t)(a.tokens - 1), hi = (int64_t)(b.tokens - 1);
+  // A piece of b `d` bytes behind one of a, or any number of steps from lo to hi further.
+  auto hits = [&](int64_t d) {
+    const int64_t above = -(int64_t)b.bytes - d;  // d + i * step > -b.bytes: i * step > above
+    int64_t i = lo;
+    if (step > 0) i = std::max(lo, (above >= 0 ? above / step : -((-above + step - 1) / step)) + 1);
+    const int64_t at = d + i * step;
+    return i <= hi && at > -(int64_t)b.bytes && at < (int64_t)a.bytes;
+  };
+  const int64_t apart = (int64_t)(y - x);
+  if (a.heads == 1 || b.heads == 1 || a.head == b.head) {
+    const int64_t head = (int64_t)(a.heads > 1 ? a.head : b.head);
+    for (int64_t h = -(int64_t)(a.heads - 1); h < (int64_t)b.heads; ++h)
+      if (hits(apart + h * head)) return true;
+    return false;
+  }
+  if (a.heads * b.heads > (size_t(1) << 16)) return true;
+  for (size_t i = 0; i < a.heads; ++i)
+    for (size_t j = 0; j < b.heads; ++j)
+      if (hits(apart + (int64_t)(j * b.head) - (int64_t)(i * a.head))) return true;
+  return false;
 }
 
 bool overlap(const void* a, size_t a_words, const void* b, size_t b_words) {
@@ -333,7 +378,17 @@ cpq_status cpq_check_kv_append_rotary_args(const cpq_kv_cache* cache, const cpq_
   const Words w[] = {{"slots", a->slots, a->n_tokens},
                      {"positions", a->positions, a->n_tokens},
                      {"frequencies", a->frequencies, a->rotary_dim / 2}};
-  return check_words(op, w, 3, 0);
+  st = check_words(op, w, 3, 0);
+  // (In place the queries' own place is the caller's word.)
+  if (st != CPQ_OK || !a->n_heads || a->q == a->q_out) return st;
+  const Rows out = rows_of("q_out", a->q_out, a->n_tokens, a->n_heads, d, a->q_out_token_stride, a->q_out_head_stride);
+  for (const Rows& in : {rows_of("q", a->q, a->n_tokens, a->n_heads, d, a->q_token_stride, a->q_head_stride),
+                         rows_of("k", a->k, a->n_tokens, heads, d, a->k_token_stride, a->k_head_stride),
+                         rows_of("v", a->v, a->n_tokens, heads, d, a->v_token_stride, a->v_head_stride),
+                         Rows{w[0].name, w[0].p, 1, 1, 0, 0, 4 * w[0].n}, Rows{w[1].name, w[1].p, 1, 1, 0, 0, 4 * w[1].n},
+                         Rows{w[2].name, w[2].p, 1, 1, 0, 0, 4 * w[2].n}})
+    if (meet(out, in)) return invalid(op, std::string("q_out overlaps ") + in.name);
+  return CPQ_OK;
 }
 
 cpq_status cpq_kv_append_rotary(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* args) {

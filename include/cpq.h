@@ -607,8 +607,9 @@ cpq_status cpq_kv_attention_scored(cpq_commands* cmds, const cpq_kv_cache* cache
  *   (a, b) becomes (a c - b s, b c + a s)
  * over the pairs (i, i + rotary_dim / 2) or, interleaved, (2 i, 2 i + 1), i <
  * rotary_dim / 2, the other dimensions stay; with the arithmetic in fp64, rounded to fp32
- * and then to T.  Queries are written to q_out (which may be q at the same strides, and
- * else must not overlap an input); keys, rotated, and values go into the cache as
+ * and then to T.  Queries are written to q_out, which may be q at the same strides (k and v
+ * then lie apart from q), and else must not overlap an input, nor lie among an input's rows
+ * at another token stride; keys, rotated, and values go into the cache as
  * cpq_kv_append puts them there, bit for bit.  Tokens whose slot is none are skipped,
  * their rows of q_out too; so are slots past the cache, which are reported as by
  * cpq_kv_append.
@@ -641,7 +642,8 @@ typedef struct cpq_kv_append_rotary_args {
 cpq_status cpq_kv_append_rotary(cpq_commands* cmds, const cpq_kv_cache* cache, const cpq_kv_append_rotary_args* args);
 
 /* Host-only argument validators of the above (callable without a GPU; of the
- * pointers only NULL, alignment and overlap are looked at). */
+ * pointers only NULL and alignment are looked at, and for kv_append_rotary that a q_out
+ * other than q overlaps no input). */
 cpq_status cpq_check_kv_cache(const cpq_kv_cache* cache);
 cpq_status cpq_check_kv_attention_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* args);
 cpq_status cpq_check_kv_attention_scored_args(const cpq_kv_cache* cache, const cpq_kv_attention_args* args,
