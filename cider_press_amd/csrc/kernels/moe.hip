@@ -369,11 +369,10 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
 // Small workgroups make more histograms, large ones leave CUs idle: four tokens each while that
 // is one for a CU, then eight, then 16 (256 experts, 1000 tokens 13.4 us, 15.5 with 16 each; 1500
 // 14.0, 15.6 with 16; 4000, in 16s either way, 16.2).
-constexpr int kFewBlocks = 256;
 constexpr int most_tokens(int nv) { return nv > 8 ? 8 : 16; }  // by the registers of a wave
-inline int grouped_tokens(int tokens, int nv) {
+inline int grouped_tokens(int tokens, int nv, int cus) {
   int per = 4;
-  while (per < most_tokens(nv) && tokens > kFewBlocks * per) per *= 2;
+  while (per < most_tokens(nv) && tokens > cus * per) per *= 2;
   return per;
 }
 // A histogram's rows of bytes (a token picks an expert once, so counts are at most 16), where the
@@ -855,16 +854,16 @@ static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, 
   return hipGetLastError();
 }
 
-size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r) {
-  const int per = grouped_tokens(tokens, GroupedRouter(r, n_experts).per), blocks = (tokens + per - 1) / per;
+size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r, int cus) {
+  const int per = grouped_tokens(tokens, GroupedRouter(r, n_experts).per, cus), blocks = (tokens + per - 1) / per;
   return (size_t)blocks * (sums_bytes(tokens, blocks, n_experts) ? (size_t)byte_row(n_experts) : (size_t)n_experts * 4);
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
-                                    int top_k, const cpq_moe_router& r, uint32_t* experts, float* scores,
+                                    int top_k, const cpq_moe_router& r, int cus, uint32_t* experts, float* scores,
                                     uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   const GroupedRouter router(r, n_experts);
-  const int per = grouped_tokens(tokens, router.per), blocks = (tokens + per - 1) / per;
+  const int per = grouped_tokens(tokens, router.per, cus), blocks = (tokens + per - 1) / per;
   const bool bytes = sums_bytes(tokens, blocks, n_experts);
   if (blocks) {
     const hipError_t e = with_logits<32>(logits_dtype, router.per, [&](auto l, auto nv) {

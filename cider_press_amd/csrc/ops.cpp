@@ -918,8 +918,9 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
   cpq_status st = cpq_check_moe_route_grouped_args(logits_dtype, tokens, n_experts, top_k, router);
   if (st != CPQ_OK) return st;
   uint32_t* hist;
+  const int cus = cpq::session_ctx(cmds).cu_count;
   st = cpq::check_route_buffers(op, cmds, tokens,
-                                cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts, *router), logits, experts,
+                                cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts, *router, cus), logits, experts,
                                 scores, lhs, rhs, inv, offsets, &hist);
   if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))
@@ -929,7 +930,7 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
                                                             static_cast<unsigned int*>(cmds->scratch)),
                          "moe_route_grouped launch");
   return cpq::launched(cpq::launch_moe_route_grouped(cmds->stream, (int)logits_dtype, logits, (int)tokens,
-                                                     (int)n_experts, (int)top_k, *router, experts, scores, hist, lhs,
+                                                     (int)n_experts, (int)top_k, *router, cus, experts, scores, hist, lhs,
                                                      rhs, inv, offsets),
                        "moe_route_grouped launch");
 }
