@@ -146,7 +146,7 @@ hipError_t launch_moe_route_sort(hipStream_t s, int logits_dtype, const void* lo
                                  uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
 // The grouped router with its sort on a device of `cus` compute units; in one launch for a few
 // tokens (`counter` zero between launches).
-size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r, int cus);
+size_t moe_grouped_scratch_bytes(int tokens, int n_experts, int top_k, const cpq_moe_router& r, int cus);
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
                                     int top_k, const cpq_moe_router& r, int cus, uint32_t* experts, float* scores,
                                     uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);

@@ -366,6 +366,7 @@ __global__ __launch_bounds__(256) void route_kernel(const void* __restrict__ log
 
 // The grouped router, a token to a wave, with the histogram of the workgroup's tokens, which
 // the sort starts from (a launch less: 8191 tokens of 256 experts 26.0 us instead of 27.4).
+// (Null `counts`: none is asked for.)
 // Small workgroups make more histograms, large ones leave CUs idle: four tokens each while that
 // is one for a CU, then eight, then 16 (256 experts, 1000 tokens 13.4 us, 15.5 with 16 each; 1500
 // 14.0, 15.6 with 16; 4000, in 16s either way, 16.2).
@@ -397,6 +398,7 @@ __global__ __launch_bounds__(most_tokens(NV) * 64) void route_grouped_kernel(
       atomicAdd(&h[pick], 1u);
     }
   }
+  if (!counts) return;
   __syncthreads();
   if (bytes) {
     for (int i = threadIdx.x; i < row / 4; i += blockDim.x)
@@ -665,10 +667,11 @@ __device__ __forceinline__ void sum_bytes(const u32x4* __restrict__ counts, int 
     }
   }
 }
-// Up to here (and below 65536 tokens) it does, which saves the scan's launch; past it the scan
-// reads less (of 256 experts 8191 tokens 22.7 us, 24.8 with the scan; 16000 38.7 and 44.2; 24000,
-// 375 KB, 59.1 and 59.3; 32000 78.3 and 74.1).
-constexpr size_t kByteSums = 320 * 1024;
+// Up to here (and below 65536 tokens) it does, which saves launches; past it counting and the
+// scan read less (of 256 experts, 8 picks: 8191 tokens 22.7 us, 25.5 with the scan; 12000 31.6
+// and 36.1; 16000, 250 KB, 38.3 and 39.2; 20480 51.4 and 47.3; 32000 77.1 and 67.4; 2 picks of
+// 20480 33.6 and 35.4, 16 picks 71.3 and 57.4).
+constexpr size_t kByteSums = 256 * 1024;
 inline bool sums_bytes(int tokens, int blocks, int n_experts) {
   return tokens < 65536 && (size_t)blocks * byte_row(n_experts) <= kByteSums;
 }
@@ -854,9 +857,18 @@ static hipError_t sort_blocks(hipStream_t s, const uint32_t* experts, int rows, 
   return hipGetLastError();
 }
 
-size_t moe_grouped_scratch_bytes(int tokens, int n_experts, const cpq_moe_router& r, int cus) {
+// Where histograms are scanned: whether they are the routing workgroups' own, of `rows` rows.
+// Those of half a sort block or less are many, each with a scatter workgroup of its own: then
+// the picks are counted again, a block at a time, a launch more (65536 tokens of 256 experts, 8
+// picks 113 us, 129 with the routing kernel's histograms of 128 rows; 2 picks 79 and 109; 131072
+// tokens of 64 experts, 1 pick 62 and 127; 65536 of 1024, 8 picks 389 and 450), in the scratch
+// that moe_route takes.
+inline bool keeps_counts(int rows) { return 2 * rows > kSortRows; }
+
+size_t moe_grouped_scratch_bytes(int tokens, int n_experts, int top_k, const cpq_moe_router& r, int cus) {
   const int per = grouped_tokens(tokens, GroupedRouter(r, n_experts).per, cus), blocks = (tokens + per - 1) / per;
-  return (size_t)blocks * (sums_bytes(tokens, blocks, n_experts) ? (size_t)byte_row(n_experts) : (size_t)n_experts * 4);
+  if (sums_bytes(tokens, blocks, n_experts)) return (size_t)blocks * byte_row(n_experts);
+  return keeps_counts(per * top_k) ? (size_t)blocks * n_experts * 4 : moe_sort_scratch_bytes(tokens * top_k, n_experts);
 }
 
 hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void* logits, int tokens, int n_experts,
@@ -864,16 +876,17 @@ hipError_t launch_moe_route_grouped(hipStream_t s, int logits_dtype, const void*
                                     uint32_t* scratch, uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets) {
   const GroupedRouter router(r, n_experts);
   const int per = grouped_tokens(tokens, router.per, cus), blocks = (tokens + per - 1) / per;
-  const bool bytes = sums_bytes(tokens, blocks, n_experts);
+  const bool bytes = sums_bytes(tokens, blocks, n_experts), counted = bytes || keeps_counts(per * top_k);
   if (blocks) {
     const hipError_t e = with_logits<32>(logits_dtype, router.per, [&](auto l, auto nv) {
       constexpr int NV = decltype(nv)::value;
       hipLaunchKernelGGL((route_grouped_kernel<decltype(l)::value, NV>), dim3((unsigned)blocks),
-                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, router, experts, scores, scratch,
-                         (int)bytes);
+                         dim3(per * 64), 0, s, logits, tokens, n_experts, top_k, router, experts, scores,
+                         counted ? scratch : nullptr, (int)bytes);
     });
     if (e != hipSuccess) return e;
   }
+  if (!counted) return launch_moe_sort(s, experts, tokens * top_k, top_k, n_experts, scratch, lhs, rhs, inv, offsets);
   if (bytes) {
     const int rows = per * top_k, together = std::max(kSortRows / rows, 1);
     hipLaunchKernelGGL(sort_scatter_kernel<true>, dim3((unsigned)std::max((blocks + together - 1) / together, 1)),

@@ -920,7 +920,7 @@ cpq_status cpq_moe_route_grouped(cpq_commands* cmds, cpq_dtype logits_dtype, con
   uint32_t* hist;
   const int cus = cpq::session_ctx(cmds).cu_count;
   st = cpq::check_route_buffers(op, cmds, tokens,
-                                cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts, *router, cus), logits, experts,
+                                cpq::moe_grouped_scratch_bytes((int)tokens, (int)n_experts, (int)top_k, *router, cus), logits, experts,
                                 scores, lhs, rhs, inv, offsets, &hist);
   if (st != CPQ_OK) return st;
   if (cpq::moe_route_sort_fits((int)tokens))

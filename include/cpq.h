@@ -400,7 +400,8 @@ cpq_status cpq_embed_tokens(cpq_commands* cmds, cpq_dtype dtype, const uint32_t*
  * expert, stably: lhs[p] = token and rhs[p] = expert of sorted row p (the
  * sorted-index inputs of cpq_affine_gather_qmm), inv[r] = sorted position
  * of row r, offsets[e] = first sorted row of expert e, offsets[E] = tokens*k.
- * n_experts <= 1024, top_k <= min(16, n_experts).  Uses session scratch. */
+ * n_experts <= 1024, top_k <= min(16, n_experts).  Uses session scratch, 4 * n_experts
+ * bytes for every 256 rows. */
 cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void* logits, size_t tokens,
                          size_t n_experts, uint32_t top_k, int normalize, uint32_t* experts, float* scores,
                          uint32_t* lhs, uint32_t* rhs, uint32_t* inv, uint32_t* offsets);
@@ -417,7 +418,9 @@ cpq_status cpq_moe_route(cpq_commands* cmds, cpq_dtype logits_dtype, const void*
  * are made in fp64 because they are whole numbers: in fp32 near scores would change
  * places with the order of a sum.  Then the sort, as moe_route.  n_experts <= 1024, top_k
  * <= min(16, n_experts / n_groups * top_groups), n_groups <= 64 divides n_experts,
- * group_best <= n_experts / n_groups, tokens <= 2^25.  Uses session scratch. */
+ * group_best <= n_experts / n_groups, tokens <= 2^25.  Uses session scratch, 256 KiB or at
+ * most 4 * n_experts bytes for every 128 rows: a default session's 64 MiB hold the sort of
+ * some 2 million rows of 1024 experts. */
 typedef struct cpq_moe_router {
   int sigmoid;
   const float* bias;
