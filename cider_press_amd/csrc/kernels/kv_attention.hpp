@@ -517,7 +517,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
   // The first key of the t-th tile of `begin` to `stop`.  With biases, which mostly fall
   // with distance, the last keys come first: forward the weights of most heads grow from tile
   // to tile, and with each the reference is raised and weights are made twice (4096 queries
-  // over 8192 keys 667 us; so 483.  Slopes below 0 still have it).
+  // over 8192 keys 667 us; so 485.  Slopes below 0 still have it).
   auto key_of = [&](int t) { return (biased(SCORES) ? begin + stop - 1 - t : t) * kKeys; };
   auto load = [&](int t) {
     const int lane = (int)opaque((uint32_t)(tid & 63));
@@ -732,8 +732,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 256 ? 1 : D == 64 && !GS ? 3 : 2)
       };
       uint32_t seen[2];  // where not all are (scored)
       // What the scores become (apart from `sc`, whose 16 registers stay one operand).  Caps
-      // bound how far they lie from the reference, which is subtracted on the way then (574
-      // us instead of 580); with biases it would take their last bits where it jumps.
+      // bound how far they lie from the reference, which is subtracted on the way then (568
+      // us instead of 578); with biases it would take their last bits where it jumps.
       constexpr bool kFolded = SCORES == Scores::kCapped;
       float rel[2];  // what `z` holds besides
       float z[kScored ? 2 : 1][16];

@@ -218,7 +218,8 @@ __device__ __forceinline__ KvSeq kv_seq(const cpq_kv_attention_args& a, int s, i
 
 // What scores become, in units of log2(e) (cpq_kv_attention_scored): nothing else, plus a
 // bias, capped, both.  (A bias costs an addition a score: 4096 capped queries over 8192 keys
-// 571 us without, 589 with.)  With a cap
+// 572 us without, 590 with.  Prefixes alone run with a bias of 0: 4096 queries over 8192 keys
+// 507 us, 451 as the plain form.)  With a cap
 //   cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)),
 // whose error is one of cap, 2^-22 of it, where s itself is small: caps are limited to
 // kKvMostCap, which leaves a weight off by 2^-11 of itself at most.  Both ends of the

@@ -31,6 +31,10 @@
 // T = f16 by its instructions too (the same three: 110 us, 4.2 TB/s), by fixed
 // phases of 9 us where they are not: launch, search, first tile, join (48 requests of
 // up to 8193 tokens: 27 us, 2.6 TB/s; one of 391 tokens, 2 heads of 64: 8.6 us).
+// With a bias 17 to 32 rows at T = f16 in groups of 32 do not fit the registers (23 to 60 of
+// them go to scratch memory): 3 drafts each of three requests of 60001 tokens, 64 heads of 128
+// on 8, 79 us without scores, 88 capped, 108 with a bias, 115 with both; of 30001 tokens, heads
+// of 256, 141, 150, 167 and 177.  In groups of 64 73, 81, 82 and 89 (256: 111, 116, 144, 152).
 #pragma once
 
 #include <algorithm>
